@@ -21,7 +21,8 @@ INCLUDE_DIR = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libsx8_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["sx8_abi.hip", "sx8_dequant.hip", "sx8_layout.hip", "sx8_quant.hip", "sx8_gemv.hip",
-           "sx8_gemm.hip", "sx8_gemm_small.hip", "sx8_decoder.hip"]
+           "sx8_gemm.hip", "sx8_gemm_small.hip", "sx8_decoder.hip", "sx8_attn_varlen.hip", "sx8_kv4.hip",
+           "sx8_pages.hip"]
 PY_SOURCE, PY_PATH = "sx8_py.cpp", os.path.join(PKG_DIR, "_sx8py.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -41,7 +42,7 @@ HIP_FLAGS = [
 _PRELOAD8 = ["-mllvm", "-amdgpu-kernarg-preload-count=8"]
 SOURCE_FLAGS = {"sx8_gemv.hip": _PRELOAD8, "sx8_decoder.hip": _PRELOAD8}
 
-# (name, restype, argtypes) for every exported symbol of include/sx8_hip.h
+# (name, restype, argtypes) for every exported symbol of include/*.h
 _P = ctypes.c_void_p
 _I32, _I64 = ctypes.c_int32, ctypes.c_int64
 SIGNATURES = [
@@ -116,8 +117,24 @@ SIGNATURES = [
     ("sx8_dec_gemv_rmsnorm_pair", _I32, [_P, _P, ctypes.c_float, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _I64, _I64,
                                          _P, _P, _P, _P]),
     ("sx8_dec_gemv_zp_add", _I32, [_P, _P, _P, _I32, _P, _P, _I64, _I64, _P, _P, _P]),
+    # include/sx8_paged.h
+    ("sx8_attn_varlen", _I32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64,
+                               _I64, _I64, _I64, _I64, ctypes.c_float, _I32, _I32, _P]),
+    ("sx8_kv4_page_bytes", _I64, [_I32, _I32, _I32]),
+    ("sx8_kv4_append", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32,
+                              _I32, _P]),
+    ("sx8_kv4_read", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32,
+                            _I32, _P]),
+    ("sx8_kv4_attend", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32,
+                              _I32, ctypes.c_float, _I32, _P, _I64, _P]),
+    ("sx8_kv4_attend_workspace_bytes", _I64, [_I32]),
+    ("sx8_kv4_pages_workspace_bytes", _I64, [_I64, _I64]),
+    ("sx8_kv4_reserve", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P, _P, _I64, _P]),
+    ("sx8_kv4_fork", _I32, [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _I64, _P]),
+    ("sx8_kv4_free", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P]),
+    ("sx8_kv4_compact", _I32, [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),
 ]
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 _lib = None
 _py = None

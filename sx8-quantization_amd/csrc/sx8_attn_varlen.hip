@@ -1,0 +1,346 @@
+// sx8_attn_varlen.hip -- attention of packed sequences (include/sx8_paged.h: sx8_attn_varlen).
+#include <type_traits>
+
+#include "sx8_buffer.h"
+#include "sx8_host.h"
+#include "sx8_kv4_dev.h"
+#include "sx8_paged.h"
+
+namespace sx8 {
+namespace {
+
+// A work-group takes 128 query rows of one head of a sequence, 32 to each of its four waves, and walks the keys in
+// tiles that all waves read from LDS.  Per 32 keys a wave computes S^T = K Q^T on the 32x32x16 MFMA with the keys as
+// rows and its queries as columns, so that lane 32 h + c holds scores of query c alone (keys 8 (r / 4) + 4 h + r % 4 in
+// accumulator r) and the online softmax needs one exchange, with lane ^ 32.  O^T += V^T P^T takes P^T from those
+// accumulators as they lie (the order of the contracted keys is free: slot t of half h of step st is key
+// 16 st + 8 (t / 4) + 4 h + t % 4), and V^T by the LDS transpose read, which hands a lane four keys of its dimension.
+// K and V go from memory to LDS directly, the next tile while this one is computed; rows past the sequence's
+// last key lie past the buffer and come as zeros.  A 16-byte chunk of a row lies at its position XOR a few bits of
+// the row, so that neither kind of read meets bank conflicts (the swap is made in the load's address).
+template <int HD>
+struct VarTile {
+    static constexpr int kKeys = HD == 256 ? 32 : 64;        // of a tile
+    static constexpr int kChunks = HD / 8;                   // 16-byte chunks of a row
+    static constexpr int kBytes = kKeys * HD * 2;            // of K or V
+    __device__ static int k_swz(int row) { return row & (HD == 128 ? 15 : 7); }
+    __device__ static int v_swz(int row) { return HD == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
+};
+
+struct VarIo {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* out;
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    int64_t Tq, Tk, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
+    int n_seq, nh, nk;
+    float scale_log2;
+};
+
+constexpr int kRows = 128;
+
+// Rows of sequence b in a packed tensor of T rows: first row and count.
+__device__ __forceinline__ void seq_rows(const int32_t* cu, int64_t T, int b, int64_t* first, int64_t* n) {
+    const int64_t a = kv4_clamp(cu[b], 0, T), e = kv4_clamp(cu[b + 1], a, T);
+    *first = a;
+    *n = e - a;
+}
+
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+
+// 16 bytes a lane from the buffer to 1 KB of LDS at dst
+__device__ __forceinline__ void load_lds(sx8_rsrc r, lds_u8* dst, int off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, dst, 16, off, 0, 0, 0);
+}
+// Lane i of 16 names the eight bytes of key i / 4 that hold dimensions 4 (i % 4) .. + 3, and gets dimension i of the four keys.
+__device__ __forceinline__ u32x2 read_tr(const unsigned char* at) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+}
+
+template <bool kBf16>
+struct Mma;
+template <>
+struct Mma<false> {
+    typedef _Float16 vec8 __attribute__((ext_vector_type(8)));
+    template <typename A>
+    __device__ static A mul(u32x4 a, u32x4 b, A c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t kExp = 0x7C007C00u, kOne = 0x04000400u;      // exponent bits, their lowest
+};
+template <>
+struct Mma<true> {
+    typedef __bf16 vec8 __attribute__((ext_vector_type(8)));
+    template <typename A>
+    __device__ static A mul(u32x4 a, u32x4 b, A c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t kExp = 0x7F807F80u, kOne = 0x00800080u;
+};
+
+// K and V of two tiles, and before that the prefix sums of the sequences' tiles
+template <int HD>
+constexpr int var_lds_bytes() {
+    constexpr int a = 4 * VarTile<HD>::kBytes, b = (kKv4MaxSlots + 1) * 8;
+    return a > b ? a : (b + 15) / 16 * 16;
+}
+
+template <int HD, bool kBf16, bool kCausal>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const VarIo io) {
+    typedef float f32x16 __attribute__((ext_vector_type(16)));
+    using T = VarTile<HD>;
+    using M = Mma<kBf16>;
+    constexpr float kInf = __builtin_inff();
+    constexpr int KB = T::kKeys, NB = KB / 32, KS = HD / 16, NT = HD / 32, CH = T::kChunks;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ __align__(16) unsigned char var_lds[var_lds_bytes<HD>()];
+    int64_t* const pre = reinterpret_cast<int64_t*>(var_lds);
+    // the tile of queries: the last ones of a sequence, which see the most keys, come first; consecutive work-groups (of
+    // different XCDs) take different KV heads, so that the query heads of one share its XCD's L2
+    prefix_sums<256>(io.n_seq, pre, [&](int b) {
+        int64_t f, n;
+        seq_rows(io.cu_q, io.Tq, b, &f, &n);
+        return (n + kRows - 1) / kRows;
+    });
+    __syncthreads();
+    const int64_t item = uniform(pre[io.n_seq]) - 1 - blockIdx.x / io.nh;
+    if (item < 0) return;
+    const int hh = blockIdx.x % io.nh, G = io.nh / io.nk, kvh = hh % io.nk, head = kvh * G + hh / io.nk;
+    const int b = find_item<256>(io.n_seq, pre, item);
+    int64_t q_first, nq, k_first, nkeys;
+    seq_rows(io.cu_q, io.Tq, b, &q_first, &nq);
+    seq_rows(io.cu_k, io.Tk, b, &k_first, &nkeys);
+    q_first = uniform(q_first);
+    nq = uniform(nq);
+    k_first = uniform(k_first);
+    nkeys = uniform(nkeys);
+    const int64_t q0 = (item - uniform(pre[b])) * kRows + 32 * w;        // the wave's first row in the sequence
+    __syncthreads();                                                     // (pre makes room for the first tile)
+    const int64_t past = nkeys - nq;                                     // row i attends keys 0 .. past + i
+    const int64_t wg_last = (q0 - 32 * w + kRows < nq ? q0 - 32 * w + kRows : nq) - 1;
+    const int64_t see = kCausal ? (past + wg_last + 1 < 0 ? 0 : past + wg_last + 1) : nkeys;    // keys of the work-group
+    const int n_tiles = (int)((see + KB - 1) / KB);
+    const int64_t w_last = (q0 + 32 < nq ? q0 + 32 : nq) - 1;            // the wave's last row
+    const int64_t w_see = q0 >= nq ? 0 : kCausal ? past + w_last + 1 : nkeys;
+    const int64_t w_all = q0 >= nq ? 0 : kCausal ? past + q0 + 1 : nkeys;   // keys that all its rows see
+    const bool row_ok = q0 + c < nq;
+    const int64_t lim = kCausal ? past + (row_ok ? q0 + c : nq - 1) : nkeys - 1;
+    u32x4 qf[KS];
+    {
+        const uint16_t* qr = io.q + (q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs + 8 * h;
+#pragma unroll
+        for (int st = 0; st < KS; ++st) qf[st] = *reinterpret_cast<const u32x4*>(qr + 16 * st);
+    }
+    const uint16_t* const kp = io.k + k_first * io.k_ts + kvh * io.k_hs;
+    const uint16_t* const vp = io.v + k_first * io.v_ts + kvh * io.v_hs;
+    // loads: a wave instruction fills 1 KB of LDS; instruction i of wave w holds rows (4 i + w) R .. (R = 512 / HD
+    // rows; for HD 256 half of one each), R rows apart by waves so that a lane's row keeps its low bits over i
+    // (the whole offset goes into the load's vector offset: only that one is checked against the buffer's end)
+    constexpr int R = 64 / CH, NI = T::kBytes / 4096;
+    const int lrow = w * R + lane / CH, lpos = lane % CH;
+    const int k_off = (int)(lrow * io.k_ts * 2) + 16 * (lpos ^ T::k_swz(lrow));
+    const int v_off = (int)(lrow * io.v_ts * 2) + 16 * (lpos ^ T::v_swz(lrow));
+    auto fetch = [&](int j, int buf) __attribute__((always_inline)) {
+        const int64_t k0 = (int64_t)j * KB, left = nkeys - k0 < KB ? nkeys - k0 : KB;
+        const sx8_rsrc kr = make_rsrc(kp + k0 * io.k_ts, (left - 1) * io.k_ts * 2 + HD * 2);
+        const sx8_rsrc vr = make_rsrc(vp + k0 * io.v_ts, (left - 1) * io.v_ts * 2 + HD * 2);
+        lds_u8* const dst = (lds_u8*)var_lds + buf * 2 * T::kBytes + w * 1024;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            load_lds(kr, dst + i * 4096, k_off + 8 * R * i * (int)io.k_ts);
+            load_lds(vr, dst + T::kBytes + i * 4096, v_off + 8 * R * i * (int)io.v_ts);
+        }
+    };
+    f32x16 o[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
+    // running maximum in powers of two, raised when a score exceeds it by more than 8: probabilities stay at or below 2^8
+    float m = -kInf, l = 0.f;
+    // V^T reads: key and dimension that the lane names
+    const int vi = lane & 15, vd = (lane >> 4 & 1) * 16 + 4 * (vi & 3), vk = 4 * h + (vi >> 2);
+    auto tile = [&](int j, int buf, auto mask) __attribute__((always_inline)) {
+        constexpr bool kMask = decltype(mask)::value;
+        const unsigned char* kt = var_lds + buf * 2 * T::kBytes;
+        const unsigned char* vt = kt + T::kBytes;
+        f32x16 s[NB];
+#pragma unroll
+        for (int a = 0; a < NB; ++a) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[a][r] = 0.f;
+            const int row = 32 * a + c;
+#pragma unroll
+            for (int st = 0; st < KS; ++st) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + row * (HD * 2) + 16 * ((2 * st + h) ^ T::k_swz(row)));
+                s[a] = M::mul(kf, qf[st], s[a]);
+            }
+        }
+        if constexpr (kMask) {
+#pragma unroll
+            for (int a = 0; a < NB; ++a)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t key = (int64_t)j * KB + 32 * a + 8 * (r >> 2) + 4 * h + (r & 3);
+                    s[a][r] = key <= lim ? s[a][r] : -kInf;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int a = 0; a < NB; ++a)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[a][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * io.scale_log2;
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
+        }
+        const float nm = m == -kInf ? 0.f : -m;
+#pragma unroll
+        for (int a = 0; a < NB; ++a)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[a][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][r], io.scale_log2, nm));
+                l += s[a][r];
+            }
+        uint32_t odd = 0;
+#pragma unroll
+        for (int st = 0; st < KB / 16; ++st) {
+            u32x4 pf;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pf[e] = pack16<kBf16>(s[st / 2][8 * (st & 1) + 2 * e], s[st / 2][8 * (st & 1) + 2 * e + 1]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                u32x4 vf;
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const int row = 16 * st + 8 * a + vk, d = 32 * n + vd;
+                    const u32x2 x = read_tr(vt + row * (HD * 2) + 16 * ((d / 8) ^ T::v_swz(row)) + 2 * (d % 8));
+                    vf[2 * a] = x.x;
+                    vf[2 * a + 1] = x.y;
+                }
+                if constexpr (kMask) {
+                    // values that are no finite numbers are left out here (below)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t top = (vf[e] & M::kExp) + M::kOne;        // its half's sign bit: not finite
+                        odd |= top;
+                        const uint32_t bad = (top >> 15 & 0x00010001u) * 0xFFFFu;
+                        vf[e] &= ~bad;
+                    }
+                }
+                o[n] = M::mul(vf, pf, o[n]);
+            }
+        }
+        if constexpr (kMask) {
+            // A key that some row may not attend has probability zero there, and 0 * NaN must not reach the row: values that
+            // are not finite are added here, to the rows that give them weight.
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) != 0) {
+                for (int key = 0; key < KB; ++key) {
+                    float p = 0.f;
+                    // the probability of the key: lane half (key >> 2) & 1, accumulator 4 (key % 32 / 8) + key % 4
+#pragma unroll
+                    for (int a = 0; a < NB; ++a)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (key >> 5 == a && (key & 31) >> 3 == r >> 2 && (key & 3) == (r & 3)) p = s[a][r];
+                    p = __shfl(p, c + 32 * (key >> 2 & 1), 64);
+                    if (p == 0.f) continue;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int d = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
+                            const float x = ld16<kBf16>(*reinterpret_cast<const uint16_t*>(
+                                vt + key * (HD * 2) + 16 * ((d / 8) ^ T::v_swz(key)) + 2 * (d % 8)));
+                            if (!(__builtin_fabsf(x) < kInf)) o[n][r] = __builtin_fmaf(p, x, o[n][r]);
+                        }
+                }
+            }
+        }
+    };
+    if (n_tiles > 0) fetch(0, 0);
+    for (int j = 0; j < n_tiles; ++j) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                          // tile j is there, and nobody reads the other buffer any more
+        if (j + 1 < n_tiles) fetch(j + 1, (j + 1) & 1);
+        const int64_t k0 = (int64_t)j * KB;
+        if (k0 < w_see) {
+            if (k0 + KB > w_all) tile(j, j & 1, std::true_type{});
+            else tile(j, j & 1, std::false_type{});
+        }
+    }
+    if (!row_ok) return;
+    l += __shfl_xor(l, 32, 64);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* const dst = io.out + (q_first + q0 + c) * io.o_ts + head * io.o_hs + 4 * h;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                x[e] = pack16<kBf16>(o[n][4 * g + 2 * e] * inv, o[n][4 * g + 2 * e + 1] * inv);
+            *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * g) = u32x2{x[0], x[1]};
+        }
+}
+
+template <int HD>
+void launch(const VarIo& io, int dtype, int causal, unsigned grid, hipStream_t st) {
+    if (dtype && causal) hipLaunchKernelGGL((k_attn_varlen<HD, true, true>), dim3(grid), dim3(256), 0, st, io);
+    else if (dtype) hipLaunchKernelGGL((k_attn_varlen<HD, true, false>), dim3(grid), dim3(256), 0, st, io);
+    else if (causal) hipLaunchKernelGGL((k_attn_varlen<HD, false, true>), dim3(grid), dim3(256), 0, st, io);
+    else hipLaunchKernelGGL((k_attn_varlen<HD, false, false>), dim3(grid), dim3(256), 0, st, io);
+}
+
+}  // namespace
+}  // namespace sx8
+
+extern "C" int32_t sx8_attn_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
+                                   const int32_t* cu_k, int64_t n_seq, int64_t Tq, int64_t Tk, int32_t nh, int32_t nk,
+                                   int32_t hd, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
+                                   int64_t v_hs, int64_t o_ts, int64_t o_hs, float scale, int32_t causal, int32_t dtype,
+                                   void* stream) {
+    using namespace sx8;
+    const char* what = "sx8_attn_varlen";
+    if (!cu_q || !cu_k || (Tq > 0 && (!q || !out)) || (Tk > 0 && (!k || !v)))
+        return fail(SX8_ERR_INVALID, "%s: null pointer", what);
+    if ((hd != 64 && hd != 128 && hd != 256) || nk <= 0 || nh <= 0 || nh % nk || nh > 65536)
+        return fail(SX8_ERR_INVALID, "%s: bad shape (hd 64, 128 or 256, nh a multiple of nk)", what);
+    if (n_seq <= 0 || n_seq > kKv4MaxSlots || Tq < 0 || Tq > 0x7FFFFFFF || Tk < 0 || Tk > 0x7FFFFFFF)
+        return fail(SX8_ERR_INVALID, "%s: bad sizes (n_seq 1..%d, Tq and Tk 0..2^31 - 1)", what, kKv4MaxSlots);
+    if (dtype != 0 && dtype != 1) return fail(SX8_ERR_INVALID, "%s: dtype must be 0 (fp16) or 1 (bf16)", what);
+    if (!(scale > 0.f) || !(scale < __builtin_inff()))
+        return fail(SX8_ERR_INVALID, "%s: scale must be positive and finite", what);
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(cu_q, 4) || !aligned(cu_k, 4))
+        return fail(SX8_ERR_INVALID, "%s: q, k, v and out must be 16-byte aligned, cu_q and cu_k 4-byte", what);
+    const int64_t strides[8] = {q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs};
+    for (int i = 0; i < 8; ++i)
+        if (strides[i] % 8 || strides[i] < 0 || strides[i] > (int64_t)1 << 40)
+            return fail(SX8_ERR_INVALID, "%s: strides must be multiples of 8", what);
+    if (k_ts < hd || v_ts < hd || k_ts > 1 << 23 || v_ts > 1 << 23)     // (a tile's rows lie within 32-bit offsets)
+        return fail(SX8_ERR_INVALID, "%s: the token strides of k and v must be hd .. 2^23", what);
+    const int64_t grid = ((Tq + kRows - 1) / kRows + (n_seq < Tq ? n_seq : Tq)) * nh;
+    if (grid > 0x7FFFFFFF) return fail(SX8_ERR_UNSUPPORTED, "%s: over 2^31 tiles of rows", what);
+    if (Tq == 0) return ok();
+    const VarIo io{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, cu_q, cu_k, Tq, Tk, q_ts, q_hs,
+                   k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, (int)n_seq, nh, nk, scale * 1.4426950408889634f};
+    const hipStream_t st = as_stream(stream);
+    if (hd == 64) launch<64>(io, dtype, causal, (unsigned)grid, st);
+    else if (hd == 128) launch<128>(io, dtype, causal, (unsigned)grid, st);
+    else launch<256>(io, dtype, causal, (unsigned)grid, st);
+    return check_launch(what);
+}

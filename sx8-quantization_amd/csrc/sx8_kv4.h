@@ -1,0 +1,90 @@
+// sx8_kv4.h -- the 4-bit KV cache format: where a value's bits lie, and how the attention over it is
+// cut into pieces.  Plain integer functions, the same on the host (tests) and in the kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#define SX8_KV4_FN __host__ __device__ __forceinline__
+
+namespace sx8 {
+
+constexpr int kKv4Group = 64;        // values that share a scale and a minimum
+constexpr int kKv4Block = 32;        // tokens of a block
+constexpr int kKv4MaxSlots = 4096;
+constexpr int64_t kKv4MaxTokens = 1 << 22;   // of a slot (max_pages * page_tokens)
+
+// A block holds the K and V rows of 32 tokens of one head:
+//   K levels (16 hd bytes) | V levels (16 hd) | K scales | K minima | V scales | V minima (hd / 64 * 64 each)
+// Levels are 4-bit, eight to a 32-bit word (value e of a word at bits 4 (e / 2) + 16 (e % 2), so that
+// (word >> 4 i) & 0x000F000F are values 2 i and 2 i + 1 as two 16-bit numbers), and lie as a 16x16x32 MFMA
+// takes them as its row operand: lane 16 h + c of 64 holds row c, steps 8 h .. 8 h + 7.
+//   K: rows are tokens (two tiles of 16), steps are dimensions: word j of a lane covers dimensions 32 j + 8 h + e.
+//   V: rows are dimensions (tile t: 16 t + c), steps are tokens: value e of the word of a lane is token
+//      16 (e / 4) + 4 h + e % 4 -- the order in which the score tiles' accumulators hold them.
+SX8_KV4_FN constexpr int kv4_block_bytes(int hd) { return 32 * hd + hd / kKv4Group * 256; }
+SX8_KV4_FN constexpr int kv4_shift(int e) { return 4 * (e >> 1) + 16 * (e & 1); }
+
+// Byte offset in the block of the word that holds dimension d of token t, and the bit it starts at.
+SX8_KV4_FN int kv4_k_word(int hd, int t, int d) {
+    const int W = hd / 32, wi = W < 4 ? W : 4, j = d / 32, lane = (d % 32) / 8 * 16 + t % 16;
+    return t / 16 * (256 * W) + (j / wi * 64 + lane) * wi * 4 + j % wi * 4;
+}
+SX8_KV4_FN int kv4_k_shift(int d) { return kv4_shift(d % 8); }
+SX8_KV4_FN int kv4_v_word(int hd, int t, int d) {
+    const int lane = (t % 16) / 4 * 16 + d % 16, tile = d / 16;
+    return 16 * hd + (tile / 4 * 64 + lane) * 16 + tile % 4 * 4;
+}
+SX8_KV4_FN int kv4_v_shift(int t) { return kv4_shift(t / 16 * 4 + t % 4); }
+
+// Scales of K (which = 0) and V (2) and minima of V (3) by group, step group h and token slot; minima of K (1)
+// by token and group.
+SX8_KV4_FN int kv4_param(int hd, int which, int t, int g) {
+    const int ng = hd / kKv4Group, base = 32 * hd + which * ng * 64;
+    return which == 1 ? base + 2 * (t * ng + g) : base + 2 * (g * 32 + (t % 16) / 4 * 8 + t / 16 * 4 + t % 4);
+}
+
+// ---- the attention's pieces -------------------------------------------------------------------
+// A unit is 16 query rows (row r = token r / G, head r % G of the group) of one KV head of a slot; it reads the
+// slot's blocks.  Units lie one after another (slots, heads, row tiles) on a line of blocks that the work-groups
+// share evenly, so a unit may be cut into several pieces, each a run of blocks.
+struct Kv4Shape {
+    int n_slots, nk, G;
+    int64_t cap, rows;             // tokens a slot can hold; query rows in the call
+};
+
+// New tokens of slot s and the row of its first one, from cu (null: one row a slot), kept inside the call's rows.
+SX8_KV4_FN int64_t kv4_clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+SX8_KV4_FN void kv4_rows(const Kv4Shape& sh, const int32_t* cu, int s, int64_t* first, int64_t* n) {
+    const int64_t a = kv4_clamp(cu ? cu[s] : s, 0, sh.rows), b = kv4_clamp(cu ? cu[s + 1] : s + 1, a, sh.rows);
+    *first = a;
+    *n = b - a;
+}
+SX8_KV4_FN int64_t kv4_len(const Kv4Shape& sh, const int32_t* lens, int s) { return kv4_clamp(lens[s], 0, sh.cap); }
+SX8_KV4_FN int64_t kv4_unit_blocks(int64_t len) { return len > 0 ? (len + kKv4Block - 1) / kKv4Block : 1; }
+SX8_KV4_FN int64_t kv4_tiles(int64_t n, int G) { return (n * G + 15) / 16; }
+SX8_KV4_FN int64_t kv4_slot_blocks(const Kv4Shape& sh, const int32_t* lens, const int32_t* cu, int s) {
+    int64_t first, n;
+    kv4_rows(sh, cu, s, &first, &n);
+    return sh.nk * kv4_tiles(n, sh.G) * kv4_unit_blocks(kv4_len(sh, lens, s));
+}
+
+// Blocks of a work-group: an even share, and enough that each of its four waves has one.
+SX8_KV4_FN int64_t kv4_share(int64_t total, int wgs) {
+    const int64_t p = (total + wgs - 1) / wgs;
+    return p < 4 ? 4 : p;
+}
+
+// Blocks of tokens that the new tokens of a slot touch (append, read): first block, and how many.  Positions
+// len - n .. len - 1; those outside the slot are left out.
+SX8_KV4_FN int64_t kv4_touched(int64_t len, int64_t n, int64_t* first) {
+    const int64_t a = len - n > 0 ? len - n : 0;
+    *first = a / kKv4Block;
+    return n > 0 && len > 0 ? (len - 1) / kKv4Block - *first + 1 : 0;
+}
+// At least the touched blocks of all slots together, from what the host knows: every slot with rows touches at
+// most (n + 30) / 32 + 1 blocks.
+SX8_KV4_FN int64_t kv4_touched_most(int64_t n_slots, int64_t rows, bool cu) {
+    return cu ? rows / kKv4Block + 2 * (n_slots < rows ? n_slots : rows) : (n_slots < rows ? n_slots : rows);
+}
+
+}  // namespace sx8

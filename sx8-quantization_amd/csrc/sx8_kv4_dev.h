@@ -1,0 +1,79 @@
+// sx8_kv4_dev.h -- device pieces shared by the kernels over packed sequences and the paged cache.
+#pragma once
+#include "sx8_device.h"
+#include "sx8_kv4.h"
+
+namespace sx8 {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// 16-bit value of dtype (fp16 or bf16) <-> float; rounding to nearest even.
+template <bool kBf16>
+__device__ __forceinline__ float ld16(uint32_t bits) {
+    if constexpr (kBf16) return __builtin_bit_cast(float, bits << 16);
+    else return sx8_h2f(bits);
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t st16(float v) {
+    if constexpr (kBf16) return __builtin_bit_cast(uint16_t, (__bf16)v);
+    else return __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+// a | b << 16
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    if constexpr (kBf16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
+}
+__device__ __forceinline__ uint32_t half_of(uint32_t word, int i) { return i & 1 ? word >> 16 : word & 0xFFFFu; }
+
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// Prefix sums of f(s) over n items into pre[0 .. n] (LDS), every thread of the work-group (kT threads) taking part.
+template <int kT, typename F>
+__device__ __forceinline__ void prefix_sums(int n, int64_t* pre, F&& f) {
+    __shared__ int64_t wsum[kT / 64];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int64_t base = 0;
+    if (tid == 0) pre[0] = 0;
+    for (int s0 = 0; s0 < n; s0 += kT) {
+        int64_t v = s0 + tid < n ? f(s0 + tid) : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t u = __shfl_up(v, o, 64);
+            if (lane >= o) v += u;
+        }
+        if (lane == 63) wsum[w] = v;
+        __syncthreads();
+        int64_t before = base, all = base;
+#pragma unroll
+        for (int i = 0; i < kT / 64; ++i) {
+            if (i < w) before += wsum[i];
+            all += wsum[i];
+        }
+        if (s0 + tid < n) pre[s0 + tid + 1] = before + v;
+        base = all;
+        __syncthreads();
+    }
+}
+
+// The item whose range of the prefix sums holds x (pre[0] <= x < pre[n]); every thread gets it.
+template <int kT>
+__device__ __forceinline__ int find_item(int n, const int64_t* pre, int64_t x) {
+    __shared__ int found;
+    for (int s = threadIdx.x; s < n; s += kT)
+        if (pre[s] <= x && x < pre[s + 1]) found = s;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(found);
+}
+
+}  // namespace sx8
