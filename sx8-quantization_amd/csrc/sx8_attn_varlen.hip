@@ -34,25 +34,35 @@ struct VarIo {
     uint16_t* out;
     const int32_t* cu_q;
     const int32_t* cu_k;
-    int64_t Tq, Tk, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
-    int n_seq, nh, nk;
+    int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
+    int Tq, Tk, n_seq, nh, nk;
     float scale_log2;
 };
 
 constexpr int kRows = 128;
 
 // Rows of sequence b in a packed tensor of T rows: first row and count.
-__device__ __forceinline__ void seq_rows(const int32_t* cu, int64_t T, int b, int64_t* first, int64_t* n) {
-    const int64_t a = kv4_clamp(cu[b], 0, T), e = kv4_clamp(cu[b + 1], a, T);
+__device__ __forceinline__ void seq_rows(const int32_t* cu, int T, int b, int* first, int* n) {
+    const int a = kv4_clamp(cu[b], 0, T), e = kv4_clamp(cu[b + 1], a, T);
     *first = a;
     *n = e - a;
 }
 
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 
-// 16 bytes a lane from the buffer to 1 KB of LDS at dst
-__device__ __forceinline__ void load_lds(sx8_rsrc r, lds_u8* dst, int off) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, dst, 16, off, 0, 0, 0);
+// A raw buffer over `bytes` bytes at p (as make_rsrc), in scalar registers for load_lds.
+__device__ __forceinline__ u32x4 scalar_rsrc(const void* p, uint32_t bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xFFFFu)),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kRsrcFlags};
+}
+// 16 bytes a lane from the buffer to the 1 KB of LDS at byte `dst`; no register is written, and the kernel waits for
+// vmcnt(0) and a barrier before it reads that LDS.  The builtin does the same, but the compiler then waits for it before
+// every LDS read that might be of the same place, which is every one (prompt of 8192: 715 us against 618).
+__device__ __forceinline__ void load_lds(const u32x4& r, int dst, int off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off), "s"(r)
+                 : "memory", "m0");
 }
 // Lane i of 16 names the eight bytes of key i / 4 that hold dimensions 4 (i % 4) .. + 3, and gets dimension i of the four keys.
 __device__ __forceinline__ u32x2 read_tr(const unsigned char* at) {
@@ -102,36 +112,36 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     // the tile of queries: the last ones of a sequence, which see the most keys, come first; consecutive work-groups (of
     // different XCDs) take different KV heads, so that the query heads of one share its XCD's L2
     prefix_sums<256>(io.n_seq, pre, [&](int b) {
-        int64_t f, n;
+        int f, n;
         seq_rows(io.cu_q, io.Tq, b, &f, &n);
-        return (n + kRows - 1) / kRows;
+        return ((int64_t)n + kRows - 1) / kRows;
     });
     __syncthreads();
-    const int64_t item = uniform(pre[io.n_seq]) - 1 - blockIdx.x / io.nh;
+    const int item = (int)uniform(pre[io.n_seq]) - 1 - (int)(blockIdx.x / io.nh);
     if (item < 0) return;
     const int hh = blockIdx.x % io.nh, G = io.nh / io.nk, kvh = hh % io.nk, head = kvh * G + hh / io.nk;
     const int b = find_item<256>(io.n_seq, pre, item);
-    int64_t q_first, nq, k_first, nkeys;
+    int q_first, nq, k_first, nkeys;
     seq_rows(io.cu_q, io.Tq, b, &q_first, &nq);
     seq_rows(io.cu_k, io.Tk, b, &k_first, &nkeys);
-    q_first = uniform(q_first);
-    nq = uniform(nq);
-    k_first = uniform(k_first);
-    nkeys = uniform(nkeys);
-    const int64_t q0 = (item - uniform(pre[b])) * kRows + 32 * w;        // the wave's first row in the sequence
+    q_first = __builtin_amdgcn_readfirstlane(q_first);
+    nq = __builtin_amdgcn_readfirstlane(nq);
+    k_first = __builtin_amdgcn_readfirstlane(k_first);
+    nkeys = __builtin_amdgcn_readfirstlane(nkeys);
+    const int wg_q0 = (item - (int)uniform(pre[b])) * kRows, q0 = wg_q0 + 32 * w;   // first rows in the sequence
     __syncthreads();                                                     // (pre makes room for the first tile)
-    const int64_t past = nkeys - nq;                                     // row i attends keys 0 .. past + i
-    const int64_t wg_last = (q0 - 32 * w + kRows < nq ? q0 - 32 * w + kRows : nq) - 1;
-    const int64_t see = kCausal ? (past + wg_last + 1 < 0 ? 0 : past + wg_last + 1) : nkeys;    // keys of the work-group
-    const int n_tiles = (int)((see + KB - 1) / KB);
-    const int64_t w_last = (q0 + 32 < nq ? q0 + 32 : nq) - 1;            // the wave's last row
-    const int64_t w_see = q0 >= nq ? 0 : kCausal ? past + w_last + 1 : nkeys;
-    const int64_t w_all = q0 >= nq ? 0 : kCausal ? past + q0 + 1 : nkeys;   // keys that all its rows see
+    const int past = nkeys - nq;                                         // row i attends keys 0 .. past + i
+    const int wg_last = min(nq - wg_q0, kRows) - 1 + wg_q0;
+    const int see = kCausal ? max(past + wg_last + 1, 0) : nkeys;        // keys of the work-group
+    const int n_tiles = (int)(((int64_t)see + KB - 1) / KB);
+    const int w_last = min(nq - q0, 32) - 1 + q0;                        // the wave's last row
+    const int w_see = q0 >= nq ? 0 : kCausal ? past + w_last + 1 : nkeys;
+    const int w_all = q0 >= nq ? 0 : kCausal ? past + q0 + 1 : nkeys;    // keys that all its rows see
     const bool row_ok = q0 + c < nq;
-    const int64_t lim = kCausal ? past + (row_ok ? q0 + c : nq - 1) : nkeys - 1;
+    const int lim = kCausal ? past + (row_ok ? q0 + c : nq - 1) : nkeys - 1;
     u32x4 qf[KS];
     {
-        const uint16_t* qr = io.q + (q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs + 8 * h;
+        const uint16_t* qr = io.q + ((int64_t)q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs + 8 * h;
 #pragma unroll
         for (int st = 0; st < KS; ++st) qf[st] = *reinterpret_cast<const u32x4*>(qr + 16 * st);
     }
@@ -144,11 +154,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     const int lrow = w * R + lane / CH, lpos = lane % CH;
     const int k_off = (int)(lrow * io.k_ts * 2) + 16 * (lpos ^ T::k_swz(lrow));
     const int v_off = (int)(lrow * io.v_ts * 2) + 16 * (lpos ^ T::v_swz(lrow));
+    const int lds0 = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(lds_u8*)var_lds);
     auto fetch = [&](int j, int buf) __attribute__((always_inline)) {
-        const int64_t k0 = (int64_t)j * KB, left = nkeys - k0 < KB ? nkeys - k0 : KB;
-        const sx8_rsrc kr = make_rsrc(kp + k0 * io.k_ts, (left - 1) * io.k_ts * 2 + HD * 2);
-        const sx8_rsrc vr = make_rsrc(vp + k0 * io.v_ts, (left - 1) * io.v_ts * 2 + HD * 2);
-        lds_u8* const dst = (lds_u8*)var_lds + buf * 2 * T::kBytes + w * 1024;
+        const int k0 = j * KB;
+        const int left = min(nkeys - k0, KB);
+        const u32x4 kr = scalar_rsrc(kp + (int64_t)k0 * io.k_ts, (uint32_t)((left - 1) * (int)io.k_ts * 2 + HD * 2));
+        const u32x4 vr = scalar_rsrc(vp + (int64_t)k0 * io.v_ts, (uint32_t)((left - 1) * (int)io.v_ts * 2 + HD * 2));
+        const int dst = lds0 + buf * 2 * T::kBytes + w * 1024;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             load_lds(kr, dst + i * 4096, k_off + 8 * R * i * (int)io.k_ts);
@@ -164,8 +176,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     float m = -kInf, l = 0.f;
     // V^T reads: key and dimension that the lane names
     const int vi = lane & 15, vd = (lane >> 4 & 1) * 16 + 4 * (vi & 3), vk = 4 * h + (vi >> 2);
-    auto tile = [&](int j, int buf, auto mask) __attribute__((always_inline)) {
-        constexpr bool kMask = decltype(mask)::value;
+    auto tile = [&](int j, int buf, bool mask) __attribute__((always_inline)) {
         const unsigned char* kt = var_lds + buf * 2 * T::kBytes;
         const unsigned char* vt = kt + T::kBytes;
         f32x16 s[NB];
@@ -180,12 +191,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
                 s[a] = M::mul(kf, qf[st], s[a]);
             }
         }
-        if constexpr (kMask) {
+        if (mask) {
 #pragma unroll
             for (int a = 0; a < NB; ++a)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int64_t key = (int64_t)j * KB + 32 * a + 8 * (r >> 2) + 4 * h + (r & 3);
+                    const int key = j * KB + 32 * a + 8 * (r >> 2) + 4 * h + (r & 3);
                     s[a][r] = key <= lim ? s[a][r] : -kInf;
                 }
         }
@@ -213,14 +224,46 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
                 s[a][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][r], io.scale_log2, nm));
                 l += s[a][r];
             }
-        uint32_t odd = 0;
+        if (mask) {
+            // A key that some row may not attend has probability zero there, and 0 * NaN must not reach the row.  So a tile
+            // with values that are no finite numbers (an exponent of all ones) is added up here, by the rows that give
+            // them weight; it costs such a tile some 30 us, and the others one look at their values.
+            uint32_t odd = 0;
+#pragma unroll 4
+            for (int i = 0; i < T::kBytes / 1024; ++i) {
+                const u32x4 x = reinterpret_cast<const u32x4*>(vt)[i * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd |= (x[e] & M::kExp) + M::kOne;
+            }
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) != 0) {
+                for (int key = 0; key < KB; ++key) {
+                    float p = 0.f;
+                    // the probability of the key: lane half (key >> 2) & 1, accumulator 4 (key % 32 / 8) + key % 4
+#pragma unroll
+                    for (int a = 0; a < NB; ++a)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (key >> 5 == a && (key & 31) >> 3 == r >> 2 && (key & 3) == (r & 3)) p = s[a][r];
+                    p = ld16<kBf16>(st16<kBf16>(__shfl(p, c + 32 * (key >> 2 & 1), 64)));
+                    if (p == 0.f) continue;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int d = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
+                            o[n][r] = __builtin_fmaf(p, ld16<kBf16>(*reinterpret_cast<const uint16_t*>(
+                                vt + key * (HD * 2) + 16 * ((d / 8) ^ T::v_swz(key)) + 2 * (d % 8))), o[n][r]);
+                        }
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int st = 0; st < KB / 16; ++st) {
             u32x4 pf;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; ++e)
                 pf[e] = pack16<kBf16>(s[st / 2][8 * (st & 1) + 2 * e], s[st / 2][8 * (st & 1) + 2 * e + 1]);
-            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 u32x4 vf;
@@ -231,61 +274,25 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
                     vf[2 * a] = x.x;
                     vf[2 * a + 1] = x.y;
                 }
-                if constexpr (kMask) {
-                    // values that are no finite numbers are left out here (below)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t top = (vf[e] & M::kExp) + M::kOne;        // its half's sign bit: not finite
-                        odd |= top;
-                        const uint32_t bad = (top >> 15 & 0x00010001u) * 0xFFFFu;
-                        vf[e] &= ~bad;
-                    }
-                }
                 o[n] = M::mul(vf, pf, o[n]);
-            }
-        }
-        if constexpr (kMask) {
-            // A key that some row may not attend has probability zero there, and 0 * NaN must not reach the row: values that
-            // are not finite are added here, to the rows that give them weight.
-            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) != 0) {
-                for (int key = 0; key < KB; ++key) {
-                    float p = 0.f;
-                    // the probability of the key: lane half (key >> 2) & 1, accumulator 4 (key % 32 / 8) + key % 4
-#pragma unroll
-                    for (int a = 0; a < NB; ++a)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (key >> 5 == a && (key & 31) >> 3 == r >> 2 && (key & 3) == (r & 3)) p = s[a][r];
-                    p = __shfl(p, c + 32 * (key >> 2 & 1), 64);
-                    if (p == 0.f) continue;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int d = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-                            const float x = ld16<kBf16>(*reinterpret_cast<const uint16_t*>(
-                                vt + key * (HD * 2) + 16 * ((d / 8) ^ T::v_swz(key)) + 2 * (d % 8)));
-                            if (!(__builtin_fabsf(x) < kInf)) o[n][r] = __builtin_fmaf(p, x, o[n][r]);
-                        }
-                }
             }
         }
     };
     if (n_tiles > 0) fetch(0, 0);
+    // the query is waited for here and not at its uses, where the wait would take in the next tile's loads
+#pragma unroll
+    for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(qf[st]));
     for (int j = 0; j < n_tiles; ++j) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                          // tile j is there, and nobody reads the other buffer any more
         if (j + 1 < n_tiles) fetch(j + 1, (j + 1) & 1);
-        const int64_t k0 = (int64_t)j * KB;
-        if (k0 < w_see) {
-            if (k0 + KB > w_all) tile(j, j & 1, std::true_type{});
-            else tile(j, j & 1, std::false_type{});
-        }
+        const int k0 = j * KB;
+        if (k0 < w_see) tile(j, j & 1, k0 + KB > w_all);
     }
     if (!row_ok) return;
     l += __shfl_xor(l, 32, 64);
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t* const dst = io.out + (q_first + q0 + c) * io.o_ts + head * io.o_hs + 4 * h;
+    uint16_t* const dst = io.out + ((int64_t)q_first + q0 + c) * io.o_ts + head * io.o_hs + 4 * h;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -320,8 +327,8 @@ extern "C" int32_t sx8_attn_varlen(const void* q, const void* k, const void* v, 
         return fail(SX8_ERR_INVALID, "%s: null pointer", what);
     if ((hd != 64 && hd != 128 && hd != 256) || nk <= 0 || nh <= 0 || nh % nk || nh > 65536)
         return fail(SX8_ERR_INVALID, "%s: bad shape (hd 64, 128 or 256, nh a multiple of nk)", what);
-    if (n_seq <= 0 || n_seq > kKv4MaxSlots || Tq < 0 || Tq > 0x7FFFFFFF || Tk < 0 || Tk > 0x7FFFFFFF)
-        return fail(SX8_ERR_INVALID, "%s: bad sizes (n_seq 1..%d, Tq and Tk 0..2^31 - 1)", what, kKv4MaxSlots);
+    if (n_seq <= 0 || n_seq > kKv4MaxSlots || Tq < 0 || Tq > 0x7FFFFF00 || Tk < 0 || Tk > 0x7FFFFF00)
+        return fail(SX8_ERR_INVALID, "%s: bad sizes (n_seq 1..%d, Tq and Tk below 2^31 - 256)", what, kKv4MaxSlots);
     if (dtype != 0 && dtype != 1) return fail(SX8_ERR_INVALID, "%s: dtype must be 0 (fp16) or 1 (bf16)", what);
     if (!(scale > 0.f) || !(scale < __builtin_inff()))
         return fail(SX8_ERR_INVALID, "%s: scale must be positive and finite", what);
@@ -336,8 +343,8 @@ extern "C" int32_t sx8_attn_varlen(const void* q, const void* k, const void* v, 
     const int64_t grid = ((Tq + kRows - 1) / kRows + (n_seq < Tq ? n_seq : Tq)) * nh;
     if (grid > 0x7FFFFFFF) return fail(SX8_ERR_UNSUPPORTED, "%s: over 2^31 tiles of rows", what);
     if (Tq == 0) return ok();
-    const VarIo io{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, cu_q, cu_k, Tq, Tk, q_ts, q_hs,
-                   k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, (int)n_seq, nh, nk, scale * 1.4426950408889634f};
+    const VarIo io{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, cu_q, cu_k, q_ts, q_hs, k_ts,
+                   k_hs, v_ts, v_hs, o_ts, o_hs, (int)Tq, (int)Tk, (int)n_seq, nh, nk, scale * 1.4426950408889634f};
     const hipStream_t st = as_stream(stream);
     if (hd == 64) launch<64>(io, dtype, causal, (unsigned)grid, st);
     else if (hd == 128) launch<128>(io, dtype, causal, (unsigned)grid, st);

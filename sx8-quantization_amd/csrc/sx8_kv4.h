@@ -45,39 +45,64 @@ SX8_KV4_FN int kv4_param(int hd, int which, int t, int g) {
 
 // ---- the attention's pieces -------------------------------------------------------------------
 // A unit is 16 query rows (row r = token r / G, head r % G of the group) of one KV head of a slot; it reads the
-// slot's blocks.  Units lie one after another (slots, heads, row tiles) on a line of blocks that the work-groups
-// share evenly, so a unit may be cut into several pieces, each a run of blocks.
+// slot's blocks.  Units lie one after another (slots, heads, row tiles) on a line that the waves of the launch share
+// evenly, so a unit may be cut into several pieces, each a run of blocks.  On the line a unit is its blocks and kKv4Begin
+// places before them, for what a piece costs beside its blocks (a wave that gets only those has nothing to do).
+constexpr int kKv4Begin = 3;
 struct Kv4Shape {
     int n_slots, nk, G;
-    int64_t cap, rows;             // tokens a slot can hold; query rows in the call
+    int cap, rows;                 // tokens a slot can hold; query rows in the call (rows * G < 2^31)
 };
 
 // New tokens of slot s and the row of its first one, from cu (null: one row a slot), kept inside the call's rows.
-SX8_KV4_FN int64_t kv4_clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
-SX8_KV4_FN void kv4_rows(const Kv4Shape& sh, const int32_t* cu, int s, int64_t* first, int64_t* n) {
-    const int64_t a = kv4_clamp(cu ? cu[s] : s, 0, sh.rows), b = kv4_clamp(cu ? cu[s + 1] : s + 1, a, sh.rows);
+SX8_KV4_FN int kv4_clamp(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+SX8_KV4_FN void kv4_rows(const Kv4Shape& sh, const int32_t* cu, int s, int* first, int* n) {
+    const int a = kv4_clamp(cu ? cu[s] : s, 0, sh.rows), b = kv4_clamp(cu ? cu[s + 1] : s + 1, a, sh.rows);
     *first = a;
     *n = b - a;
 }
-SX8_KV4_FN int64_t kv4_len(const Kv4Shape& sh, const int32_t* lens, int s) { return kv4_clamp(lens[s], 0, sh.cap); }
-SX8_KV4_FN int64_t kv4_unit_blocks(int64_t len) { return len > 0 ? (len + kKv4Block - 1) / kKv4Block : 1; }
-SX8_KV4_FN int64_t kv4_tiles(int64_t n, int G) { return (n * G + 15) / 16; }
-SX8_KV4_FN int64_t kv4_slot_blocks(const Kv4Shape& sh, const int32_t* lens, const int32_t* cu, int s) {
-    int64_t first, n;
+SX8_KV4_FN int kv4_len(const Kv4Shape& sh, const int32_t* lens, int s) { return kv4_clamp(lens[s], 0, sh.cap); }
+SX8_KV4_FN int kv4_unit_blocks(int len) { return len > 0 ? (len + kKv4Block - 1) / kKv4Block : 1; }
+SX8_KV4_FN int kv4_tiles(int n, int G) { return (n * G + 15) / 16; }
+// Places of a slot on the line.
+SX8_KV4_FN int64_t kv4_slot_places(int nk, int G, int n, int len) {
+    return (int64_t)nk * kv4_tiles(n, G) * (kv4_unit_blocks(len) + kKv4Begin);
+}
+SX8_KV4_FN int64_t kv4_slot_places(const Kv4Shape& sh, const int32_t* lens, const int32_t* cu, int s) {
+    int first, n;
     kv4_rows(sh, cu, s, &first, &n);
-    return sh.nk * kv4_tiles(n, sh.G) * kv4_unit_blocks(kv4_len(sh, lens, s));
+    return kv4_slot_places(sh.nk, sh.G, n, kv4_len(sh, lens, s));
 }
 
-// Blocks of a work-group: an even share, and enough that each of its four waves has one.
-SX8_KV4_FN int64_t kv4_share(int64_t total, int wgs) {
-    const int64_t p = (total + wgs - 1) / wgs;
-    return p < 4 ? 4 : p;
+// Places of each of 2^waves_log2 waves: an even share.
+SX8_KV4_FN int64_t kv4_share(int64_t total, int waves_log2) {
+    const int64_t p = (total + (1 << waves_log2) - 1) >> waves_log2;
+    return p < 1 ? 1 : p;
+}
+// The piece that begins at place x of the line, `off` places behind the beginning of its slot, for a wave whose share ends
+// at x1: blocks b0 .. b1 - 1 of unit `unit` of the slot (none where b0 == b1), and the places it takes.
+struct Kv4Run {
+    int64_t unit;
+    int b0, b1;
+    int64_t places;
+};
+// a / b; the wide division only where it is needed
+SX8_KV4_FN int64_t kv4_div(int64_t a, int b) { return (uint64_t)a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
+SX8_KV4_FN Kv4Run kv4_run(int64_t x, int64_t off, int64_t x1, int nb) {
+    const int all = nb + kKv4Begin;
+    const int64_t unit = kv4_div(off, all);
+    const int v0 = (int)(off - unit * all), v1 = all - v0 < x1 - x ? all : v0 + (int)(x1 - x);
+    return Kv4Run{unit, v0 > kKv4Begin ? v0 - kKv4Begin : 0, v1 > kKv4Begin ? v1 - kKv4Begin : 0, v1 - v0};
+}
+// How many waves have blocks of a unit whose first block lies at place `at`, in the share of `wave`.
+SX8_KV4_FN int kv4_parts(int64_t at, int nb, int64_t share, int wave) {
+    return (int)((at + nb - 1) / share - wave + 1);
 }
 
 // Blocks of tokens that the new tokens of a slot touch (append, read): first block, and how many.  Positions
 // len - n .. len - 1; those outside the slot are left out.
-SX8_KV4_FN int64_t kv4_touched(int64_t len, int64_t n, int64_t* first) {
-    const int64_t a = len - n > 0 ? len - n : 0;
+SX8_KV4_FN int kv4_touched(int len, int n, int* first) {
+    const int a = len - n > 0 ? len - n : 0;
     *first = a / kKv4Block;
     return n > 0 && len > 0 ? (len - 1) / kKv4Block - *first + 1 : 0;
 }

@@ -20,8 +20,8 @@ struct Kv4Pool {
 };
 
 // Byte offset of block b of head h of a slot's page, or -1 where the slot has no such page.
-__device__ __forceinline__ int64_t block_offset(const Kv4Pool& p, int slot, int head, int64_t b, int bb) {
-    const int64_t at = b >> p.bpp_log2;
+__device__ __forceinline__ int64_t block_offset(const Kv4Pool& p, int slot, int head, int b, int bb) {
+    const int at = b >> p.bpp_log2;
     if (at >= p.max_pages) return -1;
     const int page = p.table[(int64_t)slot * p.max_pages + at];
     if (page < 0 || page >= p.n_pages) return -1;
@@ -80,29 +80,26 @@ __device__ __forceinline__ void encode_group(const float (&x)[8], Enc& e) {
 // The block that work item `item` of the call names: slot, its block, and the new tokens in it (block-relative
 // [t0, t1), row of token t0).  Every thread gets it; false past the last item.
 struct Touched {
-    int slot;
-    int64_t block;
-    int t0, t1;
-    int64_t row0;
+    int slot, block, t0, t1, row0;
 };
 __device__ __forceinline__ bool find_touched(const Kv4Pool& p, int64_t item, int64_t* pre, Touched* t) {
     prefix_sums<256>(p.sh.n_slots, pre, [&](int s) {
-        int64_t first, n, b;
+        int first, n, b;
         kv4_rows(p.sh, p.cu, s, &first, &n);
-        return kv4_touched(kv4_len(p.sh, p.lens, s), n, &b);
+        return (int64_t)kv4_touched(kv4_len(p.sh, p.lens, s), n, &b);
     });
     __syncthreads();
     if (item >= pre[p.sh.n_slots]) return false;
     t->slot = find_item<256>(p.sh.n_slots, pre, item);
-    int64_t first, n, b;
+    int first, n, b;
     kv4_rows(p.sh, p.cu, t->slot, &first, &n);
-    const int64_t len = kv4_len(p.sh, p.lens, t->slot);
+    const int len = kv4_len(p.sh, p.lens, t->slot);
     kv4_touched(len, n, &b);
-    t->block = b + (item - pre[t->slot]);
-    const int64_t a = len - n > t->block * 32 ? len - n : t->block * 32;
-    const int64_t e = len < t->block * 32 + 32 ? len : t->block * 32 + 32;
-    t->t0 = (int)(a - t->block * 32);
-    t->t1 = (int)(e - t->block * 32);
+    t->block = b + (int)(item - pre[t->slot]);
+    const int a = len - n > t->block * 32 ? len - n : t->block * 32;
+    const int e = len < t->block * 32 + 32 ? len : t->block * 32 + 32;
+    t->t0 = a - t->block * 32;
+    t->t1 = e - t->block * 32;
     t->row0 = first + a - (len - n);
     return true;
 }
@@ -133,7 +130,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsI
         // (whole groups of eight lanes run together: CPR is a multiple of 8)
         for (int i = tid; i < nt * CPR; i += 256) {
             const int tok = t.t0 + i / CPR, d0 = i % CPR * 8, g = d0 / kKv4Group;
-            const u32x4 w = *reinterpret_cast<const u32x4*>(src + (t.row0 + i / CPR) * ts + head * hs + d0);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(src + (int64_t)(t.row0 + i / CPR) * ts + head * hs + d0);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = ld16<kBf16>(half_of(w[e >> 1], e));
@@ -189,9 +186,8 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
     if (!find_touched(p, blockIdx.x, pre, &t)) return;
     const int head = blockIdx.y, tid = threadIdx.x;
     const int64_t off = block_offset(p, t.slot, head, t.block, kBB);
-    if (off < 0) return;                                            // (uniform)
     for (int i = tid; i < kBB / 16; i += 256)
-        reinterpret_cast<u32x4*>(blk)[i] = reinterpret_cast<const u32x4*>(p.pages + off)[i];
+        reinterpret_cast<u32x4*>(blk)[i] = off < 0 ? u32x4{0u, 0u, 0u, 0u} : reinterpret_cast<const u32x4*>(p.pages + off)[i];
     __syncthreads();
     const int nt = t.t1 - t.t0;
     for (int i = tid; i < 2 * nt * CPR; i += 256) {
@@ -209,15 +205,15 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
             if (e & 1) w[e >> 1] |= b << 16;
             else w[e >> 1] = b;
         }
-        uint16_t* const dst = which ? out.v + (t.row0 + j / CPR) * out.v_ts + head * out.v_hs
-                                    : out.k + (t.row0 + j / CPR) * out.k_ts + head * out.k_hs;
+        uint16_t* const dst = which ? out.v + (int64_t)(t.row0 + j / CPR) * out.v_ts + head * out.v_hs
+                                    : out.k + (int64_t)(t.row0 + j / CPR) * out.k_ts + head * out.k_hs;
         *reinterpret_cast<u32x4*>(dst + d0) = w;
     }
 }
 
 // ---- attend ------------------------------------------------------------------------------------
-// Work-groups share the blocks of all units evenly (sx8_kv4.h); a piece is a run of blocks of one unit, its four
-// waves take every fourth block.  Per block a wave computes S^T = K Q^T on v_mfma_f32_16x16x32_f16 with the tokens as
+// The launch's waves share the blocks of all units evenly (sx8_kv4.h) and work apart from each other; a piece is a run
+// of blocks of one unit.  Per block a wave computes S^T = K Q^T on v_mfma_f32_16x16x32_f16 with the tokens as
 // rows and the unit's 16 query rows as columns, so that a lane (column c, step group h) holds the scores of
 // tokens 4 h + r and 16 + 4 h + r of its own query row and the softmax stays in the lane.  The levels go into the
 // MFMA as the fp16 subnormals level * 2^-24, which is one shift and one mask for two values and exact; the scale
@@ -229,12 +225,16 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // the scale: bf16 rows become fp16 without loss (but for values 2^-30 below the largest), and sum(q_g) fits.
 // p is kept at or below 8 (the running maximum is raised when a score exceeds it by 3 in powers of two), so p * s
 // fits in fp16 for every s.
-constexpr int kWgs = 512;                 // two for each of 256 CUs
 constexpr float kRaise = 3.f;
 
-struct Kv4Piece {                         // record of a unit cut after this work-group's share: parts == 0: none
-    int32_t parts, first_at, tile, head;
-    int64_t row0, n;
+template <int HD>
+constexpr int waves_log2() { return HD == 256 ? 10 : 11; }        // two or four... a SIMD of 256 CUs
+
+// Record of a cut unit for the combine; parts == 0: none.  The records lie by unit (slots, heads, tiles) where the host
+// knows that there are no more units than waves, so that the combine has a work-group for each; otherwise by the
+// wave that has the unit's first block.
+struct Kv4Piece {
+    int32_t parts, first, tile, head, row0, n, pad[2];      // first: place of its first part
 };
 static_assert(sizeof(Kv4Piece) == 32, "record");
 
@@ -243,12 +243,15 @@ struct AttendIo {
     uint16_t* out;
     int64_t q_ts, q_hs, o_ts, o_hs;
     float scale_log2;
-    float* part_o;                        // [2 kWgs][16][HD]
-    float* part_ml;                       // [2 kWgs][16][2]
-    Kv4Piece* piece;                      // [kWgs]
+    float* part_o;                        // [2 waves][16][HD]
+    float* part_ml;                       // [2 waves][16][2]
+    Kv4Piece* piece;                      // [waves]
+    int by_unit;
 };
 
-constexpr int64_t attend_ws(int64_t hd) { return 2 * kWgs * 16 * (hd + 2) * 4 + kWgs * (int64_t)sizeof(Kv4Piece); }
+constexpr int64_t attend_ws(int64_t hd) {
+    return ((int64_t)(2 * 16 * (hd + 2) * 4 + sizeof(Kv4Piece))) << (hd == 256 ? 10 : 11);
+}
 
 template <int HD>
 struct Kv4Regs {                          // a lane's share of one block
@@ -275,121 +278,110 @@ __device__ __forceinline__ float sum4(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-template <int HD, bool kBf16>
-__device__ __forceinline__ void store_row(uint16_t* dst, const float* v) {      // HD / 16 values
-    constexpr int N = HD / 16;
-    uint32_t w[N / 2];
-#pragma unroll
-    for (int e = 0; e < N / 2; ++e) w[e] = pack16<kBf16>(v[2 * e], v[2 * e + 1]);
-    if constexpr (N == 4) *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
-    else
-#pragma unroll
-        for (int i = 0; i < N / 8; ++i)
-            reinterpret_cast<u32x4*>(dst)[i] = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
-}
+// What a wave knows of the slots: with up to 64 of them lane s holds slot s and its place on the line of blocks; with
+// more the places lie in LDS.
+struct Slots {
+    int row0, n, len;
+    int64_t end;                          // places of the slots up to this lane's
+    int units;                            // (by_unit) units of the slots up to this lane's
+};
 
 template <int HD, bool kBf16>
-__global__ __launch_bounds__(256) void k_kv4_attend(const Kv4Pool p, const AttendIo io) {
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4Pool p, const AttendIo io) {
     using Regs = Kv4Regs<HD>;
-    constexpr int W = Regs::W, NT = Regs::NT, NG = Regs::NG, kBB = kv4_block_bytes(HD), kRow = HD + 4;
+    constexpr int W = Regs::W, NT = Regs::NT, NG = Regs::NG, kBB = kv4_block_bytes(HD);
     constexpr float kInf = __builtin_inff();
-    __shared__ __align__(16) float so[4][16][kRow];
-    __shared__ float sml[4][16][2];
     int64_t* const pre = reinterpret_cast<int64_t*>(dyn_lds);
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, h = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const int S = p.sh.n_slots, G = p.sh.G;
-    prefix_sums<256>(S, pre, [&](int s) { return kv4_slot_blocks(p.sh, p.lens, p.cu, s); });
-    __syncthreads();
-    const int64_t total = uniform(pre[S]), share = kv4_share(total, gridDim.x);
-    int64_t x = (int64_t)blockIdx.x * share;
-    const int64_t x0 = x, x1 = x + share < total ? x + share : total;
-    if (x >= total) {
-        if (tid == 0) io.piece[blockIdx.x].parts = 0;
-        return;
-    }
-    int slot = find_item<256>(S, pre, x);
-    bool cut = false;
-    while (x < x1) {
-        while (x >= uniform(pre[slot + 1])) ++slot;
-        int64_t row0, n;
-        kv4_rows(p.sh, p.cu, slot, &row0, &n);
-        row0 = uniform(row0);
-        n = uniform(n);
-        const int64_t len = uniform(kv4_len(p.sh, p.lens, slot)), nb = kv4_unit_blocks(len), tiles = kv4_tiles(n, G);
-        const int64_t off = x - uniform(pre[slot]), unit = off / nb, b0 = off - unit * nb;
-        const int64_t bend = nb - b0 < x1 - x ? nb : b0 + (x1 - x);
-        const int head = (int)(unit / tiles);
-        const int64_t tile = unit - head * tiles;
-        // the column's query row, and the last position it may attend
-        const int64_t r = 16 * tile + c, tok = r / G;
-        const bool row_ok = tok < n;
-        const int64_t lim = row_ok ? len - n + tok : len - 1;
-        const int64_t tok_min = 16 * tile / G, tok_max = (16 * tile + 15) / G;
-        const int64_t lim_min = len - n + tok_min, lim_max = len - n + (tok_max < n ? tok_max : n - 1);
-        const int64_t b1 = lim_max < 0 ? b0 : bend < lim_max / 32 + 1 ? bend : lim_max / 32 + 1;   // blocks it reads
-        // query fragment: fp16 with the row's largest value in [64, 128)
-        f16x8 qf[W], qm;
-        float kscale;
-        {
-            const uint16_t* qr = io.q + (row_ok ? (row0 + tok) * io.q_ts + (head * G + (int)(r - tok * G)) * io.q_hs
-                                                : row0 * io.q_ts + head * G * io.q_hs) + 8 * h;
-            u32x4 raw[W];
-#pragma unroll
-            for (int j = 0; j < W; ++j) raw[j] = *reinterpret_cast<const u32x4*>(qr + 32 * j);
-            float top = 0.f;
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(ld16<kBf16>(half_of(raw[j][e >> 1], e))));
-            top = max4(row_ok ? top : 0.f);
-            // exponent of the largest value; no scaling of rows that are zero or not finite
-            const int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
-            const int up = top > 0.f && ex < 255 && ex > 0 ? (127 + 6 - ex < 126 ? 127 + 6 - ex : 126) : 0;
-            const float mul = __builtin_ldexpf(row_ok ? 1.f : 0.f, up);
-            kscale = io.scale_log2 * __builtin_ldexpf(1.f, -up);
-            float qs[NG];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) qs[g] = 0.f;
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float raw_q = ld16<kBf16>(half_of(raw[j][e >> 1], e));
-                    const _Float16 v = (_Float16)(row_ok ? raw_q * mul : 0.f);
-                    qf[j][e] = v;
-                    qs[j / 2] += (float)v;
-                }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) qm[e] = (_Float16)0.f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const float s = sum4(qs[g]);
-                const _Float16 hi = (_Float16)s;
-                if (h == 0) {
-                    qm[g] = hi;
-                    qm[4 + g] = (_Float16)(s - (float)hi);
-                }
-            }
+    const bool few = S <= 64;
+    Slots sl = {0, 0, 0, 0, 0};
+    int32_t* const pre_units = reinterpret_cast<int32_t*>(pre + S + 1);
+    int64_t total;
+    int units = 0;
+    if (few) {
+        if (lane < S) {
+            kv4_rows(p.sh, p.cu, lane, &sl.row0, &sl.n);
+            sl.len = kv4_len(p.sh, p.lens, lane);
+            sl.end = kv4_slot_places(p.sh.nk, G, sl.n, sl.len);
+            sl.units = p.sh.nk * kv4_tiles(sl.n, G);
         }
-        f32x4 o[NT], om = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = -kInf, l = 0.f;
-        const int cnt = b1 > b0 + w ? (int)((b1 - b0 - w + 3) / 4) : 0;    // blocks of this wave: b0 + w + 4 i
-        int pages = -1;                                                    // lane i: page of block (i0 + i)
+        sl.end = wave_prefix(sl.end);
+        total = lane_of(sl.end, 63);
+        if (io.by_unit) {
+            sl.units = (int)wave_prefix(sl.units);
+            units = __builtin_amdgcn_readlane(sl.units, 63);
+        }
+    } else {
+        prefix_sums<256>(S, pre, [&](int s) { return kv4_slot_places(p.sh, p.lens, p.cu, s); });
+        if (io.by_unit)
+            prefix_sums<256>(S, pre_units, [&](int s) {
+                int first, n;
+                kv4_rows(p.sh, p.cu, s, &first, &n);
+                return (int64_t)p.sh.nk * kv4_tiles(n, G);
+            });
+        __syncthreads();
+        total = uniform(pre[S]);
+        if (io.by_unit) units = __builtin_amdgcn_readfirstlane(pre_units[S]);
+    }
+    const int64_t share = kv4_share(total, waves_log2<HD>());
+    const int64_t x0 = wave * share, x1 = x0 + share < total ? x0 + share : total;
+    int slot = 0;
+    if (x0 < total) {
+        if (few) slot = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < S && sl.end <= x0));
+        else
+            for (int s = lane; s - lane < S; s += 64) slot += __builtin_popcountll(__builtin_amdgcn_ballot_w64(s < S && pre[s < S ? s + 1 : S] <= x0));
+    }
+    if ((!io.by_unit || wave >= units) && lane == 0) io.piece[wave].parts = 0;
+    for (int64_t x = x0; x < x1;) {
+        int row0, n, len;
+        int64_t begin;
+        int unit0 = 0;
+        if (few) {
+            while (x >= lane_of(sl.end, slot)) ++slot;
+            row0 = __builtin_amdgcn_readlane(sl.row0, slot);
+            n = __builtin_amdgcn_readlane(sl.n, slot);
+            len = __builtin_amdgcn_readlane(sl.len, slot);
+            begin = slot ? lane_of(sl.end, slot - 1) : 0;
+            if (io.by_unit) unit0 = slot ? __builtin_amdgcn_readlane(sl.units, slot - 1) : 0;
+        } else {
+            while (x >= uniform(pre[slot + 1])) ++slot;
+            kv4_rows(p.sh, p.cu, slot, &row0, &n);
+            row0 = __builtin_amdgcn_readfirstlane(row0);
+            n = __builtin_amdgcn_readfirstlane(n);
+            len = __builtin_amdgcn_readfirstlane(kv4_len(p.sh, p.lens, slot));
+            begin = uniform(pre[slot]);
+            if (io.by_unit) unit0 = __builtin_amdgcn_readfirstlane(pre_units[slot]);
+        }
+        const int nb = kv4_unit_blocks(len), tiles = kv4_tiles(n, G);
+        const Kv4Run run = kv4_run(x, x - begin, x1, nb);
+        const int b0 = run.b0, bend = run.b1;
+        const int64_t here = x;
+        x += run.places;
+        if (b0 == bend) continue;
+        const int head = (int)kv4_div(run.unit, tiles), tile = (int)(run.unit - (int64_t)head * tiles);
+        // the column's query row, and the last position it may attend
+        const int r = 16 * tile + c, tok = r / G;
+        const bool row_ok = tok < n;
+        const int lim = row_ok ? len - n + tok : len - 1;
+        const int tok_min = 16 * tile / G, tok_max = (16 * tile + 15) / G;
+        const int lim_min = len - n + tok_min, lim_max = len - n + (tok_max < n ? tok_max : n - 1);
+        const int b1 = lim_max < 0 ? b0 : bend < lim_max / 32 + 1 ? bend : lim_max / 32 + 1;   // blocks it reads
+        const int cnt = b1 > b0 ? b1 - b0 : 0;
+        int pages = -1;                                                    // lane i: page of block b0 + i0 + i
         auto load_pages = [&](int i0) {
-            const int64_t b = b0 + w + 4 * (int64_t)(i0 + lane);
+            const int b = b0 + i0 + lane;
             pages = b < b1 ? p.table[(int64_t)slot * p.max_pages + (b >> p.bpp_log2)] : -1;
         };
         auto load = [&](Regs& rg, int i) __attribute__((always_inline)) {
-            if ((i & 63) == 0) load_pages(i);
-            const int64_t b = b0 + w + 4 * (int64_t)i;
+            if (i != 0 && (i & 63) == 0) load_pages(i);
+            const int b = b0 + i;
             int page = __builtin_amdgcn_readlane(pages, i & 63);
             rg.bad = page < 0 || page >= p.n_pages;
             page = rg.bad ? 0 : page;
             const uint8_t* base = p.pages + page * p.page_bytes
-                + (((int64_t)head << p.bpp_log2) + (b & ((1 << p.bpp_log2) - 1))) * kBB;
+                + (int64_t)((head << p.bpp_log2) + (b & ((1 << p.bpp_log2) - 1))) * kBB;
             const uint8_t* prm = base + 32 * HD;
             if constexpr (W == 2) {
 #pragma unroll
@@ -432,9 +424,62 @@ __global__ __launch_bounds__(256) void k_kv4_attend(const Kv4Pool p, const Atten
                 rg.vs[g] = *reinterpret_cast<const u32x4*>(prm + 2 * NG * 64 + (g * 32 + h * 8) * 2);
             rg.vm = *reinterpret_cast<const u32x4*>(prm + 3 * NG * 64 + ((c < NG ? c : 0) * 32 + h * 8) * 2);
         };
-        // kMask: the block reaches past a column's last position, or has no page
-        auto block = [&](Regs& rg, int64_t b, auto mask) __attribute__((always_inline)) {
-            constexpr bool kMask = decltype(mask)::value;
+        load_pages(0);
+        // query fragment: fp16 with the row's largest value in [64, 128)
+        u32x4 raw[W];
+        {
+            const int tk = row_ok ? tok : 0, hd = head * G + (row_ok ? r - tok * G : 0);
+            const uint16_t* qr = io.q + ((int64_t)row0 + tk) * io.q_ts + hd * io.q_hs + 8 * h;
+#pragma unroll
+            for (int j = 0; j < W; ++j) raw[j] = *reinterpret_cast<const u32x4*>(qr + 32 * j);
+        }
+        Regs r0, r1;
+        if (cnt > 0) load(r0, 0);
+        f16x8 qf[W], qm;
+        float kscale;
+        {
+            float top = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(ld16<kBf16>(half_of(raw[j][e >> 1], e))));
+            top = max4(row_ok ? top : 0.f);
+            // exponent of the largest value; no scaling of rows that are zero or not finite
+            const int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+            const int up = top > 0.f && ex < 255 && ex > 0 ? (127 + 6 - ex < 126 ? 127 + 6 - ex : 126) : 0;
+            const float mul = __builtin_ldexpf(row_ok ? 1.f : 0.f, up);
+            kscale = io.scale_log2 * __builtin_ldexpf(1.f, -up);
+            float qs[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) qs[g] = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float raw_q = ld16<kBf16>(half_of(raw[j][e >> 1], e));
+                    const _Float16 v = (_Float16)(row_ok ? raw_q * mul : 0.f);
+                    qf[j][e] = v;
+                    qs[j / 2] += (float)v;
+                }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qm[e] = (_Float16)0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const float s = sum4(qs[g]);
+                const _Float16 hi = (_Float16)s;
+                if (h == 0) {
+                    qm[g] = hi;
+                    qm[4 + g] = (_Float16)(s - (float)hi);
+                }
+            }
+        }
+        f32x4 o[NT], om = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -kInf, l = 0.f;
+        auto step = [&](Regs& rg, int i) __attribute__((always_inline)) {
+            const int b = b0 + i;
+            const bool mask = b * 32 + 31 > lim_min || rg.bad;     // past a column's last position, or no page
             float sc[8];
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
@@ -458,10 +503,10 @@ __global__ __launch_bounds__(256) void k_kv4_attend(const Kv4Pool p, const Atten
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[4 * a + e] = __builtin_fmaf(s[e], 16777216.f, mt[e]);
             }
-            if constexpr (kMask) {
+            if (mask) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int64_t key = b * 32 + (e / 4) * 16 + 4 * h + e % 4;
+                    const int key = b * 32 + (e / 4) * 16 + 4 * h + e % 4;
                     sc[e] = key <= lim && !rg.bad ? sc[e] : -kInf;
                 }
             }
@@ -487,9 +532,15 @@ __global__ __launch_bounds__(256) void k_kv4_attend(const Kv4Pool p, const Atten
             }
             u32x4 vm = rg.vm;
             if (c >= NG) vm = u32x4{0u, 0u, 0u, 0u};
-            if constexpr (kMask) {
-                // a token that some column may not attend must not reach it through 0 * NaN: its minimum is zero where
-                // it is no number (the scale, which is none either, still brings the NaN to the columns that attend it)
+            if (mask) {
+                // a token that some column may not attend must not reach it through 0 * NaN: its scale is zero for that
+                // column, and its minimum zero where it is no number (the scale, which is none either, still brings the
+                // NaN to the columns that attend it)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (pv[e] == 0.f)
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) rg.vs[g][e >> 1] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t lo = vm[e] & 0x7FFFu, hi = vm[e] >> 16 & 0x7FFFu;
@@ -510,9 +561,8 @@ __global__ __launch_bounds__(256) void k_kv4_attend(const Kv4Pool p, const Atten
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float s = sx8_h2f(half_of(rg.vs[g][e >> 1], e));
-                    const float ps = kMask && pv[e] == 0.f ? 0.f : s;
-                    ph[e] = (_Float16)(pv[e] * ps);
-                    pl[e] = (_Float16)__builtin_fmaf(pv[e], ps, -(float)ph[e]);
+                    ph[e] = (_Float16)(pv[e] * s);
+                    pl[e] = (_Float16)__builtin_fmaf(pv[e], s, -(float)ph[e]);
                 }
 #pragma unroll
                 for (int t = 4 * g; t < 4 * g + 4; ++t) {
@@ -522,13 +572,6 @@ __global__ __launch_bounds__(256) void k_kv4_attend(const Kv4Pool p, const Atten
                 }
             }
         };
-        auto step = [&](Regs& rg, int i) __attribute__((always_inline)) {
-            const int64_t b = b0 + w + 4 * (int64_t)i;
-            if (b * 32 + 31 > lim_min || rg.bad) block(rg, b, std::true_type{});
-            else block(rg, b, std::false_type{});
-        };
-        Regs r0, r1;
-        if (cnt > 0) load(r0, 0);
         for (int i = 0; i < cnt; i += 2) {
             if (i + 1 < cnt) load(r1, i + 1);
             step(r0, i);
@@ -536,122 +579,86 @@ __global__ __launch_bounds__(256) void k_kv4_attend(const Kv4Pool p, const Atten
             if (i + 2 < cnt) load(r0, i + 2);
             step(r1, i + 1);
         }
-        // the four waves' states meet in LDS: O = 2^24 (levels) + (minima's sum of the group, row g of om)
+        // O = 2^24 (levels) + (the minima's sum of the group, row g of om)
         l = sum4(l);
-        float og[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) og[g] = __shfl(om[g], c, 64);
+        const bool whole = b0 == 0 && bend == nb;
+        const float f = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const int place = 2 * wave + (here == x0 ? 0 : 1);
+        const int64_t at = place * (int64_t)16 + c;
+        float* const po = io.part_o + at * HD + 4 * h;
+        uint16_t* const dst = io.out + ((int64_t)row0 + tok) * io.o_ts + (head * G + (r - tok * G)) * io.o_hs + 4 * h;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            const float og = __shfl(om[t / 4], c, 64);
             f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(o[t][e], 16777216.f, og[t / 4]);
-            *reinterpret_cast<f32x4*>(&so[w][c][16 * t + 4 * h]) = v;
-        }
-        if (h == 0) {
-            sml[w][c][0] = m;
-            sml[w][c][1] = l;
-        }
-        __syncthreads();
-        {
-            constexpr int N = HD / 16;
-            const int col = tid >> 4, d0 = (tid & 15) * N;
-            float mm = sml[0][col][0];
-#pragma unroll
-            for (int i = 1; i < 4; ++i) mm = fmaxf(mm, sml[i][col][0]);
-            float den = 0.f, acc[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) acc[e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float f = sml[i][col][0] == mm ? 1.f : __builtin_amdgcn_exp2f(sml[i][col][0] - mm);
-                den = __builtin_fmaf(f, sml[i][col][1], den);
-#pragma unroll
-                for (int e = 0; e < N; ++e) acc[e] = __builtin_fmaf(f, so[i][col][d0 + e], acc[e]);
-            }
-            const int64_t rr = 16 * tile + col, tk = rr / G;
-            if (b0 == 0 && bend == nb) {
-                if (tk < n) {
-                    const float inv = den == 0.f ? 0.f : 1.f / den;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) acc[e] *= inv;
-                    store_row<HD, kBf16>(io.out + (row0 + tk) * io.o_ts + (head * G + (int)(rr - tk * G)) * io.o_hs + d0,
-                                         acc);
-                }
-            } else {
-                const int64_t at = 2 * (int64_t)blockIdx.x + (x == x0 ? 0 : 1);
-                float* po = io.part_o + (at * 16 + col) * HD + d0;
-#pragma unroll
-                for (int e = 0; e < N; e += 4)
-                    *reinterpret_cast<f32x4*>(po + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-                if ((tid & 15) == 0) {
-                    io.part_ml[(at * 16 + col) * 2] = mm;
-                    io.part_ml[(at * 16 + col) * 2 + 1] = den;
-                }
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(o[t][e], 16777216.f, og) * f;
+            if (row_ok) {
+                if (whole) *reinterpret_cast<u32x2*>(dst + 16 * t) = u32x2{pack16<kBf16>(v[0], v[1]), pack16<kBf16>(v[2], v[3])};
+                else *reinterpret_cast<f32x4*>(po + 16 * t) = v;
             }
         }
-        // a unit whose first piece this is and that goes on in the next work-groups: its record for the combine
-        if (bend < nb && x - b0 >= x0) {
-            cut = true;
-            if (tid == 0) {
-                Kv4Piece pc;
-                pc.parts = (int32_t)((x - b0 + nb - 1) / share - blockIdx.x + 1);
-                pc.first_at = x == x0 ? 0 : 1;
-                pc.tile = (int32_t)tile;
-                pc.head = head;
-                pc.row0 = row0;
-                pc.n = n;
-                io.piece[blockIdx.x] = pc;
-            }
+        if (!whole && h == 0 && row_ok) {
+            io.part_ml[at * 2] = m;
+            io.part_ml[at * 2 + 1] = l;
         }
-        x += bend - b0;
-        __syncthreads();
+        // the unit's record is written by its first piece; a unit that is cut goes on in the next waves
+        if (b0 == 0 && lane == 0 && (io.by_unit || !whole)) {
+            Kv4Piece pc;
+            pc.parts = whole ? 0 : kv4_parts(begin + run.unit * (nb + kKv4Begin) + kKv4Begin, nb, share, wave);
+            pc.first = place;
+            pc.tile = tile;
+            pc.head = head;
+            pc.row0 = row0;
+            pc.n = n;
+            io.piece[io.by_unit ? unit0 + run.unit : wave] = pc;
+        }
     }
-    if (!cut && tid == 0) io.piece[blockIdx.x].parts = 0;
 }
 
-// Units that were cut: work-group i merges the unit whose first piece ends the share of work-group i, its parts in their
-// order (part 0 at slot 2 i + first_at, the next ones at 2 (i + 1), 2 (i + 2), ...).  Wave = (row, quarter of the parts).
-template <int HD, bool kBf16>
+// Units that were cut: work-group i takes the record i and kRows of its 16 rows, and adds the unit's parts up in their order
+// (part 0 at its place, part j at place 2 (wave + j)).  A row's parts are shared by 16 / kRows waves, whose sums meet in LDS.
+template <int HD, bool kBf16, int kRows>
 __global__ __launch_bounds__(1024) void k_kv4_combine(const AttendIo io, int G) {
-    constexpr int N = HD / 64;
+    constexpr int N = HD / 64, kShares = 16 / kRows, kU = 8;      // kU: parts requested together
+    typedef float vecN __attribute__((ext_vector_type(N)));
     const Kv4Piece pc = io.piece[blockIdx.x];
-    if (pc.parts == 0) return;
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = w & 3;
-    const int row = 4 * blockIdx.y + (w >> 2);
-    const int64_t rr = 16 * (int64_t)pc.tile + row, tk = rr / G;
-    const bool live = tk < pc.n;
-    __shared__ float sml[16][2], so[16][HD];
-    auto at = [&](int i) { return (2 * ((int64_t)blockIdx.x + i) + (i == 0 ? pc.first_at : 0)) * 16 + row; };
-    const int per = (pc.parts + 3) / 4, i0 = quarter * per, i1 = min(i0 + per, pc.parts);
-    float m = -__builtin_inff();
+    const int row0 = kRows * blockIdx.y, rows = min(16, pc.n * G - 16 * pc.tile);
+    if (pc.parts == 0 || row0 >= rows) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mine = w % kShares, row = row0 + w / kShares;
+    __shared__ float sml[16][2];
+    __shared__ vecN so[16][64];
+    const bool live = row < rows;
+    auto at = [&](int i) { return (int64_t)(i == 0 ? pc.first : 2 * (pc.first / 2 + i)) * 16 + row; };
+    const int per = (pc.parts + kShares - 1) / kShares, i0 = mine * per, i1 = min(i0 + per, pc.parts);
+    float m = -__builtin_inff(), den = 0.f;
+    vecN acc = 0.f;
     if (live) {
-        for (int i = i0 + lane; i < i1; i += 64) m = fmaxf(m, io.part_ml[at(i) * 2]);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    }
-    float den = 0.f, acc[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = 0.f;
-    if (live) {
-        constexpr int kU = 8;                       // parts requested together
         for (int i = i0; i < i1; i += kU) {
-            float v[kU][N], pm[kU], pl[kU];
+            float pm[kU], pl[kU];
+            vecN v[kU];
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
                 const int64_t a = at(min(i + u, i1 - 1));
                 pm[u] = io.part_ml[a * 2];
                 pl[u] = io.part_ml[a * 2 + 1];
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[u][e] = io.part_o[a * HD + 64 * e + lane];
+                v[u] = reinterpret_cast<const vecN*>(io.part_o + a * HD)[lane];
             }
+            __builtin_amdgcn_sched_barrier(0);
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) mn = fmaxf(mn, pm[u]);
+            const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            den *= alpha;
+            acc *= alpha;
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-                if (i + u >= i1) break;
+                if (i + u >= i1) continue;
                 const float f = pm[u] == m ? 1.f : __builtin_amdgcn_exp2f(pm[u] - m);
                 den = __builtin_fmaf(f, pl[u], den);
-#pragma unroll
-                for (int e = 0; e < N; ++e) acc[e] = __builtin_fmaf(f, v[u][e], acc[e]);
+                acc = __builtin_elementwise_fma(vecN(f), v[u], acc);
             }
         }
     }
@@ -659,28 +666,28 @@ __global__ __launch_bounds__(1024) void k_kv4_combine(const AttendIo io, int G) 
         sml[w][0] = m;
         sml[w][1] = den;
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) so[w][64 * e + lane] = acc[e];
+    so[w][lane] = acc;
     __syncthreads();
-    if (quarter != 0 || !live) return;
+    if (mine != 0 || !live) return;
     float mm = m;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) mm = fmaxf(mm, sml[w + i][0]);
+    for (int i = 1; i < kShares; ++i) mm = fmaxf(mm, sml[w + i][0]);
     const float f0 = m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm);
     den *= f0;
+    acc *= f0;
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] *= f0;
-#pragma unroll
-    for (int i = 1; i < 4; ++i) {
+    for (int i = 1; i < kShares; ++i) {
         const float f = sml[w + i][0] == mm ? 1.f : __builtin_amdgcn_exp2f(sml[w + i][0] - mm);
         den = __builtin_fmaf(f, sml[w + i][1], den);
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = __builtin_fmaf(f, so[w + i][64 * e + lane], acc[e]);
+        acc = __builtin_elementwise_fma(vecN(f), so[w + i][lane], acc);
     }
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    uint16_t* dst = io.out + (pc.row0 + tk) * io.o_ts + (pc.head * G + (int)(rr - tk * G)) * io.o_hs;
+    acc *= den == 0.f ? 0.f : 1.f / den;
+    const int rr = 16 * pc.tile + row, tk = rr / G;
+    uint16_t* dst = io.out + ((int64_t)pc.row0 + tk) * io.o_ts + (pc.head * G + (rr - tk * G)) * io.o_hs + N * lane;
+    if constexpr (N == 1) *dst = (uint16_t)st16<kBf16>(acc[0]);
+    else
 #pragma unroll
-    for (int e = 0; e < N; ++e) dst[64 * e + lane] = (uint16_t)st16<kBf16>(acc[e] * inv);
+        for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack16<kBf16>(acc[e], acc[e + 1]);
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -711,7 +718,7 @@ int32_t make_pool(const char* what, Kv4Pool* p, const uint8_t* pages, const int3
     p->max_pages = (int)max_pages;
     p->n_pages = (int)n_pages;
     p->bpp_log2 = page_tokens == 32 ? 0 : page_tokens == 64 ? 1 : page_tokens == 128 ? 2 : 3;
-    p->sh = Kv4Shape{(int)n_slots, nk, 1, max_pages * page_tokens, rows};
+    p->sh = Kv4Shape{(int)n_slots, nk, 1, (int)(max_pages * page_tokens), (int)rows};
     return SX8_OK;
 }
 
@@ -809,21 +816,32 @@ extern "C" int32_t sx8_kv4_attend(const uint8_t* pages, const int32_t* table, co
         return fail(SX8_ERR_INVALID, "%s: scale must be positive and finite", what);
     if (!workspace || workspace_bytes < attend_ws(hd) || !aligned(workspace, 256))
         return fail(SX8_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", what, (long long)attend_ws(hd));
+    if (rows * (nh / nk) > 0x7FFFFF00) return fail(SX8_ERR_UNSUPPORTED, "%s: over 2^31 query rows of a KV head", what);
     if (rows == 0) return ok();
     p.sh.G = nh / nk;
+    const int64_t waves = (int64_t)1 << (hd == 256 ? 10 : 11);
     AttendIo io{(const uint16_t*)q, (uint16_t*)out, q_ts, q_hs, o_ts, o_hs, scale * 1.4426950408889634f, nullptr, nullptr,
-                nullptr};
+                nullptr, 0};
     io.piece = reinterpret_cast<Kv4Piece*>(workspace);
-    io.part_o = reinterpret_cast<float*>(io.piece + kWgs);
-    io.part_ml = io.part_o + 2 * kWgs * 16 * (int64_t)hd;
-    // rows of a unit that can be in use: all 16, or those of one token a slot
-    const int64_t used = cu ? rows * p.sh.G : p.sh.G;
-    const unsigned groups = (unsigned)((used < 16 ? used : 16) + 3) / 4;
+    io.part_o = reinterpret_cast<float*>(io.piece + waves);
+    io.part_ml = io.part_o + 2 * waves * 16 * hd;
+    // units at most: a slot with n rows has nk ceil(n G / 16) of them
+    const int64_t G = p.sh.G, live = n_slots < rows ? n_slots : rows;
+    const int64_t units = nk * (cu ? rows * G / 16 + live : n_slots * ((G + 15) / 16));
+    io.by_unit = units <= waves;
+    const unsigned entries = (unsigned)(io.by_unit ? units : waves), used = (unsigned)(cu ? (rows * G < 16 ? rows * G : 16) : (G < 16 ? G : 16));
+    // few rows in all: a row's parts are shared by 16 waves, else by four
+    const bool narrow = entries * used <= 512;
     by_kind(hd, dtype, [&](auto d, auto b) {
-        hipLaunchKernelGGL((k_kv4_attend<decltype(d)::value, decltype(b)::value>), dim3(kWgs), dim3(256), prefix_bytes(p),
-                           as_stream(stream), p, io);
-        hipLaunchKernelGGL((k_kv4_combine<decltype(d)::value, decltype(b)::value>), dim3(kWgs, groups), dim3(1024), 0,
-                           as_stream(stream), io, p.sh.G);
+        constexpr int HD = decltype(d)::value;
+        constexpr bool kBf = decltype(b)::value;
+        hipLaunchKernelGGL((k_kv4_attend<HD, kBf>), dim3((1 << waves_log2<HD>()) / 4), dim3(256),
+                           n_slots <= 64 ? 0 : prefix_bytes(p) * 3 / 2, as_stream(stream), p, io);
+        if (narrow)
+            hipLaunchKernelGGL((k_kv4_combine<HD, kBf, 1>), dim3(entries, used), dim3(1024), 0, as_stream(stream), io, p.sh.G);
+        else
+            hipLaunchKernelGGL((k_kv4_combine<HD, kBf, 4>), dim3(entries, (used + 3) / 4), dim3(1024), 0, as_stream(stream), io,
+                               p.sh.G);
     });
     return check_launch(what);
 }

@@ -38,20 +38,36 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
                      (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+
+// Sum of v over the lanes up to this one: shifts within rows of 16 lanes, then each row's last lane to the rows above.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int64_t add_dpp(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), kCtrl, kRows, 0xF, false);
+    return v + (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t wave_prefix(int64_t v) {
+    v = add_dpp<0x111, 0xF>(v);                      // row_shr 1, 2, 4, 8
+    v = add_dpp<0x112, 0xF>(v);
+    v = add_dpp<0x114, 0xF>(v);
+    v = add_dpp<0x118, 0xF>(v);
+    v = add_dpp<0x142, 0xA>(v);                      // row_bcast 15 into rows 1 and 3
+    return add_dpp<0x143, 0xC>(v);                   // row_bcast 31 into rows 2 and 3
+}
+
 // Prefix sums of f(s) over n items into pre[0 .. n] (LDS), every thread of the work-group (kT threads) taking part.
-template <int kT, typename F>
-__device__ __forceinline__ void prefix_sums(int n, int64_t* pre, F&& f) {
+template <int kT, typename P, typename F>
+__device__ __forceinline__ void prefix_sums(int n, P* pre, F&& f) {
     __shared__ int64_t wsum[kT / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     int64_t base = 0;
     if (tid == 0) pre[0] = 0;
     for (int s0 = 0; s0 < n; s0 += kT) {
-        int64_t v = s0 + tid < n ? f(s0 + tid) : 0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t u = __shfl_up(v, o, 64);
-            if (lane >= o) v += u;
-        }
+        const int64_t v = wave_prefix(s0 + tid < n ? f(s0 + tid) : 0);
         if (lane == 63) wsum[w] = v;
         __syncthreads();
         int64_t before = base, all = base;
@@ -60,7 +76,7 @@ __device__ __forceinline__ void prefix_sums(int n, int64_t* pre, F&& f) {
             if (i < w) before += wsum[i];
             all += wsum[i];
         }
-        if (s0 + tid < n) pre[s0 + tid + 1] = before + v;
+        if (s0 + tid < n) pre[s0 + tid + 1] = (P)(before + v);
         base = all;
         __syncthreads();
     }

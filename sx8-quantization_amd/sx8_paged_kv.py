@@ -177,14 +177,14 @@ class PagedKV4:
 
     def read(self, layer, rows, cu=None, dtype=torch.float16, out=None):
         """The values of the slots' last tokens: k and v (rows, n_kv, head_dim), packed as `append` takes them (cu of
-        all lengths reads whole slots).  out: (k, v) to write into.  Rows of tokens without a page stay as they are
-        (new tensors begin as zeros)."""
+        all lengths reads whole slots).  out: (k, v) to write into.  Tokens without a page give zeros; rows of no token stay as
+        they are (in new tensors: unset)."""
         if dtype not in _DTYPES:
             raise RuntimeError(f"dtype must be float16 or bfloat16, got {dtype}")
         with torch.cuda.device(self.device):
             like = torch.empty(int(rows), 0, 0, dtype=dtype, device=self.device)
             if out is None:
-                out = tuple(torch.zeros(int(rows), self.n_kv, self.head_dim, dtype=dtype, device=self.device)
+                out = tuple(torch.empty(int(rows), self.n_kv, self.head_dim, dtype=dtype, device=self.device)
                             for _ in range(2))
             k, v = (_out(n, t, like, self.n_kv, self.head_dim) for n, t in zip(("k", "v"), out))
             _L.call("sx8_kv4_read", *self._slots(layer, cu), k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1),

@@ -24,11 +24,11 @@ def emul(hiplib):                                                      # (torch'
                     os.path.join(REPO, "sx8-quantization_amd", "csrc"), "-o", out,
                     os.path.join(HERE, "emul", "sx8_kv4_emul.hip")], check=True, capture_output=True)
     L = ctypes.CDLL(out)
-    L.sx8e_kv4_pieces.restype = L.sx8e_kv4_slot_blocks.restype = I64
+    L.sx8e_kv4_pieces.restype = L.sx8e_kv4_slot_places.restype = I64
     L.sx8e_kv4_touched.restype = L.sx8e_kv4_touched_most.restype = I64
-    L.sx8e_kv4_pieces.argtypes = [I32, I32, I32, I64, I64, P, P, I32, P, I64]
-    L.sx8e_kv4_slot_blocks.argtypes = [I32, I32, I32, I64, I64, P, P, I32]
-    L.sx8e_kv4_touched.argtypes = [I64, I64, P]
+    L.sx8e_kv4_pieces.argtypes = [I32, I32, I32, I32, I32, P, P, I32, P, I64]
+    L.sx8e_kv4_slot_places.argtypes = [I32, I32, I32, I32, I32, P, P, I32]
+    L.sx8e_kv4_touched.argtypes = [I32, I32, P]
     L.sx8e_kv4_touched_most.argtypes = [I64, I64, I32]
     return L
 
@@ -74,35 +74,43 @@ def _lists(rng):
 
 
 def test_work_split_covers_every_block_once(emul):
-    """Every block of every unit belongs to one piece; a work-group has at most one piece that starts its share and
-    one that ends it, so the partial results' places are distinct; the parts of a cut unit lie in consecutive
-    work-groups, whose number is what the combine is told."""
+    """Every block of every unit belongs to one piece; a wave has at most one piece that starts its share and one
+    that ends it, so the partial results' places are distinct; the parts of a cut unit lie in consecutive waves, whose
+    number is what the combine is told."""
     rng = random.Random(5)
     for it in range(60):
         S, nk, G, cap, rows, lens, cu = _lists(rng)
-        wgs = rng.choice([1, 3, 512])
+        log2 = rng.choice([0, 2, 11])
+        waves = 1 << log2
         la = np.array(lens, np.int32)
         ca = None if cu is None else np.array(cu, np.int32)
         cp = None if ca is None else ca.ctypes.data
         args = (S, nk, G, cap, rows, la.ctypes.data, cp)
-        n = emul.sx8e_kv4_pieces(*args, wgs, None, 0)
-        out = np.zeros((max(n, 1), 7), np.int64)
-        assert emul.sx8e_kv4_pieces(*args, wgs, out.ctypes.data, n) == n
+        n = emul.sx8e_kv4_pieces(*args, log2, None, 0)
+        out = np.zeros((max(n, 1), 8), np.int64)
+        assert emul.sx8e_kv4_pieces(*args, log2, out.ctypes.data, n) == n
         out = out[:n]
         seen, places, total = {}, set(), 0
-        for wg, s, unit, b0, e, nb, place in out:
+        parts = {}
+        for wave, s, unit, b0, e, nb, place, told in out:
             assert b0 == seen.get((s, unit), (0, None))[0] and b0 < e <= nb
-            if b0 > 0:                                              # goes on: the next work-group, as its first piece
-                assert wg == seen[s, unit][1] + 1 and place % 2 == 0
-            seen[s, unit] = (e, wg, nb)
+            if b0 > 0:                                              # goes on: the next wave, as its first piece
+                assert wave == seen[s, unit][1] + 1 and place % 2 == 0
+                parts[s, unit][1] += 1
+            else:
+                parts[s, unit] = [told, 1]
+            seen[s, unit] = (e, wave, nb)
             if not (b0 == 0 and e == nb):
-                assert place not in places and 0 <= place < 2 * wgs
+                assert place not in places and 0 <= place < 2 * waves
                 places.add(place)
             total += e - b0
         assert all(e == nb for e, _, nb in seen.values())
-        sums = [emul.sx8e_kv4_slot_blocks(*args, s) for s in range(S)]
-        assert total == sum(sums)
-        share = max(4, -(-total // wgs))
+        sums = [emul.sx8e_kv4_slot_places(*args, s) for s in range(S)]
+        assert all(a == b for a, b in parts.values())
+        units = len(seen)
+        assert total + 3 * units == sum(sums)
+        total = sum(sums)
+        share = max(1, -(-total // waves))
         assert all(out[:, 0] * share < total)
         for s in range(S):                                          # units as rows and heads say
             new = 1 if cu is None else int(cu[s + 1] - cu[s])
@@ -113,7 +121,7 @@ def test_work_split_covers_every_block_once(emul):
 def test_touched_blocks(emul):
     """The blocks of a slot's new tokens, and the grid's bound on those of all slots."""
     rng = random.Random(6)
-    first = I64()
+    first = I32()
     for _ in range(300):
         S = rng.choice([1, 3, 20])
         lens = [rng.randrange(0, 200) for _ in range(S)]
@@ -205,5 +213,5 @@ def test_varlen_entry_point_refuses(hiplib):
                dict(st=(-128, 64, 64, 64, 64, 64, 128, 64))):
         assert call(**kw) == 1, kw
         assert "sx8_attn_varlen" in L.sx8_last_error().decode()
-    assert call(tq=(1 << 31) - 1, nh=4096, n=1) == 3
+    assert call(tq=(1 << 31) - 300, nh=4096, n=1) == 3
     assert call(tq=0, q=null, out=null) == 0

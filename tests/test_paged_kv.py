@@ -255,6 +255,27 @@ def test_attend_long_and_cut(hiplib, cuda):
     assert torch.equal(again, p.attend(0, q, scale=0.3))
 
 
+@pytest.mark.parametrize("n_slots", [64, 65, 300, 4096])
+@pytest.mark.parametrize("nk", [1, 9])
+def test_attend_many_slots(hiplib, cuda, n_slots, nk):
+    """More slots than a wave has lanes, more units than the launch has waves, with and without cu."""
+    lens = [(37 * i) % 71 for i in range(n_slots)]
+    p, k, v = make(cuda, lens, nk, 64, 32)
+    kk, vv = q4(k), q4(v)
+    some = [i for i in range(n_slots) if i < 70 or i % 97 == 0 or i > n_slots - 3]
+    ends = torch.tensor(lens).cumsum(0).tolist()
+    for new in ([1] * n_slots, [(5 * i) % 4 for i in range(n_slots)]):
+        q = rand((sum(new), 2 * nk, 64), 3, F16, cuda)
+        got = p.attend(0, q, cum(new, cuda))
+        if new[0] == 1:
+            assert torch.equal(got, p.attend(0, q))
+        firsts = torch.tensor([0] + new).cumsum(0).tolist()
+        for i in some:
+            a, b, e = firsts[i], ends[i], lens[i]
+            want = attention(q[a:a + new[i]].double(), kk[b - e:b], vv[b - e:b], e - new[i])
+            close(got[a:a + new[i]], want, F16, 4.0)
+
+
 def test_attend_more_rows_than_tokens(hiplib, cuda):
     """More new rows than the slot has tokens: the first rows see none and give zeros."""
     p, k, v = make(cuda, [2, 40], 2, 64, 32)
