@@ -60,7 +60,7 @@ int32_t sx8_kv4_append(uint8_t* pages, const int32_t* table, const int32_t* lens
                        int32_t dtype, void* stream);
 
 /* The values of the slots' last tokens (as sx8_kv4_append takes them), rounded to dtype.  Tokens without a page
- * give zeros; rows without a token (a slot with more rows than tokens) are left as they are. */
+ * and rows without a token (a slot with more rows than tokens) give zeros. */
 int32_t sx8_kv4_read(const uint8_t* pages, const int32_t* table, const int32_t* lens, const int32_t* cu, int64_t n_slots,
                      int64_t max_pages, int64_t n_pages, void* k, void* v, int64_t rows, int64_t k_ts, int64_t k_hs,
                      int64_t v_ts, int64_t v_hs, int32_t nk, int32_t hd, int32_t page_tokens, int32_t dtype,

@@ -100,11 +100,11 @@ SX8_KV4_FN int kv4_parts(int64_t at, int nb, int64_t share, int wave) {
 }
 
 // Blocks of tokens that the new tokens of a slot touch (append, read): first block, and how many.  Positions
-// len - n .. len - 1; those outside the slot are left out.
+// len - n .. len - 1; those below zero (more rows than tokens) lie in blocks below zero, which have no page.
+SX8_KV4_FN int kv4_floor_block(int pos) { return pos >= 0 ? pos / kKv4Block : -((-pos + kKv4Block - 1) / kKv4Block); }
 SX8_KV4_FN int kv4_touched(int len, int n, int* first) {
-    const int a = len - n > 0 ? len - n : 0;
-    *first = a / kKv4Block;
-    return n > 0 && len > 0 ? (len - 1) / kKv4Block - *first + 1 : 0;
+    *first = kv4_floor_block(len - n);
+    return n > 0 ? kv4_floor_block(len - 1) - *first + 1 : 0;
 }
 // At least the touched blocks of all slots together, from what the host knows: every slot with rows touches at
 // most (n + 30) / 32 + 1 blocks.

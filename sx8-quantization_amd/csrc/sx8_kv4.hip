@@ -22,7 +22,7 @@ struct Kv4Pool {
 // Byte offset of block b of head h of a slot's page, or -1 where the slot has no such page.
 __device__ __forceinline__ int64_t block_offset(const Kv4Pool& p, int slot, int head, int b, int bb) {
     const int at = b >> p.bpp_log2;
-    if (at >= p.max_pages) return -1;
+    if (b < 0 || at >= p.max_pages) return -1;
     const int page = p.table[(int64_t)slot * p.max_pages + at];
     if (page < 0 || page >= p.n_pages) return -1;
     return page * p.page_bytes + (((int64_t)head << p.bpp_log2) + (b & ((1 << p.bpp_log2) - 1))) * bb;

@@ -25,8 +25,10 @@
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
+#include <string>
 
 #include "sx8_hip.h"
+#include "sx8_paged.h"
 
 namespace {
 
@@ -43,6 +45,14 @@ struct Lib {
                           int64_t, void*);
     int32_t (*dequant)(CP, CP, CP, CP, CP, CP, CP, CP, int64_t, int64_t, int64_t, void*, void*);
     int32_t (*embed)(CP, int64_t, CP, CP, int32_t, CP, CP, int64_t, int64_t, int64_t, void*, void*);
+    decltype(&sx8_attn_varlen) varlen;
+    decltype(&sx8_kv4_append) kv4_append;
+    decltype(&sx8_kv4_read) kv4_read;
+    decltype(&sx8_kv4_attend) kv4_attend;
+    decltype(&sx8_kv4_reserve) kv4_reserve;
+    decltype(&sx8_kv4_fork) kv4_fork;
+    decltype(&sx8_kv4_free) kv4_free;
+    decltype(&sx8_kv4_compact) kv4_compact;
 } lib;
 
 constexpr int32_t kUnsupported = SX8_ERR_UNSUPPORTED;
@@ -120,6 +130,14 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     SX8_BIND(gemm_split, "sx8_gemm_prefill_split")
     SX8_BIND(dequant, "sx8_dequant_f16")
     SX8_BIND(embed, "sx8_embed_gather")
+    SX8_BIND(varlen, "sx8_attn_varlen")
+    SX8_BIND(kv4_append, "sx8_kv4_append")
+    SX8_BIND(kv4_read, "sx8_kv4_read")
+    SX8_BIND(kv4_attend, "sx8_kv4_attend")
+    SX8_BIND(kv4_reserve, "sx8_kv4_reserve")
+    SX8_BIND(kv4_fork, "sx8_kv4_fork")
+    SX8_BIND(kv4_free, "sx8_kv4_free")
+    SX8_BIND(kv4_compact, "sx8_kv4_compact")
 #undef SX8_BIND
     Py_RETURN_NONE;
 }
@@ -402,6 +420,229 @@ PyObject* py_to_host(PyObject*, PyObject* const* a, Py_ssize_t na) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- packed sequences and the paged cache (sx8_paged_kv.py) ------------------------------------
+// A (rows, heads, hd) tensor of fp16 or bf16 that the kernels read in place (sx8_paged_kv._in_place), else null.
+const at::Tensor* head_rows(PyObject* o, int64_t min_ts) {
+    const at::Tensor* x = plain(o);
+    if (!x || !x->is_cuda() || x->layout() != at::kStrided || x->dim() != 3 || x->size(0) < 1 ||
+        (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16))
+        return nullptr;
+    const int64_t ts = x->stride(0), hs = x->stride(1);
+    const bool ok = x->stride(2) == 1 && ts % 8 == 0 && hs % 8 == 0 && hs >= 0 && ts >= min_ts && ts <= 1 << 23 &&
+                    reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0;
+    return ok ? x : nullptr;
+}
+
+// A contiguous int32 vector of n values (any number: n < 0) on the device of `like`, else null.
+const at::Tensor* int_vector(PyObject* o, int64_t n, const at::Tensor& like) {
+    const at::Tensor* x = dense(o, at::kInt);
+    return x && x->dim() == 1 && x->numel() > 0 && (n < 0 || x->numel() == n) && x->device() == like.device() ? x : nullptr;
+}
+
+int32_t dtype_of(const at::Tensor& x) { return x.scalar_type() == at::kBFloat16; }
+
+// varlen(q, k, v, cu_q, cu_k or None, scale, causal): attn_varlen into a new tensor.
+PyObject* py_varlen(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(7)
+    const at::Tensor* q = head_rows(a[0], 0);
+    if (!q) Py_RETURN_NONE;
+    const int64_t hd = q->size(2);
+    const at::Tensor* k = head_rows(a[1], hd);
+    const at::Tensor* v = head_rows(a[2], hd);
+    const at::Tensor* cq = int_vector(a[3], -1, *q);
+    const at::Tensor* ck = a[4] == Py_None ? cq : int_vector(a[4], cq ? cq->numel() : 0, *q);
+    if (!k || !v || !cq || !ck || k->sizes() != v->sizes() || k->size(2) != hd || k->scalar_type() != q->scalar_type() ||
+        v->scalar_type() != q->scalar_type() || k->device() != q->device() || v->device() != q->device() ||
+        !PyFloat_Check(a[5]) || !PyBool_Check(a[6]))
+        Py_RETURN_NONE;
+    const float scale = (float)PyFloat_AS_DOUBLE(a[5]);
+    int32_t rc;
+    at::Tensor o;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(q->device());
+        o = empty_like_device(q->sizes(), q->scalar_type(), *q);
+        rc = lib.varlen(q->data_ptr(), k->data_ptr(), v->data_ptr(), o.data_ptr(), cq->data_ptr<int32_t>(),
+                        ck->data_ptr<int32_t>(), cq->numel() - 1, q->size(0), k->size(0), (int32_t)q->size(1),
+                        (int32_t)k->size(1), (int32_t)hd, q->stride(0), q->stride(1), k->stride(0), k->stride(1), v->stride(0),
+                        v->stride(1), o.stride(0), o.stride(1), scale, a[6] == Py_True, dtype_of(*q), stream_of(*q));
+    }
+    if (rc) return failed("sx8_attn_varlen", rc);
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// What PagedKV4 keeps for these calls: (pages, table, lens, refs, status, page_bytes, n_kv, head_dim, page_tokens,
+// bytes of attend's workspace, bytes of the page operations' workspace); the wrapper checked it.
+struct Cache {
+    const at::Tensor *pages, *table, *lens, *refs, *status;
+    int64_t layers, n_pages, slots, width, page_bytes, ws_attend, ws_pages;
+    int32_t nk, hd, pt;
+    void* stream;
+    int32_t* ints(const at::Tensor* t) const { return t->data_ptr<int32_t>(); }
+    uint8_t* layer(int64_t i) const { return pages->data_ptr<uint8_t>() + i * n_pages * page_bytes; }
+};
+bool cache(PyObject* o, Cache* c) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 11) return false;
+    const at::Tensor** t[5] = {&c->pages, &c->table, &c->lens, &c->refs, &c->status};
+    for (int i = 0; i < 5; ++i)
+        if (!(*t[i] = plain(PyTuple_GET_ITEM(o, i)))) return false;
+    int64_t n[6];
+    for (int i = 0; i < 6; ++i) n[i] = num(PyTuple_GET_ITEM(o, 5 + i));
+    c->page_bytes = n[0];
+    c->nk = (int32_t)n[1];
+    c->hd = (int32_t)n[2];
+    c->pt = (int32_t)n[3];
+    c->ws_attend = n[4];
+    c->ws_pages = n[5];
+    c->layers = c->pages->size(0);
+    c->n_pages = c->pages->size(1);
+    c->slots = c->table->size(0);
+    c->width = c->table->size(1);
+    c->stream = stream_of(*c->pages);
+    return true;
+}
+// cu (None or a vector of slots + 1) and layer of a call with rows
+bool cache_call(PyObject* desc, PyObject* layer, PyObject* cu, Cache* c, int64_t* li, const int32_t** cup) {
+    if (!cache(desc, c)) return false;
+    *li = num(layer);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    if (*li < 0 || *li >= c->layers) return false;
+    *cup = nullptr;
+    if (cu == Py_None) return true;
+    const at::Tensor* t = int_vector(cu, c->slots + 1, *c->pages);
+    if (!t) return false;
+    *cup = t->data_ptr<int32_t>();
+    return true;
+}
+
+// kv4_append(cache, layer, k, v, cu or None) -> True
+PyObject* py_kv4_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(5)
+    Cache c;
+    int64_t layer;
+    const int32_t* cu;
+    const at::Tensor* k = head_rows(a[2], 0);
+    const at::Tensor* v = head_rows(a[3], 0);
+    if (!k || !v || !cache_call(a[0], a[1], a[4], &c, &layer, &cu) || k->sizes() != v->sizes() || k->size(1) != c.nk ||
+        k->size(2) != c.hd || k->scalar_type() != v->scalar_type() || k->device() != c.pages->device() ||
+        v->device() != c.pages->device())
+        Py_RETURN_NONE;
+    int32_t rc;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(c.pages->device());
+        rc = lib.kv4_append(c.layer(layer), c.ints(c.table), c.ints(c.lens), cu, c.slots, c.width, c.n_pages, k->data_ptr(),
+                            v->data_ptr(), k->size(0), k->stride(0), k->stride(1), v->stride(0), v->stride(1), c.nk, c.hd, c.pt,
+                            dtype_of(*k), c.stream);
+    }
+    if (rc) return failed("sx8_kv4_append", rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_read(cache, layer, rows, cu or None, bf16) -> (k, v)
+PyObject* py_kv4_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(5)
+    Cache c;
+    int64_t layer;
+    const int32_t* cu;
+    const int64_t rows = num(a[2]);
+    SX8_SIZES_OK()
+    if (rows < 1 || !cache_call(a[0], a[1], a[3], &c, &layer, &cu)) Py_RETURN_NONE;
+    const bool bf = a[4] == Py_True;
+    int32_t rc;
+    at::Tensor k, v;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(c.pages->device());
+        k = empty_like_device({rows, c.nk, c.hd}, bf ? at::kBFloat16 : at::kHalf, *c.pages);
+        v = empty_like_device({rows, c.nk, c.hd}, bf ? at::kBFloat16 : at::kHalf, *c.pages);
+        rc = lib.kv4_read(c.layer(layer), c.ints(c.table), c.ints(c.lens), cu, c.slots, c.width, c.n_pages, k.data_ptr(),
+                          v.data_ptr(), rows, k.stride(0), k.stride(1), v.stride(0), v.stride(1), c.nk, c.hd, c.pt, bf, c.stream);
+    }
+    if (rc) return failed("sx8_kv4_read", rc);
+    PyObject* pk = THPVariable_Wrap(std::move(k));
+    PyObject* pv = THPVariable_Wrap(std::move(v));
+    PyObject* both = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
+    Py_XDECREF(pk);
+    Py_XDECREF(pv);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_attend(cache, layer, q, cu or None, scale) -> out
+PyObject* py_kv4_attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(5)
+    Cache c;
+    int64_t layer;
+    const int32_t* cu;
+    const at::Tensor* q = head_rows(a[2], 0);
+    if (!q || !PyFloat_Check(a[4]) || !cache_call(a[0], a[1], a[3], &c, &layer, &cu) || q->size(2) != c.hd ||
+        q->device() != c.pages->device())
+        Py_RETURN_NONE;
+    const float scale = (float)PyFloat_AS_DOUBLE(a[4]);
+    int32_t rc;
+    at::Tensor o;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(c.pages->device());
+        o = empty_like_device(q->sizes(), q->scalar_type(), *q);
+        const at::Tensor ws = empty_like_device({c.ws_attend}, at::kByte, *q);
+        rc = lib.kv4_attend(c.layer(layer), c.ints(c.table), c.ints(c.lens), cu, c.slots, c.width, c.n_pages, q->data_ptr(),
+                            o.data_ptr(), q->size(0), q->stride(0), q->stride(1), o.stride(0), o.stride(1), (int32_t)q->size(1),
+                            c.nk, c.hd, c.pt, scale, dtype_of(*q), ws.data_ptr(), c.ws_attend, c.stream);
+    }
+    if (rc) return failed("sx8_kv4_attend", rc);
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_pages(cache, "reserve", add) / ("fork", src, dst) / ("free", slots) / ("compact") -> True
+PyObject* py_kv4_pages(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    Cache c;
+    if (na < 2 || na > 4 || !PyUnicode_Check(a[1]) || !cache(a[0], &c)) Py_RETURN_NONE;
+    const char* what = PyUnicode_AsUTF8(a[1]);
+    if (!what) return nullptr;
+    const at::Tensor* x = na > 2 ? int_vector(a[2], what[0] == 'r' ? c.slots : -1, *c.pages) : nullptr;
+    const at::Tensor* y = na > 3 && x ? int_vector(a[3], x->numel(), *c.pages) : nullptr;
+    if ((na > 2 && !x) || (na > 3 && !y)) Py_RETURN_NONE;
+    int32_t rc;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(c.pages->device());
+        at::Tensor ws;
+        if (std::strcmp(what, "free") != 0) ws = empty_like_device({c.ws_pages}, at::kByte, *c.pages);
+        void* const w = ws.defined() ? ws.data_ptr() : nullptr;
+        int32_t *const table = c.ints(c.table), *const lens = c.ints(c.lens), *const refs = c.ints(c.refs),
+                       *const status = c.ints(c.status);
+        if (!std::strcmp(what, "reserve") && na == 3)
+            rc = lib.kv4_reserve(table, lens, refs, c.ints(x), c.slots, c.width, c.n_pages, c.pt, status, w, c.ws_pages, c.stream);
+        else if (!std::strcmp(what, "fork") && na == 4)
+            rc = lib.kv4_fork(c.layer(0), c.layers, c.page_bytes, table, lens, refs, c.ints(x), c.ints(y), x->numel(), c.slots,
+                              c.width, c.n_pages, c.pt, status, w, c.ws_pages, c.stream);
+        else if (!std::strcmp(what, "free") && na == 3)
+            rc = lib.kv4_free(table, lens, refs, c.ints(x), x->numel(), c.slots, c.width, c.n_pages, status, c.stream);
+        else if (!std::strcmp(what, "compact") && na == 2)
+            rc = lib.kv4_compact(c.layer(0), c.layers, c.page_bytes, table, refs, c.slots, c.width, c.n_pages, w, c.ws_pages,
+                                 c.stream);
+        else
+            rc = -1;
+    }
+    if (rc == -1) Py_RETURN_NONE;
+    if (rc) return failed(("sx8_kv4_" + std::string(what)).c_str(), rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 #define SX8_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
 PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"linear", SX8_FAST(py_linear), nullptr},
@@ -411,6 +652,11 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"dequant", SX8_FAST(py_dequant), nullptr},
                          {"embed", SX8_FAST(py_embed), nullptr},
                          {"to_host", SX8_FAST(py_to_host), nullptr},
+                         {"varlen", SX8_FAST(py_varlen), nullptr},
+                         {"kv4_append", SX8_FAST(py_kv4_append), nullptr},
+                         {"kv4_read", SX8_FAST(py_kv4_read), nullptr},
+                         {"kv4_attend", SX8_FAST(py_kv4_attend), nullptr},
+                         {"kv4_pages", SX8_FAST(py_kv4_pages), nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_sx8py", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

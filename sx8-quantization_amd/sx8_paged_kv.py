@@ -76,7 +76,11 @@ def attn_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
     the device; cu_k = None: cu_q, keys and queries of the same tokens).  causal: the last query of a
     sequence attends all of its keys, the one before it one key less, and so on; a query with no key gives
     zeros.  Rows of no sequence are left as they are (in a new `out`: unset).  hd 64, 128 or 256; scale
-    1 / sqrt(hd) unless given.  Returns out (Tq, heads, hd)."""
+    1 / sqrt(hd) unless given.  Forward only.  Returns out (Tq, heads, hd)."""
+    if out is None and q.dim() == 3:
+        got = _L.py().varlen(q, k, v, cu_q, cu_k, _scale(scale, q.shape[2]), causal)
+        if got is not None:
+            return got
     if q.dim() != 3 or k.dim() != 3 or q.device.type != "cuda":
         raise RuntimeError("q, k and v must be (rows, heads, hd) tensors on the GPU")
     nh, hd, nk = q.shape[1], q.shape[2], k.shape[1]
@@ -147,13 +151,20 @@ class PagedKV4:
         _ints("table", table.view(-1), None, self.device)
         _ints("lens", lens, self.n_slots, self.device)
         _ints("refs", refs, self.n_pages, self.device)
-        self.pages, self.table, self.lens, self.refs = pages, table, lens, refs
         self.n_kv, self.head_dim, self.page_tokens, self.page_bytes = int(n_kv), int(head_dim), int(page_tokens), nb
-        self.status = torch.zeros(2, dtype=torch.int32, device=self.device)
+        status = torch.zeros(2, dtype=torch.int32, device=self.device)
         self._ws_pages = int(_L.lib().sx8_kv4_pages_workspace_bytes(self.n_slots, self.n_pages))
         if self._ws_pages < 0 or self.max_pages * self.page_tokens > 1 << 22:
             raise RuntimeError("a cache has 1..4096 slots of up to 2^22 tokens and up to 2^28 pages")
         self._ws_attend = int(_L.lib().sx8_kv4_attend_workspace_bytes(self.head_dim))
+        self._t = (pages, table, lens, refs, status, nb, self.n_kv, self.head_dim, self.page_tokens, self._ws_attend,
+                   self._ws_pages)
+
+    pages = property(lambda self: self._t[0])
+    table = property(lambda self: self._t[1])
+    lens = property(lambda self: self._t[2])
+    refs = property(lambda self: self._t[3])
+    status = property(lambda self: self._t[4])
 
     # ---------------------------------------------------------------- rows
     def _slots(self, layer, cu):
@@ -166,6 +177,8 @@ class PagedKV4:
 
     def append(self, layer, k, v, cu=None):
         """Write the new tokens' k and v rows (rows, n_kv, head_dim), fp16 or bf16, into the slots' pages."""
+        if _L.py().kv4_append(self._t, layer, k, v, cu):
+            return
         with torch.cuda.device(self.device):
             k = _rows("k", k, self.n_kv, self.head_dim, self.device)
             v = _rows("v", v, self.n_kv, self.head_dim, self.device, k.dtype)
@@ -177,10 +190,14 @@ class PagedKV4:
 
     def read(self, layer, rows, cu=None, dtype=torch.float16, out=None):
         """The values of the slots' last tokens: k and v (rows, n_kv, head_dim), packed as `append` takes them (cu of
-        all lengths reads whole slots).  out: (k, v) to write into.  Tokens without a page give zeros; rows of no token stay as
-        they are (in new tensors: unset)."""
+        all lengths reads whole slots).  out: (k, v) to write into.  Tokens without a page and rows without a token give zeros;
+        rows of no slot are left as they are (in new tensors: unset)."""
         if dtype not in _DTYPES:
             raise RuntimeError(f"dtype must be float16 or bfloat16, got {dtype}")
+        if out is None:
+            got = _L.py().kv4_read(self._t, layer, rows, cu, dtype is torch.bfloat16)
+            if got is not None:
+                return got
         with torch.cuda.device(self.device):
             like = torch.empty(int(rows), 0, 0, dtype=dtype, device=self.device)
             if out is None:
@@ -195,6 +212,10 @@ class PagedKV4:
     def attend(self, layer, q, cu=None, scale=None, out=None):
         """Attention of the new query rows q (rows, heads, head_dim), fp16 or bf16: row i of a slot's n new ones attends
         the slot's tokens 0 .. lens - n + i (zeros where that is none).  Returns out (rows, heads, head_dim)."""
+        if out is None:
+            got = _L.py().kv4_attend(self._t, layer, q, cu, _scale(scale, self.head_dim))
+            if got is not None:
+                return got
         with torch.cuda.device(self.device):
             nh = q.shape[1] if q.dim() == 3 else 0
             q = _rows("q", q, nh, self.head_dim, self.device)
@@ -212,6 +233,8 @@ class PagedKV4:
 
     def reserve(self, add):
         """Slot s grows by add[s] tokens (int32 on the device): lens, and pages for them, lowest free page first."""
+        if _L.py().kv4_pages(self._t, "reserve", add):
+            return
         with torch.cuda.device(self.device):
             _ints("add", add, self.n_slots, self.device)
             ws = self._ws()
@@ -222,6 +245,8 @@ class PagedKV4:
     def fork(self, src, dst):
         """The empty slots dst[i] become copies of the slots src[i] (int32 on the device): full pages are shared, a last
         page that is partly filled is copied."""
+        if _L.py().kv4_pages(self._t, "fork", src, dst):
+            return
         with torch.cuda.device(self.device):
             _ints("src", src, None, self.device)
             _ints("dst", dst, src.numel(), self.device)
@@ -233,6 +258,8 @@ class PagedKV4:
 
     def free(self, slots):
         """Empty the slots (int32 on the device); pages that no other slot holds are free."""
+        if _L.py().kv4_pages(self._t, "free", slots):
+            return
         with torch.cuda.device(self.device):
             _ints("slots", slots, None, self.device)
             _L.call("sx8_kv4_free", self.table.data_ptr(), self.lens.data_ptr(), self.refs.data_ptr(), slots.data_ptr(),
@@ -241,6 +268,8 @@ class PagedKV4:
 
     def compact(self):
         """Move the used pages to the front of the pool: pages 0 .. (number of used ones) - 1."""
+        if _L.py().kv4_pages(self._t, "compact"):
+            return
         with torch.cuda.device(self.device):
             ws = self._ws()
             _L.call("sx8_kv4_compact", self.pages.data_ptr(), self.n_layers, self.page_bytes, self.table.data_ptr(),

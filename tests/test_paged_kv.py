@@ -284,6 +284,13 @@ def test_attend_more_rows_than_tokens(hiplib, cuda):
     want = want_attend(q, q4(k), q4(v), [2, 40], [5, 4])
     close(got, want, F16, q4(v).abs().max().item())
     assert not got[:3].any() and got[3].any()
+    before = p.pages.clone()
+    rk, _ = p.read(0, 9, cum([5, 4], cuda), out=(torch.full_like(q, 7.0), torch.full_like(q, 7.0)))
+    assert not rk[:3].any() and torch.equal(rk[3:5], q4(k[:2]).half())
+    p.append(0, q, q, cum([40, 4], cuda)[:1].repeat(3) + ints([0, 5, 9], cuda))
+    p.append(0, k[:2], v[:2], ints([0, 2, 2], cuda))
+    p.append(0, k[-4:], v[-4:], ints([0, 0, 4], cuda))
+    assert torch.equal(p.pages, before)
 
 
 @pytest.mark.parametrize("dt", [F16, BF16])
@@ -752,6 +759,30 @@ def test_varlen_in_a_graph_and_streams(hiplib, cuda):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, attn_varlen(q, k, v, cu))
+
+
+def test_general_path_gives_the_same(hiplib, cuda, monkeypatch):
+    """Without the host module every call takes the wrappers' general path: the same results."""
+    import _sx8lib
+    from sx8_paged_kv import attn_varlen
+
+    def run():
+        p, k, v = make(cuda, [40, 0, 70], 2, 128, 32, spare=3, layers=2)
+        q = rand((3, 4, 128), 5, F16, cuda)
+        outs = [p.attend(1, q), p.attend(0, q, cum([1, 0, 2], cuda), scale=0.2), *p.read(0, 110, cum([40, 0, 70], cuda)),
+                *p.read(1, 3, dtype=BF16), attn_varlen(q, k, v, cum([1, 0, 2], cuda), cum([40, 0, 70], cuda), causal=False),
+                attn_varlen(k, k, v, cum([40, 0, 70], cuda))]
+        p.fork(ints([0], cuda), ints([1], cuda))
+        p.free(ints([2], cuda))
+        p.compact()
+        p.check()
+        return outs + [p.table, p.lens, p.refs, p.pages[:, :4]]
+
+    fast = run()
+    assert isinstance(_sx8lib.py().varlen, type(len))               # the module is there
+    monkeypatch.setattr(_sx8lib, "_py", _sx8lib._NoHostModule())
+    for a, b in zip(fast, run()):
+        assert torch.equal(a, b)
 
 
 # ------------------------------------------------------------------------------ refusals of the wrappers
