@@ -31,14 +31,32 @@ __device__ __forceinline__ int64_t block_offset(const Kv4Pool& p, int slot, int 
 // ---- append ------------------------------------------------------------------------------------
 // A work-group encodes the new rows of one block of one head, so that no word of the cache has two writers.
 // Eight lanes hold a group of 64 values (16 bytes each): minimum and maximum by three lane exchanges, then each
-// lane's eight levels.  The level is decided in binary64, where x - m is exact for fp16 rows and the quotient is put
-// right by its exact remainder, so that ties fall as the definition says.  K's eight levels of a lane are one
-// word; V's word holds eight tokens of a dimension, so V's levels meet in LDS, and a word with tokens of
-// earlier calls keeps their bits.
+// lane's eight levels.  K's eight levels of a lane are one word; V's word holds eight tokens of a dimension, so V's
+// levels meet in LDS, and a word with tokens of earlier calls keeps their bits.
 struct Enc {
     float s, m;
     uint32_t lv[8];
 };
+
+// The level of x: (x - m) / s to the nearest, ties to even.  In binary32 the quotient is within 2^-18 of the true one (two
+// roundings of a number below 32 and one of 1 / s), so only a quotient within 2^-16 of a border is decided in binary64:
+// there x - m is exact for fp16 rows, and the rounded quotient is put right by its exact remainder.  (All of them in
+// binary64: 13081 rows of 8 heads of 128, K and V, 50 us against 27.)
+__device__ __forceinline__ uint32_t level_of(float x, float m, float s, float inv) {
+#pragma clang fp contract(off)
+    const float t = (x - m) * inv;
+    float n = __builtin_rintf(t);
+    if (!(__builtin_fabsf(t - n) < 0.5f - 0x1p-16f) && t > -1.f && t < 16.f) {
+        const double d = (double)x - (double)m, s64 = s;
+        double q = __builtin_rint(d / s64);
+        const double rem = d - q * s64;
+        const bool odd = (int)q & 1;
+        if (2.0 * rem > s64 || (2.0 * rem == s64 && odd)) q += 1.0;
+        else if (-2.0 * rem > s64 || (-2.0 * rem == s64 && odd)) q -= 1.0;
+        n = (float)q;
+    }
+    return (uint32_t)(int)fminf(fmaxf(n, 0.f), 15.f);
+}
 
 // rows outside the call come as zeros (their results are unused)
 __device__ __forceinline__ void encode_group(const float (&x)[8], Enc& e) {
@@ -51,53 +69,64 @@ __device__ __forceinline__ void encode_group(const float (&x)[8], Enc& e) {
         hi = fmaxf(hi, x[i]);
         bad |= !(__builtin_fabsf(x[i]) < __builtin_inff());
     }
-    int b = bad;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, o, 8));
-        hi = fmaxf(hi, __shfl_xor(hi, o, 8));
-        b |= __shfl_xor(b, o, 8);
-    }
+    // over the eight lanes of the group; a bad one makes both ends NaN for all of them
+    if (bad) lo = hi = __builtin_inff();
+    lo = fminf(lo, dpp_lane<0xB1>(lo));
+    hi = fmaxf(hi, dpp_lane<0xB1>(hi));
+    lo = fminf(lo, dpp_lane<0x4E>(lo));
+    hi = fmaxf(hi, dpp_lane<0x4E>(hi));
+    lo = fminf(lo, dpp_lane<0x141>(lo));
+    hi = fmaxf(hi, dpp_lane<0x141>(hi));
+    const bool none = !(hi < __builtin_inff());
     const float r = hi - lo;
-    e.s = (float)(_Float16)fminf(r * (1.0f / 15.0f), 65504.0f);
-    e.m = (float)(_Float16)fminf(fmaxf(lo, -65504.0f), 65504.0f);
-    if (b) e.s = e.m = __builtin_nanf("");
-    const double s = e.s, m = e.m, inv = 1.0 / s;
+    e.s = none ? __builtin_nanf("") : (float)(_Float16)fminf(r * (1.0f / 15.0f), 65504.0f);
+    e.m = none ? __builtin_nanf("") : (float)(_Float16)fminf(fmaxf(lo, -65504.0f), 65504.0f);
+    const float inv = 1.0f / e.s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const double d = (double)x[i] - m;
-        double n = __builtin_rint(d * inv);
-        n = n < 0.0 ? 0.0 : n > 15.0 ? 15.0 : n;
-        // remainder d - n s (exact: n s has 15 bits); one step further where it is over half a step, or half and n odd
-        const double rem = d - n * s;
-        const bool odd = (int)n & 1;
-        if (n < 15.0 && (2.0 * rem > s || (2.0 * rem == s && odd))) n += 1.0;
-        else if (n > 0.0 && (-2.0 * rem > s || (-2.0 * rem == s && odd))) n -= 1.0;
-        e.lv[i] = !b && s > 0.0 ? (uint32_t)(int)n : 0u;
-    }
+    for (int i = 0; i < 8; ++i) e.lv[i] = e.s > 0.f ? level_of(x[i], e.m, e.s, inv) : 0u;
 }
 
 // The block that work item `item` of the call names: slot, its block, and the new tokens in it (block-relative
-// [t0, t1), row of token t0).  Every thread gets it; false past the last item.
+// [t0, t1), row of token t0).  Every wave finds it; false past the last item.
 struct Touched {
     int slot, block, t0, t1, row0;
 };
 __device__ __forceinline__ bool find_touched(const Kv4Pool& p, int64_t item, int64_t* pre, Touched* t) {
-    prefix_sums<256>(p.sh.n_slots, pre, [&](int s) {
-        int first, n, b;
+    const int S = p.sh.n_slots, lane = threadIdx.x & 63;
+    int first, n, len, b;
+    int64_t before;
+    auto count = [&](int s) {
         kv4_rows(p.sh, p.cu, s, &first, &n);
-        return (int64_t)kv4_touched(kv4_len(p.sh, p.lens, s), n, &b);
-    });
-    __syncthreads();
-    if (item >= pre[p.sh.n_slots]) return false;
-    t->slot = find_item<256>(p.sh.n_slots, pre, item);
-    int first, n, b;
-    kv4_rows(p.sh, p.cu, t->slot, &first, &n);
-    const int len = kv4_len(p.sh, p.lens, t->slot);
+        len = kv4_len(p.sh, p.lens, s);
+        return (int64_t)kv4_touched(len, n, &b);
+    };
+    if (!p.cu) {                            // one row a slot touches one block
+        t->slot = (int)item;
+        before = item;
+        count(t->slot);
+    } else if (S <= 64) {
+        const int64_t mine = lane < S ? count(lane) : 0, end = wave_prefix(mine);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(lane < S && end <= item);
+        t->slot = __builtin_popcountll(past);
+        if (t->slot >= S) return false;
+        before = lane_of(end - mine, t->slot);
+        first = __builtin_amdgcn_readlane(first, t->slot);
+        n = __builtin_amdgcn_readlane(n, t->slot);
+        len = __builtin_amdgcn_readlane(len, t->slot);
+    } else {
+        prefix_sums<256>(S, pre, count);
+        __syncthreads();
+        if (item >= uniform(pre[S])) return false;
+        t->slot = find_item<256>(S, pre, item);
+        before = uniform(pre[t->slot]);
+        count(t->slot);
+    }
+    first = __builtin_amdgcn_readfirstlane(first);
+    n = __builtin_amdgcn_readfirstlane(n);
+    len = __builtin_amdgcn_readfirstlane(len);
     kv4_touched(len, n, &b);
-    t->block = b + (int)(item - pre[t->slot]);
-    const int a = len - n > t->block * 32 ? len - n : t->block * 32;
-    const int e = len < t->block * 32 + 32 ? len : t->block * 32 + 32;
+    t->block = b + (int)(item - before);
+    const int a = max(len - n, t->block * 32), e = min(len, t->block * 32 + 32);
     t->t0 = a - t->block * 32;
     t->t1 = e - t->block * 32;
     t->row0 = first + a - (len - n);
@@ -114,26 +143,37 @@ extern __shared__ __align__(16) unsigned char dyn_lds[];
 
 template <int HD, bool kBf16>
 __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsIn in) {
-    constexpr int kBB = kv4_block_bytes(HD), CPR = HD / 8;
-    __shared__ uint8_t lv[32][HD + 4];
+    constexpr int kBB = kv4_block_bytes(HD), CPR = HD / 8, NI = 32 * CPR / 256;   // chunks of a row; rounds of K or V
+    __shared__ __align__(8) uint8_t lv[32][HD + 8];
     int64_t* const pre = reinterpret_cast<int64_t*>(dyn_lds);
     Touched t;
     if (!find_touched(p, blockIdx.x, pre, &t)) return;
     const int head = blockIdx.y, tid = threadIdx.x;
     const int64_t off = block_offset(p, t.slot, head, t.block, kBB);
+    const int nt = t.t1 - t.t0;
+    // every row of the block's share is requested before the first is encoded (and while the page number is on its way)
+    u32x4 raw[2][NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int ch = tid + 256 * i;
+        if (ch < nt * CPR) {
+            const int64_t row = t.row0 + ch / CPR;
+            raw[0][i] = *reinterpret_cast<const u32x4*>(in.k + row * in.k_ts + head * in.k_hs + ch % CPR * 8);
+            raw[1][i] = *reinterpret_cast<const u32x4*>(in.v + row * in.v_ts + head * in.v_hs + ch % CPR * 8);
+        }
+    }
     if (off < 0) return;                                            // (uniform)
     uint8_t* const blk = const_cast<uint8_t*>(p.pages) + off;
-    const int nt = t.t1 - t.t0;
-    for (int which = 0; which < 2; ++which) {
-        const uint16_t* src = which ? in.v : in.k;
-        const int64_t ts = which ? in.v_ts : in.k_ts, hs = which ? in.v_hs : in.k_hs;
-        // (whole groups of eight lanes run together: CPR is a multiple of 8)
-        for (int i = tid; i < nt * CPR; i += 256) {
-            const int tok = t.t0 + i / CPR, d0 = i % CPR * 8, g = d0 / kKv4Group;
-            const u32x4 w = *reinterpret_cast<const u32x4*>(src + (int64_t)(t.row0 + i / CPR) * ts + head * hs + d0);
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int ch = tid + 256 * i;
+            if (ch >= nt * CPR) break;                              // (eight lanes of a group alike: CPR is a multiple of 8)
+            const int tok = t.t0 + ch / CPR, d0 = ch % CPR * 8, g = d0 / kKv4Group;
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = ld16<kBf16>(half_of(w[e >> 1], e));
+            for (int e = 0; e < 8; ++e) x[e] = ld16<kBf16>(half_of(raw[which][i][e >> 1], e));
             Enc en;
             encode_group(x, en);
             if (which == 0) {
@@ -142,15 +182,16 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsI
                 for (int e = 0; e < 8; ++e) word |= en.lv[e] << kv4_shift(e);
                 *reinterpret_cast<uint32_t*>(blk + kv4_k_word(HD, tok, d0)) = word;
             } else {
+                u32x2 bytes = {0u, 0u};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) lv[tok][d0 + e] = (uint8_t)en.lv[e];
+                for (int e = 0; e < 8; ++e) bytes[e >> 2] |= en.lv[e] << 8 * (e & 3);
+                *reinterpret_cast<u32x2*>(&lv[tok][d0]) = bytes;
             }
-            if (i % 8 == 0) {
+            if (tid % 8 == 0) {
                 *reinterpret_cast<uint16_t*>(blk + kv4_param(HD, 2 * which, tok, g)) = (uint16_t)st16<false>(en.s);
                 *reinterpret_cast<uint16_t*>(blk + kv4_param(HD, 2 * which + 1, tok, g)) = (uint16_t)st16<false>(en.m);
             }
         }
-    }
     __syncthreads();
     for (int i = tid; i < HD * 4; i += 256) {
         const int d = i % HD, h = i / HD;                           // word: tokens 4 h + r and 16 + 4 h + r
@@ -170,7 +211,8 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsI
 }
 
 // ---- read --------------------------------------------------------------------------------------
-// The same cut: a work-group takes one block of one head into LDS (coalesced) and writes its new tokens' rows.
+// The same cut: a work-group takes one block of one head into LDS (coalesced) and writes its new tokens' rows, K by
+// words (eight dimensions of a token), V by four words side by side (eight tokens of four dimensions).
 struct RowsOut {
     uint16_t* k;
     uint16_t* v;
@@ -190,24 +232,36 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
         reinterpret_cast<u32x4*>(blk)[i] = off < 0 ? u32x4{0u, 0u, 0u, 0u} : reinterpret_cast<const u32x4*>(p.pages + off)[i];
     __syncthreads();
     const int nt = t.t1 - t.t0;
-    for (int i = tid; i < 2 * nt * CPR; i += 256) {
-        const int which = i >= nt * CPR, j = i - which * nt * CPR;
-        const int tok = t.t0 + j / CPR, d0 = j % CPR * 8, g = d0 / kKv4Group;
-        const float s = sx8_h2f(*reinterpret_cast<const uint16_t*>(blk + kv4_param(HD, 2 * which, tok, g)));
-        const float m = sx8_h2f(*reinterpret_cast<const uint16_t*>(blk + kv4_param(HD, 2 * which + 1, tok, g)));
-        const uint32_t kw = *reinterpret_cast<const uint32_t*>(blk + kv4_k_word(HD, tok, d0));
+    auto value = [](uint32_t level, float s, float m) { return __builtin_fmaf((float)(int)level, s, m); };
+    for (int i = tid; i < nt * CPR; i += 256) {
+        const int tok = t.t0 + i / CPR, d0 = i % CPR * 8, g = d0 / kKv4Group;
+        const float s = sx8_h2f(*reinterpret_cast<const uint16_t*>(blk + kv4_param(HD, 0, tok, g)));
+        const float m = sx8_h2f(*reinterpret_cast<const uint16_t*>(blk + kv4_param(HD, 1, tok, g)));
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(blk + kv4_k_word(HD, tok, d0));
         u32x4 w;
 #pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = pack16<kBf16>(value(word >> kv4_shift(2 * e) & 15u, s, m), value(word >> kv4_shift(2 * e + 1) & 15u, s, m));
+        *reinterpret_cast<u32x4*>(out.k + (int64_t)(t.row0 + i / CPR) * out.k_ts + head * out.k_hs + d0) = w;
+    }
+    for (int i = tid; i < HD; i += 256) {
+        const int h = i / (HD / 4), d0 = i % (HD / 4) * 4, g = d0 / kKv4Group;
+        uint32_t words[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) words[e] = *reinterpret_cast<const uint32_t*>(blk + kv4_v_word(HD, 4 * h, d0 + e));
+        const u32x4 s8 = *reinterpret_cast<const u32x4*>(blk + kv4_param(HD, 2, 4 * h, g));
+        const u32x4 m8 = *reinterpret_cast<const u32x4*>(blk + kv4_param(HD, 3, 4 * h, g));
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t vw = *reinterpret_cast<const uint32_t*>(blk + kv4_v_word(HD, tok, d0 + e));
-            const uint32_t l = which ? (vw >> kv4_v_shift(tok)) & 15u : (kw >> kv4_shift(e)) & 15u;
-            const uint32_t b = st16<kBf16>(__builtin_fmaf((float)(int)l, s, m));
-            if (e & 1) w[e >> 1] |= b << 16;
-            else w[e >> 1] = b;
+            const int tok = e / 4 * 16 + 4 * h + e % 4;
+            if (tok < t.t0 || tok >= t.t1) continue;
+            const float s = sx8_h2f(half_of(s8[e >> 1], e)), m = sx8_h2f(half_of(m8[e >> 1], e));
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = value(words[k] >> kv4_shift(e) & 15u, s, m);
+            *reinterpret_cast<u32x2*>(out.v + (int64_t)(t.row0 + tok - t.t0) * out.v_ts + head * out.v_hs + d0) =
+                u32x2{pack16<kBf16>(x[0], x[1]), pack16<kBf16>(x[2], x[3])};
         }
-        uint16_t* const dst = which ? out.v + (int64_t)(t.row0 + j / CPR) * out.v_ts + head * out.v_hs
-                                    : out.k + (int64_t)(t.row0 + j / CPR) * out.k_ts + head * out.k_hs;
-        *reinterpret_cast<u32x4*>(dst + d0) = w;
     }
 }
 
@@ -769,8 +823,8 @@ extern "C" int32_t sx8_kv4_append(uint8_t* pages, const int32_t* table, const in
     const RowsIn in{(const uint16_t*)k, (const uint16_t*)v, k_ts, k_hs, v_ts, v_hs};
     const dim3 grid((unsigned)kv4_touched_most(n_slots, rows, cu != nullptr), (unsigned)nk);
     by_kind(hd, dtype, [&](auto d, auto b) {
-        hipLaunchKernelGGL((k_kv4_append<decltype(d)::value, decltype(b)::value>), grid, dim3(256), prefix_bytes(p),
-                           as_stream(stream), p, in);
+        hipLaunchKernelGGL((k_kv4_append<decltype(d)::value, decltype(b)::value>), grid, dim3(256),
+                           cu && n_slots > 64 ? prefix_bytes(p) : 0, as_stream(stream), p, in);
     });
     return check_launch(what);
 }
@@ -790,8 +844,8 @@ extern "C" int32_t sx8_kv4_read(const uint8_t* pages, const int32_t* table, cons
     const RowsOut out{(uint16_t*)k, (uint16_t*)v, k_ts, k_hs, v_ts, v_hs};
     const dim3 grid((unsigned)kv4_touched_most(n_slots, rows, cu != nullptr), (unsigned)nk);
     by_kind(hd, dtype, [&](auto d, auto b) {
-        hipLaunchKernelGGL((k_kv4_read<decltype(d)::value, decltype(b)::value>), grid, dim3(256), prefix_bytes(p),
-                           as_stream(stream), p, out);
+        hipLaunchKernelGGL((k_kv4_read<decltype(d)::value, decltype(b)::value>), grid, dim3(256),
+                           cu && n_slots > 64 ? prefix_bytes(p) : 0, as_stream(stream), p, out);
     });
     return check_launch(what);
 }

@@ -43,6 +43,11 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
                      (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
 }
 
+template <int kCtrl>
+__device__ __forceinline__ float dpp_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xF, 0xF, false));
+}
+
 // Sum of v over the lanes up to this one: shifts within rows of 16 lanes, then each row's last lane to the rows above.
 template <int kCtrl, int kRows>
 __device__ __forceinline__ int64_t add_dpp(int64_t v) {
