@@ -23,6 +23,7 @@ import torch
 import torch.nn as nn
 
 import _sx8lib as _L
+from sx8_paged_kv import PagedKV4, attn_varlen
 from integrate_fused_v44 import SX8LinearV44
 from prepare_v44 import to_v44_device
 from quantize_sx8 import quantize_tensor
@@ -172,8 +173,11 @@ class SX8Decoder(nn.Module):
     def _prefill_bufs(self, T):
         """Activation buffers of prefill_fused for T tokens (built once per T)."""
         pb = getattr(self, "_pb", None)
-        if pb is not None and pb["T"] == T:
-            return pb
+        if pb is None or pb["T"] != T:
+            self._pb = pb = self._make_bufs(T)
+        return pb
+
+    def _make_bufs(self, T):
         cfg, dev = self.cfg, self.device
         H, nh, nk, hd, I = cfg["hidden"], cfg["n_heads"], cfg["n_kv"], cfg["head_dim"], cfg["inter"]
         f32 = dict(dtype=torch.float32, device=dev)
@@ -212,7 +216,6 @@ class SX8Decoder(nn.Module):
                          self._group_args((ly.gate, ly.up), ()),         # (no float32 outputs)
                          self._group_args((ly.o,), (pb["o"],)),
                          self._group_args((ly.down,), (pb["d"],))) for ly in self.layers]
-        self._pb = pb
         return pb
 
     @staticmethod
@@ -539,3 +542,209 @@ class SX8Decoder(nn.Module):
         if lg is not None:
             return out, t_prefill, t_decode, lg
         return out, t_prefill, t_decode
+
+    @torch.no_grad()
+    def generate_batch(self, prompts, n_new, prefix=None, page_tokens=64, use_graph=True):
+        """Greedy generation of several sequences at once over a paged 4-bit KV cache (PagedDecoder): prompts, a
+        list of (T_i,) int64 tensors, with `prefix` (T,) in front of each of them, which is run once and whose
+        pages the sequences share.  Returns (len(prompts), n_new) int64 tokens on the device."""
+        n = len(prompts)
+        first = 0 if prefix is None else prefix.shape[0]
+        longest = first + max(p.shape[0] for p in prompts) + n_new
+        pd = PagedDecoder(self, n + (prefix is not None), longest, page_tokens=page_tokens)
+        if prefix is not None:
+            pd.prompt([n], [prefix])
+            pd.fork([n] * n, list(range(n)))
+            pd.free([n])
+        out = torch.empty(n, n_new, dtype=torch.int64, device=self.device)
+        out[:, 0] = pd.prompt(list(range(n)), prompts)
+        for i in range(1, n_new):
+            out[:, i] = pd.step(use_graph)[:n]
+        pd.cache.check()
+        return out
+
+
+class PagedDecoder:
+    """Several sequences of one SX8Decoder, each in a slot of a paged 4-bit KV cache (sx8_paged_kv).
+
+    ``prompt`` runs the prompts of any slots as one packed pass (a slot that has tokens already goes on from them),
+    ``step`` decodes one token of every slot in use, replayed from a HIP graph; ``fork``, ``free`` and ``compact`` are the
+    cache's.  Linears, norms and RoPE are the kernels of prefill_fused with one row per new token; K and V rows go
+    into the pages as they leave RoPE.  New prompts attend their own fp16 rows (attn_varlen); rows with
+    earlier tokens, and every decoded token, attend the pages (PagedKV4.attend).  The reference serves one sequence
+    (scripts/infer_sx8.py:109-173)."""
+
+    def __init__(self, dec, n_slots, max_len=None, n_pages=None, page_tokens=64):
+        cfg = dec.cfg
+        self.dec, self.n_slots = dec, n_slots
+        self.max_len = dec.max_len if max_len is None else max_len
+        if self.max_len > dec.max_len:
+            raise ValueError(f"max_len {self.max_len} exceeds the decoder's {dec.max_len}")
+        width = -(-self.max_len // page_tokens)
+        self.cache = PagedKV4(cfg["n_layers"], cfg["n_kv"], cfg["head_dim"], n_pages or n_slots * width, n_slots, width,
+                              page_tokens, device=dec.device)
+        self.lens = [0] * n_slots                                   # as cache.lens, known without asking the device
+        self.tok = torch.zeros(n_slots, dtype=torch.int64, device=dec.device)
+        self.active = torch.zeros(n_slots, dtype=torch.int32, device=dec.device)
+        self.logits = None                                          # of the last prompt or step
+        self._pb, self._graph = {}, None
+
+    def _ints(self, xs):
+        return torch.tensor(list(xs), dtype=torch.int32, device=self.dec.device)
+
+    def _set_active(self):
+        self.active.copy_(self._ints(int(n > 0) for n in self.lens))
+
+    def _rows(self, pb, ids, pos, attend):
+        """The layers over T packed rows at positions `pos`; attend(layer, q, k, v) -> (T, heads, hd).  The residual
+        stream of the rows is left in pb["resid"] + pb["d"]."""
+        d = self.dec
+        cfg, P = d.cfg, _L.ptr
+        H, nh, nk, hd, eps, T = cfg["hidden"], cfg["n_heads"], cfg["n_kv"], cfg["head_dim"], cfg["eps"], pb["T"]
+        st = _L.stream(d.device)
+        emb = d.embed(ids)
+        # RoPE and its K/V rows as a prompt's at position 0 of a table and a cache of T rows
+        cos, sin = d.cos.index_select(0, pos), d.sin.index_select(0, pos)
+        pend, last = (None, 0, 0), len(d.layers) - 1
+        for li, ly in enumerate(d.layers):
+            g_qkv, g_mlp, g_o, g_down = pb["groups"][li]
+            d._norm_packed(pb, g_qkv, pb["resid"], None if li == 0 else pb["d"], emb if li == 0 else None, ly.in_norm, pend,
+                           eps, st)
+            qp = d._gemm_packed(g_qkv, pb["xn"], pb["zn"], T, H, pb["ws"], st)
+            _L.call("sx8_dec_qk_rope_cache_rows_parts", P(pb["q"]), P(pb["k"]), P(pb["v"]), P(ly.q_norm), P(ly.k_norm),
+                    P(cos), P(sin), P(pb["pos0"]), T, P(pb["qh"]), P(pb["kr"]), P(pb["vr"]), nh, nk, hd, T, eps, qp[0],
+                    qp[1], qp[2], st)
+            a = attend(li, pb["qh"], pb["kr"].permute(1, 0, 2), pb["vr"].permute(1, 0, 2))
+            op = d._gemm_group_deferred(g_o, a.view(T, nh * hd), pb["ws"], st)
+            d._norm_packed(pb, g_mlp, pb["resid"], pb["o"], None, ly.post_norm, op, eps, st)
+            _, hdrs, lvls, bas, sca, _, gcb, _ = g_mlp
+            _, _, dbas, dsca = ly.down._t44
+            _L.call("sx8_dec_gemm_gateup_silu", None, P(pb["xn"]),
+                    (ctypes.c_void_p * 2)(*[z.data_ptr() for z in pb["zn"][:2]]), T, H, hdrs, lvls, 6, bas, sca,
+                    cfg["inter"], gcb, P(dbas), P(dsca), P(pb["xpd"]), P(pb["zhld"]), P(pb["ws"]), pb["ws"].numel(), st)
+            pend = d._gemm_packed(g_down, pb["xpd"], [pb["zhld"]], T, cfg["inter"], pb["ws"], st, defer=li < last)
+
+    def _bufs(self, T):
+        """Activation buffers for T rows: those of the step are kept, a prompt's replace the last prompt's."""
+        pb = self._pb.get(T)
+        if pb is None:
+            cfg = self.dec.cfg
+            pb = self.dec._make_bufs(T)
+            for name in ("kr", "vr"):
+                pb[name] = torch.empty(cfg["n_kv"], T, cfg["head_dim"], dtype=torch.float16, device=self.dec.device)
+            self._pb = {t: b for t, b in self._pb.items() if t == self.n_slots}
+            self._pb[T] = pb
+        return pb
+
+    def _head(self, resid, delta, M):
+        """Logits of M rows: final norm of resid + delta and the lm_head."""
+        d = self.dec
+        st, V = _L.stream(d.device), d.cfg["vocab"]
+        h = torch.empty(M, d.cfg["hidden"], dtype=torch.float16, device=d.device)
+        _L.call("sx8_dec_add_rmsnorm", _L.ptr(resid), _L.ptr(delta), None, _L.ptr(d.final_norm), _L.ptr(h), M,
+                d.cfg["hidden"], d.cfg["eps"], st)
+        logits = torch.empty(M, V, dtype=torch.float32, device=d.device)
+        ws, _ = _L.gemm_workspace(M, (V,), d.head.qt["n_cb"], d.device)
+        d._gemm(d.head, h, logits, ws, st)
+        return logits
+
+    @torch.no_grad()
+    def prompt(self, slots, prompts):
+        """Append `prompts` (a list of int64 token vectors) to the slots and return the next token of each (len(slots),)."""
+        by = {}
+        for s, p in zip(slots, prompts):
+            if not 0 <= s < self.n_slots or s in by or p.numel() == 0 or self.lens[s] + p.numel() > self.max_len:
+                raise ValueError(f"slot {s}: out of range, named twice, an empty prompt or past {self.max_len} tokens")
+            by[s] = p.to(self.dec.device)
+        if not by or len(slots) != len(prompts):
+            raise ValueError("as many slots as prompts, and at least one")
+        order = sorted(by)
+        ids = torch.cat([by[s] for s in order])
+        pos = torch.cat([torch.arange(self.lens[s], self.lens[s] + by[s].numel(), device=self.dec.device) for s in order])
+        new = [by[s].numel() if s in by else 0 for s in range(self.n_slots)]
+        cu = self._ints([0] + [sum(new[:i + 1]) for i in range(self.n_slots)])
+        self.cache.reserve(self._ints(new))
+        self.cache.check()
+        fresh = all(self.lens[s] == 0 for s in by)
+        scale = 1.0 / math.sqrt(self.dec.cfg["head_dim"])
+
+        def attend(li, q, k, v):
+            self.cache.append(li, k, v, cu)
+            return attn_varlen(q, k, v, cu, scale=scale) if fresh else self.cache.attend(li, q, cu, scale)
+
+        pb = self._bufs(ids.numel())
+        self._rows(pb, ids, pos, attend)
+        for s in by:
+            self.lens[s] += new[s]
+        self._set_active()
+        ends = torch.tensor([int(sum(new[:s + 1])) - 1 for s in order], device=self.dec.device)
+        self.logits = self._head(pb["resid"].index_select(0, ends), pb["d"].index_select(0, ends), len(order))
+        nxt = self.logits.argmax(-1)
+        self.tok[torch.tensor(order, device=self.dec.device)] = nxt
+        return nxt[torch.tensor([order.index(s) for s in slots], device=self.dec.device)]
+
+    def _step(self):
+        self.cache.reserve(self.active)
+        pos = (self.cache.lens.long() - 1).clamp_(min=0)
+        pb = self._bufs(self.n_slots)
+        scale = 1.0 / math.sqrt(self.dec.cfg["head_dim"])
+
+        def attend(li, q, k, v):
+            self.cache.append(li, k, v)
+            return self.cache.attend(li, q, None, scale)
+
+        self._rows(pb, self.tok, pos, attend)
+        return self._head(pb["resid"], pb["d"], self.n_slots)
+
+    @torch.no_grad()
+    def step(self, use_graph=True):
+        """Decode one token of every slot in use: returns the next tokens (n_slots,), kept as the step's input of the
+        next call (slots not in use: meaningless)."""
+        if any(n >= self.max_len for n in self.lens):
+            raise ValueError(f"a slot is full ({self.max_len} tokens)")
+        if use_graph and self._graph is None:
+            # warm-up on a side stream, then the step is captured; the cache and the token are put back between
+            state = [t.clone() for t in (self.cache.table, self.cache.lens, self.cache.refs, self.cache.status)]
+            side = torch.cuda.Stream(self.dec.device)
+            side.wait_stream(torch.cuda.current_stream(self.dec.device))
+            with torch.cuda.stream(side):
+                self._step()
+            torch.cuda.current_stream(self.dec.device).wait_stream(side)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                logits = self._step()
+            for t, was in zip((self.cache.table, self.cache.lens, self.cache.refs, self.cache.status), state):
+                t.copy_(was)
+            self._graph = (g, logits)
+        if use_graph:
+            self._graph[0].replay()
+            self.logits = self._graph[1]
+        else:
+            self.logits = self._step()
+        self.lens = [n + (n > 0) for n in self.lens]
+        self.tok.copy_(self.logits.argmax(-1))
+        return self.tok.clone()
+
+    def fork(self, src, dst):
+        """The empty slots dst[i] go on from where the slots src[i] are."""
+        if len(src) != len(dst) or len(set(dst)) != len(dst) or any(self.lens[b] or not self.lens[a] for a, b in zip(src, dst)):
+            raise ValueError("fork: as many used sources as empty, distinct targets")
+        self.cache.fork(self._ints(src), self._ints(dst))
+        self.cache.check()
+        self.tok[torch.tensor(dst, device=self.tok.device)] = self.tok[torch.tensor(src, device=self.tok.device)]
+        for a, b in zip(src, dst):
+            self.lens[b] = self.lens[a]
+        self._set_active()
+
+    def free(self, slots):
+        """Empty the slots; pages that no other slot shares are free again."""
+        if any(not 0 <= s < self.n_slots for s in slots):
+            raise ValueError(f"free: slots are 0..{self.n_slots - 1}")
+        self.cache.free(self._ints(slots))
+        for s in slots:
+            self.lens[s] = 0
+        self._set_active()
+
+    def compact(self):
+        """Move the used pages to the front of the pool (a pool that is to be saved or cut)."""
+        self.cache.compact()
