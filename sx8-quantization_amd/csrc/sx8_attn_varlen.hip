@@ -98,6 +98,41 @@ constexpr int var_lds_bytes() {
     return a > b ? a : (b + 15) / 16 * 16;
 }
 
+// A wave's rows key by key, without products of a zero probability: for the rows beside a value that is no finite number
+// (about 1 us a key).  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
+template <int HD, bool kBf16, typename V, int NT>
+__device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, const uint16_t* v, const VarIo& io,
+                                                    int see, int lim, int h, V (&o)[NT], float& l) {
+    float m = -__builtin_inff();
+    l = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n] = 0.f;
+    for (int key = 0; key < see; ++key) {
+        float s = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
+                s = __builtin_fmaf(ld16<kBf16>(q[d]), ld16<kBf16>(k[key * io.k_ts + d]), s);
+            }
+        s = (s + __shfl_xor(s, 32, 64)) * io.scale_log2;
+        if (key > lim) continue;
+        const float mn = fmaxf(m, s), alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float p = __builtin_amdgcn_exp2f(mn == -__builtin_inff() ? s : s - mn);
+        m = mn;
+        l = l * alpha + p;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float x = ld16<kBf16>(v[key * io.v_ts + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3)]);
+                o[n][r] = o[n][r] * alpha;
+                if (p != 0.f) o[n][r] = __builtin_fmaf(p, x, o[n][r]);
+            }
+    }
+}
+
 template <int HD, bool kBf16, bool kCausal>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const VarIo io) {
     typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -176,9 +211,23 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     float m = -kInf, l = 0.f;
     // V^T reads: key and dimension that the lane names
     const int vi = lane & 15, vd = (lane >> 4 & 1) * 16 + 4 * (vi & 3), vk = 4 * h + (vi >> 2);
+    bool odd = false;
     auto tile = [&](int j, int buf, bool mask) __attribute__((always_inline)) {
         const unsigned char* kt = var_lds + buf * 2 * T::kBytes;
         const unsigned char* vt = kt + T::kBytes;
+        if (mask) {
+            // A key that some row may not attend has probability zero there, and 0 * NaN must not reach the row: a tile with
+            // values that are no finite numbers (an exponent of all ones) leaves the wave's rows to slow_rows.
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int i = 0; i < T::kBytes / 1024; ++i) {
+                const u32x4 x = reinterpret_cast<const u32x4*>(vt)[i * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) any |= (x[e] & M::kExp) + M::kOne;
+            }
+            odd = __builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0) != 0;
+            if (odd) return;
+        }
         f32x16 s[NB];
 #pragma unroll
         for (int a = 0; a < NB; ++a) {
@@ -192,6 +241,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
             }
         }
         if (mask) {
+            asm volatile("");                    // (a branch: as selects these would run for every tile)
 #pragma unroll
             for (int a = 0; a < NB; ++a)
 #pragma unroll
@@ -224,40 +274,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
                 s[a][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][r], io.scale_log2, nm));
                 l += s[a][r];
             }
-        if (mask) {
-            // A key that some row may not attend has probability zero there, and 0 * NaN must not reach the row.  So a tile
-            // with values that are no finite numbers (an exponent of all ones) is added up here, by the rows that give
-            // them weight; it costs such a tile some 30 us, and the others one look at their values.
-            uint32_t odd = 0;
-#pragma unroll 4
-            for (int i = 0; i < T::kBytes / 1024; ++i) {
-                const u32x4 x = reinterpret_cast<const u32x4*>(vt)[i * 64 + lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd |= (x[e] & M::kExp) + M::kOne;
-            }
-            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) != 0) {
-                for (int key = 0; key < KB; ++key) {
-                    float p = 0.f;
-                    // the probability of the key: lane half (key >> 2) & 1, accumulator 4 (key % 32 / 8) + key % 4
-#pragma unroll
-                    for (int a = 0; a < NB; ++a)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (key >> 5 == a && (key & 31) >> 3 == r >> 2 && (key & 3) == (r & 3)) p = s[a][r];
-                    p = ld16<kBf16>(st16<kBf16>(__shfl(p, c + 32 * (key >> 2 & 1), 64)));
-                    if (p == 0.f) continue;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int d = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-                            o[n][r] = __builtin_fmaf(p, ld16<kBf16>(*reinterpret_cast<const uint16_t*>(
-                                vt + key * (HD * 2) + 16 * ((d / 8) ^ T::v_swz(key)) + 2 * (d % 8))), o[n][r]);
-                        }
-                }
-                return;
-            }
-        }
 #pragma unroll
         for (int st = 0; st < KB / 16; ++st) {
             u32x4 pf;
@@ -287,10 +303,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
         __syncthreads();                          // tile j is there, and nobody reads the other buffer any more
         if (j + 1 < n_tiles) fetch(j + 1, (j + 1) & 1);
         const int k0 = j * KB;
-        if (k0 < w_see) tile(j, j & 1, k0 + KB > w_all);
+        if (k0 < w_see && !odd) tile(j, j & 1, k0 + KB > w_all);
     }
-    if (!row_ok) return;
     l += __shfl_xor(l, 32, 64);
+    if (odd) slow_rows<HD, kBf16>(io.q + ((int64_t)q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs, kp, vp, io,
+                                  w_see, lim, h, o, l);
+    if (!row_ok) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint16_t* const dst = io.out + ((int64_t)q_first + q0 + c) * io.o_ts + head * io.o_hs + 4 * h;
 #pragma unroll
