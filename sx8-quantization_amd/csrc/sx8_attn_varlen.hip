@@ -79,7 +79,6 @@ struct Mma<false> {
     __device__ static A mul(u32x4 a, u32x4 b, A c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
     }
-    static constexpr uint32_t kExp = 0x7C007C00u, kOne = 0x04000400u;      // exponent bits, their lowest
 };
 template <>
 struct Mma<true> {
@@ -88,7 +87,6 @@ struct Mma<true> {
     __device__ static A mul(u32x4 a, u32x4 b, A c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
     }
-    static constexpr uint32_t kExp = 0x7F807F80u, kOne = 0x00800080u;
 };
 
 // K and V of two tiles, and before that the prefix sums of the sequences' tiles
@@ -98,8 +96,8 @@ constexpr int var_lds_bytes() {
     return a > b ? a : (b + 15) / 16 * 16;
 }
 
-// A wave's rows key by key, without products of a zero probability: for the rows beside a value that is no finite number
-// (about 1 us a key).  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
+// A wave's rows key by key, without products of a zero probability: for rows in whose sums there is a value that is no
+// finite number (about 1 us a key).  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
 template <int HD, bool kBf16, typename V, int NT>
 __device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, const uint16_t* v, const VarIo& io,
                                                     int see, int lim, int h, V (&o)[NT], float& l) {
@@ -143,28 +141,54 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     __shared__ __align__(16) unsigned char var_lds[var_lds_bytes<HD>()];
-    int64_t* const pre = reinterpret_cast<int64_t*>(var_lds);
-    // the tile of queries: the last ones of a sequence, which see the most keys, come first; consecutive work-groups (of
-    // different XCDs) take different KV heads, so that the query heads of one share its XCD's L2
-    prefix_sums<256>(io.n_seq, pre, [&](int b) {
-        int f, n;
-        seq_rows(io.cu_q, io.Tq, b, &f, &n);
-        return ((int64_t)n + kRows - 1) / kRows;
-    });
-    __syncthreads();
-    const int item = (int)uniform(pre[io.n_seq]) - 1 - (int)(blockIdx.x / io.nh);
-    if (item < 0) return;
-    const int hh = blockIdx.x % io.nh, G = io.nh / io.nk, kvh = hh % io.nk, head = kvh * G + hh / io.nk;
-    const int b = find_item<256>(io.n_seq, pre, item);
-    int q_first, nq, k_first, nkeys;
-    seq_rows(io.cu_q, io.Tq, b, &q_first, &nq);
-    seq_rows(io.cu_k, io.Tk, b, &k_first, &nkeys);
-    q_first = __builtin_amdgcn_readfirstlane(q_first);
-    nq = __builtin_amdgcn_readfirstlane(nq);
-    k_first = __builtin_amdgcn_readfirstlane(k_first);
-    nkeys = __builtin_amdgcn_readfirstlane(nkeys);
-    const int wg_q0 = (item - (int)uniform(pre[b])) * kRows, q0 = wg_q0 + 32 * w;   // first rows in the sequence
-    __syncthreads();                                                     // (pre makes room for the first tile)
+    // The tile of queries.  Tiles that see the most keys come first: with up to 64 sequences the tiles of all of them by
+    // their place in the sequence, from the back, with more each sequence's own from the back.  Consecutive work-groups (of
+    // different XCDs) take different KV heads, so that the query heads of one share its XCD's L2.
+    const int item = (int)(blockIdx.x / io.nh), hh = blockIdx.x % io.nh, G = io.nh / io.nk, kvh = hh % io.nk;
+    const int head = kvh * G + hh / io.nk;
+    int q_first = 0, nq = 0, k_first = 0, nkeys = 0, t;
+    if (io.n_seq <= 64) {
+        if (lane < io.n_seq) {
+            seq_rows(io.cu_q, io.Tq, lane, &q_first, &nq);
+            seq_rows(io.cu_k, io.Tk, lane, &k_first, &nkeys);
+        }
+        const int tiles = nq > 0 ? (nq - 1) / kRows + 1 : 0;
+        // tiles at place t of their sequence or behind it, over all sequences: the places from the back hold items 0, 1, ...
+        auto from = [&](int place) { return wave_sum(max(tiles - place, 0)); };
+        if (item >= from(0)) return;
+        t = 0;                                   // the last place whose tiles end behind the item
+        int step = 1;
+        while (from(step) > item) step *= 2;
+        for (step /= 2; step > 0; step /= 2)
+            if (from(t + step) > item) t += step;
+        uint64_t have = __builtin_amdgcn_ballot_w64(tiles > t);
+        for (int skip = item - from(t + 1); skip > 0; --skip) have &= have - 1;
+        const int b = __builtin_ctzll(have);
+        q_first = __builtin_amdgcn_readlane(q_first, b);
+        nq = __builtin_amdgcn_readlane(nq, b);
+        k_first = __builtin_amdgcn_readlane(k_first, b);
+        nkeys = __builtin_amdgcn_readlane(nkeys, b);
+    } else {
+        int64_t* const pre = reinterpret_cast<int64_t*>(var_lds);
+        prefix_sums<256>(io.n_seq, pre, [&](int b) {
+            int f, n;
+            seq_rows(io.cu_q, io.Tq, b, &f, &n);
+            return ((int64_t)n + kRows - 1) / kRows;
+        });
+        __syncthreads();
+        const int at = (int)uniform(pre[io.n_seq]) - 1 - item;
+        if (at < 0) return;
+        const int b = find_item<256>(io.n_seq, pre, at);
+        t = at - (int)uniform(pre[b]);
+        seq_rows(io.cu_q, io.Tq, b, &q_first, &nq);
+        seq_rows(io.cu_k, io.Tk, b, &k_first, &nkeys);
+        q_first = __builtin_amdgcn_readfirstlane(q_first);
+        nq = __builtin_amdgcn_readfirstlane(nq);
+        k_first = __builtin_amdgcn_readfirstlane(k_first);
+        nkeys = __builtin_amdgcn_readfirstlane(nkeys);
+        __syncthreads();                         // (pre makes room for the first tile)
+    }
+    const int wg_q0 = t * kRows, q0 = wg_q0 + 32 * w;                    // first rows in the sequence
     const int past = nkeys - nq;                                         // row i attends keys 0 .. past + i
     const int wg_last = min(nq - wg_q0, kRows) - 1 + wg_q0;
     const int see = kCausal ? max(past + wg_last + 1, 0) : nkeys;        // keys of the work-group
@@ -211,23 +235,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     float m = -kInf, l = 0.f;
     // V^T reads: key and dimension that the lane names
     const int vi = lane & 15, vd = (lane >> 4 & 1) * 16 + 4 * (vi & 3), vk = 4 * h + (vi >> 2);
-    bool odd = false;
     auto tile = [&](int j, int buf, bool mask) __attribute__((always_inline)) {
         const unsigned char* kt = var_lds + buf * 2 * T::kBytes;
         const unsigned char* vt = kt + T::kBytes;
-        if (mask) {
-            // A key that some row may not attend has probability zero there, and 0 * NaN must not reach the row: a tile with
-            // values that are no finite numbers (an exponent of all ones) leaves the wave's rows to slow_rows.
-            uint32_t any = 0;
-#pragma unroll 4
-            for (int i = 0; i < T::kBytes / 1024; ++i) {
-                const u32x4 x = reinterpret_cast<const u32x4*>(vt)[i * 64 + lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) any |= (x[e] & M::kExp) + M::kOne;
-            }
-            odd = __builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0) != 0;
-            if (odd) return;
-        }
         f32x16 s[NB];
 #pragma unroll
         for (int a = 0; a < NB; ++a) {
@@ -303,11 +313,19 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
         __syncthreads();                          // tile j is there, and nobody reads the other buffer any more
         if (j + 1 < n_tiles) fetch(j + 1, (j + 1) & 1);
         const int k0 = j * KB;
-        if (k0 < w_see && !odd) tile(j, j & 1, k0 + KB > w_all);
+        if (k0 < w_see) tile(j, j & 1, k0 + KB > w_all);
     }
     l += __shfl_xor(l, 32, 64);
-    if (odd) slow_rows<HD, kBf16>(io.q + ((int64_t)q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs, kp, vp, io,
-                                  w_see, lim, h, o, l);
+    // A key that a row may not attend has probability zero there, and 0 * NaN or 0 * infinity must not reach the row:
+    // where a sum is no finite number, the wave's rows are computed again by what they attend alone.
+    float odd = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(0.f, o[n][r], odd);
+    if (__builtin_amdgcn_ballot_w64(odd != 0.f) != 0)
+        slow_rows<HD, kBf16>(io.q + ((int64_t)q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs, kp, vp, io, w_see, lim,
+                              h, o, l);
     if (!row_ok) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint16_t* const dst = io.out + ((int64_t)q_first + q0 + c) * io.o_ts + head * io.o_hs + 4 * h;

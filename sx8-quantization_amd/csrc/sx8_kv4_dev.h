@@ -64,6 +64,17 @@ __device__ __forceinline__ int64_t wave_prefix(int64_t v) {
     return add_dpp<0x143, 0xC>(v);                   // row_bcast 31 into rows 2 and 3
 }
 
+// Sum of v over the wave, in a scalar register.
+__device__ __forceinline__ int wave_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 // Prefix sums of f(s) over n items into pre[0 .. n] (LDS), every thread of the work-group (kT threads) taking part.
 template <int kT, typename P, typename F>
 __device__ __forceinline__ void prefix_sums(int n, P* pre, F&& f) {
