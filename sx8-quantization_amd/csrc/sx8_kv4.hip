@@ -320,6 +320,27 @@ __device__ __forceinline__ f16x8 levels(uint32_t w) {
     const u32x4 v = {w & 0x000F000Fu, (w >> 4) & 0x000F000Fu, (w >> 8) & 0x000F000Fu, (w >> 12) & 0x000F000Fu};
     return __builtin_bit_cast(f16x8, v);
 }
+// The same with values 2, 3, 6 and 7 sixteen times as large: one shift less (their factors are sixteen times smaller).
+__device__ __forceinline__ f16x8 levels16(uint32_t w) {
+    const uint32_t u = w >> 8;
+    return __builtin_bit_cast(f16x8, u32x4{w & 0x000F000Fu, w & 0x00F000F0u, u & 0x000F000Fu, u & 0x00F000F0u});
+}
+// p s of four values (s: two words of fp16) as two fp16 numbers each, hi + lo: an instruction for each number, where the
+// compiler takes three.  (A word's halves are written one instruction apart from each other.)
+__device__ __forceinline__ void split4(const float* p, uint32_t s0, uint32_t s1, uint32_t* hi, uint32_t* lo) {
+    asm("v_fma_mixlo_f16 %0, %2, %6, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixlo_f16 %1, %4, %7, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixhi_f16 %0, %3, %6, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixhi_f16 %1, %5, %7, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]"
+        : "=&v"(hi[0]), "=&v"(hi[1])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(s0), "v"(s1));
+    asm("v_fma_mixlo_f16 %0, %2, %6, -%8 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixlo_f16 %1, %4, %7, -%9 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixhi_f16 %0, %3, %6, -%8 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixhi_f16 %1, %5, %7, -%9 op_sel:[0,1,1] op_sel_hi:[0,1,1]"
+        : "=&v"(lo[0]), "=&v"(lo[1])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(s0), "v"(s1), "v"(hi[0]), "v"(hi[1]));
+}
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -512,7 +533,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
                 for (int e = 0; e < 8; ++e) {
                     const float raw_q = ld16<kBf16>(half_of(raw[j][e >> 1], e));
                     const _Float16 v = (_Float16)(row_ok ? raw_q * mul : 0.f);
-                    qf[j][e] = v;
+                    qf[j][e] = e & 2 ? v * (_Float16)0.0625f : v;                  // (levels16)
                     qs[j / 2] += (float)v;
                 }
 #pragma unroll
@@ -541,8 +562,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                    acc = mfma16(levels(rg.kw[a][2 * g]), qf[2 * g], acc);
-                    acc = mfma16(levels(rg.kw[a][2 * g + 1]), qf[2 * g + 1], acc);
+                    acc = mfma16(levels16(rg.kw[a][2 * g]), qf[2 * g], acc);
+                    acc = mfma16(levels16(rg.kw[a][2 * g + 1]), qf[2 * g + 1], acc);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         s[e] = __builtin_fmaf(sx8_h2f(half_of(rg.ks[g][2 * a + (e >> 1)], e)), acc[e], s[e]);
@@ -558,6 +579,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
                 for (int e = 0; e < 4; ++e) sc[4 * a + e] = __builtin_fmaf(s[e], 16777216.f, mt[e]);
             }
             if (mask) {
+                asm volatile("");                // (a branch: as selects these would run for every block)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int key = b * 32 + (e / 4) * 16 + 4 * h + e % 4;
@@ -590,6 +612,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
                 // a token that some column may not attend must not reach it through 0 * NaN: its scale is zero for that
                 // column, and its minimum zero where it is no number (the scale, which is none either, still brings the
                 // NaN to the columns that attend it)
+                asm volatile("");
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (pv[e] == 0.f)
@@ -601,28 +624,30 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
                     vm[e] = (lo >= 0x7C00u ? 0u : vm[e] & 0xFFFFu) | (hi >= 0x7C00u ? 0u : vm[e] & 0xFFFF0000u);
                 }
             }
-            f16x8 ph, pl;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ph[e] = (_Float16)pv[e];
-                pl[e] = (_Float16)(pv[e] - (float)ph[e]);
+            u32x4 ph, pl;
+            constexpr uint32_t kOnes = 0x3C003C00u;
+            {
+                uint32_t hi[4], lo[4];
+                split4(pv, kOnes, kOnes, hi, lo);
+                split4(pv + 4, kOnes, kOnes, hi + 2, lo + 2);
+                ph = u32x4{hi[0], hi[1], hi[2], hi[3]};
+                pl = u32x4{lo[0], lo[1], lo[2], lo[3]};
             }
             const f16x8 vm8 = __builtin_bit_cast(f16x8, vm);
-            om = mfma16(vm8, ph, om);
-            om = mfma16(vm8, pl, om);
+            om = mfma16(vm8, __builtin_bit_cast(f16x8, ph), om);
+            om = mfma16(vm8, __builtin_bit_cast(f16x8, pl), om);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float s = sx8_h2f(half_of(rg.vs[g][e >> 1], e));
-                    ph[e] = (_Float16)(pv[e] * s);
-                    pl[e] = (_Float16)__builtin_fmaf(pv[e], s, -(float)ph[e]);
-                }
+                uint32_t hi[4], lo[4];
+                split4(pv, rg.vs[g][0], rg.vs[g][1], hi, lo);
+                split4(pv + 4, rg.vs[g][2], rg.vs[g][3], hi + 2, lo + 2);
+                const f16x8 h8 = __builtin_bit_cast(f16x8, (u32x4{hi[0], hi[1], hi[2], hi[3]}));
+                const f16x8 l8 = __builtin_bit_cast(f16x8, (u32x4{lo[0], lo[1], lo[2], lo[3]}));
 #pragma unroll
                 for (int t = 4 * g; t < 4 * g + 4; ++t) {
                     const f16x8 lv = levels(rg.vw[t]);
-                    o[t] = mfma16(lv, ph, o[t]);
-                    o[t] = mfma16(lv, pl, o[t]);
+                    o[t] = mfma16(lv, h8, o[t]);
+                    o[t] = mfma16(lv, l8, o[t]);
                 }
             }
         };
