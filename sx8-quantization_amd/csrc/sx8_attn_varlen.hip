@@ -62,7 +62,7 @@ __device__ __forceinline__ u32x4 scalar_rsrc(const void* p, uint32_t bytes) {
 // every LDS read that might be of the same place, which is every one (prompt of 8192: 715 us against 618).
 __device__ __forceinline__ void load_lds(const u32x4& r, int dst, int off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off), "s"(r)
-                 : "memory", "m0");
+                 : "memory");
 }
 // Lane i of 16 names the eight bytes of key i / 4 that hold dimensions 4 (i % 4) .. + 3, and gets dimension i of the four keys.
 __device__ __forceinline__ u32x2 read_tr(const unsigned char* at) {
@@ -374,6 +374,7 @@ extern "C" int32_t sx8_attn_varlen(const void* q, const void* k, const void* v, 
     for (int i = 0; i < 8; ++i)
         if (strides[i] % 8 || strides[i] < 0 || strides[i] > (int64_t)1 << 40)
             return fail(SX8_ERR_INVALID, "%s: strides must be multiples of 8", what);
+    if (Tq > 0 && !rows_apart(o_ts, o_hs, Tq, nh, hd)) return fail(SX8_ERR_INVALID, "%s: rows of out overlap", what);
     if (k_ts < hd || v_ts < hd || k_ts > 1 << 23 || v_ts > 1 << 23)     // (a tile's rows lie within 32-bit offsets)
         return fail(SX8_ERR_INVALID, "%s: the token strides of k and v must be hd .. 2^23", what);
     const int64_t grid = ((Tq + kRows - 1) / kRows + (n_seq < Tq ? n_seq : Tq)) * nh;

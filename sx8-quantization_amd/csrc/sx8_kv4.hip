@@ -809,6 +809,12 @@ int32_t check_rows(const char* what, const char* name, const void* ptr, int64_t 
     return SX8_OK;
 }
 
+// Output rows of `heads` heads: no two of them share memory.
+int32_t check_apart(const char* what, const char* name, int64_t ts, int64_t hs, int64_t rows, int64_t heads, int64_t hd) {
+    if (rows == 0 || rows_apart(ts, hs, rows, heads, hd)) return SX8_OK;
+    return fail(SX8_ERR_INVALID, "%s: rows of %s overlap", what, name);
+}
+
 // f(integral_constant<hd>, integral_constant<bf16>)
 template <typename F>
 void by_kind(int hd, int dtype, F&& f) {
@@ -864,6 +870,8 @@ extern "C" int32_t sx8_kv4_read(const uint8_t* pages, const int32_t* table, cons
     int32_t rc = make_pool(what, &p, pages, table, lens, cu, n_slots, max_pages, n_pages, rows, nk, hd, page_tokens, dtype);
     if (rc == SX8_OK) rc = check_rows(what, "k", k, k_ts, k_hs, rows);
     if (rc == SX8_OK) rc = check_rows(what, "v", v, v_ts, v_hs, rows);
+    if (rc == SX8_OK) rc = check_apart(what, "k", k_ts, k_hs, rows, nk, hd);
+    if (rc == SX8_OK) rc = check_apart(what, "v", v_ts, v_hs, rows, nk, hd);
     if (rc != SX8_OK) return rc;
     if (rows == 0) return ok();
     const RowsOut out{(uint16_t*)k, (uint16_t*)v, k_ts, k_hs, v_ts, v_hs};
@@ -891,6 +899,8 @@ extern "C" int32_t sx8_kv4_attend(const uint8_t* pages, const int32_t* table, co
     if (rc != SX8_OK) return rc;
     if (nh <= 0 || nh % nk || nh / nk > 256)
         return fail(SX8_ERR_INVALID, "%s: nh must be a multiple of nk, at most 256 nk", what);
+    rc = check_apart(what, "out", o_ts, o_hs, rows, nh, hd);
+    if (rc != SX8_OK) return rc;
     if (!(scale > 0.f) || !(scale < __builtin_inff()))
         return fail(SX8_ERR_INVALID, "%s: scale must be positive and finite", what);
     if (!workspace || workspace_bytes < attend_ws(hd) || !aligned(workspace, 256))

@@ -684,7 +684,7 @@ class PagedDecoder:
         return nxt[torch.tensor([order.index(s) for s in slots], device=self.dec.device)]
 
     def _step(self):
-        self.cache.reserve(self.active)
+        """The layers and the lm_head for one token of every slot, whose place in the cache is reserved."""
         pos = (self.cache.lens.long() - 1).clamp_(min=0)
         pb = self._bufs(self.n_slots)
         scale = 1.0 / math.sqrt(self.dec.cfg["head_dim"])
@@ -702,9 +702,11 @@ class PagedDecoder:
         next call (slots not in use: meaningless)."""
         if any(n >= self.max_len for n in self.lens):
             raise ValueError(f"a slot is full ({self.max_len} tokens)")
+        self.cache.reserve(self.active)
+        if any(n and n % self.cache.page_tokens == 0 for n in self.lens):
+            self.cache.check()                                      # (a slot needs a page: is there one?)
         if use_graph and self._graph is None:
-            # warm-up on a side stream, then the step is captured; the cache and the token are put back between
-            state = [t.clone() for t in (self.cache.table, self.cache.lens, self.cache.refs, self.cache.status)]
+            # once on a side stream, then captured (both write the rows that the replay writes)
             side = torch.cuda.Stream(self.dec.device)
             side.wait_stream(torch.cuda.current_stream(self.dec.device))
             with torch.cuda.stream(side):
@@ -713,8 +715,6 @@ class PagedDecoder:
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
                 logits = self._step()
-            for t, was in zip((self.cache.table, self.cache.lens, self.cache.refs, self.cache.status), state):
-                t.copy_(was)
             self._graph = (g, logits)
         if use_graph:
             self._graph[0].replay()

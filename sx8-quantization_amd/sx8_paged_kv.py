@@ -50,8 +50,10 @@ def _out(name, out, like, heads, hd):
         return torch.empty(like.shape[0], heads, hd, dtype=like.dtype, device=like.device)
     if out.shape != (like.shape[0], heads, hd) or out.dtype != like.dtype or out.device != like.device:
         raise RuntimeError(f"{name} must be {(like.shape[0], heads, hd)} {like.dtype} on {like.device}")
-    # two rows of the output may not share memory
-    if not _in_place(out) or (out.shape[0] > 1 and out.stride(0) < hd) or (heads > 1 and out.stride(1) < hd):
+    # no two rows of the output may share memory
+    ts, hs = out.stride()[:2]
+    apart = hs >= hd and ts >= (heads - 1) * hs + hd or ts >= hd and hs >= (out.shape[0] - 1) * ts + hd
+    if out.shape[0] and not (_in_place(out) and apart):
         raise RuntimeError(f"{name} needs contiguous head rows that begin on 16 bytes and do not overlap")
     return out
 

@@ -159,7 +159,7 @@ def test_paged_entry_points_refuse(hiplib):
                dict(pages=odd), dict(q=odd), dict(out=odd), dict(w=P(4096 + 128)), dict(wb=ws - 1), dict(slots=0),
                dict(slots=4097, rows=4097), dict(width=0), dict(width=1 << 18), dict(n_pages=0), dict(n_pages=1 << 31),
                dict(rows=3), dict(rows=-1, cu=p), dict(rows=1 << 31, cu=p), dict(st=(4, 64, 128, 64)),
-               dict(st=(128, -64, 128, 64)), dict(nh=3, nk=2), dict(nh=0), dict(nk=0), dict(nh=257), dict(hd=96), dict(pt=16),
+               dict(st=(128, -64, 128, 64)), dict(st=(128, 64, 64, 64)), dict(st=(128, 64, 0, 64)), dict(nh=3, nk=2), dict(nh=0), dict(nk=0), dict(nh=257), dict(hd=96), dict(pt=16),
                dict(scale=0.0), dict(scale=-1.0), dict(scale=inf), dict(scale=nan), dict(dt=2), dict(cu=P(4098))):
         assert attend(**kw) == 1, kw
         assert "sx8_kv4_attend" in err()
@@ -172,6 +172,7 @@ def test_paged_entry_points_refuse(hiplib):
         for kw in (dict(k=null), dict(v=null), dict(k=odd), dict(v=odd), dict(rows=5), dict(st=(60, 64, 64, 64)), dict(dt=3)):
             assert rows_call(fn, **kw) == 1, kw
         assert rows_call(fn, rows=0, cu=p) == 0
+    assert rows_call(L.sx8_kv4_read, st=(0, 64, 64, 64)) == 1 and "overlap" in err()
 
     nb = L.sx8_kv4_pages_workspace_bytes(4, 32)
 
@@ -210,8 +211,8 @@ def test_varlen_entry_point_refuses(hiplib):
                dict(tk=1 << 31), dict(nh=3, nk=2), dict(nk=0), dict(hd=32), dict(hd=96), dict(scale=0.0),
                dict(scale=float("nan")), dict(dt=2), dict(st=(128, 64, 60, 64, 64, 64, 128, 64)),
                dict(st=(128, 64, 0, 64, 64, 64, 128, 64)), dict(st=(128, 64, 64, 64, 1 << 24, 64, 128, 64)),
-               dict(st=(-128, 64, 64, 64, 64, 64, 128, 64))):
+               dict(st=(-128, 64, 64, 64, 64, 64, 128, 64)), dict(st=(128, 64, 64, 64, 64, 64, 64, 64))):
         assert call(**kw) == 1, kw
         assert "sx8_attn_varlen" in L.sx8_last_error().decode()
-    assert call(tq=(1 << 31) - 300, nh=4096, n=1) == 3
+    assert call(tq=(1 << 31) - 300, nh=4096, n=1, st=(128, 64, 64, 64, 64, 64, 4096 * 64, 64)) == 3
     assert call(tq=0, q=null, out=null) == 0

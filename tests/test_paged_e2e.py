@@ -167,3 +167,15 @@ def test_paged_decoder_refuses(dec, cuda):
         pd.fork([0], [1])
     with pytest.raises(ValueError):
         pd.free([2])
+    # a step that would need a page too many is refused before it changes anything
+    pd = PagedDecoder(d, 2, max_len=64, n_pages=2, page_tokens=32)
+    pd.prompt([0, 1], [ids(31, 1, cuda), ids(32, 2, cuda)])
+    state = pd.cache.table.clone(), pd.cache.lens.clone(), pd.cache.pages.clone()
+    with pytest.raises(RuntimeError, match="no free pages"):
+        pd.step()
+    assert all(torch.equal(a, b) for a, b in zip(state, (pd.cache.table, pd.cache.lens, pd.cache.pages)))
+    pd.free([1])
+    pd.step()
+    pd.step()
+    pd.cache.check()
+    assert pd.cache.lens.tolist() == pd.lens == [33, 0]

@@ -615,6 +615,48 @@ def test_step_in_a_graph(hiplib, cuda):
         assert torch.equal(p.pages, eager.pages) and torch.equal(p.table, eager.table)
 
 
+def test_pool_past_four_gib(hiplib, cuda):
+    """Pages whose bytes lie past 2^32: written, read, attended, forked and moved."""
+    from sx8_paged_kv import PagedKV4
+    nk, hd, pt = 8, 128, 128
+    n_pages = (1 << 32) // PagedKV4._page_bytes(nk, hd, pt) + 40
+    p = PagedKV4(1, nk, hd, n_pages, 3, 4, pt, device=cuda)
+    p.refs[:n_pages - 8] = 1                                        # all but the last pages are taken
+    n = 300
+    p.reserve(ints([n, 0, 0], cuda))
+    assert p.table[0, 0] == n_pages - 8 and (n_pages - 8) * p.page_bytes > 1 << 32
+    k, v = rand((n, nk, hd), 1, F16, cuda), rand((n, nk, hd), 2, F16, cuda)
+    p.append(0, k, v, ints([0, n, n, n], cuda))
+    p.fork(ints([0], cuda), ints([2], cuda))
+    p.check()
+    q = rand((2, nk, hd), 3, F16, cuda)
+    want = attention(q[:1].double(), q4(k), q4(v), n - 1)
+    cu = ints([0, 1, 1, 2], cuda)
+    q[1] = q[0]
+    got = p.attend(0, q, cu)
+    close(got[:1], want, F16, 4.0)
+    assert torch.equal(got[0], got[1])
+    p.refs[:n_pages - 8] = 0
+    p.compact()
+    assert p.table.max() == 3 and torch.equal(p.attend(0, q, cu), got)
+    rk, _ = p.read(0, 2 * n, ints([0, n, n, 2 * n], cuda))
+    assert torch.equal(rk, torch.cat([q4(k).half()] * 2))
+
+
+def test_varlen_rows_past_four_gib(hiplib, cuda):
+    """Keys and values whose offsets pass 2^32 bytes (rows 2 MB apart)."""
+    from sx8_paged_kv import attn_varlen
+    T, ts = 2100, 1 << 20
+    big = torch.zeros(T * ts, dtype=F16, device=cuda)
+    k = torch.as_strided(big, (T, 1, 64), (ts, 64, 1))
+    v = torch.as_strided(big, (T, 1, 64), (ts, 64, 1), 64)
+    k.copy_(rand((T, 1, 64), 1, F16, cuda))
+    v.copy_(rand((T, 1, 64), 2, F16, cuda))
+    q = rand((5, 2, 64), 3, F16, cuda)
+    got = attn_varlen(q, k, v, ints([0, 3, 5], cuda), ints([0, 50, T], cuda))
+    close(got, want_varlen(q, k, v, [3, 2], [50, T - 50]), F16, 5.0, 2.0 ** -11)
+
+
 def test_two_streams(hiplib, cuda):
     """Two caches worked on by two streams at once give what they give one after the other."""
     pools = [make(cuda, [900 + 200 * i, 64], 2, 128, 64, seed=i)[0] for i in range(2)]
@@ -796,6 +838,7 @@ def test_wrappers_refuse(hiplib, cuda):
                  lambda: p.attend(0, q.cpu()), lambda: p.attend(0, q, scale=0.0), lambda: p.attend(0, q, scale=math.nan),
                  lambda: p.attend(0, rand((2, 2, 64), 1, F16, cuda)), lambda: p.attend(0, q, out=q.float()),
                  lambda: p.attend(0, q, out=q[:, :1].expand(1, 2, 64)),
+                 lambda: p.attend(0, q.expand(1, 2, 64), out=torch.as_strided(q, (1, 2, 64), (128, 8, 1))),
                  lambda: p.append(0, k, v), lambda: p.append(0, k, v[:3], cum([40], cuda)),
                  lambda: p.append(0, k, v.bfloat16(), cum([40], cuda)), lambda: p.read(0, 2),
                  lambda: p.read(0, 1, dtype=torch.float32), lambda: p.reserve(ints([1, 1], cuda)),
