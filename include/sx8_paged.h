@@ -44,11 +44,15 @@ extern "C" {
  * (cu_* (n_seq + 1) int32).  out = softmax(scale * q . k) v over its keys; causal != 0: row i of nq attends keys
  * 0 .. nk_b - nq + i (its own is the last).  A row with no key gives zeros; rows of no sequence are left as
  * they are.  hd 64, 128 or 256, nh a multiple of nk, scale > 0; n_seq <= 4096; one head's keys and values are
- * addressed in 64 bits.  Softmax sums and products are held in float32, probabilities rounded to dtype. */
+ * addressed in 64 bits.  Softmax sums and products are held in float32, probabilities rounded to dtype.
+ * workspace (256-byte aligned, sx8_attn_varlen_workspace_bytes, no clearing needed) lets calls of few rows cut their
+ * keys into parts that are added up by a second launch; without one (NULL) they run as one part. */
+int64_t sx8_attn_varlen_workspace_bytes(int64_t n_seq, int64_t Tq, int64_t Tk, int32_t nh, int32_t hd);
 int32_t sx8_attn_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
                         const int32_t* cu_k, int64_t n_seq, int64_t Tq, int64_t Tk, int32_t nh, int32_t nk, int32_t hd,
                         int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs,
-                        int64_t o_ts, int64_t o_hs, float scale, int32_t causal, int32_t dtype, void* stream);
+                        int64_t o_ts, int64_t o_hs, float scale, int32_t causal, int32_t dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 /* Bytes of a page (nk heads of hd 64, 128 or 256), or -1 for bad arguments. */
 int64_t sx8_kv4_page_bytes(int32_t nk, int32_t hd, int32_t page_tokens);

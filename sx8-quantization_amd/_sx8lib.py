@@ -119,7 +119,8 @@ SIGNATURES = [
     ("sx8_dec_gemv_zp_add", _I32, [_P, _P, _P, _I32, _P, _P, _I64, _I64, _P, _P, _P]),
     # include/sx8_paged.h
     ("sx8_attn_varlen", _I32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64,
-                               _I64, _I64, _I64, _I64, ctypes.c_float, _I32, _I32, _P]),
+                               _I64, _I64, _I64, _I64, ctypes.c_float, _I32, _I32, _P, _I64, _P]),
+    ("sx8_attn_varlen_workspace_bytes", _I64, [_I64, _I64, _I64, _I32, _I32]),
     ("sx8_kv4_page_bytes", _I64, [_I32, _I32, _I32]),
     ("sx8_kv4_append", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32,
                               _I32, _P]),

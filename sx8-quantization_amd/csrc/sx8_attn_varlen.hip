@@ -37,6 +37,14 @@ struct VarIo {
     int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
     int Tq, Tk, n_seq, nh, nk;
     float scale_log2;
+    // keys in `splits` parts (gridDim.y): per work-group (x, y) 128 rows of sums and their (maximum, sum of weights)
+    int splits;
+    float* part_o;                        // [x][y][128][HD]
+    float* part_ml;                       // [x][y][128][2]
+    struct VarRecord* record;             // [x]
+};
+struct VarRecord {                        // rows that the parts of x are for; n == 0: none
+    int32_t q_first, q0, n, head;
 };
 
 constexpr int kRows = 128;
@@ -100,12 +108,12 @@ constexpr int var_lds_bytes() {
 // finite number (about 1 us a key).  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
 template <int HD, bool kBf16, typename V, int NT>
 __device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, const uint16_t* v, const VarIo& io,
-                                                    int see, int lim, int h, V (&o)[NT], float& l) {
-    float m = -__builtin_inff();
+                                          int from, int to, int lim, int h, V (&o)[NT], float& m, float& l) {
+    m = -__builtin_inff();
     l = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n] = 0.f;
-    for (int key = 0; key < see; ++key) {
+    for (int key = from; key < to; ++key) {
         float s = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -131,7 +139,8 @@ __device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, 
     }
 }
 
-template <int HD, bool kBf16, bool kCausal>
+// kSplit: the work-group takes part blockIdx.y of its rows' keys (a kernel of its own: as one, whole calls take 3% longer).
+template <int HD, bool kBf16, bool kCausal, bool kSplit>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const VarIo io) {
     typedef float f32x16 __attribute__((ext_vector_type(16)));
     using T = VarTile<HD>;
@@ -155,7 +164,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
         const int tiles = nq > 0 ? (nq - 1) / kRows + 1 : 0;
         // tiles at place t of their sequence or behind it, over all sequences: the places from the back hold items 0, 1, ...
         auto from = [&](int place) { return wave_sum(max(tiles - place, 0)); };
-        if (item >= from(0)) return;
+        if (item >= from(0)) {
+            if (kSplit && blockIdx.y == 0 && tid == 0) io.record[blockIdx.x].n = 0;
+            return;
+        }
         t = 0;                                   // the last place whose tiles end behind the item
         int step = 1;
         while (from(step) > item) step *= 2;
@@ -177,7 +189,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
         });
         __syncthreads();
         const int at = (int)uniform(pre[io.n_seq]) - 1 - item;
-        if (at < 0) return;
+        if (at < 0) {
+            if (kSplit && blockIdx.y == 0 && tid == 0) io.record[blockIdx.x].n = 0;
+            return;
+        }
         const int b = find_item<256>(io.n_seq, pre, at);
         t = at - (int)uniform(pre[b]);
         seq_rows(io.cu_q, io.Tq, b, &q_first, &nq);
@@ -192,7 +207,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     const int past = nkeys - nq;                                         // row i attends keys 0 .. past + i
     const int wg_last = min(nq - wg_q0, kRows) - 1 + wg_q0;
     const int see = kCausal ? max(past + wg_last + 1, 0) : nkeys;        // keys of the work-group
-    const int n_tiles = (int)(((int64_t)see + KB - 1) / KB);
+    const int all_tiles = (int)(((int64_t)see + KB - 1) / KB);
+    const int j0 = kSplit ? (int)((int64_t)all_tiles * blockIdx.y / io.splits) : 0;      // this part's tiles
+    const int j1 = kSplit ? (int)((int64_t)all_tiles * (blockIdx.y + 1) / io.splits) : all_tiles;
     const int w_last = min(nq - q0, 32) - 1 + q0;                        // the wave's last row
     const int w_see = q0 >= nq ? 0 : kCausal ? past + w_last + 1 : nkeys;
     const int w_all = q0 >= nq ? 0 : kCausal ? past + q0 + 1 : nkeys;    // keys that all its rows see
@@ -304,16 +321,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
             }
         }
     };
-    if (n_tiles > 0) fetch(0, 0);
+    if (j0 < j1) fetch(j0, 0);
     // the query is waited for here and not at its uses, where the wait would take in the next tile's loads
 #pragma unroll
     for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(qf[st]));
-    for (int j = 0; j < n_tiles; ++j) {
+    for (int j = j0; j < j1; ++j) {
+        const int buf = (j - j0) & 1;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                          // tile j is there, and nobody reads the other buffer any more
-        if (j + 1 < n_tiles) fetch(j + 1, (j + 1) & 1);
+        if (j + 1 < j1) fetch(j + 1, buf ^ 1);
         const int k0 = j * KB;
-        if (k0 < w_see) tile(j, j & 1, k0 + KB > w_all);
+        if (k0 < w_see) tile(j, buf, k0 + KB > w_all);
     }
     l += __shfl_xor(l, 32, 64);
     // A key that a row may not attend has probability zero there, and 0 * NaN or 0 * infinity must not reach the row:
@@ -324,8 +342,24 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(0.f, o[n][r], odd);
     if (__builtin_amdgcn_ballot_w64(odd != 0.f) != 0)
-        slow_rows<HD, kBf16>(io.q + ((int64_t)q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs, kp, vp, io, w_see, lim,
-                              h, o, l);
+        slow_rows<HD, kBf16>(io.q + ((int64_t)q_first + (row_ok ? q0 + c : nq - 1)) * io.q_ts + head * io.q_hs, kp, vp, io, j0 * KB,
+                              min(w_see, j1 * KB), lim, h, o, m, l);
+    if constexpr (kSplit) {
+        const int64_t at = (int64_t)blockIdx.x * io.splits + blockIdx.y;
+        if (blockIdx.y == 0 && tid == 0) io.record[blockIdx.x] = VarRecord{q_first, wg_q0, nq, head};
+        if (!row_ok) return;
+        float* const po = io.part_o + (at * kRows + 32 * w + c) * HD + 4 * h;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(po + 32 * n + 8 * g) = f32x4{o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]};
+        if (h == 0) {
+            io.part_ml[(at * kRows + 32 * w + c) * 2] = m;
+            io.part_ml[(at * kRows + 32 * w + c) * 2 + 1] = l;
+        }
+        return;
+    }
     if (!row_ok) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint16_t* const dst = io.out + ((int64_t)q_first + q0 + c) * io.o_ts + head * io.o_hs + 4 * h;
@@ -341,22 +375,84 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
         }
 }
 
+// The parts of 16 rows of an item, added up in their order: 16 threads a row.
+template <int HD, bool kBf16>
+__global__ __launch_bounds__(256) void k_varlen_combine(const VarIo io) {
+    constexpr int N = HD / 16;
+    const VarRecord rec = io.record[blockIdx.x];
+    const int row = 16 * blockIdx.y + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * N;
+    if (rec.n == 0 || rec.q0 + row >= rec.n) return;
+    const int64_t base = (int64_t)blockIdx.x * io.splits * kRows + row;
+    float m = -__builtin_inff(), l = 0.f;
+    for (int i = 0; i < io.splits; ++i) m = fmaxf(m, io.part_ml[(base + (int64_t)i * kRows) * 2]);
+    f32x4 acc[N / 4];
+#pragma unroll
+    for (int e = 0; e < N / 4; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < io.splits; ++i) {
+        const int64_t at = base + (int64_t)i * kRows;
+        const float pm = io.part_ml[at * 2], f = pm == m ? 1.f : __builtin_amdgcn_exp2f(pm - m);
+        l = __builtin_fmaf(f, io.part_ml[at * 2 + 1], l);
+#pragma unroll
+        for (int e = 0; e < N / 4; ++e)
+            acc[e] = __builtin_elementwise_fma(f32x4(f), reinterpret_cast<const f32x4*>(io.part_o + at * HD + d0)[e], acc[e]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* const dst = io.out + ((int64_t)rec.q_first + rec.q0 + row) * io.o_ts + rec.head * io.o_hs + d0;
+#pragma unroll
+    for (int e = 0; e < N / 4; ++e)
+        reinterpret_cast<u32x2*>(dst)[e] = u32x2{pack16<kBf16>(acc[e][0] * inv, acc[e][1] * inv),
+                                                 pack16<kBf16>(acc[e][2] * inv, acc[e][3] * inv)};
+}
+
+// Work-groups of a call at most (a tile of rows of a head each), and the parts that its keys are cut into: with few
+// work-groups the keys of each are shared by up to 16, so that about 1024 run, each with at least 256 keys of a sequence of
+// average length, or 1024 where there is a work-group for every CU already.  With the reader of the cache before it, 32
+// heads over 8: 8 rows after 16000 keys 298 -> 60 us, 128 rows after 4000 92 -> 40; 8 sequences of 8 rows after 16000 keys
+// 440 -> 380; 1024 rows after 500 keys in three parts of 500 42 -> 51, so they stay whole.
+int64_t var_items(int64_t n_seq, int64_t Tq, int64_t nh) { return ((Tq + kRows - 1) / kRows + (n_seq < Tq ? n_seq : Tq)) * nh; }
+int var_splits(int64_t n_seq, int64_t Tk, int64_t items) {
+    const int64_t a = items > 0 ? 1024 / items : 1, b = Tk / (n_seq * (items < 256 ? 256 : 1024)), c = a < b ? a : b;
+    return (int)(c < 2 ? 1 : c > 16 ? 16 : c);
+}
+int64_t var_ws(int64_t items, int splits, int64_t hd) {
+    return splits > 1 ? items * (splits * (int64_t)kRows * (hd + 2) * 4 + (int64_t)sizeof(VarRecord)) : 0;
+}
+
 template <int HD>
 void launch(const VarIo& io, int dtype, int causal, unsigned grid, hipStream_t st) {
-    if (dtype && causal) hipLaunchKernelGGL((k_attn_varlen<HD, true, true>), dim3(grid), dim3(256), 0, st, io);
-    else if (dtype) hipLaunchKernelGGL((k_attn_varlen<HD, true, false>), dim3(grid), dim3(256), 0, st, io);
-    else if (causal) hipLaunchKernelGGL((k_attn_varlen<HD, false, true>), dim3(grid), dim3(256), 0, st, io);
-    else hipLaunchKernelGGL((k_attn_varlen<HD, false, false>), dim3(grid), dim3(256), 0, st, io);
+    const dim3 g(grid, (unsigned)io.splits), c(grid, kRows / 16);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, st, io); };
+    if (io.splits == 1) {
+        if (dtype && causal) go(k_attn_varlen<HD, true, true, false>);
+        else if (dtype) go(k_attn_varlen<HD, true, false, false>);
+        else if (causal) go(k_attn_varlen<HD, false, true, false>);
+        else go(k_attn_varlen<HD, false, false, false>);
+        return;
+    }
+    if (dtype && causal) go(k_attn_varlen<HD, true, true, true>);
+    else if (dtype) go(k_attn_varlen<HD, true, false, true>);
+    else if (causal) go(k_attn_varlen<HD, false, true, true>);
+    else go(k_attn_varlen<HD, false, false, true>);
+    if (dtype) hipLaunchKernelGGL((k_varlen_combine<HD, true>), c, dim3(256), 0, st, io);
+    else hipLaunchKernelGGL((k_varlen_combine<HD, false>), c, dim3(256), 0, st, io);
 }
 
 }  // namespace
 }  // namespace sx8
 
+extern "C" int64_t sx8_attn_varlen_workspace_bytes(int64_t n_seq, int64_t Tq, int64_t Tk, int32_t nh, int32_t hd) {
+    using namespace sx8;
+    if (n_seq <= 0 || n_seq > kKv4MaxSlots || Tq < 0 || Tk < 0 || nh <= 0) return -1;
+    const int64_t items = var_items(n_seq, Tq, nh);
+    return var_ws(items, var_splits(n_seq, Tk, items), hd);
+}
+
 extern "C" int32_t sx8_attn_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
                                    const int32_t* cu_k, int64_t n_seq, int64_t Tq, int64_t Tk, int32_t nh, int32_t nk,
                                    int32_t hd, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
                                    int64_t v_hs, int64_t o_ts, int64_t o_hs, float scale, int32_t causal, int32_t dtype,
-                                   void* stream) {
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace sx8;
     const char* what = "sx8_attn_varlen";
     if (!cu_q || !cu_k || (Tq > 0 && (!q || !out)) || (Tk > 0 && (!k || !v)))
@@ -377,14 +473,25 @@ extern "C" int32_t sx8_attn_varlen(const void* q, const void* k, const void* v, 
     if (Tq > 0 && !rows_apart(o_ts, o_hs, Tq, nh, hd)) return fail(SX8_ERR_INVALID, "%s: rows of out overlap", what);
     if (k_ts < hd || v_ts < hd || k_ts > 1 << 23 || v_ts > 1 << 23)     // (a tile's rows lie within 32-bit offsets)
         return fail(SX8_ERR_INVALID, "%s: the token strides of k and v must be hd .. 2^23", what);
-    const int64_t grid = ((Tq + kRows - 1) / kRows + (n_seq < Tq ? n_seq : Tq)) * nh;
-    if (grid > 0x7FFFFFFF) return fail(SX8_ERR_UNSUPPORTED, "%s: over 2^31 tiles of rows", what);
+    const int64_t items = var_items(n_seq, Tq, nh);
+    if (items > 0x7FFFFFFF) return fail(SX8_ERR_UNSUPPORTED, "%s: over 2^31 tiles of rows", what);
+    int splits = var_splits(n_seq, Tk, items);
+    if (splits > 1 && !workspace) splits = 1;
+    if (splits > 1 && (workspace_bytes < var_ws(items, splits, hd) || !aligned(workspace, 256)))
+        return fail(SX8_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", what,
+                    (long long)var_ws(items, splits, hd));
     if (Tq == 0) return ok();
-    const VarIo io{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, cu_q, cu_k, q_ts, q_hs, k_ts,
-                   k_hs, v_ts, v_hs, o_ts, o_hs, (int)Tq, (int)Tk, (int)n_seq, nh, nk, scale * 1.4426950408889634f};
+    VarIo io{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, cu_q, cu_k, q_ts, q_hs, k_ts,
+             k_hs, v_ts, v_hs, o_ts, o_hs, (int)Tq, (int)Tk, (int)n_seq, nh, nk, scale * 1.4426950408889634f, splits,
+             nullptr, nullptr, nullptr};
+    if (splits > 1) {
+        io.record = reinterpret_cast<VarRecord*>(workspace);
+        io.part_o = reinterpret_cast<float*>(io.record + items);
+        io.part_ml = io.part_o + items * splits * kRows * (int64_t)hd;
+    }
     const hipStream_t st = as_stream(stream);
-    if (hd == 64) launch<64>(io, dtype, causal, (unsigned)grid, st);
-    else if (hd == 128) launch<128>(io, dtype, causal, (unsigned)grid, st);
-    else launch<256>(io, dtype, causal, (unsigned)grid, st);
+    if (hd == 64) launch<64>(io, dtype, causal, (unsigned)items, st);
+    else if (hd == 128) launch<128>(io, dtype, causal, (unsigned)items, st);
+    else launch<256>(io, dtype, causal, (unsigned)items, st);
     return check_launch(what);
 }

@@ -114,8 +114,8 @@ SX8_KV4_FN int64_t kv4_touched_most(int64_t n_slots, int64_t rows, bool cu) {
 
 // Whether the head rows (hd values each) of a (rows, heads, hd) tensor lie apart from each other.
 inline bool rows_apart(int64_t ts, int64_t hs, int64_t rows, int64_t heads, int64_t hd) {
-    return (hs >= hd || heads == 1) && (rows == 1 || ts >= (heads - 1) * hs + hd) ||
-           (ts >= hd || rows == 1) && (heads == 1 || hs >= (rows - 1) * ts + hd);
+    const bool by_rows = (hs >= hd || heads == 1) && (rows == 1 || ts >= (heads - 1) * hs + hd);
+    return by_rows || ((ts >= hd || rows == 1) && (heads == 1 || hs >= (rows - 1) * ts + hd));
 }
 
 }  // namespace sx8

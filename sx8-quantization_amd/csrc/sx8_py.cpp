@@ -46,6 +46,7 @@ struct Lib {
     int32_t (*dequant)(CP, CP, CP, CP, CP, CP, CP, CP, int64_t, int64_t, int64_t, void*, void*);
     int32_t (*embed)(CP, int64_t, CP, CP, int32_t, CP, CP, int64_t, int64_t, int64_t, void*, void*);
     decltype(&sx8_attn_varlen) varlen;
+    decltype(&sx8_attn_varlen_workspace_bytes) varlen_ws;
     decltype(&sx8_kv4_append) kv4_append;
     decltype(&sx8_kv4_read) kv4_read;
     decltype(&sx8_kv4_attend) kv4_attend;
@@ -131,6 +132,7 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     SX8_BIND(dequant, "sx8_dequant_f16")
     SX8_BIND(embed, "sx8_embed_gather")
     SX8_BIND(varlen, "sx8_attn_varlen")
+    SX8_BIND(varlen_ws, "sx8_attn_varlen_workspace_bytes")
     SX8_BIND(kv4_append, "sx8_kv4_append")
     SX8_BIND(kv4_read, "sx8_kv4_read")
     SX8_BIND(kv4_attend, "sx8_kv4_attend")
@@ -463,10 +465,14 @@ PyObject* py_varlen(PyObject*, PyObject* const* a, Py_ssize_t na) {
         Unlocked u;
         c10::DeviceGuard on(q->device());
         o = empty_like_device(q->sizes(), q->scalar_type(), *q);
+        const int64_t nb = lib.varlen_ws(cq->numel() - 1, q->size(0), k->size(0), (int32_t)q->size(1), (int32_t)hd);
+        at::Tensor ws;
+        if (nb > 0) ws = empty_like_device({nb}, at::kByte, *q);
         rc = lib.varlen(q->data_ptr(), k->data_ptr(), v->data_ptr(), o.data_ptr(), cq->data_ptr<int32_t>(),
                         ck->data_ptr<int32_t>(), cq->numel() - 1, q->size(0), k->size(0), (int32_t)q->size(1),
                         (int32_t)k->size(1), (int32_t)hd, q->stride(0), q->stride(1), k->stride(0), k->stride(1), v->stride(0),
-                        v->stride(1), o.stride(0), o.stride(1), scale, a[6] == Py_True, dtype_of(*q), stream_of(*q));
+                        v->stride(1), o.stride(0), o.stride(1), scale, a[6] == Py_True, dtype_of(*q),
+                        nb > 0 ? ws.data_ptr() : nullptr, nb > 0 ? nb : 0, stream_of(*q));
     }
     if (rc) return failed("sx8_attn_varlen", rc);
     return THPVariable_Wrap(std::move(o));

@@ -97,10 +97,12 @@ def attn_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
         out = _out("out", out, q, nh, hd)
         _ints("cu_q", cu_q, None, q.device)
         _ints("cu_k", cu_k, cu_q.numel(), q.device)
+        nb = int(_L.lib().sx8_attn_varlen_workspace_bytes(cu_q.numel() - 1, q.shape[0], k.shape[0], nh, hd))
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb > 0 else None
         _L.call("sx8_attn_varlen", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
                 cu_q.numel() - 1, q.shape[0], k.shape[0], nh, nk, hd, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
                 v.stride(0), v.stride(1), out.stride(0), out.stride(1), _scale(scale, hd), int(bool(causal)),
-                _DTYPES[q.dtype], _L.stream(q.device))
+                _DTYPES[q.dtype], None if ws is None else ws.data_ptr(), max(nb, 0), _L.stream(q.device))
     return out
 
 

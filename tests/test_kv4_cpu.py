@@ -203,8 +203,8 @@ def test_varlen_entry_point_refuses(hiplib):
     p, odd, null = P(4096), P(4104), P(None)
 
     def call(q=p, k=p, v=p, out=p, cq=p, ck=p, n=2, tq=8, tk=8, nh=2, nk=1, hd=64, st=(128, 64, 64, 64, 64, 64, 128, 64),
-             scale=0.1, causal=1, dt=0):
-        return L.sx8_attn_varlen(q, k, v, out, cq, ck, n, tq, tk, nh, nk, hd, *st, scale, causal, dt, null)
+             scale=0.1, causal=1, dt=0, w=null, wb=0):
+        return L.sx8_attn_varlen(q, k, v, out, cq, ck, n, tq, tk, nh, nk, hd, *st, scale, causal, dt, w, wb, null)
 
     for kw in (dict(q=null), dict(k=null), dict(v=null), dict(out=null), dict(cq=null), dict(ck=null), dict(q=odd),
                dict(k=odd), dict(v=odd), dict(out=odd), dict(cq=P(4098)), dict(n=0), dict(n=4097), dict(tq=-1),
@@ -216,3 +216,10 @@ def test_varlen_entry_point_refuses(hiplib):
         assert "sx8_attn_varlen" in L.sx8_last_error().decode()
     assert call(tq=(1 << 31) - 300, nh=4096, n=1, st=(128, 64, 64, 64, 64, 64, 4096 * 64, 64)) == 3
     assert call(tq=0, q=null, out=null) == 0
+    # few rows and many keys: keys in parts, and a workspace that is given has to hold them
+    need = L.sx8_attn_varlen_workspace_bytes(2, 8, 9000, 2, 64)
+    assert need > 0 and L.sx8_attn_varlen_workspace_bytes(2, 8, 100, 2, 64) == 0
+    assert L.sx8_attn_varlen_workspace_bytes(1, 1 << 20, 1 << 20, 32, 128) == 0
+    assert L.sx8_attn_varlen_workspace_bytes(0, 8, 8, 2, 64) == -1
+    assert call(tk=9000, w=p, wb=need - 1) == 1 and "workspace" in L.sx8_last_error().decode()
+    assert call(tk=9000, w=P(4096 + 128), wb=need) == 1

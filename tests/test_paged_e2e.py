@@ -136,6 +136,24 @@ def test_shared_prefix_fork_free_compact(dec, cuda):
     pd.cache.check()
 
 
+def test_long_prompts_after_a_prefix(dec, cuda):
+    """Many new tokens behind tokens that the cache holds: the pages' values read back and attended."""
+    from e2e_decoder import PagedDecoder
+    d, W = dec
+    pd = PagedDecoder(d, 3, max_len=160, page_tokens=64)
+    refs = [Ref(d, W) for _ in range(2)]
+    first, tails = [ids(11, 1, cuda), ids(3, 2, cuda)], [ids(140, 3, cuda), ids(131, 4, cuda)]
+    pd.prompt([2, 0], first)
+    pd.prompt([2, 0], tails)
+    for row, i in ((1, 0), (0, 1)):
+        refs[i].run(first[i])
+        near(pd.logits[row], refs[i].run(tails[i]))
+    fed = pd.tok.clone()
+    pd.step()
+    near(pd.logits[2], refs[0].run(fed[2:3]))
+    pd.cache.check()
+
+
 def test_generate_batch(dec, cuda):
     """generate_batch: graph and eager steps give the same tokens, with and without a shared prefix."""
     d, _ = dec

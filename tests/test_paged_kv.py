@@ -727,6 +727,37 @@ def test_varlen_long(hiplib, cuda):
         assert torch.equal(got, attn_varlen(q, k, v, cum([2500], cuda)))
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_varlen_few_rows_many_keys(hiplib, cuda, hd, dt):
+    """Calls whose keys are cut into parts: sequences of very different lengths, rows without keys, empty parts, values that are
+    no finite numbers; and the same without a workspace."""
+    import _sx8lib as L
+    from sx8_paged_kv import attn_varlen
+    nq, nkeys = [3, 130, 1, 6, 2], [5000, 900, 0, 4, 2700]
+    assert L.lib().sx8_attn_varlen_workspace_bytes(5, sum(nq), sum(nkeys), 4, hd) > 0
+    q = rand((sum(nq) + 1, 4, hd), 1, dt, cuda)
+    k, v = rand((sum(nkeys), 2, hd), 2, dt, cuda), rand((sum(nkeys), 2, hd), 3, dt, cuda)
+    cq, ck = cum(nq, cuda), cum(nkeys, cuda)
+    for causal in (True, False):
+        got = attn_varlen(q, k, v, cq, ck, causal=causal, out=torch.full_like(q, 5.0))
+        close(got[:-1], want_varlen(q, k, v, nq, nkeys, causal), dt, v.abs().max().item(), torch.finfo(dt).eps / 2)
+        assert (got[-1] == 5).all()
+        one = torch.full_like(q, 5.0)
+        L.call("sx8_attn_varlen", q.data_ptr(), k.data_ptr(), v.data_ptr(), one.data_ptr(), cq.data_ptr(), ck.data_ptr(), 5,
+               q.shape[0], k.shape[0], 4, 2, hd, 4 * hd, hd, 2 * hd, hd, 2 * hd, hd, 4 * hd, hd, hd ** -0.5, causal,
+               int(dt is BF16), None, 0, L.stream(cuda))
+        close(one[:-1], want_varlen(q, k, v, nq, nkeys, causal), dt, v.abs().max().item(), torch.finfo(dt).eps / 2)
+    v[4998, 1, 5] = math.nan                                       # seen by rows 1 and 2 of the first sequence
+    got = attn_varlen(q, k, v, cq, ck)
+    nan = torch.isnan(got[:-1])
+    assert nan[1:3, 2:, 5].all() and nan.sum() == 4
+    vz = v.clone()
+    vz[4998, 1, 5] = 0
+    want = want_varlen(q, k, vz, nq, nkeys)
+    close(torch.where(nan, 0, got[:-1]), torch.where(nan, 0.0, want), dt, vz.abs().max().item(), torch.finfo(dt).eps / 2)
+
+
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_varlen_not_finite(hiplib, cuda, dt, bad):
