@@ -18,6 +18,12 @@ namespace {
 // K and V go from memory to LDS directly, the next tile while this one is computed; rows past the sequence's
 // last key lie past the buffer and come as zeros.  A 16-byte chunk of a row lies at its position XOR a few bits of
 // the row, so that neither kind of read meets bank conflicts (the swap is made in the load's address).
+// Bound by the matrix cores and the softmax's VALU, which two waves a SIMD of different work-groups overlap: one prompt of
+// 8192 tokens (32 heads over 8 of 128, bf16) takes 515-535 us, 1028-1067 TFLOP/s, where a library product of 8192^3
+// reaches 1100-1150.  Short prompts are bound by a work-group's start (about 5 us: lengths, query, first tile): 24 of
+// 40 .. 2000 tokens 230 us, three of up to 96 tokens 7.  s_setprio around the products (541 us against 533), tiles of 32
+// keys with three waves a SIMD (544 against 528) and work-groups that stay and request the next rows ahead (561 against
+// 515) were slower.
 template <int HD>
 struct VarTile {
     static constexpr int kKeys = HD == 256 ? 32 : 64;        // of a tile
@@ -67,7 +73,7 @@ __device__ __forceinline__ u32x4 scalar_rsrc(const void* p, uint32_t bytes) {
 }
 // 16 bytes a lane from the buffer to the 1 KB of LDS at byte `dst`; no register is written, and the kernel waits for
 // vmcnt(0) and a barrier before it reads that LDS.  The builtin does the same, but the compiler then waits for it before
-// every LDS read that might be of the same place, which is every one (prompt of 8192: 715 us against 618).
+// every LDS read that might be of the same place, which is every one (prompt of 8192: 730 us against 603).
 __device__ __forceinline__ void load_lds(const u32x4& r, int dst, int off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off), "s"(r)
                  : "memory");
