@@ -688,7 +688,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
             io.part_ml[at * 2 + 1] = l;
         }
         // the unit's record is written by its first piece; a unit that is cut goes on in the next waves
-        if (b0 == 0 && lane == 0 && (io.by_unit || !whole)) {
+        // (a cu that runs backwards can name more units than rows allow: those have no record)
+        const int64_t rec = io.by_unit ? unit0 + run.unit : wave;
+        if (b0 == 0 && lane == 0 && (io.by_unit || !whole) && rec < (1 << waves_log2<HD>())) {
             Kv4Piece pc;
             pc.parts = whole ? 0 : kv4_parts(begin + run.unit * (nb + kKv4Begin) + kKv4Begin, nb, share, wave);
             pc.first = place;
@@ -696,7 +698,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
             pc.head = head;
             pc.row0 = row0;
             pc.n = n;
-            io.piece[io.by_unit ? unit0 + run.unit : wave] = pc;
+            io.piece[rec] = pc;
         }
     }
 }

@@ -255,6 +255,21 @@ def test_attend_long_and_cut(hiplib, cuda):
     assert torch.equal(again, p.attend(0, q, scale=0.3))
 
 
+def test_attend_cu_backwards(hiplib, cuda):
+    """A cu that names the same rows for many slots: more units than rows allow, still inside the memory."""
+    from sx8_paged_kv import PagedKV4
+    p = PagedKV4(1, 1, 64, 2, 4096, 1, 32, device=cuda)
+    p.reserve(ints([1, 1] + [0] * 4094, cuda))
+    q = rand((64, 256, 64), 1, F16, cuda)
+    k = rand((64, 1, 64), 1, F16, cuda)
+    cu = ints([0, 64] * 2048 + [64], cuda)
+    out = p.attend(0, q, cu)
+    p.append(0, k, k, cu)
+    p.read(0, 64, cu)
+    torch.cuda.synchronize()
+    assert out.shape == q.shape and p.refs.tolist() == [1, 1]
+
+
 @pytest.mark.parametrize("n_slots", [64, 65, 300, 4096])
 @pytest.mark.parametrize("nk", [1, 9])
 def test_attend_many_slots(hiplib, cuda, n_slots, nk):
@@ -364,7 +379,7 @@ def test_attend_odd_lengths_of_the_tables(hiplib, cuda):
     assert not got[1].any()
     p.append(0, q, q)
     p.lens.copy_(ints([64, 32], cuda))
-    for cu in ([0, 50, -3], [-9, 1, 1 << 30], [5, 2, 1]):
+    for cu in ([0, 50, -3], [-9, 1, 1 << 30], [5, 2, 1], [0, 2, 0]):
         out = torch.full_like(q, 3.0)
         p.attend(0, q, ints(cu, cuda), out=out)
         p.read(0, 2, ints(cu, cuda))
