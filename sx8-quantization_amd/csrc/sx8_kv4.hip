@@ -280,12 +280,14 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // So nothing is rounded to fewer than 22 bits between the cache and the output.
 // Query rows are multiplied by a power of two that brings their largest value into [64, 128), which is undone in
 // the scale: bf16 rows become fp16 without loss (but for values 2^-30 below the largest), and sum(q_g) fits.
-// p is kept at or below 8 (the running maximum is raised when a score exceeds it by 3 in powers of two), so p * s
-// fits in fp16 for every s.
+// The running maximum is kept kUp powers of two below the largest score and raised when a score exceeds it by kUp + kSlack,
+// so that p is at most 2^13 and p * s holds its 22 bits for small values as well (down to p * s = 2^-3 in those units).
+// That is for scales under 2, groups that span less than 30: a lane that holds a larger one (to 65504) has p at most 1, and
+// p * s never leaves fp16.  (Raised at every larger score, four long slots take 52.2 us instead of 49.4.)
 // Bound by memory once it runs, by its chain of loads (lengths, table, block) before: a first block takes 6.2 us, then the
 // blocks come at 5 TB/s.  8 KV heads of 128: 48 slots of 60 .. 8000 tokens 21 us and the combine 4.6, 32 slots of 16384
 // tokens 122 us (4.96 TB/s).  Three sets of registers ahead instead of two: no faster.
-constexpr float kRaise = 3.f;
+constexpr float kUp = 10.f, kSlack = 3.f;
 
 template <int HD>
 constexpr int waves_log2() { return HD == 256 ? 10 : 11; }        // one or two a SIMD of 256 CUs, as registers allow
@@ -596,8 +598,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
             mx *= kscale;
-            if (__builtin_amdgcn_ballot_w64(mx > m + kRaise) != 0) {
-                const float mn = fmaxf(m, max4(mx));
+            uint32_t any = 0;                    // bit 14 of a scale: 2 or more (or NaN)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) any |= rg.vs[g][0] | rg.vs[g][1] | rg.vs[g][2] | rg.vs[g][3];
+            const float up = any & 0x40004000u ? 0.f : kUp, slack = any & 0x40004000u ? 0.f : kUp + kSlack;
+            if (__builtin_amdgcn_ballot_w64(mx > m + slack) != 0) {
+                const float mn = fmaxf(m, max4(mx - up));
                 const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= alpha;

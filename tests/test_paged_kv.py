@@ -325,6 +325,55 @@ def test_attend_query_sizes(hiplib, cuda, dt):
             close(got[rows], want[rows], dt, q4(v).abs().max().item())
 
 
+@pytest.mark.parametrize("dt,size", [(F16, 65504.0), (F16, 60.0), (F16, 2e-3), (BF16, 3e38), (BF16, 1e6), (BF16, 1e-3)])
+def test_attend_value_sizes(hiplib, cuda, dt, size):
+    """Values from small ones to the ends of fp16 and far past them keep their precision: scales of every size times weights of
+    every size."""
+    from sx8_paged_kv import PagedKV4
+    n = 100
+    p = PagedKV4(1, 1, 64, 4, 1, 4, 32, device=cuda)
+    p.reserve(ints([n], cuda))
+    k = rand((n, 1, 64), 1, dt, cuda)
+    v = (torch.rand(n, 1, 64, generator=torch.Generator().manual_seed(2)) * 2 - 1).to(cuda)
+    v[0, 0, 0], v[0, 0, 1] = 1, -1
+    v = (v.double() * size).to(dt)
+    p.append(0, k, v, cum([n], cuda))
+    q = rand((1, 2, 64), 3, dt, cuda) * torch.tensor([1, 40], device=cuda, dtype=dt)[:, None]
+    got = p.attend(0, q).double()
+    vv = q4(v)
+    want = attention(q.double(), q4(k), vv, n - 1)
+    want = want.clamp(-torch.finfo(dt).max, torch.finfo(dt).max) if dt is F16 else want
+    err = (got - want).abs().max().item()
+    assert err <= (torch.finfo(dt).eps / 2 + LOOSE) * vv.abs().max().item()
+
+
+def test_attend_scales_that_grow(hiplib, cuda):
+    """Blocks whose values grow from nothing to fp16's ends and back: the weights' common power of two
+    follows them."""
+    from sx8_paged_kv import PagedKV4
+    sizes = [0.0, 1e-6, 1e-3, 1.0, 100.0, 65504.0, 1.0, 0.0, 30.0]
+    n = 32 * len(sizes)
+    p = PagedKV4(1, 1, 128, 9, 1, 9, 32, device=cuda)
+    p.reserve(ints([n], cuda))
+    k, v = rand((n, 1, 128), 1, F16, cuda), torch.zeros(n, 1, 128, dtype=F16, device=cuda)
+    for i, size in enumerate(sizes):
+        v[32 * i:32 * i + 32] = ((torch.rand(32, 1, 128, generator=torch.Generator().manual_seed(i)) * 2 - 1) * size).half().to(cuda)
+    p.append(0, k, v, cum([n], cuda))
+    # queries that pick out one block each, and one that sees all
+    q = torch.zeros(1, 10, 128, dtype=F16, device=cuda)
+    vv = q4(v)
+    for i in range(9):
+        q[0, i] = k[32 * i + 5, 0] * 4
+    got = p.attend(0, q).double()
+    want = attention(q.double(), q4(k), vv, n - 1)
+    # a row's bound goes by the values that it gives weight: those of its block (others weigh below 2^-50 there)
+    w = torch.softmax(torch.matmul(q[0].double(), q4(k)[:, 0].T.contiguous()) / 128 ** 0.5, -1)
+    top = (w @ vv[:, 0].abs().amax(-1, keepdim=True)).flatten()
+    for i in range(10):
+        err = (got[0, i] - want[0, i]).abs().max().item()
+        assert err <= (2.0 ** -11 + LOOSE) * max(top[i].item(), want[0, i].abs().max().item()) + 2.0 ** -25, (i, err)
+
+
 def test_attend_not_finite(hiplib, cuda):
     """NaN and infinity reach the rows that see them, and no others; garbage past the last token reaches none."""
     from sx8_paged_kv import PagedKV4
