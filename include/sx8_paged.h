@@ -7,7 +7,7 @@
  * nothing synchronised, lengths and tables are read on the device, so every call can be captured in a
  * graph.  dtype: 0 = fp16, 1 = bf16 (both as 16-bit words).  Strides are in elements; a head's hd values
  * are contiguous; pointers of rows are 16-byte aligned and their strides
- * multiples of 8; output rows may not overlap.
+ * multiples of 8; output rows may not overlap each other or what the call reads, but for out on the rows of q alone.
  *
  * The cache.  A pool has n_pages pages for each layer, a page page_tokens (32, 64, 128 or 256) tokens of
  * all nk KV heads: sx8_kv4_page_bytes bytes, [head][block of 32 tokens][block bytes].  A block is

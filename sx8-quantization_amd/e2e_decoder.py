@@ -549,6 +549,8 @@ class SX8Decoder(nn.Module):
         list of (T_i,) int64 tensors, with `prefix` (T,) in front of each of them, which is run once and whose
         pages the sequences share.  Returns (len(prompts), n_new) int64 tokens on the device."""
         n = len(prompts)
+        if n == 0 or n_new < 1:
+            raise ValueError("at least one prompt and one new token")
         first = 0 if prefix is None else prefix.shape[0]
         longest = first + max(p.shape[0] for p in prompts) + n_new
         pd = PagedDecoder(self, n + (prefix is not None), longest, page_tokens=page_tokens)
@@ -664,6 +666,7 @@ class PagedDecoder:
         pos = torch.cat([torch.arange(self.lens[s], self.lens[s] + by[s].numel(), device=self.dec.device) for s in order])
         new = [by[s].numel() if s in by else 0 for s in range(self.n_slots)]
         cu = self._ints([0] + [sum(new[:i + 1]) for i in range(self.n_slots)])
+        pb = self._bufs(ids.numel())
         self.cache.reserve(self._ints(new))
         self.cache.check()
         fresh = all(self.lens[s] == 0 for s in by)
@@ -686,11 +689,10 @@ class PagedDecoder:
                 return attn_varlen(q, k, v, cu, cu_held, scale)
             return self.cache.attend(li, q, cu, scale)
 
-        pb = self._bufs(ids.numel())
-        self._rows(pb, ids, pos, attend)
-        for s in by:
+        for s in by:                                                # (as the cache has it, whatever comes of the rows)
             self.lens[s] += new[s]
         self._set_active()
+        self._rows(pb, ids, pos, attend)
         ends = torch.tensor([int(sum(new[:s + 1])) - 1 for s in order], device=self.dec.device)
         self.logits = self._head(pb["resid"].index_select(0, ends), pb["d"].index_select(0, ends), len(order))
         nxt = self.logits.argmax(-1)
@@ -719,6 +721,8 @@ class PagedDecoder:
         self.cache.reserve(self.active)
         if any(n and n % self.cache.page_tokens == 0 for n in self.lens):
             self.cache.check()                                      # (a slot needs a page: is there one?)
+        self.lens = [n + (n > 0) for n in self.lens]
+        self._bufs(self.n_slots)                                    # (on this stream, which uses and frees them)
         if use_graph and self._graph is None:
             # once on a side stream, then captured (both write the rows that the replay writes)
             side = torch.cuda.Stream(self.dec.device)
@@ -735,7 +739,6 @@ class PagedDecoder:
             self.logits = self._graph[1]
         else:
             self.logits = self._step()
-        self.lens = [n + (n > 0) for n in self.lens]
         self.tok.copy_(self.logits.argmax(-1))
         return self.tok.clone()
 

@@ -77,7 +77,7 @@ def attn_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
     bf16, sequence b the query rows cu_q[b] .. cu_q[b + 1] - 1 and the keys cu_k[b] .. cu_k[b + 1] - 1 (int32 on
     the device; cu_k = None: cu_q, keys and queries of the same tokens).  causal: the last query of a
     sequence attends all of its keys, the one before it one key less, and so on; a query with no key gives
-    zeros.  Rows of no sequence are left as they are (in a new `out`: unset).  hd 64, 128 or 256; scale
+    zeros.  Rows of no sequence are left as they are (in a new `out`: unset); out shares no memory with k and v.  hd 64, 128 or 256; scale
     1 / sqrt(hd) unless given.  Forward only.  Returns out (Tq, heads, hd)."""
     if out is None and q.dim() == 3:
         got = _L.py().varlen(q, k, v, cu_q, cu_k, _scale(scale, q.shape[2]), causal)
@@ -95,6 +95,8 @@ def attn_varlen(q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None):
         k = _rows("k", k, nk, hd, q.device, q.dtype, hd)
         v = _rows("v", v, nk, hd, q.device, q.dtype, hd)
         out = _out("out", out, q, nh, hd)
+        if out.data_ptr() and out.data_ptr() in (k.data_ptr(), v.data_ptr()):
+            raise RuntimeError("out may not be k or v")
         _ints("cu_q", cu_q, None, q.device)
         _ints("cu_k", cu_k, cu_q.numel(), q.device)
         nb = int(_L.lib().sx8_attn_varlen_workspace_bytes(cu_q.numel() - 1, q.shape[0], k.shape[0], nh, hd))
@@ -208,6 +210,8 @@ class PagedKV4:
                 out = tuple(torch.empty(int(rows), self.n_kv, self.head_dim, dtype=dtype, device=self.device)
                             for _ in range(2))
             k, v = (_out(n, t, like, self.n_kv, self.head_dim) for n, t in zip(("k", "v"), out))
+            if k.shape[0] and k.data_ptr() == v.data_ptr():
+                raise RuntimeError("k and v may not share memory")
             _L.call("sx8_kv4_read", *self._slots(layer, cu), k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1),
                     v.stride(0), v.stride(1), self.n_kv, self.head_dim, self.page_tokens, _DTYPES[dtype],
                     _L.stream(self.device))

@@ -197,3 +197,30 @@ def test_paged_decoder_refuses(dec, cuda):
     pd.step()
     pd.cache.check()
     assert pd.cache.lens.tolist() == pd.lens == [33, 0]
+
+
+def test_generate_batch_refuses(dec, cuda):
+    d, _ = dec
+    for prompts, n in (([], 3), ([ids(3, 1, cuda)], 0), ([ids(3, 1, cuda)], 500), ([ids(0, 1, cuda)], 2)):
+        with pytest.raises(ValueError):
+            d.generate_batch(prompts, n)
+
+
+def test_a_pass_that_fails_midway(dec, cuda, monkeypatch):
+    """Where the layers raise, the decoder's lengths are still the cache's: the slot can be freed and used again."""
+    from e2e_decoder import PagedDecoder
+    d, _ = dec
+    pd = PagedDecoder(d, 2, max_len=64, page_tokens=32)
+    pd.prompt([0], [ids(9, 1, cuda)])
+    with monkeypatch.context() as m:
+        m.setattr(pd, "_rows", lambda *a: (_ for _ in ()).throw(MemoryError()))
+        with pytest.raises(MemoryError):
+            pd.prompt([1], [ids(5, 2, cuda)])
+        with pytest.raises(MemoryError):
+            pd.step(use_graph=False)
+    assert pd.lens == pd.cache.lens.tolist() == [10, 6]
+    pd.free([0, 1])
+    a = pd.prompt([0, 1], [ids(9, 1, cuda), ids(5, 2, cuda)])
+    fresh = PagedDecoder(d, 2, max_len=64, page_tokens=32)
+    assert torch.equal(a, fresh.prompt([0, 1], [ids(9, 1, cuda), ids(5, 2, cuda)]))
+    assert torch.equal(pd.step(), fresh.step())

@@ -791,6 +791,29 @@ def test_varlen_long(hiplib, cuda):
         assert torch.equal(got, attn_varlen(q, k, v, cum([2500], cuda)))
 
 
+def test_outputs_on_inputs(hiplib, cuda):
+    """out on the rows of q; outputs that are each other or K or V are refused."""
+    from sx8_paged_kv import attn_varlen
+    for nkeys in (300, 6000):                                           # (whole, in parts)
+        q, k, v = rand((300, 4, 128), 1, F16, cuda), rand((nkeys, 4, 128), 2, F16, cuda), rand((nkeys, 4, 128), 3, F16, cuda)
+        v[7] = math.nan
+        cq, ck = cum([300], cuda), cum([nkeys], cuda)
+        want = attn_varlen(q, k, v, cq, ck)
+        for bad in (k, v):
+            if nkeys == 300:
+                with pytest.raises(RuntimeError, match="k or v"):
+                    attn_varlen(q, k, v, cq, ck, out=bad)
+        attn_varlen(q, k, v, cq, ck, out=q)
+        assert torch.equal(q.view(torch.int16), want.view(torch.int16))
+    p, _, _ = make(cuda, [900, 64], 2, 128, 64)
+    q = rand((2, 8, 128), 1, F16, cuda)
+    want = p.attend(0, q)
+    assert torch.equal(p.attend(0, q, out=q), want)
+    x = torch.empty(2, 2, 128, dtype=F16, device=cuda)
+    with pytest.raises(RuntimeError, match="share memory"):
+        p.read(0, 2, out=(x, x))
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("dt", [F16, BF16])
 def test_varlen_few_rows_many_keys(hiplib, cuda, hd, dt):
