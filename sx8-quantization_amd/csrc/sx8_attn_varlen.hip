@@ -254,7 +254,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
-    // running maximum in powers of two, raised when a score exceeds it by more than 8: probabilities stay at or below 2^8
+    // running maximum in powers of two, kept kUp below the largest score and raised when one exceeds it by more than kUp + 8:
+    // probabilities stay at or below 2^15 in fp16, where many small ones (each over 2^-21 of the largest) keep their 11
+    // bits, and at or below 2^8 in bf16, which holds small ones as well as large
+    constexpr float kUp = kBf16 ? 0.f : 7.f;
     float m = -kInf, l = 0.f;
     // V^T reads: key and dimension that the lane names
     const int vi = lane & 15, vd = (lane >> 4 & 1) * 16 + 4 * (vi & 3), vk = 4 * h + (vi >> 2);
@@ -289,8 +292,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[a][r]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * io.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
-            const float mn = fmaxf(m, mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m + (kUp + 8.f)) != 0) {
+            const float mn = fmaxf(m, mx - kUp);
             const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= alpha;

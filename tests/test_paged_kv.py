@@ -791,6 +791,19 @@ def test_varlen_long(hiplib, cuda):
         assert torch.equal(got, attn_varlen(q, k, v, cum([2500], cuda)))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_varlen_many_small_weights(hiplib, cuda, dt):
+    """A key with nearly all of the weight and 100000 with 2^-22.7 of it each: each weight is within eps / 2 of itself."""
+    from sx8_paged_kv import attn_varlen
+    n, s = 100001, 15.76
+    q = torch.zeros(1, 1024, 64, dtype=dt, device=cuda)
+    k, v = torch.zeros(n, 1, 64, dtype=dt, device=cuda), torch.ones(n, 1, 64, dtype=dt, device=cuda)
+    q[..., 0], k[0, 0, 0], v[0] = 8, 2, 0
+    got = attn_varlen(q, k, v, cum([1], cuda), cum([n], cuda), scale=s / 16)
+    w = (n - 1) * math.exp(-s)
+    close(got, torch.full_like(got, w / (1 + w), dtype=torch.float64), dt, 1.0, torch.finfo(dt).eps / 2)
+
+
 def test_outputs_on_inputs(hiplib, cuda):
     """out on the rows of q; outputs that are each other or K or V are refused."""
     from sx8_paged_kv import attn_varlen
