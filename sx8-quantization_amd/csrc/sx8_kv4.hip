@@ -37,42 +37,45 @@ __device__ __forceinline__ int64_t block_offset(const Kv4Pool& p, int slot, int 
 // slots 5.8, where the chain of lengths, table and rows is all there is.
 struct Enc {
     float s, m;
-    uint32_t lv[8];
+    uint32_t lv[8];               // kLevel0 + level
 };
+constexpr uint32_t kLevel0 = 0x4B400000u;      // 1.5 2^23 as a float: adding it rounds to an integer, in the low bits
 
-// The level of x: (x - m) / s to the nearest, ties to even.  In binary32 the quotient is within 2^-18 of the true one (two
-// roundings of a number below 32 and one of 1 / s), so only a quotient within 2^-16 of a border is decided in binary64:
-// there x - m is exact for fp16 rows, and the rounded quotient is put right by its exact remainder.  (All of them in
-// binary64: 13081 rows of 8 heads of 128, K and V, 50 us against 27.)
-__device__ __forceinline__ uint32_t level_of(float x, float m, float s, float inv) {
+// The level of x: (x - m) / s to the nearest, ties to even, in exact arithmetic: x - m is exact in binary64, and the
+// rounded quotient is put right by its exact remainder.
+__device__ __noinline__ uint32_t exact_level(float x, float m, float s) {
 #pragma clang fp contract(off)
-    const float t = (x - m) * inv;
-    float n = __builtin_rintf(t);
-    if (!(__builtin_fabsf(t - n) < 0.5f - 0x1p-16f) && t > -1.f && t < 16.f) {
-        const double d = (double)x - (double)m, s64 = s;
-        double q = __builtin_rint(d / s64);
-        const double rem = d - q * s64;
-        const bool odd = (int)q & 1;
-        if (2.0 * rem > s64 || (2.0 * rem == s64 && odd)) q += 1.0;
-        else if (-2.0 * rem > s64 || (-2.0 * rem == s64 && odd)) q -= 1.0;
-        n = (float)q;
-    }
-    return (uint32_t)(int)fminf(fmaxf(n, 0.f), 15.f);
+    const double d = (double)x - (double)m, s64 = s;
+    double q = __builtin_rint(d / s64);
+    const double rem = d - q * s64;
+    const bool odd = (int)q & 1;
+    if (2.0 * rem > s64 || (2.0 * rem == s64 && odd)) q += 1.0;
+    else if (-2.0 * rem > s64 || (-2.0 * rem == s64 && odd)) q -= 1.0;
+    return kLevel0 + (uint32_t)(int)fmin(fmax(q, 0.0), 15.0);
 }
 
-// rows outside the call come as zeros (their results are unused)
-__device__ __forceinline__ void encode_group(const float (&x)[8], Enc& e) {
+// In binary32 the quotient is within 2^-17 of the true one (below 16; two roundings and a reciprocal to one place in 2^-23),
+// so only a quotient within 2^-16 of a border is decided by exact_level: one look for the lane's eight values.  (A look
+// for each of them: 13081 rows of 8 heads of 128, K and V, 27 us; all of them in binary64: 50.)
+// Rows outside the call come as zeros (their results are unused).
+template <bool kBf16>
+__device__ __forceinline__ void encode_group(const u32x4& raw, Enc& e) {
 #pragma clang fp contract(off)
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = ld16<kBf16>(half_of(raw[i >> 1], i));
     float lo = x[0], hi = x[0];
-    bool bad = false;
+    u16x2 top = {0, 0};           // magnitudes order as integers, NaN above all
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         lo = fminf(lo, x[i]);
         hi = fmaxf(hi, x[i]);
-        bad |= !(__builtin_fabsf(x[i]) < __builtin_inff());
     }
-    // over the eight lanes of the group; a bad one makes both ends NaN for all of them
-    if (bad) lo = hi = __builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, (uint32_t)(raw[i] & 0x7FFF7FFFu)));
+    // over the eight lanes of the group; a bad one makes both ends infinite for all of them
+    if (max(top[0], top[1]) >= (kBf16 ? 0x7F80 : 0x7C00)) lo = hi = __builtin_inff();
     lo = fminf(lo, dpp_lane<0xB1>(lo));
     hi = fmaxf(hi, dpp_lane<0xB1>(hi));
     lo = fminf(lo, dpp_lane<0x4E>(lo));
@@ -83,9 +86,22 @@ __device__ __forceinline__ void encode_group(const float (&x)[8], Enc& e) {
     const float r = hi - lo;
     e.s = none ? __builtin_nanf("") : (float)(_Float16)fminf(r * (1.0f / 15.0f), 65504.0f);
     e.m = none ? __builtin_nanf("") : (float)(_Float16)fminf(fmaxf(lo, -65504.0f), 65504.0f);
-    const float inv = 1.0f / e.s;
+    const float inv = e.s > 0.f ? __builtin_amdgcn_rcpf(e.s) : 0.f;
+    const float big = __builtin_bit_cast(float, kLevel0);
+    float u[8], far = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e.lv[i] = e.s > 0.f ? level_of(x[i], e.m, e.s, inv) : 0u;
+    for (int i = 0; i < 8; ++i) {
+        u[i] = fminf(fmaxf((x[i] - e.m) * inv, 0.f), 15.f);       // (NaN: 0)
+        const float n = u[i] + big;
+        e.lv[i] = __builtin_bit_cast(uint32_t, n);
+        u[i] = u[i] - (n - big);
+        far = fmaxf(far, __builtin_fabsf(u[i]));
+    }
+    if (far >= 0.5f - 0x1p-16f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (__builtin_fabsf(u[i]) >= 0.5f - 0x1p-16f) e.lv[i] = exact_level(x[i], e.m, e.s);
+    }
 }
 
 // The block that work item `item` of the call names: slot, its block, and the new tokens in it (block-relative
@@ -173,20 +189,22 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsI
             const int ch = tid + 256 * i;
             if (ch >= nt * CPR) break;                              // (eight lanes of a group alike: CPR is a multiple of 8)
             const int tok = t.t0 + ch / CPR, d0 = ch % CPR * 8, g = d0 / kKv4Group;
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = ld16<kBf16>(half_of(raw[which][i][e >> 1], e));
             Enc en;
-            encode_group(x, en);
+            encode_group<kBf16>(raw[which][i], en);
+            // (kLevel0 is taken off the sums: its bits up to 21 are zero)
             if (which == 0) {
-                uint32_t word = 0;
+                uint32_t word = 0u - (kLevel0 + (kLevel0 << 4) + (kLevel0 << 8));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) word |= en.lv[e] << kv4_shift(e);
+                for (int e = 0; e < 8; ++e) word += en.lv[e] << kv4_shift(e);
                 *reinterpret_cast<uint32_t*>(blk + kv4_k_word(HD, tok, d0)) = word;
             } else {
-                u32x2 bytes = {0u, 0u};
+                u32x2 bytes;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) bytes[e >> 2] |= en.lv[e] << 8 * (e & 3);
+                for (int w = 0; w < 2; ++w) {
+                    bytes[w] = 0u - (kLevel0 + (kLevel0 << 8));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bytes[w] += en.lv[4 * w + e] << 8 * e;
+                }
                 *reinterpret_cast<u32x2*>(&lv[tok][d0]) = bytes;
             }
             if (tid % 8 == 0) {
@@ -195,20 +213,26 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsI
             }
         }
     __syncthreads();
-    for (int i = tid; i < HD * 4; i += 256) {
-        const int d = i % HD, h = i / HD;                           // word: tokens 4 h + r and 16 + 4 h + r
-        uint32_t word = 0, fresh = 0;
+    // words of four dimensions d0 .. d0 + 3: tokens 4 h + r and 16 + 4 h + r
+    for (int i = tid; i < HD; i += 256) {
+        const int h = i / (HD / 4), d0 = i % (HD / 4) * 4;
+        uint32_t b[8], fresh = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int tok = e / 4 * 16 + 4 * h + e % 4;
-            if (tok >= t.t0 && tok < t.t1) {
-                word |= (uint32_t)lv[tok][d] << kv4_shift(e);
-                fresh |= 15u << kv4_shift(e);
-            }
+            b[e] = *reinterpret_cast<const uint32_t*>(&lv[tok][d0]) & 0x0F0F0F0Fu;     // (old tokens' bytes were never set)
+            if (tok >= t.t0 && tok < t.t1) fresh |= 15u << kv4_shift(e);
         }
         if (fresh == 0) continue;
-        uint32_t* const at = reinterpret_cast<uint32_t*>(blk + kv4_v_word(HD, 4 * h, d));
-        *at = fresh == 0xFFFFFFFFu ? word : (*at & ~fresh) | word;
+        // bytes of four dimensions with the levels of two tokens each; byte j of a word is byte d of c[j]
+        const uint32_t c[4] = {b[0] | b[2] << 4, b[4] | b[6] << 4, b[1] | b[3] << 4, b[5] | b[7] << 4};
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const uint32_t word = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0C0C0400u + 0x0101u * d),
+                                                        __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u + 0x0101u * d), 0x05040100u);
+            uint32_t* const at = reinterpret_cast<uint32_t*>(blk + kv4_v_word(HD, 4 * h, d0 + d));
+            *at = fresh == 0xFFFFFFFFu ? word : (*at & ~fresh) | (word & fresh);
+        }
     }
 }
 
