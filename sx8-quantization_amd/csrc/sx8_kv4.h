@@ -25,21 +25,21 @@ SX8_KV4_FN constexpr int kv4_block_bytes(int hd) { return 32 * hd + hd / kKv4Gro
 SX8_KV4_FN constexpr int kv4_shift(int e) { return 4 * (e >> 1) + 16 * (e & 1); }
 
 // Byte offset in the block of the word that holds dimension d of token t, and the bit it starts at.
-SX8_KV4_FN int kv4_k_word(int hd, int t, int d) {
-    const int W = hd / 32, wi = W < 4 ? W : 4, j = d / 32, lane = (d % 32) / 8 * 16 + t % 16;
+SX8_KV4_FN uint32_t kv4_k_word(uint32_t hd, uint32_t t, uint32_t d) {
+    const uint32_t W = hd / 32, wi = W < 4 ? W : 4, j = d / 32, lane = (d % 32) / 8 * 16 + t % 16;
     return t / 16 * (256 * W) + (j / wi * 64 + lane) * wi * 4 + j % wi * 4;
 }
 SX8_KV4_FN int kv4_k_shift(int d) { return kv4_shift(d % 8); }
-SX8_KV4_FN int kv4_v_word(int hd, int t, int d) {
-    const int lane = (t % 16) / 4 * 16 + d % 16, tile = d / 16;
+SX8_KV4_FN uint32_t kv4_v_word(uint32_t hd, uint32_t t, uint32_t d) {
+    const uint32_t lane = (t % 16) / 4 * 16 + d % 16, tile = d / 16;
     return 16 * hd + (tile / 4 * 64 + lane) * 16 + tile % 4 * 4;
 }
 SX8_KV4_FN int kv4_v_shift(int t) { return kv4_shift(t / 16 * 4 + t % 4); }
 
 // Scales of K (which = 0) and V (2) and minima of V (3) by group, step group h and token slot; minima of K (1)
 // by token and group.
-SX8_KV4_FN int kv4_param(int hd, int which, int t, int g) {
-    const int ng = hd / kKv4Group, base = 32 * hd + which * ng * 64;
+SX8_KV4_FN uint32_t kv4_param(uint32_t hd, uint32_t which, uint32_t t, uint32_t g) {
+    const uint32_t ng = hd / kKv4Group, base = 32 * hd + which * ng * 64;
     return which == 1 ? base + 2 * (t * ng + g) : base + 2 * (g * 32 + (t % 16) / 4 * 8 + t / 16 * 4 + t % 4);
 }
 

@@ -54,53 +54,70 @@ __device__ __noinline__ uint32_t exact_level(float x, float m, float s) {
     return kLevel0 + (uint32_t)(int)fmin(fmax(q, 0.0), 15.0);
 }
 
-// In binary32 the quotient is within 2^-17 of the true one (below 16; two roundings and a reciprocal to one place in 2^-23),
-// so only a quotient within 2^-16 of a border is decided by exact_level: one look for the lane's eight values.  (A look
-// for each of them: 13081 rows of 8 heads of 128, K and V, 27 us; all of them in binary64: 50.)
+// x[i] - m of the eight rows' values (fp16: without a conversion of its own)
+template <bool kBf16, int kHalf>
+__device__ __forceinline__ float less(uint32_t word, float m) {
+    if constexpr (kBf16) return ld16<true>(half_of(word, kHalf)) - m;
+    float d;
+    if constexpr (kHalf) asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(word), "v"(m));
+    else asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(word), "v"(m));
+    return d;
+}
+
+// The ends of a group come from integers that order as the values do (infinities and NaN beyond all others), the minimum and
+// the complement of the maximum in one word.  In binary32 the quotient is within 2^-17 of the true one (a fifteenth of it is
+// within 2.5 2^-23 of itself: three roundings, and a reciprocal good to one place), so only a quotient within 2^-16 of a
+// border is decided by exact_level: one look for the lane's eight values.  (A look for each of them, and the ends in
+// binary32: 13081 rows of 8 heads of 128, K and V, 27 us; all quotients in binary64: 50.)
 // Rows outside the call come as zeros (their results are unused).
 template <bool kBf16>
 __device__ __forceinline__ void encode_group(const u32x4& raw, Enc& e) {
 #pragma clang fp contract(off)
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    float x[8];
+    typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+    constexpr int kLowest = ~(kBf16 ? 0x7F80 : 0x7C00);          // -infinity
+    auto ordered = [](uint32_t w) {
+        const uint32_t sign = __builtin_bit_cast(uint32_t, (i16x2)(__builtin_bit_cast(i16x2, w) >> 15));
+        return w ^ (sign & 0x7FFF7FFFu);
+    };
+    auto least = [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(i16x2, a), __builtin_bit_cast(i16x2, b)));
+    };
+    uint32_t lows = ordered(raw[0]), highs = ~lows;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ld16<kBf16>(half_of(raw[i >> 1], i));
-    float lo = x[0], hi = x[0];
-    u16x2 top = {0, 0};           // magnitudes order as integers, NaN above all
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
+    for (int i = 1; i < 4; ++i) {
+        const uint32_t w = ordered(raw[i]);
+        lows = least(lows, w);
+        highs = least(highs, ~w);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, (uint32_t)(raw[i] & 0x7FFF7FFFu)));
-    // over the eight lanes of the group; a bad one makes both ends infinite for all of them
-    if (max(top[0], top[1]) >= (kBf16 ? 0x7F80 : 0x7C00)) lo = hi = __builtin_inff();
-    lo = fminf(lo, dpp_lane<0xB1>(lo));
-    hi = fmaxf(hi, dpp_lane<0xB1>(hi));
-    lo = fminf(lo, dpp_lane<0x4E>(lo));
-    hi = fmaxf(hi, dpp_lane<0x4E>(hi));
-    lo = fminf(lo, dpp_lane<0x141>(lo));
-    hi = fmaxf(hi, dpp_lane<0x141>(hi));
-    const bool none = !(hi < __builtin_inff());
-    const float r = hi - lo;
+    // low half: the minimum, high half: the complement of the maximum; over the eight lanes of the group
+    uint32_t ends = least(__builtin_amdgcn_perm(highs, lows, 0x05040100u), __builtin_amdgcn_perm(highs, lows, 0x07060302u));
+    ends = least(ends, __builtin_amdgcn_mov_dpp((int)ends, 0xB1, 0xF, 0xF, true));
+    ends = least(ends, __builtin_amdgcn_mov_dpp((int)ends, 0x4E, 0xF, 0xF, true));
+    ends = least(ends, __builtin_amdgcn_mov_dpp((int)ends, 0x141, 0xF, 0xF, true));
+    const bool none = min((int)(int16_t)ends, (int)ends >> 16) <= kLowest;
+    const uint32_t both = ordered(ends ^ 0xFFFF0000u);
+    const float lo = ld16<kBf16>(both & 0xFFFFu), r = ld16<kBf16>(both >> 16) - lo;
     e.s = none ? __builtin_nanf("") : (float)(_Float16)fminf(r * (1.0f / 15.0f), 65504.0f);
     e.m = none ? __builtin_nanf("") : (float)(_Float16)fminf(fmaxf(lo, -65504.0f), 65504.0f);
-    const float inv = e.s > 0.f ? __builtin_amdgcn_rcpf(e.s) : 0.f;
+    const float part = e.s > 0.f ? __builtin_amdgcn_rcpf(e.s) * (1.0f / 15.0f) : 0.f;
     const float big = __builtin_bit_cast(float, kLevel0);
-    float u[8], far = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        u[i] = fminf(fmaxf((x[i] - e.m) * inv, 0.f), 15.f);       // (NaN: 0)
-        const float n = u[i] + big;
+    float off[8], far = 0.f;
+    auto level = [&](int i, float d) {
+        const float u = fminf(fmaxf(d * part, 0.f), 1.f);        // (NaN: 0)
+        const float n = __builtin_fmaf(u, 15.f, big);
         e.lv[i] = __builtin_bit_cast(uint32_t, n);
-        u[i] = u[i] - (n - big);
-        far = fmaxf(far, __builtin_fabsf(u[i]));
+        off[i] = __builtin_fmaf(u, 15.f, big - n);
+        far = fmaxf(far, __builtin_fabsf(off[i]));
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        level(2 * i, less<kBf16, 0>(raw[i], e.m));
+        level(2 * i + 1, less<kBf16, 1>(raw[i], e.m));
     }
     if (far >= 0.5f - 0x1p-16f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (__builtin_fabsf(u[i]) >= 0.5f - 0x1p-16f) e.lv[i] = exact_level(x[i], e.m, e.s);
+            if (__builtin_fabsf(off[i]) >= 0.5f - 0x1p-16f) e.lv[i] = exact_level(ld16<kBf16>(half_of(raw[i >> 1], i)), e.m, e.s);
     }
 }
 
@@ -170,15 +187,17 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsI
     const int64_t off = block_offset(p, t.slot, head, t.block, kBB);
     const int nt = t.t1 - t.t0;
     // every row of the block's share is requested before the first is encoded (and while the page number is on its way)
+    constexpr int kStep = 256 / CPR;                                // rows between a thread's chunks
     u32x4 raw[2][NI];
+    {
+        const uint16_t* const k = in.k + t.row0 * in.k_ts + head * in.k_hs + ((uint32_t)tid / CPR * in.k_ts + tid % CPR * 8);
+        const uint16_t* const v = in.v + t.row0 * in.v_ts + head * in.v_hs + ((uint32_t)tid / CPR * in.v_ts + tid % CPR * 8);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int ch = tid + 256 * i;
-        if (ch < nt * CPR) {
-            const int64_t row = t.row0 + ch / CPR;
-            raw[0][i] = *reinterpret_cast<const u32x4*>(in.k + row * in.k_ts + head * in.k_hs + ch % CPR * 8);
-            raw[1][i] = *reinterpret_cast<const u32x4*>(in.v + row * in.v_ts + head * in.v_hs + ch % CPR * 8);
-        }
+        for (int i = 0; i < NI; ++i)
+            if (tid + 256 * i < nt * CPR) {
+                raw[0][i] = *reinterpret_cast<const u32x4*>(k + i * (kStep * in.k_ts));
+                raw[1][i] = *reinterpret_cast<const u32x4*>(v + i * (kStep * in.v_ts));
+            }
     }
     if (off < 0) return;                                            // (uniform)
     uint8_t* const blk = const_cast<uint8_t*>(p.pages) + off;
@@ -189,22 +208,20 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Pool p, const RowsI
             const int ch = tid + 256 * i;
             if (ch >= nt * CPR) break;                              // (eight lanes of a group alike: CPR is a multiple of 8)
             const int tok = t.t0 + ch / CPR, d0 = ch % CPR * 8, g = d0 / kKv4Group;
+            __builtin_assume(tok >= 0 && tok < 32);
             Enc en;
             encode_group<kBf16>(raw[which][i], en);
-            // (kLevel0 is taken off the sums: its bits up to 21 are zero)
+            // (the low 22 bits of lv are the level)
             if (which == 0) {
-                uint32_t word = 0u - (kLevel0 + (kLevel0 << 4) + (kLevel0 << 8));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) word += en.lv[e] << kv4_shift(e);
-                *reinterpret_cast<uint32_t*>(blk + kv4_k_word(HD, tok, d0)) = word;
+                const uint32_t even = en.lv[0] | en.lv[2] << 4 | en.lv[4] << 8 | en.lv[6] << 12;
+                const uint32_t odd = en.lv[1] | en.lv[3] << 4 | en.lv[5] << 8 | en.lv[7] << 12;
+                *reinterpret_cast<uint32_t*>(blk + kv4_k_word(HD, tok, d0)) = __builtin_amdgcn_perm(odd, even, 0x05040100u);
             } else {
                 u32x2 bytes;
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    bytes[w] = 0u - (kLevel0 + (kLevel0 << 8));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) bytes[w] += en.lv[4 * w + e] << 8 * e;
-                }
+                for (int w = 0; w < 2; ++w)
+                    bytes[w] = __builtin_amdgcn_perm(en.lv[4 * w + 1], en.lv[4 * w], 0x0C0C0400u) |
+                               __builtin_amdgcn_perm(en.lv[4 * w + 3], en.lv[4 * w + 2], 0x04000C0Cu);
                 *reinterpret_cast<u32x2*>(&lv[tok][d0]) = bytes;
             }
             if (tid % 8 == 0) {
