@@ -23,10 +23,11 @@ namespace {
 // reaches 1100-1150.  Short prompts are bound by a work-group's start (about 5 us: lengths, query, first tile): 24 of
 // 40 .. 2000 tokens 230 us, three of up to 96 tokens 7.  s_setprio around the products (541 us against 533), tiles of 32
 // keys with three waves a SIMD (544 against 528) and work-groups that stay and request the next rows ahead (561 against
-// 515) were slower.
+// 515) were slower.  Heads of 256 leave room for one wave a SIMD: 8192 tokens of 16 heads over 4 take 699 us (787 TFLOP/s;
+// tiles of 32 keys 719); the next tile's scores computed beside this one's softmax 767 (881 with tiles of 32).
 template <int HD>
 struct VarTile {
-    static constexpr int kKeys = HD == 256 ? 32 : 64;        // of a tile
+    static constexpr int kKeys = 64;                         // of a tile
     static constexpr int kChunks = HD / 8;                   // 16-byte chunks of a row
     static constexpr int kBytes = kKeys * HD * 2;            // of K or V
     __device__ static int k_swz(int row) { return row & (HD == 128 ? 15 : 7); }
