@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     const uint16_t* const kp = io.k + k_first * io.k_ts + kvh * io.k_hs;
     const uint16_t* const vp = io.v + k_first * io.v_ts + kvh * io.v_hs;
     // loads: a wave instruction fills 1 KB of LDS; instruction i of wave w holds rows (4 i + w) R .. (R = 512 / HD
-    // rows; for HD 256 half of one each), R rows apart by waves so that a lane's row keeps its low bits over i
+    // rows), R rows apart by waves so that a lane's row keeps its low bits over i
     // (the whole offset goes into the load's vector offset: only that one is checked against the buffer's end)
     constexpr int R = 64 / CH, NI = T::kBytes / 4096;
     const int lrow = w * R + lane / CH, lpos = lane % CH;

@@ -750,50 +750,49 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
     }
 }
 
-// Units that were cut: work-group i takes the record i and kRows of its 16 rows, and adds the unit's parts up in their order
-// (part 0 at its place, part j at place 2 (wave + j)).  A row's parts are shared by 16 / kRows waves, whose sums meet in LDS.
-template <int HD, bool kBf16, int kRows>
-__global__ __launch_bounds__(1024) void k_kv4_combine(const AttendIo io, int G) {
-    constexpr int N = HD / 64, kShares = 16 / kRows, kU = 8;      // kU: parts requested together
+// Units that were cut: work-group (i, row) takes a row of record i and adds the unit's parts up in their order (part 0 at its
+// place, part j at place 2 (wave + j)).  The parts are shared by kWaves waves, whose sums meet in LDS.  A launch costs 1.8
+// us and three dependent loads; 48 slots of up to 8000 tokens take 4.7 us, 16 slots of 8 new tokens 5.8 (work-groups of
+// 16 waves for four rows at once: 5.9 and 6.5; two waves a row: 4.8 and 5.1, but twice the rounds where one slot of
+// many has most of the tokens).
+template <int HD, bool kBf16, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void k_kv4_combine(const AttendIo io, int G) {
+    constexpr int N = HD / 64, kU = 8;                            // kU: parts requested together
     typedef float vecN __attribute__((ext_vector_type(N)));
     const Kv4Piece pc = io.piece[blockIdx.x];
-    const int row0 = kRows * blockIdx.y, rows = min(16, pc.n * G - 16 * pc.tile);
-    if (pc.parts == 0 || row0 >= rows) return;
+    const int row = blockIdx.y;
+    if (pc.parts == 0 || row >= min(16, pc.n * G - 16 * pc.tile)) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int mine = w % kShares, row = row0 + w / kShares;
-    __shared__ float sml[16][2];
-    __shared__ vecN so[16][64];
-    const bool live = row < rows;
+    __shared__ float sml[kWaves][2];
+    __shared__ vecN so[kWaves][64];
     auto at = [&](int i) { return (int64_t)(i == 0 ? pc.first : 2 * (pc.first / 2 + i)) * 16 + row; };
-    const int per = (pc.parts + kShares - 1) / kShares, i0 = mine * per, i1 = min(i0 + per, pc.parts);
+    const int per = (pc.parts + kWaves - 1) / kWaves, i0 = w * per, i1 = min(i0 + per, pc.parts);
     float m = -__builtin_inff(), den = 0.f;
     vecN acc = 0.f;
-    if (live) {
-        for (int i = i0; i < i1; i += kU) {
-            float pm[kU], pl[kU];
-            vecN v[kU];
+    for (int i = i0; i < i1; i += kU) {
+        float pm[kU], pl[kU];
+        vecN v[kU];
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int64_t a = at(min(i + u, i1 - 1));
-                pm[u] = io.part_ml[a * 2];
-                pl[u] = io.part_ml[a * 2 + 1];
-                v[u] = reinterpret_cast<const vecN*>(io.part_o + a * HD)[lane];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            float mn = m;
+        for (int u = 0; u < kU; ++u) {
+            const int64_t a = at(min(i + u, i1 - 1));
+            pm[u] = io.part_ml[a * 2];
+            pl[u] = io.part_ml[a * 2 + 1];
+            v[u] = reinterpret_cast<const vecN*>(io.part_o + a * HD)[lane];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float mn = m;
 #pragma unroll
-            for (int u = 0; u < kU; ++u) mn = fmaxf(mn, pm[u]);
-            const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            den *= alpha;
-            acc *= alpha;
+        for (int u = 0; u < kU; ++u) mn = fmaxf(mn, pm[u]);
+        const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        den *= alpha;
+        acc *= alpha;
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                if (i + u >= i1) continue;
-                const float f = pm[u] == m ? 1.f : __builtin_amdgcn_exp2f(pm[u] - m);
-                den = __builtin_fmaf(f, pl[u], den);
-                acc = __builtin_elementwise_fma(vecN(f), v[u], acc);
-            }
+        for (int u = 0; u < kU; ++u) {
+            if (i + u >= i1) continue;
+            const float f = pm[u] == m ? 1.f : __builtin_amdgcn_exp2f(pm[u] - m);
+            den = __builtin_fmaf(f, pl[u], den);
+            acc = __builtin_elementwise_fma(vecN(f), v[u], acc);
         }
     }
     if (lane == 0) {
@@ -802,18 +801,18 @@ __global__ __launch_bounds__(1024) void k_kv4_combine(const AttendIo io, int G) 
     }
     so[w][lane] = acc;
     __syncthreads();
-    if (mine != 0 || !live) return;
+    if (w != 0) return;
     float mm = m;
 #pragma unroll
-    for (int i = 1; i < kShares; ++i) mm = fmaxf(mm, sml[w + i][0]);
+    for (int i = 1; i < kWaves; ++i) mm = fmaxf(mm, sml[i][0]);
     const float f0 = m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm);
     den *= f0;
     acc *= f0;
 #pragma unroll
-    for (int i = 1; i < kShares; ++i) {
-        const float f = sml[w + i][0] == mm ? 1.f : __builtin_amdgcn_exp2f(sml[w + i][0] - mm);
-        den = __builtin_fmaf(f, sml[w + i][1], den);
-        acc = __builtin_elementwise_fma(vecN(f), so[w + i][lane], acc);
+    for (int i = 1; i < kWaves; ++i) {
+        const float f = sml[i][0] == mm ? 1.f : __builtin_amdgcn_exp2f(sml[i][0] - mm);
+        den = __builtin_fmaf(f, sml[i][1], den);
+        acc = __builtin_elementwise_fma(vecN(f), so[i][lane], acc);
     }
     acc *= den == 0.f ? 0.f : 1.f / den;
     const int rr = 16 * pc.tile + row, tk = rr / G;
@@ -981,11 +980,9 @@ extern "C" int32_t sx8_kv4_attend(const uint8_t* pages, const int32_t* table, co
         constexpr bool kBf = decltype(b)::value;
         hipLaunchKernelGGL((k_kv4_attend<HD, kBf>), dim3((1 << waves_log2<HD>()) / 4), dim3(256),
                            n_slots <= 64 ? 0 : prefix_bytes(p) * 3 / 2, as_stream(stream), p, io);
-        if (narrow)
-            hipLaunchKernelGGL((k_kv4_combine<HD, kBf, 1>), dim3(entries, used), dim3(1024), 0, as_stream(stream), io, p.sh.G);
-        else
-            hipLaunchKernelGGL((k_kv4_combine<HD, kBf, 4>), dim3(entries, (used + 3) / 4), dim3(1024), 0, as_stream(stream), io,
-                               p.sh.G);
+        const dim3 grid(entries, used);
+        if (narrow) hipLaunchKernelGGL((k_kv4_combine<HD, kBf, 16>), grid, dim3(1024), 0, as_stream(stream), io, p.sh.G);
+        else hipLaunchKernelGGL((k_kv4_combine<HD, kBf, 4>), grid, dim3(256), 0, as_stream(stream), io, p.sh.G);
     });
     return check_launch(what);
 }
