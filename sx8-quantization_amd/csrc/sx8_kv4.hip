@@ -33,8 +33,8 @@ __device__ __forceinline__ int64_t block_offset(const Kv4Pool& p, int slot, int 
 // Eight lanes hold a group of 64 values (16 bytes each): minimum and maximum by three lane exchanges, then each
 // lane's eight levels.  K's eight levels of a lane are one word; V's word holds eight tokens of a dimension, so V's
 // levels meet in LDS, and a word with tokens of earlier calls keeps their bits.
-// 13081 rows of 8 heads of 128 take 27 us (69 MB, 2.5 TB/s: two rounds of work-groups of 4-5 us each), a row of each of 64
-// slots 5.8, where the chain of lengths, table and rows is all there is.
+// 13081 rows of 8 heads of 128 take 20 us (69 MB, 3.5 TB/s; the VALU is busy 56% of the time, 1.7 rounds of work-groups), a
+// row of each of 64 slots 4.8, where the chain of lengths, table and rows is all there is.
 struct Enc {
     float s, m;
     uint32_t lv[8];               // kLevel0 + level
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // That is for scales under 2, groups that span less than 30: a lane that holds a larger one (to 65504) has p at most 1, and
 // p * s never leaves fp16.  (Raised at every larger score, four long slots take 52.2 us instead of 49.4.)
 // Bound by memory once it runs, by its chain of loads (lengths, table, block) before: a first block takes 6.2 us, then the
-// blocks come at 5 TB/s.  8 KV heads of 128: 48 slots of 60 .. 8000 tokens 21 us and the combine 4.6, 32 slots of 16384
+// blocks come at 5 TB/s.  8 KV heads of 128: 48 slots of 60 .. 8000 tokens 21 us and the combine 4.7, 32 slots of 16384
 // tokens 122 us (4.96 TB/s).  Three sets of registers ahead instead of two: no faster.
 constexpr float kUp = 10.f, kSlack = 3.f;
 
