@@ -167,6 +167,31 @@ def test_append_special_values(hiplib, cuda):
         assert torch.equal(torch.nan_to_num(k), torch.nan_to_num(v))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_append_near_borders(hiplib, cuda, dt):
+    """Values at the middle between two levels and next to it, over groups of every size and offset: the exact level."""
+    from sx8_paged_kv import PagedKV4
+    n, hd = 4096, 128
+    g = torch.Generator().manual_seed(7)
+    lo = torch.randn(n, 2, 1, generator=g).double() * 10.0 ** (torch.rand(n, 2, 1, generator=g) * 8 - 5)
+    lo = lo.clamp(-6e4, 6e4).to(dt)
+    hi = (lo.double() + 10.0 ** (torch.rand(n, 2, 1, generator=g).double() * 8 - 5)).clamp(-6e4, 6e4).to(dt)
+    s = ((hi.float() - lo.float()) * torch.tensor(1 / 15, dtype=torch.float32)).half().double()
+    m = lo.float().half().double()
+    x = (m + (torch.randint(0, 15, (n, 2, 64), generator=g) + 0.5) * s).to(dt)
+    step = torch.randint(-1, 2, (n, 2, 64), generator=g, dtype=torch.int16)
+    x = (x.view(torch.int16) + step * (x != 0)).view(dt)
+    x = torch.minimum(torch.maximum(x, lo), hi)
+    x[..., 0], x[..., 63] = lo[..., 0], hi[..., 0]
+    k = x.reshape(n, 1, hd).to(cuda)
+    v = k.flip(0).contiguous()
+    p = PagedKV4(1, 1, hd, n // 64, 1, n // 64, 64, device=cuda)
+    p.reserve(ints([n], cuda))
+    p.append(0, k, v, cum([n], cuda))
+    gk, gv = p.read(0, n, cum([n], cuda), dtype=dt)
+    assert torch.equal(gk, q4(k).to(dt)) and torch.equal(gv, q4(v).to(dt))
+
+
 def test_append_keeps_other_bytes(hiplib, cuda):
     """Bytes of tokens that a call does not bring stay as they are, and so do pages of other slots."""
     p, k, v = make(cuda, [45, 70], pt=64, spare=2)
