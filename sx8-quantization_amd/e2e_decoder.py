@@ -16,6 +16,7 @@ replayed for every generated token.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import time
 
@@ -566,6 +567,15 @@ class SX8Decoder(nn.Module):
         return out
 
 
+def _on_device(method):
+    """A PagedDecoder method run with the decoder's device as the current one."""
+    @functools.wraps(method)
+    def run(self, *args, **kw):
+        with torch.cuda.device(self.dec.device):
+            return method(self, *args, **kw)
+    return run
+
+
 class PagedDecoder:
     """Several sequences of one SX8Decoder, each in a slot of a paged 4-bit KV cache (sx8_paged_kv).
 
@@ -651,6 +661,7 @@ class PagedDecoder:
         d._gemm(d.head, h, logits, ws, st)
         return logits
 
+    @_on_device
     @torch.no_grad()
     def prompt(self, slots, prompts):
         """Append `prompts` (a list of int64 token vectors) to the slots and return the next token of each (len(slots),)."""
@@ -712,6 +723,7 @@ class PagedDecoder:
         self._rows(pb, self.tok, pos, attend)
         return self._head(pb["resid"], pb["d"], self.n_slots)
 
+    @_on_device
     @torch.no_grad()
     def step(self, use_graph=True):
         """Decode one token of every slot in use: returns the next tokens (n_slots,), kept as the step's input of the
