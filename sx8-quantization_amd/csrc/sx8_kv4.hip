@@ -627,21 +627,25 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[4 * a + e] = __builtin_fmaf(s[e], 16777216.f, mt[e]);
             }
+            uint32_t any = 0;                    // bits 14 and 30: a scale of 2 or more (or NaN)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) any |= rg.vs[g][0] | rg.vs[g][1] | rg.vs[g][2] | rg.vs[g][3];
             if (mask) {
                 asm volatile("");                // (a branch: as selects these would run for every block)
+                any = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int key = b * 32 + (e / 4) * 16 + 4 * h + e % 4;
-                    sc[e] = key <= lim && !rg.bad ? sc[e] : -kInf;
+                    const bool seen = key <= lim && !rg.bad;
+                    sc[e] = seen ? sc[e] : -kInf;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) any |= seen ? rg.vs[g][e >> 1] & (e & 1 ? 0x40000000u : 0x4000u) : 0u;
                 }
             }
             float mx = sc[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
             mx *= kscale;
-            uint32_t any = 0;                    // bit 14 of a scale: 2 or more (or NaN)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) any |= rg.vs[g][0] | rg.vs[g][1] | rg.vs[g][2] | rg.vs[g][3];
             const float up = any & 0x40004000u ? 0.f : kUp, slack = any & 0x40004000u ? 0.f : kUp + kSlack;
             if (__builtin_amdgcn_ballot_w64(mx > m + slack) != 0) {
                 const float mn = fmaxf(m, max4(mx - up));

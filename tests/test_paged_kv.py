@@ -399,6 +399,23 @@ def test_attend_scales_that_grow(hiplib, cuda):
         assert err <= (2.0 ** -11 + LOOSE) * max(top[i].item(), want[0, i].abs().max().item()) + 2.0 ** -25, (i, err)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attend_bits_do_not_depend_on_old_bytes(hiplib, cuda, hd):
+    """What lies behind a slot's last token in its page does not change a bit of the result."""
+    from sx8_paged_kv import PagedKV4
+    lens, got = [45, 1, 130], []
+    k, v = rand((sum(lens), 2, hd), 1, F16, cuda), rand((sum(lens), 2, hd), 2, F16, cuda)
+    q = rand((3, 4, hd), 3, F16, cuda)
+    for seed in (0, 1, 2):
+        p = PagedKV4(1, 2, hd, 8, 3, 3, 64, device=cuda)
+        if seed:
+            p.pages.copy_(torch.randint(0, 256, p.pages.shape, generator=torch.Generator().manual_seed(seed), dtype=torch.uint8))
+        p.reserve(ints(lens, cuda))
+        p.append(0, k, v, cum(lens, cuda))
+        got.append(p.attend(0, q))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
 def test_attend_not_finite(hiplib, cuda):
     """NaN and infinity reach the rows that see them, and no others; garbage past the last token reaches none."""
     from sx8_paged_kv import PagedKV4
