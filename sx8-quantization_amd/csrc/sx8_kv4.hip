@@ -314,11 +314,15 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // of blocks of one unit.  Per block a wave computes S^T = K Q^T on v_mfma_f32_16x16x32_f16 with the tokens as
 // rows and the unit's 16 query rows as columns, so that a lane (column c, step group h) holds the scores of
 // tokens 4 h + r and 16 + 4 h + r of its own query row and the softmax stays in the lane.  The levels go into the
-// MFMA as the fp16 subnormals level * 2^-24, which is one shift and one mask for two values and exact; the scale
+// MFMA as the fp16 subnormals level * 2^-20, which is a shift and a mask for two values and exact; the scale
 // multiplies each group's 32-bit sum (q . k = sum_g s_g (q_g . level_g) + m_g sum(q_g)), and the minima's part is
 // one more MFMA with sum(q_g) as two fp16 numbers.  O^T += V^T P^T takes the levels in the same way, with p * s of
 // each token rounded to two fp16 numbers (22 bits), and the minima's part sum_t p_t m_t,g as MFMAs of their own.
 // So nothing is rounded to fewer than 22 bits between the cache and the output.
+// The MFMA aligns its products by their exponent fields, a subnormal's being 2^-14, and cuts what lies about 25 places below the
+// largest: always downwards, so a sum of levels comes out too small by up to half a place a product.  As level * 2^-24 that
+// is 2^-16 of a level, which many tokens do not average away while their values do (four slots of up to 131000 tokens: 5.5e-4
+// of the outputs); as level * 2^-20 it is 2^-20 of one (1e-5 of them, the plain float32 form 4e-6).
 // Query rows are multiplied by a power of two that brings their largest value into [64, 128), which is undone in
 // the scale: bf16 rows become fp16 without loss (but for values 2^-30 below the largest), and sum(q_g) fits.
 // The running maximum is kept kUp powers of two below the largest score and raised when a score exceeds it by kUp + kSlack,
@@ -366,10 +370,10 @@ struct Kv4Regs {                          // a lane's share of one block
 };
 
 __device__ __forceinline__ f16x8 levels(uint32_t w) {
-    const u32x4 v = {w & 0x000F000Fu, (w >> 4) & 0x000F000Fu, (w >> 8) & 0x000F000Fu, (w >> 12) & 0x000F000Fu};
+    const u32x4 v = {w << 4 & 0x00F000F0u, w & 0x00F000F0u, w >> 4 & 0x00F000F0u, w >> 8 & 0x00F000F0u};
     return __builtin_bit_cast(f16x8, v);
 }
-// The same with values 2, 3, 6 and 7 sixteen times as large: one shift less (their factors are sixteen times smaller).
+// K's, as level * 2^-24, values 2, 3, 6 and 7 sixteen times as large: two shifts less (their factors are sixteen times smaller).
 __device__ __forceinline__ f16x8 levels16(uint32_t w) {
     const uint32_t u = w >> 8;
     return __builtin_bit_cast(f16x8, u32x4{w & 0x000F000Fu, w & 0x00F000F0u, u & 0x000F000Fu, u & 0x00F000F0u});
@@ -715,7 +719,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
             if (i + 2 < cnt) load(r0, i + 2);
             step(r1, i + 1);
         }
-        // O = 2^24 (levels) + (the minima's sum of the group, row g of om)
+        // O = 2^20 (levels) + (the minima's sum of the group, row g of om)
         l = sum4(l);
         const bool whole = b0 == 0 && bend == nb;
         const float f = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
@@ -728,7 +732,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
             const float og = __shfl(om[t / 4], c, 64);
             f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(o[t][e], 16777216.f, og) * f;
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(o[t][e], 1048576.f, og) * f;
             if (row_ok) {
                 if (whole) *reinterpret_cast<u32x2*>(dst + 16 * t) = u32x2{pack16<kBf16>(v[0], v[1]), pack16<kBf16>(v[2], v[3])};
                 else *reinterpret_cast<f32x4*>(po + 16 * t) = v;

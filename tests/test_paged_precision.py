@@ -1,0 +1,50 @@
+"""How many bits the attention over the 4-bit pages and the attention of packed prompts keep, against 64 bits: cases that
+averages over many tokens hide."""
+import math
+
+import pytest
+import torch
+
+from test_paged_kv import BF16, F16, attention, cum, ints, q4, rand
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(shape, seed, cuda):
+    """Uniform in (-1, 1), fp16."""
+    return (torch.rand(*shape, generator=torch.Generator().manual_seed(seed)) * 2 - 1).half().to(cuda)
+
+
+def pool(k, v, cuda, slots=1):
+    """A cache whose `slots` slots hold these rows each (n, nk, hd)."""
+    from sx8_paged_kv import PagedKV4
+    n, nk, hd = k.shape
+    width = -(-n // 32)
+    p = PagedKV4(1, nk, hd, slots * width, slots, width, 32, device=cuda)
+    p.reserve(ints([n] * slots, cuda))
+    p.append(0, torch.cat([k] * slots), torch.cat([v] * slots), cum([n] * slots, cuda))
+    p.check()
+    return p
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attend_sums_of_levels_are_not_short(hiplib, cuda, hd):
+    """The sum of the levels and the sum of the minima nearly cancel over many tokens, so a sum of levels that always falls
+    short shows in the mean error.  A level enters as 2^-20 times itself, aligned as if at 2^-14, and what lies about 25 places
+    below the largest product of a block is cut: a product loses half of 2^-19 levels of the block's largest weight, an
+    output 2^-20 scales times 32 of those largest weights' sum.  The outputs' own rounding is of either sign: half a step at
+    most, a third of its square on average, so four times the root of that over their number."""
+    n, nk, rep, new = 4096, 4, 4, 16
+    k, v = rand((n, nk, hd), 1, F16, cuda), rows((n, nk, hd), 2, cuda)
+    q = rand((new, nk * rep, hd), 3, F16, cuda)
+    got, kk, vv = pool(k, v, cuda).attend(0, q, ints([0, new], cuda)).double(), q4(k), q4(v)
+    want = attention(q.double(), kk, vv, n - new)
+    w = torch.matmul(q.double().permute(1, 0, 2).contiguous(), kk.repeat_interleave(rep, 1).permute(1, 2, 0).contiguous())
+    w = (w / hd ** 0.5).masked_fill(torch.arange(n, device=cuda) > n - new + torch.arange(new, device=cuda)[:, None], -math.inf)
+    top = torch.softmax(w, -1).unflatten(-1, (-1, 32)).amax(-1).sum(-1).mean().item()
+    half = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -14))) - 11)
+    noise = half.square().mean().sqrt().item() / (3 * want.numel()) ** 0.5
+    mean = (got - want).mean().item()
+    bound = 2.0 ** -20 * (2 / 15) * 32 * top + 4 * noise
+    print("mean error", mean, "bound", bound, flush=True)
+    assert abs(mean) <= bound
