@@ -324,7 +324,8 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // is 2^-16 of a level, which many tokens do not average away while their values do (four slots of up to 131000 tokens: 5.5e-4
 // of the outputs); as level * 2^-20 it is 2^-20 of one (1e-5 of them, the plain float32 form 4e-6).
 // Query rows are multiplied by a power of two that brings their largest value into [64, 128), which is undone in
-// the scale: bf16 rows become fp16 without loss (but for values 2^-30 below the largest), and sum(q_g) fits.
+// the scale: rows become fp16 within 2^-31 of their largest value (exact where they hold nothing 2^-20 below it, bf16: 2^-23),
+// and sum(q_g) fits.
 // The running maximum is kept kUp powers of two below the largest score and raised when a score exceeds it by kUp + kSlack,
 // so that p is at most 2^13 and p * s holds its 22 bits for small values as well (down to p * s = 2^-3 in those units).
 // That is for scales under 2, groups that span less than 30: a lane that holds a larger one (to 65504) has p at most 1, and
@@ -372,11 +373,6 @@ struct Kv4Regs {                          // a lane's share of one block
 __device__ __forceinline__ f16x8 levels(uint32_t w) {
     const u32x4 v = {w << 4 & 0x00F000F0u, w & 0x00F000F0u, w >> 4 & 0x00F000F0u, w >> 8 & 0x00F000F0u};
     return __builtin_bit_cast(f16x8, v);
-}
-// K's, as level * 2^-24, values 2, 3, 6 and 7 sixteen times as large: two shifts less (their factors are sixteen times smaller).
-__device__ __forceinline__ f16x8 levels16(uint32_t w) {
-    const uint32_t u = w >> 8;
-    return __builtin_bit_cast(f16x8, u32x4{w & 0x000F000Fu, w & 0x00F000F0u, u & 0x000F000Fu, u & 0x00F000F0u});
 }
 // p s of four values (s: two words of fp16) as two fp16 numbers each, hi + lo: an instruction for each number, where the
 // compiler takes three.  (A word's halves are written one instruction apart from each other.)
@@ -586,7 +582,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
                 for (int e = 0; e < 8; ++e) {
                     const float raw_q = ld16<kBf16>(half_of(raw[j][e >> 1], e));
                     const _Float16 v = (_Float16)(row_ok ? raw_q * mul : 0.f);
-                    qf[j][e] = e & 2 ? v * (_Float16)0.0625f : v;                  // (levels16)
+                    qf[j][e] = v;
                     qs[j / 2] += (float)v;
                 }
 #pragma unroll
@@ -615,8 +611,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                    acc = mfma16(levels16(rg.kw[a][2 * g]), qf[2 * g], acc);
-                    acc = mfma16(levels16(rg.kw[a][2 * g + 1]), qf[2 * g + 1], acc);
+                    acc = mfma16(levels(rg.kw[a][2 * g]), qf[2 * g], acc);
+                    acc = mfma16(levels(rg.kw[a][2 * g + 1]), qf[2 * g + 1], acc);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         s[e] = __builtin_fmaf(sx8_h2f(half_of(rg.ks[g][2 * a + (e >> 1)], e)), acc[e], s[e]);
@@ -629,7 +625,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
                 }
                 const f32x4 mt = mfma16(__builtin_bit_cast(f16x8, mw), qm, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[4 * a + e] = __builtin_fmaf(s[e], 16777216.f, mt[e]);
+                for (int e = 0; e < 4; ++e) sc[4 * a + e] = __builtin_fmaf(s[e], 1048576.f, mt[e]);
             }
             uint32_t any = 0;                    // bits 14 and 30: a scale of 2 or more (or NaN)
 #pragma unroll

@@ -48,3 +48,26 @@ def test_attend_sums_of_levels_are_not_short(hiplib, cuda, hd):
     bound = 2.0 ** -20 * (2 / 15) * 32 * top + 4 * noise
     print("mean error", mean, "bound", bound, flush=True)
     assert abs(mean) <= bound
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_attend_small_query_values(hiplib, cuda, hd, dt):
+    """Query values about 2^-19 of their row's largest decide the scores (the keys' level is zero where that one is): they
+    enter exactly.  A score is then good to the products' alignment, hd times 2^-19 levels of the largest of these values
+    (2^-11), times the scale 2^12 / sqrt(hd): 2^-14 for hd of 256, and an average of values below 1 to twice that."""
+    n = 200
+    k = torch.randint(0, 16, (n, 1, hd), generator=torch.Generator().manual_seed(1)).half().to(cuda)
+    k[..., 0::64], k[..., 1::64] = 0, 15
+    v = rows((n, 1, hd), 2, cuda)
+    assert torch.equal(q4(k), k.double())
+    q = rand((1, 8, hd), 3, torch.float32, cuda).clamp(-4, 4) * 2.0 ** -13
+    q = torch.where(q.abs() < 2.0 ** -16, 0.0, q)                   # (bf16's eight bits at 2^-16 are fp16's at 2^-24)
+    q[..., 0] = 64
+    q = q.to(dt)
+    scale = 2.0 ** 12 / hd ** 0.5
+    p = pool(k, v, cuda)
+    got, want = p.attend(0, q, scale=scale).double(), attention(q.double(), q4(k), q4(v), n - 1, scale)
+    err = ((got - want).abs() - torch.finfo(dt).eps / 2 * want.abs()).max().item()
+    print("error past half a step", err, flush=True)
+    assert err <= 2.0 ** -13
