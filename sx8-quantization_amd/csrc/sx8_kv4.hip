@@ -374,21 +374,35 @@ __device__ __forceinline__ f16x8 levels(uint32_t w) {
     const u32x4 v = {w << 4 & 0x00F000F0u, w & 0x00F000F0u, w >> 4 & 0x00F000F0u, w >> 8 & 0x00F000F0u};
     return __builtin_bit_cast(f16x8, v);
 }
-// p s of four values (s: two words of fp16) as two fp16 numbers each, hi + lo: an instruction for each number, where the
-// compiler takes three.  (A word's halves are written one instruction apart from each other.)
-__device__ __forceinline__ void split4(const float* p, uint32_t s0, uint32_t s1, uint32_t* hi, uint32_t* lo) {
-    asm("v_fma_mixlo_f16 %0, %2, %6, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
-        "v_fma_mixlo_f16 %1, %4, %7, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
-        "v_fma_mixhi_f16 %0, %3, %6, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
-        "v_fma_mixhi_f16 %1, %5, %7, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]"
-        : "=&v"(hi[0]), "=&v"(hi[1])
-        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(s0), "v"(s1));
-    asm("v_fma_mixlo_f16 %0, %2, %6, -%8 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
-        "v_fma_mixlo_f16 %1, %4, %7, -%9 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
-        "v_fma_mixhi_f16 %0, %3, %6, -%8 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
-        "v_fma_mixhi_f16 %1, %5, %7, -%9 op_sel:[0,1,1] op_sel_hi:[0,1,1]"
-        : "=&v"(lo[0]), "=&v"(lo[1])
-        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(s0), "v"(s1), "v"(hi[0]), "v"(hi[1]));
+// p s of eight values (s: four words of fp16) as two fp16 numbers each, hi + lo: an instruction for each number, where the
+// compiler takes three.  The compiler does not see what an asm block reads and writes at its ends, so the waits are here: one
+// state between an exp2 and its use, two between the last word and an MFMA that reads it.  (A word's halves, and a number and
+// its use, are written four instructions apart from each other.)
+__device__ __forceinline__ void split8(const float* p, const u32x4& s, u32x4* hi, u32x4* lo) {
+    uint32_t a[4], b[4];
+    asm("s_nop 0\n\t"
+        "v_fma_mixlo_f16 %0, %8, %16, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixlo_f16 %1, %10, %17, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixlo_f16 %2, %12, %18, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixlo_f16 %3, %14, %19, 0 op_sel:[0,0,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixhi_f16 %0, %9, %16, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixhi_f16 %1, %11, %17, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixhi_f16 %2, %13, %18, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixhi_f16 %3, %15, %19, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+        "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixlo_f16 %5, %10, %17, -%1 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixlo_f16 %6, %12, %18, -%2 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixlo_f16 %7, %14, %19, -%3 op_sel:[0,0,0] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixhi_f16 %4, %9, %16, -%0 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixhi_f16 %5, %11, %17, -%1 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixhi_f16 %6, %13, %18, -%2 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+        "v_fma_mixhi_f16 %7, %15, %19, -%3 op_sel:[0,1,1] op_sel_hi:[0,1,1]\n\t"
+        "s_nop 1"
+        : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "v"(s[0]), "v"(s[1]),
+          "v"(s[2]), "v"(s[3]));
+    *hi = u32x4{a[0], a[1], a[2], a[3]};
+    *lo = u32x4{b[0], b[1], b[2], b[3]};
 }
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -683,23 +697,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
             }
             u32x4 ph, pl;
             constexpr uint32_t kOnes = 0x3C003C00u;
-            {
-                uint32_t hi[4], lo[4];
-                split4(pv, kOnes, kOnes, hi, lo);
-                split4(pv + 4, kOnes, kOnes, hi + 2, lo + 2);
-                ph = u32x4{hi[0], hi[1], hi[2], hi[3]};
-                pl = u32x4{lo[0], lo[1], lo[2], lo[3]};
-            }
+            split8(pv, u32x4{kOnes, kOnes, kOnes, kOnes}, &ph, &pl);
             const f16x8 vm8 = __builtin_bit_cast(f16x8, vm);
             om = mfma16(vm8, __builtin_bit_cast(f16x8, ph), om);
             om = mfma16(vm8, __builtin_bit_cast(f16x8, pl), om);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                uint32_t hi[4], lo[4];
-                split4(pv, rg.vs[g][0], rg.vs[g][1], hi, lo);
-                split4(pv + 4, rg.vs[g][2], rg.vs[g][3], hi + 2, lo + 2);
-                const f16x8 h8 = __builtin_bit_cast(f16x8, (u32x4{hi[0], hi[1], hi[2], hi[3]}));
-                const f16x8 l8 = __builtin_bit_cast(f16x8, (u32x4{lo[0], lo[1], lo[2], lo[3]}));
+                u32x4 hi, lo;
+                split8(pv, rg.vs[g], &hi, &lo);
+                const f16x8 h8 = __builtin_bit_cast(f16x8, hi), l8 = __builtin_bit_cast(f16x8, lo);
 #pragma unroll
                 for (int t = 4 * g; t < 4 * g + 4; ++t) {
                     const f16x8 lv = levels(rg.vw[t]);

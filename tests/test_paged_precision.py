@@ -71,3 +71,26 @@ def test_attend_small_query_values(hiplib, cuda, hd, dt):
     err = ((got - want).abs() - torch.finfo(dt).eps / 2 * want.abs()).max().item()
     print("error past half a step", err, flush=True)
     assert err <= 2.0 ** -13
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_attend_every_token_of_a_block(hiplib, cuda, hd, dt):
+    """32 queries that give 0.4 of their weight to one token of a block each and the rest to a token whose values are zero: the
+    weight times the scale needs both of its fp16 numbers (22 bits), for every token of the block, in values whose level and
+    minimum nearly cancel.  A weight is within 2^-18 of itself (scores of 58 powers of two), weight times scale within
+    2^-22, a product within 2^-18 levels (2 / 15): all of it below 2^-18 of the value and 2^-20 * 3."""
+    n = 64
+    k, v = torch.zeros(n, 1, hd, dtype=F16, device=cuda), rows((n, 1, hd), 1, cuda)
+    k[range(32), 0, range(32)] = 15
+    k[40, 0, 40] = 15
+    v[40] = 0
+    assert torch.equal(q4(k), k.double())
+    q = torch.zeros(1, 32, hd, device=cuda)
+    q[0, range(32), range(32)] = 39.6 / 15
+    q[..., 40] = 40 / 15
+    q = q.to(dt)
+    got, want = pool(k, v, cuda).attend(0, q, scale=1.0).double(), attention(q.double(), q4(k), q4(v), n - 1, 1.0)
+    err = (got - want).abs() - (torch.finfo(dt).eps / 2 + 2.0 ** -18) * want.abs() - 3 * 2.0 ** -20
+    print("largest error over the bound", err.max().item(), flush=True)
+    assert err.max() <= 0
