@@ -318,7 +318,6 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // multiplies each group's 32-bit sum (q . k = sum_g s_g (q_g . level_g) + m_g sum(q_g)), and the minima's part is
 // one more MFMA with sum(q_g) as two fp16 numbers.  O^T += V^T P^T takes the levels in the same way, with p * s of
 // each token rounded to two fp16 numbers (22 bits), and the minima's part sum_t p_t m_t,g as MFMAs of their own.
-// So nothing is rounded to fewer than 22 bits between the cache and the output.
 // The MFMA aligns its products by their exponent fields, a subnormal's being 2^-14, and cuts what lies about 25 places below the
 // largest: always downwards, so a sum of levels comes out too small by up to half a place a product.  As level * 2^-24 that
 // is 2^-16 of a level, which many tokens do not average away while their values do (four slots of up to 131000 tokens: 5.5e-4
@@ -327,9 +326,11 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // the scale: rows become fp16 within 2^-31 of their largest value (exact where they hold nothing 2^-20 below it, bf16: 2^-23),
 // and sum(q_g) fits.
 // The running maximum is kept kUp powers of two below the largest score and raised when a score exceeds it by kUp + kSlack,
-// so that p is at most 2^13 and p * s holds its 22 bits for small values as well (down to p * s = 2^-3 in those units).
-// That is for scales under 2, groups that span less than 30: a lane that holds a larger one (to 65504) has p at most 1, and
-// p * s never leaves fp16.  (Raised at every larger score, four long slots take 52.2 us instead of 49.4.)
+// so that p is at most 2^13, the largest weight at least 2^10, and p * s holds its 22 bits down to p * s = 2^-3 in those
+// units (below that it is within 2^-25).  (Raised at every larger score, four long slots take 52.2 us instead of 49.4.)
+// Scales of 2 or more (groups that span 30 or more) would take p * s out of fp16: those go in 2^k times smaller, below 2 and
+// from 1/16 on, with their levels 2^k times as large, in matrix products of their own for each of k = 5, 10 and 15 that a
+// block has.  So what is kept of a token does not depend on the scales of other groups or tokens.
 // Bound by memory once it runs, by its chain of loads (lengths, table, block) before: a first block takes 6.2 us, then the
 // blocks come at 5 TB/s.  8 KV heads of 128: 48 slots of 60 .. 8000 tokens 21 us and the combine 4.7, 32 slots of 16384
 // tokens 122 us (4.96 TB/s).  Three sets of registers ahead instead of two: no faster.
@@ -403,6 +404,14 @@ __device__ __forceinline__ void split8(const float* p, const u32x4& s, u32x4* hi
           "v"(s[2]), "v"(s[3]));
     *hi = u32x4{a[0], a[1], a[2], a[3]};
     *lo = u32x4{b[0], b[1], b[2], b[3]};
+}
+// The scales (two a word) of 2^(k - 4) to 2^(k + 1), for k = 15 all from 2^11 on (NaN too); zeros for the others.
+__device__ __forceinline__ u32x4 large_scales(const u32x4& s, int k) {
+    auto in = [k](uint32_t half) { return (half >> 10 & 31u) - (uint32_t)(k + 11) < (k == 15 ? 6u : 5u); };
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (in(s[e]) ? s[e] & 0xFFFFu : 0u) | (in(s[e] >> 16) ? s[e] & 0xFFFF0000u : 0u);
+    return r;
 }
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -641,28 +650,20 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[4 * a + e] = __builtin_fmaf(s[e], 1048576.f, mt[e]);
             }
-            uint32_t any = 0;                    // bits 14 and 30: a scale of 2 or more (or NaN)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) any |= rg.vs[g][0] | rg.vs[g][1] | rg.vs[g][2] | rg.vs[g][3];
             if (mask) {
                 asm volatile("");                // (a branch: as selects these would run for every block)
-                any = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int key = b * 32 + (e / 4) * 16 + 4 * h + e % 4;
-                    const bool seen = key <= lim && !rg.bad;
-                    sc[e] = seen ? sc[e] : -kInf;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) any |= seen ? rg.vs[g][e >> 1] & (e & 1 ? 0x40000000u : 0x4000u) : 0u;
+                    sc[e] = key <= lim && !rg.bad ? sc[e] : -kInf;
                 }
             }
             float mx = sc[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
             mx *= kscale;
-            const float up = any & 0x40004000u ? 0.f : kUp, slack = any & 0x40004000u ? 0.f : kUp + kSlack;
-            if (__builtin_amdgcn_ballot_w64(mx > m + slack) != 0) {
-                const float mn = fmaxf(m, max4(mx - up));
+            if (__builtin_amdgcn_ballot_w64(mx > m + (kUp + kSlack)) != 0) {
+                const float mn = fmaxf(m, max4(mx - kUp));
                 const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= alpha;
@@ -701,6 +702,33 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
             const f16x8 vm8 = __builtin_bit_cast(f16x8, vm);
             om = mfma16(vm8, __builtin_bit_cast(f16x8, ph), om);
             om = mfma16(vm8, __builtin_bit_cast(f16x8, pl), om);
+            uint32_t large = 0;                  // bits 14 and 30: a scale of 2 or more (or NaN)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) large |= rg.vs[g][0] | rg.vs[g][1] | rg.vs[g][2] | rg.vs[g][3];
+            if (__builtin_amdgcn_ballot_w64((large & 0x40004000u) != 0) != 0) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+#pragma unroll 1
+                    for (int k = 5; k <= 15; k += 5) {
+                        u32x4 s = large_scales(rg.vs[g], k);
+                        if (__builtin_amdgcn_ballot_w64((s[0] | s[1] | s[2] | s[3]) != 0) == 0) continue;
+                        const _Float16 down = (_Float16)__builtin_ldexpf(1.f, -k), up = (_Float16)__builtin_ldexpf(1.f, k);
+                        s = __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, s) * f16x8(down));
+                        u32x4 hi, lo;
+                        split8(pv, s, &hi, &lo);
+#pragma unroll
+                        for (int t = 4 * g; t < 4 * g + 4; ++t) {
+                            uint32_t w = rg.vw[t];
+                            asm volatile("" : "+v"(w));          // (here, not ahead of the loop: registers)
+                            const f16x8 lv = levels(w) * f16x8(up);
+                            o[t] = mfma16(lv, __builtin_bit_cast(f16x8, hi), o[t]);
+                            o[t] = mfma16(lv, __builtin_bit_cast(f16x8, lo), o[t]);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rg.vs[g][e] &= ~((rg.vs[g][e] >> 14 & 0x00010001u) * 0xFFFFu);
+                }
+            }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 u32x4 hi, lo;

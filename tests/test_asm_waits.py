@@ -1,7 +1,8 @@
 """Wait states around inline assembly, in the compiler's output: the compiler keeps them between instructions that it writes
 itself and does not look into asm blocks.  For gfx950: two states between a VALU result and an MFMA that reads it, one between
 a transcendental's result and a VALU instruction that reads it, five between a scalar register that the VALU wrote and
-a memory access that reads it, one between m0 and the load to LDS that uses it."""
+a memory access that reads it, one between m0 and the load to LDS that uses it, 19 at most between an MFMA's result and an
+instruction that reads or overwrites it."""
 import os
 import re
 import subprocess
@@ -44,8 +45,11 @@ def short_waits(text):
         reads = set().union(*(regs(w) for o in ops[0 if stores else 1:] for w in o.split())) if ops else set()
         if to_lds:
             reads |= {"m0"}
-        for wname, wrote, w_asm, at in past[-12:]:
+        writes = set() if stores or not ops else regs(ops[0])
+        for wname, wrote, w_asm, at in past[-24:]:
             gap, hit = clock - at - 1, wrote & reads
+            if in_asm and wname.startswith("v_mfma") and wrote & (reads | writes) and gap < 19:
+                found.append((kernel, "result", wname, code))
             if not hit or not (in_asm or w_asm):
                 continue
             valu = wname.startswith("v_") and not wname.startswith("v_mfma")
@@ -57,7 +61,7 @@ def short_waits(text):
                 found.append((kernel, "sgpr", wname, code))
             if "m0" in hit and gap < 1:
                 found.append((kernel, "m0", wname, code))
-        past.append((name, set() if stores or not ops else regs(ops[0]), in_asm, clock))
+        past = [(n, w - writes, a, at) for n, w, a, at in past[-24:]] + [(name, writes, in_asm, clock)]
         clock += 1
     return found
 
@@ -78,6 +82,8 @@ def test_the_check_sees_short_waits():
     ;;#ASMEND
 """
     assert [f[1] for f in short_waits(asm)] == ["trans", "mfma", "sgpr", "m0"]
+    late = "_Zk:\n v_mfma_f32_16x16x32_f16 v[0:3], v[4:7], v[8:11], 0\n s_nop 3\n ;;#ASMSTART\n v_mov_b32_e32 v2, v20\n ;;#ASMEND\n"
+    assert [f[1] for f in short_waits(late)] == ["result"] and short_waits(late.replace("v2,", "v12,")) == []
     mended = asm.replace("    v_fma_mixlo", "    s_nop 0\n    v_fma_mixlo").replace("    v_and_b32", "    s_nop 0\n    v_and_b32")
     mended = mended.replace("    s_mov_b32 m0", "    s_nop 4\n    s_mov_b32 m0").replace("    buffer_load", "    s_nop 0\n    buffer_load")
     assert short_waits(mended) == []

@@ -94,3 +94,41 @@ def test_attend_every_token_of_a_block(hiplib, cuda, hd, dt):
     err = (got - want).abs() - (torch.finfo(dt).eps / 2 + 2.0 ** -18) * want.abs() - 3 * 2.0 ** -20
     print("largest error over the bound", err.max().item(), flush=True)
     assert err.max() <= 0
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("sizes", [(4.0, 2.0 ** -10), (2.0 ** 12, 0.25), (2.0 ** -10, 2.0 ** -10), (64.0, 2.0)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_attend_scales_of_groups(hiplib, cuda, dt, sizes, mixed):
+    """A head with a group of large and one of small scales (mixed: the first group's scale changes from token to
+    token), a key with 0.6 of the weight and 65000 that share the rest: each group keeps its own precision.  The
+    largest weight counts at least 2^10, so a token's weight times scale (below 2; a larger one divided by 2^k into 1/16 .. 2) is
+    within 2^-25, of either sign: levels' root square sum times that over the sum of the weights, a third of the square on
+    average, six times that.  Weights are within 2^-17 of themselves."""
+    n, hd = 65000, 128
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randint(0, 16, (n, 1, hd), generator=g).double() for _ in range(2))
+    k[:, :, 64:] = 0
+    k[..., 0], k[..., 1], k[0] = 0, 15, 0
+    k[0, 0, 0] = 15
+    v[..., 0::64], v[..., 1::64] = 0, 15
+    s = torch.tensor(sizes).double().repeat_interleave(64).expand(n, 1, hd).clone()
+    if mixed:
+        s[1::3, :, :64] *= 2.0 ** -6 if sizes[0] > 1 else 2.0 ** 6
+    k, v = k.half().to(cuda), (v * s).half().to(cuda)
+    assert torch.equal(q4(k), k.double()) and torch.equal(q4(v), v.double())
+    q = torch.zeros(1, 4, hd)
+    q[..., 0] = 10.7 / 15
+    q[..., 2:64] = torch.randn(1, 4, 62, generator=g) * 0.01
+    q = q.to(dt).to(cuda)
+    got, want = pool(k, v, cuda).attend(0, q, scale=1.0).double(), attention(q.double(), k.double(), v.double(), n - 1, 1.0)
+    w = torch.matmul(q[0].double(), k[:, 0].double().T.contiguous())
+    total = 2.0 ** 10 * torch.exp(w - w.amax(-1, keepdim=True)).sum(-1).min().item()
+    for i in range(2):
+        a = slice(64 * i, 64 * i + 64)
+        unit = max(1.0, s[..., a].max().item() * 8)                 # 2^k at most for scales in 2^(k - 4) .. 2^(k + 1)
+        unit = unit if s[..., a].max() >= 2 else 1.0
+        more = 6 * 2.0 ** -25 * unit * 15 * n ** 0.5 / 3 ** 0.5 / total + 2.0 ** -17 * v[..., a].max().item()
+        err = ((got - want).abs() - torch.finfo(dt).eps / 2 * want.abs())[..., a].max().item()
+        print("group", i, "error past half a step", err, "of", more, "mean value", want[..., a].abs().mean().item(), flush=True)
+        assert err <= more
