@@ -683,13 +683,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
             if (mask) {
                 // a token that some column may not attend must not reach it through 0 * NaN: its scale is zero for that
                 // column, and its minimum zero where it is no number (the scale, which is none either, still brings the
-                // NaN to the columns that attend it)
+                // NaN to the columns that attend it, however small its weight)
                 asm volatile("");
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (pv[e] == 0.f)
+                for (int e = 0; e < 8; ++e) {
+                    const int key = b * 32 + (e / 4) * 16 + 4 * h + e % 4;
+                    if (key > lim || rg.bad)
 #pragma unroll
                         for (int g = 0; g < NG; ++g) rg.vs[g][e >> 1] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t lo = vm[e] & 0x7FFFu, hi = vm[e] >> 16 & 0x7FFFu;

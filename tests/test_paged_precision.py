@@ -132,3 +132,18 @@ def test_attend_scales_of_groups(hiplib, cuda, dt, sizes, mixed):
         err = ((got - want).abs() - torch.finfo(dt).eps / 2 * want.abs())[..., a].max().item()
         print("group", i, "error past half a step", err, "of", more, "mean value", want[..., a].abs().mean().item(), flush=True)
         assert err <= more
+
+
+@pytest.mark.parametrize("token", [3, 31, 33, 38])
+def test_attend_not_finite_with_a_small_weight(hiplib, cuda, token):
+    """A value that is no number reaches a row that attends it with a weight of e^-120, in a block that the row sees
+    whole (0 .. 31) and in one that ends inside."""
+    k, v = torch.zeros(40, 1, 64, dtype=F16, device=cuda), rows((40, 1, 64), 1, cuda)
+    k[39, 0, 0] = 15
+    v[token, 0, 5] = math.nan
+    q = torch.zeros(1, 2, 64, dtype=F16, device=cuda)
+    q[..., 0] = 8
+    p = pool(k, v, cuda)
+    assert torch.isnan(p.attend(0, q, scale=1.0)).all()
+    v[token, 0, 5] = 0
+    assert torch.isfinite(pool(k, v, cuda).attend(0, q, scale=1.0)).all()
