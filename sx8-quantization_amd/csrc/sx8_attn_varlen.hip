@@ -111,8 +111,9 @@ constexpr int var_lds_bytes() {
     return a > b ? a : (b + 15) / 16 * 16;
 }
 
-// A wave's rows key by key, without products of a zero probability: for rows in whose sums there is a value that is no
-// finite number (about 1 us a key).  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
+// A wave's rows key by key, over the keys that each attends alone: for rows in whose sums there is a value that is no
+// finite number (about 1 us a key).  Such a value reaches the row however small its weight: one that underflows counts as 1
+// there, and a sum that is not finite is not scaled.  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
 template <int HD, bool kBf16, typename V, int NT>
 __device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, const uint16_t* v, const VarIo& io,
                                           int from, int to, int lim, int h, V (&o)[NT], float& m, float& l) {
@@ -140,8 +141,8 @@ __device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, 
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float x = ld16<kBf16>(v[key * io.v_ts + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3)]);
-                o[n][r] = o[n][r] * alpha;
-                if (p != 0.f) o[n][r] = __builtin_fmaf(p, x, o[n][r]);
+                const float pw = p != 0.f || s == -__builtin_inff() || __builtin_isfinite(x) ? p : 1.f;
+                o[n][r] = __builtin_fmaf(pw, x, __builtin_isfinite(o[n][r]) ? o[n][r] * alpha : o[n][r]);
             }
     }
 }
@@ -404,8 +405,12 @@ __global__ __launch_bounds__(256) void k_varlen_combine(const VarIo io) {
         const float pm = io.part_ml[at * 2], f = pm == m ? 1.f : __builtin_amdgcn_exp2f(pm - m);
         l = __builtin_fmaf(f, io.part_ml[at * 2 + 1], l);
 #pragma unroll
-        for (int e = 0; e < N / 4; ++e)
-            acc[e] = __builtin_elementwise_fma(f32x4(f), reinterpret_cast<const f32x4*>(io.part_o + at * HD + d0)[e], acc[e]);
+        for (int e = 0; e < N / 4; ++e) {
+            const f32x4 po = reinterpret_cast<const f32x4*>(io.part_o + at * HD + d0)[e];
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)       // (0 * infinity: see slow_rows)
+                acc[e][i4] = __builtin_fmaf(f != 0.f || __builtin_isfinite(po[i4]) ? f : 1.f, po[i4], acc[e][i4]);
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint16_t* const dst = io.out + ((int64_t)rec.q_first + rec.q0 + row) * io.o_ts + rec.head * io.o_hs + d0;

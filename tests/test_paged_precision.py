@@ -147,3 +147,21 @@ def test_attend_not_finite_with_a_small_weight(hiplib, cuda, token):
     assert torch.isnan(p.attend(0, q, scale=1.0)).all()
     v[token, 0, 5] = 0
     assert torch.isfinite(pool(k, v, cuda).attend(0, q, scale=1.0)).all()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("nkeys,at", [(50, 3), (50, 48), (300, 3), (9000, 3), (9000, 8500)])
+def test_varlen_not_finite_with_a_small_weight(hiplib, cuda, dt, bad, nkeys, at):
+    """A value that is no finite number reaches the rows that attend it with a weight of e^-120 before and behind the key that
+    has the rest, in tiles that the rows see whole or in part and in keys cut into parts."""
+    from sx8_paged_kv import attn_varlen
+    q, k, v = torch.zeros(4, 2, 64, dtype=dt, device=cuda), torch.zeros(nkeys, 1, 64, dtype=dt, device=cuda), rand((nkeys, 1, 64), 1, dt, cuda)
+    q[..., 0], k[20, 0, 0], v[at, 0, 7] = 8, 15, bad
+    got = attn_varlen(q, k, v, cum([4], cuda), cum([nkeys], cuda), scale=1.0)
+    sees = torch.arange(nkeys - 4, nkeys, device=cuda) >= at
+    want = torch.full_like(got[..., 7], bad)
+    same = torch.isnan(got[..., 7]) if math.isnan(bad) else got[..., 7] == want
+    assert same[sees].all() and torch.isfinite(got[~sees]).all()
+    got[..., 7] = 0
+    assert torch.isfinite(got).all()
