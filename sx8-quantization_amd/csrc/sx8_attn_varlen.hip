@@ -77,7 +77,7 @@ __device__ __forceinline__ u32x4 scalar_rsrc(const void* p, uint32_t bytes) {
 // every LDS read that might be of the same place, which is every one (prompt of 8192: 730 us against 603).
 __device__ __forceinline__ void load_lds(const u32x4& r, int dst, int off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off), "s"(r)
-                 : "memory");
+                 : "memory", "m0");
 }
 // Lane i of 16 names the eight bytes of key i / 4 that hold dimensions 4 (i % 4) .. + 3, and gets dimension i of the four keys.
 __device__ __forceinline__ u32x2 read_tr(const unsigned char* at) {

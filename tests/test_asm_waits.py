@@ -98,3 +98,15 @@ def test_waits_around_asm(source, tmp_path):
     found = short_waits(out.read_text())
     assert "#ASMSTART" in out.read_text()
     assert not found, found[:4]
+
+
+def test_asm_names_m0():
+    """An asm statement that writes m0 names it among what it overwrites."""
+    seen = 0
+    for name in sorted(os.listdir(L.CSRC_DIR)):
+        text = open(os.path.join(L.CSRC_DIR, name)).read()
+        for m in re.finditer(r'asm volatile\((?:[^;"]|"[^"]*")*\);|asm\((?:[^;"]|"[^"]*")*\);', text):
+            if re.search(r"s_mov_b32 m0|s_add_u32 m0", m[0]):
+                seen += 1
+                assert re.search(r':[^:]*"m0"[^:]*\);$', m[0]), (name, m[0])
+    assert seen
