@@ -65,12 +65,15 @@ __device__ __forceinline__ void seq_rows(const int32_t* cu, int T, int b, int* f
 
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 
-// A raw buffer over `bytes` bytes at p (as make_rsrc), in scalar registers for load_lds.
+// A raw buffer over `bytes` bytes at p (as make_rsrc), in scalar registers for load_lds.  A memory access may read a scalar
+// register that the VALU wrote five states later, which the compiler does not see to in an asm block: the wait is here.
 __device__ __forceinline__ u32x4 scalar_rsrc(const void* p, uint32_t bytes) {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
-    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
-                 (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xFFFFu)),
-                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kRsrcFlags};
+    u32x4 r = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xFFFFu)),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kRsrcFlags};
+    asm volatile("s_nop 4" : "+s"(r));
+    return r;
 }
 // 16 bytes a lane from the buffer to the 1 KB of LDS at byte `dst`; no register is written, and the kernel waits for
 // vmcnt(0) and a barrier before it reads that LDS.  The builtin does the same, but the compiler then waits for it before
