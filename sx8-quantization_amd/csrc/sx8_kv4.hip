@@ -41,16 +41,17 @@ struct Enc {
 };
 constexpr uint32_t kLevel0 = 0x4B400000u;      // 1.5 2^23 as a float: adding it rounds to an integer, in the low bits
 
-// The level of x: (x - m) / s to the nearest, ties to even, in exact arithmetic: x - m is exact in binary64, and the
-// rounded quotient is put right by its exact remainder.
+// The level of x: (x - m) / s to the nearest, ties to even, in exact arithmetic.  The quotient in binary64 is at most one
+// level off (bf16's x - m is rounded where x is far smaller than m), and x lies on one side or the other of the borders of its
+// level, m + (q +- 1/2) s, which are exact: multiples of 2^-25 below 2^21.
 __device__ __noinline__ uint32_t exact_level(float x, float m, float s) {
 #pragma clang fp contract(off)
-    const double d = (double)x - (double)m, s64 = s;
-    double q = __builtin_rint(d / s64);
-    const double rem = d - q * s64;
+    const double v = x, m64 = m, s64 = s;
+    double q = __builtin_rint((v - m64) / s64);
+    const double above = m64 + (q + 0.5) * s64, below = m64 + (q - 0.5) * s64;
     const bool odd = (int)q & 1;
-    if (2.0 * rem > s64 || (2.0 * rem == s64 && odd)) q += 1.0;
-    else if (-2.0 * rem > s64 || (-2.0 * rem == s64 && odd)) q -= 1.0;
+    if (v > above || (v == above && odd)) q += 1.0;
+    else if (v < below || (v == below && odd)) q -= 1.0;
     return kLevel0 + (uint32_t)(int)fmin(fmax(q, 0.0), 15.0);
 }
 

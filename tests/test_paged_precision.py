@@ -165,3 +165,29 @@ def test_varlen_not_finite_with_a_small_weight(hiplib, cuda, dt, bad, nkeys, at)
     assert same[sees].all() and torch.isfinite(got[~sees]).all()
     got[..., 7] = 0
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_append_levels_exactly(hiplib, cuda, dt):
+    """Values on the border between two levels and next to it by any amount (bf16: far below what binary64 holds beside the
+    minimum) get the level of the definition, decided here in rational numbers."""
+    from fractions import Fraction
+    tiny = [2.0 ** -e for e in ((20, 40, 60, 100, 126) if dt is BF16 else (12, 14, 20, 24))]
+    groups = []
+    for lo in (-1.5, -0.5, -7.5, -14.5, -2.5):                       # steps of 1: zero is the border of two levels
+        groups.append([lo, lo + 15, 0.0, -0.0] + tiny + [-t for t in tiny])
+        groups.append([4 * x for x in groups[-1][:2]] + groups[-1][2:])
+    x = torch.zeros(len(groups), 1, 64, dtype=torch.float64)
+    for i, g in enumerate(groups):
+        x[i, 0, :len(g)] = torch.tensor(g, dtype=torch.float64)
+    x = x.to(dt)
+    want = torch.zeros(len(groups), 1, 64, dtype=torch.float64)
+    for i, row in enumerate(x[:, 0].double().tolist()):
+        lo, hi = min(row), max(row)
+        s = ((torch.tensor(hi) - torch.tensor(lo)) * torch.tensor(1 / 15)).half().double().item()
+        for d, value in enumerate(row):
+            t = (Fraction(value) - Fraction(lo)) / Fraction(s)
+            want[i, 0, d] = lo + s * min(max(round(t), 0), 15)
+    k, _ = pool(x.to(cuda), x.to(cuda), cuda).read(0, len(groups), cum([len(groups)], cuda), dtype=dt)
+    _, v = pool(x.to(cuda), x.to(cuda), cuda).read(0, len(groups), cum([len(groups)], cuda), dtype=dt)
+    assert torch.equal(k.cpu(), want.to(dt)) and torch.equal(v, k)
