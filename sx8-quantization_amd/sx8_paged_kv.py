@@ -36,6 +36,7 @@ def _rows(name, t, heads, hd, device, dtype=None, min_ts=0):
     if dtype is not None and t.dtype != dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
     _dtype(name, t)
+    t = t.resolve_neg()                                             # (a view that negates on reading)
     return t if _in_place(t, min_ts) else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -50,6 +51,8 @@ def _out(name, out, like, heads, hd):
         return torch.empty(like.shape[0], heads, hd, dtype=like.dtype, device=like.device)
     if out.shape != (like.shape[0], heads, hd) or out.dtype != like.dtype or out.device != like.device:
         raise RuntimeError(f"{name} must be {(like.shape[0], heads, hd)} {like.dtype} on {like.device}")
+    if out.is_neg():
+        raise RuntimeError(f"{name} may not be a view that negates on reading")
     # no two rows of the output may share memory
     ts, hs = out.stride()[:2]
     apart = hs >= hd and ts >= (heads - 1) * hs + hd or ts >= hd and hs >= (out.shape[0] - 1) * ts + hd
@@ -60,7 +63,7 @@ def _out(name, out, like, heads, hd):
 
 def _ints(name, t, n, device):
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 1 \
-            or (n is not None and t.numel() != n) or not t.is_contiguous():
+            or (n is not None and t.numel() != n) or not t.is_contiguous() or t.is_neg():
         raise RuntimeError(f"{name} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on {device}")
     return t
 
@@ -147,7 +150,7 @@ class PagedKV4:
     def _bind(self, pages, table, lens, refs, n_kv, head_dim, page_tokens):
         nb = self._page_bytes(n_kv, head_dim, page_tokens)
         if pages.dtype != torch.uint8 or pages.dim() != 3 or pages.shape[2] != nb or not pages.is_contiguous() \
-                or pages.numel() == 0 or pages.device.type != "cuda":
+                or pages.numel() == 0 or pages.device.type != "cuda" or pages.is_neg():
             raise RuntimeError(f"pages must be a contiguous (layers, pages, {nb}) uint8 tensor on the GPU")
         if table.dim() != 2 or not table.is_contiguous():
             raise RuntimeError("table must be a contiguous (slots, pages) int32 tensor")
