@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import itertools
 import math
 import time
 
@@ -582,9 +583,9 @@ class PagedDecoder:
     ``prompt`` runs the prompts of any slots as one packed pass (a slot that has tokens already goes on from them),
     ``step`` decodes one token of every slot in use, replayed from a HIP graph; ``fork``, ``free`` and ``compact`` are the
     cache's.  Linears, norms and RoPE are the kernels of prefill_fused with one row per new token; K and V rows go
-    into the pages as they leave RoPE.  New prompts attend their own fp16 rows (attn_varlen); rows with
-    earlier tokens, and every decoded token, attend the pages (PagedKV4.attend; many rows at once read the
-    pages' values back and attend those).  The reference serves one sequence
+    into the pages as they leave RoPE.  New prompts attend their own fp16 rows (attn_varlen), whatever else the call
+    brings; rows with earlier tokens, and every decoded token, attend the pages (PagedKV4.attend; many rows at once
+    read the pages' values back and attend those).  The reference serves one sequence
     (scripts/infer_sx8.py:109-173)."""
 
     def __init__(self, dec, n_slots, max_len=None, n_pages=None, page_tokens=64):
@@ -672,40 +673,58 @@ class PagedDecoder:
             by[s] = p.to(self.dec.device)
         if not by or len(slots) != len(prompts):
             raise ValueError("as many slots as prompts, and at least one")
+        # new sequences first, then those that go on from earlier tokens: the rows of each kind lie together
         order = sorted(by)
-        ids = torch.cat([by[s] for s in order])
-        pos = torch.cat([torch.arange(self.lens[s], self.lens[s] + by[s].numel(), device=self.dec.device) for s in order])
-        new = [by[s].numel() if s in by else 0 for s in range(self.n_slots)]
-        cu = self._ints([0] + [sum(new[:i + 1]) for i in range(self.n_slots)])
+        new = {s: by[s].numel() for s in order if self.lens[s] == 0}
+        old = {s: by[s].numel() for s in order if self.lens[s] > 0}
+        held = {s: self.lens[s] + n for s, n in (*new.items(), *old.items())}
+        ids = torch.cat([by[s] for s in held])
+        pos = torch.cat([torch.arange(self.lens[s], n, device=self.dec.device) for s, n in held.items()])
         pb = self._bufs(ids.numel())
-        self.cache.reserve(self._ints(new))
+        self.cache.reserve(self._ints(by[s].numel() if s in by else 0 for s in range(self.n_slots)))
         self.cache.check()
-        fresh = all(self.lens[s] == 0 for s in by)
         scale = 1.0 / math.sqrt(self.dec.cfg["head_dim"])
 
         # From about 256 query rows of a KV head and slot on, reading the slots back and attending the values is the
         # faster way (32 heads over 8, 8 slots, 4000 tokens before: 32 new tokens 94 us against 72, 64 new 96 against
         # 125, 512 new 347 against 840; one slot of 500: 64 new 18.2 against 17.6, 128 new 19.9 against 25.4).
         group = self.dec.cfg["n_heads"] // self.dec.cfg["n_kv"]
-        many = ids.numel() * group >= 256 * len(by)
-        held = [self.lens[s] + new[s] if s in by else 0 for s in range(self.n_slots)]
-        cu_held = self._ints([0] + [sum(held[:i + 1]) for i in range(self.n_slots)]) if many and not fresh else None
+        many = sum(old.values()) * group >= 256 * len(old)
+        first, total = sum(new.values()), sum(held[s] for s in old)
+
+        def packed(n):                                              # where the rows of n's slots begin
+            return self._ints([0, *itertools.accumulate(n.get(s, 0) for s in range(self.n_slots))])
+
+        cu_new, cu_old, cu_held = map(packed, (new, old, {s: held[s] for s in old}))
+
+        def attend_new(li, q, k, v, out=None):
+            self.cache.append(li, k, v, cu_new)
+            return attn_varlen(q, k, v, cu_new, scale=scale, out=out)
+
+        def attend_old(li, q, k, v, out=None):
+            self.cache.append(li, k, v, cu_old)
+            if many:
+                k, v = self.cache.read(li, total, cu_held)
+                return attn_varlen(q, k, v, cu_old, cu_held, scale, out=out)
+            return self.cache.attend(li, q, cu_old, scale, out=out)
 
         def attend(li, q, k, v):
-            self.cache.append(li, k, v, cu)
-            if fresh:
-                return attn_varlen(q, k, v, cu, scale=scale)
-            if many:
-                k, v = self.cache.read(li, sum(held), cu_held)
-                return attn_varlen(q, k, v, cu, cu_held, scale)
-            return self.cache.attend(li, q, cu, scale)
+            if not old:
+                return attend_new(li, q, k, v)
+            if not new:
+                return attend_old(li, q, k, v)
+            out = torch.empty_like(q)
+            attend_new(li, q[:first], k[:first], v[:first], out[:first])
+            attend_old(li, q[first:], k[first:], v[first:], out[first:])
+            return out
 
         for s in by:                                                # (as the cache has it, whatever comes of the rows)
-            self.lens[s] += new[s]
+            self.lens[s] = held[s]
         self._set_active()
         self._rows(pb, ids, pos, attend)
-        ends = torch.tensor([int(sum(new[:s + 1])) - 1 for s in order], device=self.dec.device)
-        self.logits = self._head(pb["resid"].index_select(0, ends), pb["d"].index_select(0, ends), len(order))
+        ends = dict(zip(held, itertools.accumulate(by[s].numel() for s in held)))
+        last = torch.tensor([ends[s] - 1 for s in order], device=self.dec.device)
+        self.logits = self._head(pb["resid"].index_select(0, last), pb["d"].index_select(0, last), len(order))
         nxt = self.logits.argmax(-1)
         self.tok[torch.tensor(order, device=self.dec.device)] = nxt
         return nxt[torch.tensor([order.index(s) for s in slots], device=self.dec.device)]

@@ -1,0 +1,54 @@
+"""Prompts of new slots and of slots that have tokens already, in one call of the batched decoder."""
+import pytest
+import torch
+
+from test_e2e import TINY
+from test_paged_e2e import ids
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dec(hiplib, cuda):
+    from e2e_decoder import SX8Decoder
+    return SX8Decoder(TINY, device=cuda, seed=3, n_distinct=2, max_len=160)
+
+
+def start(dec, n_slots=4, **kw):
+    """A decoder whose slots 0 and 2 hold tokens."""
+    from e2e_decoder import PagedDecoder
+    pd = PagedDecoder(dec, n_slots, max_len=160, page_tokens=32, **kw)
+    pd.prompt([0, 2], [ids(11, 1, dec.device), ids(40, 2, dec.device)])
+    return pd
+
+
+def rel(a, b):
+    return ((a - b).abs().max() / b.abs().max()).item()
+
+
+@pytest.mark.parametrize("n_old", [4, 100])
+def test_new_and_continuing_slots(dec, cuda, n_old):
+    """Each sequence gets what it gets without the others (few rows behind earlier tokens, and so many that the pages are read
+    back): its attention is the same, and its linears may sum in another order for another number of rows, which moves
+    an fp16 activation by a rounding: 2^-11 of itself, some ten of them a layer, in other directions: 2^-8 of the
+    largest logit for all of them."""
+    from e2e_decoder import PagedDecoder
+    new = {1: ids(25, 3, cuda), 3: ids(70, 4, cuda)}
+    old = {0: ids(n_old, 5, cuda), 2: ids(n_old + 1, 6, cuda)}
+    want = {}
+    alone = PagedDecoder(dec, 4, max_len=160, page_tokens=32)
+    alone.prompt(list(new), list(new.values()))
+    want.update(zip(new, alone.logits))
+    alone = start(dec)
+    alone.prompt(list(old), list(old.values()))
+    want.update(zip(old, alone.logits))
+    pd = start(dec)
+    slots = [3, 0, 1, 2]
+    nxt = pd.prompt(slots, [{**new, **old}[s] for s in slots])
+    far = {s: rel(pd.logits[s], want[s]) for s in range(4)}
+    print("apart by", far, flush=True)
+    assert max(far.values()) <= 2.0 ** -8
+    assert torch.equal(nxt, pd.logits.argmax(-1)[torch.tensor(slots, device=cuda)]) and torch.equal(pd.tok, pd.logits.argmax(-1))
+    assert pd.lens == pd.cache.lens.tolist() == [11 + n_old, 25, 41 + n_old, 70]
+    pd.step()
+    pd.cache.check()
