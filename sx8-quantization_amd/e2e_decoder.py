@@ -692,20 +692,21 @@ class PagedDecoder:
         many = sum(old.values()) * group >= 256 * len(old)
         first, total = sum(new.values()), sum(held[s] for s in old)
 
-        def packed(n):                                              # where the rows of n's slots begin
-            return self._ints([0, *itertools.accumulate(n.get(s, 0) for s in range(self.n_slots))])
+        def packed(n):                                              # where the rows of n's slots begin: of all slots, and of those alone
+            return (self._ints([0, *itertools.accumulate(n.get(s, 0) for s in range(self.n_slots))]),
+                    self._ints([0, *itertools.accumulate(n.values())]))
 
-        cu_new, cu_old, cu_held = map(packed, (new, old, {s: held[s] for s in old}))
+        (cu_new, seq_new), (cu_old, seq_old), (cu_held, seq_held) = map(packed, (new, old, {s: held[s] for s in old}))
 
         def attend_new(li, q, k, v, out=None):
             self.cache.append(li, k, v, cu_new)
-            return attn_varlen(q, k, v, cu_new, scale=scale, out=out)
+            return attn_varlen(q, k, v, seq_new, scale=scale, out=out)
 
         def attend_old(li, q, k, v, out=None):
             self.cache.append(li, k, v, cu_old)
             if many:
                 k, v = self.cache.read(li, total, cu_held)
-                return attn_varlen(q, k, v, cu_old, cu_held, scale, out=out)
+                return attn_varlen(q, k, v, seq_old, seq_held, scale, out=out)
             return self.cache.attend(li, q, cu_old, scale, out=out)
 
         def attend(li, q, k, v):

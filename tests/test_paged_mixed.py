@@ -18,7 +18,7 @@ def start(dec, n_slots=4, **kw):
     """A decoder whose slots 0 and 2 hold tokens."""
     from e2e_decoder import PagedDecoder
     pd = PagedDecoder(dec, n_slots, max_len=160, page_tokens=32, **kw)
-    pd.prompt([0, 2], [ids(11, 1, dec.device), ids(40, 2, dec.device)])
+    pd.prompt([0, 2], [ids(11, 1, dec.device), ids(20, 2, dec.device)])
     return pd
 
 
@@ -26,7 +26,7 @@ def rel(a, b):
     return ((a - b).abs().max() / b.abs().max()).item()
 
 
-@pytest.mark.parametrize("n_old", [4, 100])
+@pytest.mark.parametrize("n_old", [4, 138])
 def test_new_and_continuing_slots(dec, cuda, n_old):
     """Each sequence gets what it gets without the others (few rows behind earlier tokens, and so many that the pages are read
     back): its attention is the same, and its linears may sum in another order for another number of rows, which moves
@@ -49,6 +49,27 @@ def test_new_and_continuing_slots(dec, cuda, n_old):
     print("apart by", far, flush=True)
     assert max(far.values()) <= 2.0 ** -8
     assert torch.equal(nxt, pd.logits.argmax(-1)[torch.tensor(slots, device=cuda)]) and torch.equal(pd.tok, pd.logits.argmax(-1))
-    assert pd.lens == pd.cache.lens.tolist() == [11 + n_old, 25, 41 + n_old, 70]
+    assert pd.lens == pd.cache.lens.tolist() == [11 + n_old, 25, 21 + n_old, 70]
     pd.step()
     pd.cache.check()
+
+
+def test_idle_slots_are_no_sequences(dec, cuda, monkeypatch):
+    """The prompt attention gets the call's sequences alone: slots that bring nothing do not count when it cuts keys into
+    parts, and launch nothing."""
+    import e2e_decoder
+    seen = []
+
+    def spy(q, k, v, cu_q, cu_k=None, *args, **kw):
+        seen.append((cu_q.tolist(), None if cu_k is None else cu_k.tolist()))
+        return attn_varlen(q, k, v, cu_q, cu_k, *args, **kw)
+
+    attn_varlen = e2e_decoder.attn_varlen
+    monkeypatch.setattr(e2e_decoder, "attn_varlen", spy)
+    pd = start(dec, 70)
+    assert seen and all(s == ([0, 11, 31], None) for s in seen)
+    del seen[:]
+    pd.prompt([69, 0, 33], [ids(9, 1, cuda), ids(140, 2, cuda), ids(5, 3, cuda)])
+    layers = TINY["n_layers"]
+    assert seen == [([0, 5, 14], None), ([0, 140], [0, 151])] * layers
+    assert pd.lens == pd.cache.lens.tolist()
