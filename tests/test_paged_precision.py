@@ -191,3 +191,31 @@ def test_append_levels_exactly(hiplib, cuda, dt):
     k, _ = pool(x.to(cuda), x.to(cuda), cuda).read(0, len(groups), cum([len(groups)], cuda), dtype=dt)
     _, v = pool(x.to(cuda), x.to(cuda), cuda).read(0, len(groups), cum([len(groups)], cuda), dtype=dt)
     assert torch.equal(k.cpu(), want.to(dt)) and torch.equal(v, k)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("nq,nkeys", [([700], [3000]), ([3, 90], [5000, 2500])])
+def test_varlen_near_equal_weights(hiplib, cuda, hd, dt, nq, nkeys):
+    """Long rows of nearly equal weights, whose outputs are far smaller than the values: a weight is rounded to the type, within
+    eps / 2 of itself, so an output is within eps / 2 of sum p |v| and its own half step, beside 2^-15 of that sum for scores
+    and sums in 32 bits; and the roundings are independent, each with a third of its largest square: the root mean square."""
+    from sx8_paged_kv import attn_varlen
+    q, k, v = (rand((sum(n), h, hd), i, dt, cuda) for i, (n, h) in enumerate(((nq, 4), (nkeys, 2), (nkeys, 2))))
+    q = q * 0.1
+    got = attn_varlen(q, k, v, cum(nq, cuda), cum(nkeys, cuda)).double()
+    half, a, b = torch.finfo(dt).eps / 2, 0, 0
+    for n, keys in zip(nq, nkeys):
+        qq, kk, vv = q[a:a + n].double(), k[b:b + keys].double(), v[b:b + keys].double()
+        want, size = attention(qq, kk, vv, keys - n), attention(qq, kk, vv.abs(), keys - n)
+        w = torch.matmul(qq.permute(1, 0, 2).contiguous(), kk.repeat_interleave(2, 1).permute(1, 2, 0).contiguous()) / hd ** 0.5
+        w = w.masked_fill(torch.arange(keys, device=cuda) > keys - n + torch.arange(n, device=cuda)[:, None], -math.inf)
+        p = torch.softmax(w, -1)
+        square = torch.matmul(p.square(), vv.square().repeat_interleave(2, 1).permute(1, 0, 2).contiguous()).permute(1, 0, 2)
+        err = got[a:a + n] - want
+        over = (err.abs() - half * want.abs() * (1 + half) - (half + 2.0 ** -15) * size - torch.finfo(dt).tiny).max().item()
+        rms = err.square().mean().sqrt().item()
+        most = half * ((want.square() + square).mean().item() / 3) ** 0.5 * (1 + 4 / (2 * err.numel()) ** 0.5) + 2.0 ** -17 * size.mean().item()
+        print("over", over, "rms", rms, "of", most, flush=True)
+        assert over <= 0 and rms <= most
+        a, b = a + n, b + keys
