@@ -616,7 +616,7 @@ class PagedDecoder:
         cfg, P = d.cfg, _L.ptr
         H, nh, nk, hd, eps, T = cfg["hidden"], cfg["n_heads"], cfg["n_kv"], cfg["head_dim"], cfg["eps"], pb["T"]
         st = _L.stream(d.device)
-        emb = d.embed(ids)
+        emb = d.embed.rows(ids, pb["emb"])                          # (the captured step's own: the module's may be replaced)
         # RoPE and its K/V rows as a prompt's at position 0 of a table and a cache of T rows
         cos, sin = d.cos.index_select(0, pos), d.sin.index_select(0, pos)
         pend, last = (None, 0, 0), len(d.layers) - 1
@@ -644,6 +644,7 @@ class PagedDecoder:
         if pb is None:
             cfg = self.dec.cfg
             pb = self.dec._make_bufs(T)
+            pb["emb"] = torch.empty(T, cfg["hidden"], dtype=torch.float16, device=self.dec.device)
             for name in ("kr", "vr"):
                 pb[name] = torch.empty(cfg["n_kv"], T, cfg["head_dim"], dtype=torch.float16, device=self.dec.device)
             self._pb = {t: b for t, b in self._pb.items() if t == self.n_slots}

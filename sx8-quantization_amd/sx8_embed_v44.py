@@ -71,11 +71,17 @@ class SX8EmbeddingV44(nn.Module):
         T = ids.numel()
         if self._out is None or self._out.shape[0] < T:
             self._out = torch.empty(T, self.K, dtype=torch.float16, device=DEV)
-        y = _L.py().embed(ids, self._hdr, self._lvl, self._bas, self._sca, self.K, self.N, self.n_cb, self._out)
+        return self.rows(ids, self._out)
+
+    def rows(self, ids, out):
+        """The rows of ids, written into the first ones of `out` (at least as many rows, K) fp16: for a caller with a
+        buffer of its own, which no later call with more ids replaces."""
+        self._load()
+        y = _L.py().embed(ids, self._hdr, self._lvl, self._bas, self._sca, self.K, self.N, self.n_cb, out)
         if y is not None:
             return y
         ids_c = ids.reshape(-1).to(torch.long)
-        out = self._out[:T]
+        out = out[:ids_c.numel()]
         ext().sx8_embed_v44(ids_c, self._hdr, self._lvl, self._bas, self._sca,
                             self.K, self.N, self.n_cb, out)
         return out.reshape(*ids.shape, self.K)

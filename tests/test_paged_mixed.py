@@ -73,3 +73,52 @@ def test_idle_slots_are_no_sequences(dec, cuda, monkeypatch):
     layers = TINY["n_layers"]
     assert seen == [([0, 5, 14], None), ([0, 140], [0, 151])] * layers
     assert pd.lens == pd.cache.lens.tolist()
+
+
+def test_embedding_rows_are_the_decoders_own(dec, cuda):
+    """Prompts and steps, captured ones too, write none of the embedding module's buffer, which a longer call replaces: a graph
+    that wrote it would go on writing freed memory."""
+    pd = start(dec)
+    dec.embed(ids(90, 1, cuda))
+    dec.embed._out.fill_(7)
+    pd.step()
+    pd.prompt([1], [ids(30, 2, cuda)])
+    pd.step()
+    pd.step(use_graph=False)
+    torch.cuda.synchronize()
+    assert (dec.embed._out == 7).all()
+    kept = dec.embed._out.data_ptr()
+    pd.prompt([3], [ids(150, 3, cuda)])
+    assert dec.embed._out.data_ptr() == kept
+    # the captured step after a longer prompt: the tokens of eager steps
+    other = start(dec)
+    other.step(use_graph=False)
+    other.prompt([1], [ids(30, 2, cuda)])
+    for _ in range(2):
+        other.step(use_graph=False)
+    other.prompt([3], [ids(150, 3, cuda)])
+    for _ in range(4):
+        assert torch.equal(pd.step(), other.step(use_graph=False))
+    pd.cache.check()
+
+
+def test_two_decoders_at_once(dec, cuda):
+    """Two batched decoders over one set of weights, on two streams at once, give what they give one after the other."""
+    def run(streams):
+        pds = [start(dec) for _ in range(2)]
+        for i, pd in enumerate(pds):
+            pd.prompt([1], [ids(20 + i, 7 + i, cuda)])
+            pd.step()
+        torch.cuda.synchronize()
+        out = [[], []]
+        for _ in range(5):
+            for i, pd in enumerate(pds):
+                with torch.cuda.stream(streams[i]):
+                    out[i].append(pd.step())
+        torch.cuda.synchronize()
+        return [torch.stack(o) for o in out]
+
+    one = torch.cuda.current_stream()
+    want = run([one, one])
+    got = run([torch.cuda.Stream(), torch.cuda.Stream()])
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
