@@ -19,8 +19,8 @@ namespace {
 // last key lie past the buffer and come as zeros.  A 16-byte chunk of a row lies at its position XOR a few bits of
 // the row, so that neither kind of read meets bank conflicts (the swap is made in the load's address).
 // Bound by the matrix cores and the softmax's VALU, which two waves a SIMD of different work-groups overlap: one prompt of
-// 8192 tokens (32 heads over 8 of 128, bf16) takes 515-535 us, 1028-1067 TFLOP/s, where a library product of 8192^3
-// reaches 1100-1150.  Short prompts are bound by a work-group's start (about 5 us: lengths, query, first tile): 24 of
+// 8192 tokens (32 heads over 8 of 128, bf16) takes 515-550 us by machine, 1000-1067 TFLOP/s, where a library product of
+// 8192^3 reaches 1100-1150: the MFMA is busy 51% of a SIMD's cycles and the VALU 46%.  Short prompts are bound by a work-group's start (about 5 us: lengths, query, first tile): 24 of
 // 40 .. 2000 tokens 230 us, three of up to 96 tokens 7.  s_setprio around the products (541 us against 533), tiles of 32
 // keys with three waves a SIMD (544 against 528) and work-groups that stay and request the next rows ahead (561 against
 // 515) were slower.  Heads of 256 leave room for one wave a SIMD: 8192 tokens of 16 heads over 4 take 699 us (787 TFLOP/s;
@@ -115,7 +115,8 @@ constexpr int var_lds_bytes() {
 }
 
 // A wave's rows key by key, over the keys that each attends alone: for rows in whose sums there is a value that is no
-// finite number (about 1 us a key).  Such a value reaches the row however small its weight: one that underflows counts as 1
+// finite number (2 to 5 us a key: 8192 tokens of 32 heads take 18 ms with a NaN in one of the last keys' values, 41 with one in
+// the first's).  Such a value reaches the row however small its weight: one that underflows counts as 1
 // there, and a sum that is not finite is not scaled.  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
 template <int HD, bool kBf16, typename V, int NT>
 __device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, const uint16_t* v, const VarIo& io,
@@ -259,6 +260,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_varlen(const Va
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
+    // The weights enter the matrix cores in the type, as the values do (their sum stays in 32 bits): as two numbers each they
+    // would double the products of V, half of what the matrix cores do here, for an output that is 2.1 to 2.5e-4 off
+    // in fp16 where its own rounding is 1.8 to 2.0e-4 (bf16 2.1e-3 and 1.6e-3).
     // running maximum in powers of two, kept kUp below the largest score and raised when one exceeds it by more than kUp + 8:
     // probabilities stay at or below 2^15 in fp16, where many small ones (each over 2^-21 of the largest) keep their 11
     // bits, and at or below 2^8 in bf16, which holds small ones as well as large
@@ -425,9 +429,10 @@ __global__ __launch_bounds__(256) void k_varlen_combine(const VarIo io) {
 
 // Work-groups of a call at most (a tile of rows of a head each), and the parts that its keys are cut into: with few
 // work-groups the keys of each are shared by up to 16, so that about 1024 run, each with at least 256 keys of a sequence of
-// average length, or 1024 where there is a work-group for every CU already.  With the reader of the cache before it, 32
-// heads over 8: 8 rows after 16000 keys 298 -> 60 us, 128 rows after 4000 92 -> 40; 8 sequences of 8 rows after 16000 keys
-// 440 -> 380; 1024 rows after 500 keys in three parts of 500 42 -> 51, so they stay whole.
+// average length, or 1024 where there is a work-group for every CU already.  32 heads over 8, alone: 8 rows after 16000 keys
+// 44 us and 8 sequences of such 233, where their bytes take 11 and 86.  With the reader of the cache before it: 8 rows
+// after 16000 keys 298 -> 60 us, 128 rows after 4000 92 -> 40; 8 sequences of 8 rows after 16000 keys 440 -> 380; 1024 rows
+// after 500 keys in three parts of 500 42 -> 51, so they stay whole.
 int64_t var_items(int64_t n_seq, int64_t Tq, int64_t nh) { return ((Tq + kRows - 1) / kRows + (n_seq < Tq ? n_seq : Tq)) * nh; }
 int var_splits(int64_t n_seq, int64_t Tk, int64_t items) {
     const int64_t a = items > 0 ? 1024 / items : 1, b = Tk / (n_seq * (items < 256 ? 256 : 1024)), c = a < b ? a : b;

@@ -48,7 +48,7 @@ SX8_KV4_FN uint32_t kv4_param(uint32_t hd, uint32_t which, uint32_t t, uint32_t 
 // slot's blocks.  Units lie one after another (slots, heads, row tiles) on a line that the waves of the launch share
 // evenly, so a unit may be cut into several pieces, each a run of blocks.  On the line a unit is its blocks and kKv4Begin
 // places before them, for what a piece costs beside its blocks (a wave that gets only those has nothing to do).  With 1,
-// 3 and 6 of them 48 slots of 60 .. 8000 tokens take 28.2, 26.3 and 25.4 us, 16 slots of 8 new tokens 21.5, 19.7 and 20.2.
+// 3 and 6 of them 48 slots of 60 .. 8000 tokens take 27.3, 25.0 and 24.7 us, 16 slots of 8 new tokens 20.5, 19.2 and 19.5.
 constexpr int kKv4Begin = 3;
 struct Kv4Shape {
     int n_slots, nk, G;

@@ -328,13 +328,14 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Pool p, const RowsOut
 // and sum(q_g) fits.
 // The running maximum is kept kUp powers of two below the largest score and raised when a score exceeds it by kUp + kSlack,
 // so that p is at most 2^13, the largest weight at least 2^10, and p * s holds its 22 bits down to p * s = 2^-3 in those
-// units (below that it is within 2^-25).  (Raised at every larger score, four long slots take 52.2 us instead of 49.4.)
+// units (below that it is within 2^-25).  (Raised at every larger score, four long slots take 54.4 us instead of 51.7.)
 // Scales of 2 or more (groups that span 30 or more) would take p * s out of fp16: those go in 2^k times smaller, below 2 and
 // from 1/16 on, with their levels 2^k times as large, in matrix products of their own for each of k = 5, 10 and 15 that a
 // block has.  So what is kept of a token does not depend on the scales of other groups or tokens.
-// Bound by memory once it runs, by its chain of loads (lengths, table, block) before: a first block takes 6.2 us, then the
-// blocks come at 5 TB/s.  8 KV heads of 128: 48 slots of 60 .. 8000 tokens 21 us and the combine 4.7, 32 slots of 16384
-// tokens 122 us (4.96 TB/s).  Three sets of registers ahead instead of two: no faster.
+// Bound by its chain of loads (lengths, table, block) first: a first block takes 6.2 us; then by memory and the VALU together: the
+// blocks come at 4.3-5 TB/s, a stream that is only read at 6.1, with the VALU active 55% of the time (four long
+// slots).  8 KV heads of 128: 48 slots of 60 .. 8000 tokens 21.7 us and the combine 4.0, 32 slots of 16384 tokens 122-139 us
+// by machine.  Three sets of registers ahead instead of two: no faster.
 constexpr float kUp = 10.f, kSlack = 3.f;
 
 template <int HD>
@@ -793,7 +794,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attend(const Kv4
 
 // Units that were cut: work-group (i, row) takes a row of record i and adds the unit's parts up in their order (part 0 at its
 // place, part j at place 2 (wave + j)).  The parts are shared by kWaves waves, whose sums meet in LDS.  A launch costs 1.8
-// us and three dependent loads; 48 slots of up to 8000 tokens take 4.7 us, 16 slots of 8 new tokens 5.8 (work-groups of
+// us and three dependent loads; 48 slots of up to 8000 tokens take 4.0-4.7 us, 16 slots of 8 new tokens 5.6-6.0 (work-groups of
 // 16 waves for four rows at once: 5.9 and 6.5; two waves a row: 4.8 and 5.1, but twice the rounds where one slot of
 // many has most of the tokens).
 template <int HD, bool kBf16, int kWaves>
