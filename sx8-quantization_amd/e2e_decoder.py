@@ -19,6 +19,7 @@ import ctypes
 import functools
 import itertools
 import math
+import operator
 import time
 
 import torch
@@ -568,6 +569,11 @@ class SX8Decoder(nn.Module):
         return out
 
 
+def _numbers(slots):
+    """Slot numbers as ints: a list, or a vector of integers of torch or numpy."""
+    return [operator.index(s) for s in slots]
+
+
 def _on_device(method):
     """A PagedDecoder method run with the decoder's device as the current one."""
     @functools.wraps(method)
@@ -667,7 +673,7 @@ class PagedDecoder:
     @torch.no_grad()
     def prompt(self, slots, prompts):
         """Append `prompts` (a list of int64 token vectors) to the slots and return the next token of each (len(slots),)."""
-        by = {}
+        by, slots = {}, _numbers(slots)
         for s, p in zip(slots, prompts):
             if not 0 <= s < self.n_slots or s in by or p.numel() == 0 or self.lens[s] + p.numel() > self.max_len:
                 raise ValueError(f"slot {s}: out of range, named twice, an empty prompt or past {self.max_len} tokens")
@@ -777,6 +783,7 @@ class PagedDecoder:
 
     def fork(self, src, dst):
         """The empty slots dst[i] go on from where the slots src[i] are."""
+        src, dst = _numbers(src), _numbers(dst)
         if len(src) != len(dst) or len(set(dst)) != len(dst) or any(self.lens[b] or not self.lens[a] for a, b in zip(src, dst)):
             raise ValueError("fork: as many used sources as empty, distinct targets")
         self.cache.fork(self._ints(src), self._ints(dst))
@@ -788,6 +795,7 @@ class PagedDecoder:
 
     def free(self, slots):
         """Empty the slots; pages that no other slot shares are free again."""
+        slots = _numbers(slots)
         if any(not 0 <= s < self.n_slots for s in slots):
             raise ValueError(f"free: slots are 0..{self.n_slots - 1}")
         self.cache.free(self._ints(slots))

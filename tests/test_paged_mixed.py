@@ -122,3 +122,25 @@ def test_two_decoders_at_once(dec, cuda):
     want = run([one, one])
     got = run([torch.cuda.Stream(), torch.cuda.Stream()])
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_slot_numbers_as_vectors(dec, cuda):
+    """Slot numbers in torch or numpy vectors are the slots that ints name; numbers that are no integers are refused."""
+    import numpy as np
+    from e2e_decoder import PagedDecoder
+    a, b = (PagedDecoder(dec, 5, max_len=100, page_tokens=32) for _ in range(2))
+    prompts = [ids(9, 1, cuda), ids(40, 2, cuda)]
+    want = a.prompt([3, 1], prompts)
+    assert torch.equal(b.prompt(torch.tensor([3, 1]), prompts), want) and a.lens == b.lens == b.cache.lens.tolist()
+    a.fork([1, 1], [0, 2])
+    with pytest.raises(ValueError):
+        b.fork(torch.tensor([1, 1]), torch.tensor([0, 0]))
+    b.fork(np.array([1, 1]), torch.tensor([0, 2]))
+    a.free([3])
+    b.free(np.array([3]))
+    assert a.lens == b.lens == b.cache.lens.tolist() == [40, 40, 40, 0, 0]
+    assert torch.equal(a.step(), b.step())
+    with pytest.raises(ValueError):
+        b.prompt(torch.tensor([3, 3]), prompts)
+    with pytest.raises(TypeError):
+        b.prompt([3.0], prompts[:1])
