@@ -687,9 +687,13 @@ class PagedDecoder:
         held = {s: self.lens[s] + n for s, n in (*new.items(), *old.items())}
         ids = torch.cat([by[s] for s in held])
         pos = torch.cat([torch.arange(self.lens[s], n, device=self.dec.device) for s, n in held.items()])
-        pb = self._bufs(ids.numel())
         self.cache.reserve(self._ints(by[s].numel() if s in by else 0 for s in range(self.n_slots)))
         self.cache.check()
+        for s in by:                                                # (as the cache has it, whatever comes of the rows)
+            self.lens[s] = held[s]
+        self._set_active()
+        # the last prompt's buffers may go now: check waited for this stream, whichever stream they were made on
+        pb = self._bufs(ids.numel())
         scale = 1.0 / math.sqrt(self.dec.cfg["head_dim"])
 
         # From about 256 query rows of a KV head and slot on, reading the slots back and attending the values is the
@@ -726,9 +730,6 @@ class PagedDecoder:
             attend_old(li, q[first:], k[first:], v[first:], out[first:])
             return out
 
-        for s in by:                                                # (as the cache has it, whatever comes of the rows)
-            self.lens[s] = held[s]
-        self._set_active()
         self._rows(pb, ids, pos, attend)
         ends = dict(zip(held, itertools.accumulate(by[s].numel() for s in held)))
         last = torch.tensor([ends[s] - 1 for s in order], device=self.dec.device)

@@ -144,3 +144,29 @@ def test_slot_numbers_as_vectors(dec, cuda):
         b.prompt(torch.tensor([3, 3]), prompts)
     with pytest.raises(TypeError):
         b.prompt([3.0], prompts[:1])
+
+
+def test_buffers_go_when_nothing_runs_on_them(dec, cuda, monkeypatch):
+    """A prompt replaces the last one's buffers behind the wait of the cache's check, on whatever stream they were made and
+    used; where there is no memory for the new ones, lengths are still the cache's."""
+    pd = start(dec)
+    order = []
+    check, bufs = pd.cache.check, pd._bufs
+    monkeypatch.setattr(pd.cache, "check", lambda: order.append("check") or check())
+    monkeypatch.setattr(pd, "_bufs", lambda n: order.append("bufs") or bufs(n))
+    pd.prompt([1], [ids(7, 1, cuda)])
+    assert order == ["check", "bufs"]
+
+    def none(n):
+        raise torch.cuda.OutOfMemoryError("none left")
+
+    monkeypatch.setattr(pd, "_bufs", none)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        pd.prompt([1, 3], [ids(7, 1, cuda), ids(9, 1, cuda)])
+    assert pd.lens == pd.cache.lens.tolist() == [11, 14, 20, 9] and pd.active.tolist() == [1] * 4
+    monkeypatch.setattr(pd, "_bufs", bufs)
+    pd.free([1, 3])
+    other = start(dec)
+    assert torch.equal(pd.prompt([3], [ids(9, 1, cuda)]), other.prompt([3], [ids(9, 1, cuda)]))
+    used = torch.tensor([0, 2, 3], device=cuda)
+    assert torch.equal(pd.step()[used], other.step()[used]) and pd.active.tolist() == [1, 0, 1, 1]
