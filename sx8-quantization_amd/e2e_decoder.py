@@ -755,9 +755,11 @@ class PagedDecoder:
     @torch.no_grad()
     def step(self, use_graph=True):
         """Decode one token of every slot in use: returns the next tokens (n_slots,), kept as the step's input of the
-        next call (slots not in use: meaningless)."""
-        if any(n >= self.max_len for n in self.lens):
-            raise ValueError(f"a slot is full ({self.max_len} tokens)")
+        next call (slots not in use: meaningless).  A slot that has max_len tokens has to be freed first (ValueError,
+        nothing changed), as every step takes all slots in use."""
+        full = [s for s, n in enumerate(self.lens) if n >= self.max_len]
+        if full:
+            raise ValueError(f"slots {full} are full ({self.max_len} tokens): free them first")
         self.cache.reserve(self.active)
         if any(n and n % self.cache.page_tokens == 0 for n in self.lens):
             self.cache.check()                                      # (a slot needs a page: is there one?)

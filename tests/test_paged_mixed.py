@@ -170,3 +170,15 @@ def test_buffers_go_when_nothing_runs_on_them(dec, cuda, monkeypatch):
     assert torch.equal(pd.prompt([3], [ids(9, 1, cuda)]), other.prompt([3], [ids(9, 1, cuda)]))
     used = torch.tensor([0, 2, 3], device=cuda)
     assert torch.equal(pd.step()[used], other.step()[used]) and pd.active.tolist() == [1, 0, 1, 1]
+
+
+def test_full_slots_are_named(dec, cuda):
+    from e2e_decoder import PagedDecoder
+    pd = PagedDecoder(dec, 3, max_len=40, page_tokens=32)
+    pd.prompt([0, 2], [ids(12, 1, cuda), ids(40, 2, cuda)])
+    with pytest.raises(ValueError, match=r"slots \[2\] are full"):
+        pd.step()
+    assert pd.lens == pd.cache.lens.tolist() == [12, 0, 40]
+    pd.free([2])
+    pd.step()
+    assert pd.lens == pd.cache.lens.tolist() == [13, 0, 0]
