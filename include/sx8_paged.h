@@ -73,7 +73,9 @@ int32_t sx8_kv4_read(const uint8_t* pages, const int32_t* table, const int32_t* 
 
 /* Attention of the slots' new rows q (rows, nh, hd) over their pages: row i of a slot's n sits at position
  * lens - n + i and attends positions 0 .. that one; out (rows, nh, hd).  No position: zeros.  scale > 0,
- * nh a multiple of nk.  Levels and scales enter exactly; sums are held in float32.  Two launches;
+ * nh a multiple of nk.  Levels and scales enter exactly, weights times scales as two fp16 numbers: to 22 bits, or within
+ * 2^-35 of the largest weight (for scales of 2, 64 or 2048 on: 2^5, 2^10 or 2^15 times that); sums are held in float32.
+ * Two launches;
  * workspace: sx8_kv4_attend_workspace_bytes(hd) bytes, 256-byte aligned, no clearing needed. */
 int32_t sx8_kv4_attend(const uint8_t* pages, const int32_t* table, const int32_t* lens, const int32_t* cu,
                        int64_t n_slots, int64_t max_pages, int64_t n_pages, const void* q, void* out, int64_t rows,
