@@ -20,7 +20,8 @@ namespace {
 // the row, so that neither kind of read meets bank conflicts (the swap is made in the load's address).
 // Bound by the matrix cores and the softmax's VALU, which two waves a SIMD of different work-groups overlap: one prompt of
 // 8192 tokens (32 heads over 8 of 128, bf16) takes 515-550 us by machine, 1000-1067 TFLOP/s, where a library product of
-// 8192^3 reaches 1100-1150: the MFMA is busy 51% of a SIMD's cycles and the VALU 46%.  Short prompts are bound by a work-group's start (about 5 us: lengths, query, first tile): 24 of
+// 8192^3 reaches 1100-1150: the MFMA is busy 51% of a SIMD's cycles and the VALU 46%.  Short prompts are bound by a
+// work-group's start (about 5 us: lengths, query, first tile): 24 of
 // 40 .. 2000 tokens 230 us, three of up to 96 tokens 7.  s_setprio around the products (541 us against 533), tiles of 32
 // keys with three waves a SIMD (544 against 528) and work-groups that stay and request the next rows ahead (561 against
 // 515) were slower.  Heads of 256 leave room for one wave a SIMD: 8192 tokens of 16 heads over 4 take 699 us (787 TFLOP/s;
@@ -117,7 +118,8 @@ constexpr int var_lds_bytes() {
 // A wave's rows key by key, over the keys that each attends alone: for rows in whose sums there is a value that is no
 // finite number (2 to 5 us a key: 8192 tokens of 32 heads take 18 ms with a NaN in one of the last keys' values, 41 with one in
 // the first's).  Such a value reaches the row however small its weight: one that underflows counts as 1
-// there, and a sum that is not finite is not scaled.  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the accumulators do.
+// there, and a sum that is not finite is not scaled.  Lane 32 h + c holds the row c's dimensions 32 n + 8 g + 4 h + r, as the
+// accumulators do.
 template <int HD, bool kBf16, typename V, int NT>
 __device__ __forceinline__ void slow_rows(const uint16_t* q, const uint16_t* k, const uint16_t* v, const VarIo& io,
                                           int from, int to, int lim, int h, V (&o)[NT], float& m, float& l) {

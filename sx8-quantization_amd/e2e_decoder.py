@@ -703,7 +703,7 @@ class PagedDecoder:
         many = sum(old.values()) * group >= 256 * len(old)
         first, total = sum(new.values()), sum(held[s] for s in old)
 
-        def packed(n):                                              # where the rows of n's slots begin: of all slots, and of those alone
+        def packed(n):                                              # where rows begin: of all slots, and of n's alone
             return (self._ints([0, *itertools.accumulate(n.get(s, 0) for s in range(self.n_slots))]),
                     self._ints([0, *itertools.accumulate(n.values())]))
 
