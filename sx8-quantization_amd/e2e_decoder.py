@@ -703,11 +703,15 @@ class PagedDecoder:
         many = sum(old.values()) * group >= 256 * len(old)
         first, total = sum(new.values()), sum(held[s] for s in old)
 
-        def packed(n):                                              # where rows begin: of all slots, and of n's alone
-            return (self._ints([0, *itertools.accumulate(n.get(s, 0) for s in range(self.n_slots))]),
-                    self._ints([0, *itertools.accumulate(n.values())]))
+        def packed(n, wanted):                                      # where rows begin: of all slots, and of n's alone
+            if not wanted:
+                return None, None
+            return self._ints([0, *itertools.accumulate(n.get(s, 0) for s in range(self.n_slots)),
+                               0, *itertools.accumulate(n.values())]).split((self.n_slots + 1, len(n) + 1))
 
-        (cu_new, seq_new), (cu_old, seq_old), (cu_held, seq_held) = map(packed, (new, old, {s: held[s] for s in old}))
+        cu_new, seq_new = packed(new, new)
+        cu_old, seq_old = packed(old, old)
+        cu_held, seq_held = packed({s: held[s] for s in old}, old and many)
 
         def attend_new(li, q, k, v, out=None):
             self.cache.append(li, k, v, cu_new)
