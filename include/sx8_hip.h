@@ -44,7 +44,7 @@ extern "C" {
  * 6: sx8_linear_f16, sx8_quant_pca(_workspace_bytes); sx8_dec_attn_workspace_bytes returns the
  *    bytes of 64 chunks (the entry points still run with those of 16)
  * 7: sx8_paged.h: sx8_attn_varlen, sx8_kv4_* */
-#define SX8_ABI_VERSION 7
+#define SX8_ABI_VERSION 8
 
 #define SX8_OK 0
 #define SX8_ERR_INVALID 1      /* bad argument (null pointer, size, hdr_bytes, alignment) */

@@ -84,6 +84,33 @@ int32_t sx8_kv4_attend(const uint8_t* pages, const int32_t* table, const int32_t
                        void* stream);
 int64_t sx8_kv4_attend_workspace_bytes(int32_t hd);
 
+/* Drafted tokens (sx8_draft.h): sx8_kv4_append for rows as the linears leave them.  Per head row x of q and k:
+ * x <- x / sqrt(mean x^2 + eps) w where weights q_norm, k_norm (hd values of dtype, or NULL) are given, then the pairs (a, b) of the
+ * first rot dimensions (a multiple of 16) become (a cos - b sin, b cos + a sin): (i, i + rot / 2), interleaved != 0: (2 i, 2 i + 1).
+ * cos and sin are rows of rot / 2 float32 values (cos_t, sin_t, table_rows of them, 16-byte aligned, any scaling of angles and
+ * lengths in them); a row takes the one of its position: lens - n + depth[row] (int32), or lens - n + i without depth.  That
+ * is computed in 64 bits and rounded to float32 and from there to dtype; q goes to out (rows, nh, hd), k and v (rounded to dtype) into the
+ * pages as sx8_kv4_append puts them.  in_dtype: dtype, or 2 (float32).  A row whose position lies outside the tables gets
+ * zeros in out and is not written to the pages.  out shares no memory with q, k, v and the tables. */
+int32_t sx8_kv4_append_rope(uint8_t* pages, const int32_t* table, const int32_t* lens, const int32_t* cu, int64_t n_slots,
+                            int64_t max_pages, int64_t n_pages, const void* q, const void* k, const void* v, void* out,
+                            int64_t rows, int64_t q_ts, int64_t q_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
+                            int64_t v_hs, int64_t o_ts, int64_t o_hs, int32_t nh, int32_t nk, int32_t hd,
+                            int32_t page_tokens, const float* cos_t, const float* sin_t, int64_t table_rows, int32_t rot,
+                            int32_t interleaved, const int32_t* depth, const void* q_norm, const void* k_norm, double eps,
+                            int32_t in_dtype, int32_t dtype, void* stream);
+
+/* sx8_kv4_attend where the new rows form a tree: row i of a slot's n attends the lens - n tokens before them and those new rows
+ * j whose bit (j % 64 of word j / 64) is set in mask (rows, words) uint64, words 1..4; new rows from 64 words on are attended by
+ * none.  A row that attends nothing gives zeros.  out shares no memory with q.  Two launches; workspace:
+ * sx8_kv4_attend_tree_workspace_bytes(hd) bytes, 256-byte aligned, no clearing needed. */
+int32_t sx8_kv4_attend_tree(const uint8_t* pages, const int32_t* table, const int32_t* lens, const int32_t* cu,
+                            int64_t n_slots, int64_t max_pages, int64_t n_pages, const void* q, void* out, int64_t rows,
+                            int64_t q_ts, int64_t q_hs, int64_t o_ts, int64_t o_hs, const uint64_t* mask, int32_t words,
+                            int32_t nh, int32_t nk, int32_t hd, int32_t page_tokens, float scale, int32_t dtype,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+int64_t sx8_kv4_attend_tree_workspace_bytes(int32_t hd);
+
 /* Page operations.  Each takes free pages lowest number first, in the order of its slots or entries, and does all
  * of it or nothing: where it cannot, status (2 int32: code, slot or entry) is set if it was zero, and nothing
  * else changes.  Codes: 1 bad slot or count, 2 no free pages, 3 the slot's table row is full, 4 the target slot
@@ -95,7 +122,17 @@ int64_t sx8_kv4_attend_workspace_bytes(int32_t hd);
  * free: the slots' pages lose a reference, their rows become -1 and their lengths 0.  A slot named twice is freed
  *   once.  One launch, no workspace.
  * compact: the used pages above the number of used pages move to the free ones below it, highest
- *   free places last (i-th such page to the i-th such place); tables and refs follow. */
+ *   free places last (i-th such page to the i-th such place); tables and refs follow.
+ * keep: of its n new rows (cu, rows as above) a slot keeps counts[s], the rows path[cu[s]] < path[cu[s] + 1] < .. (row numbers in
+ *   the slot, (rows) int32 as sx8_draft_verify gives them): in every layer they move together behind the tokens before the new ones,
+ *   lens becomes lens - n + counts[s], pages behind that lose a reference and leave the table.  Slots without new rows stay as they
+ *   are (counts 0).  The pages of the new rows must be the slot's own; a row or place without a page is not moved.  Code 1: a count
+ *   outside 0 .. n, rows out of order, fewer tokens than rows.  workspace: sx8_kv4_keep_workspace_bytes, 16-byte aligned. */
+int64_t sx8_kv4_keep_workspace_bytes(int64_t n_slots, int64_t rows);
+int32_t sx8_kv4_keep(uint8_t* pages, int64_t n_layers, int32_t* table, int32_t* lens, int32_t* refs, const int32_t* cu,
+                     const int32_t* path, const int32_t* counts, int64_t rows, int64_t n_slots, int64_t max_pages,
+                     int64_t n_pages, int32_t nk, int32_t hd, int32_t page_tokens, int32_t* status, void* workspace,
+                     int64_t workspace_bytes, void* stream);
 int64_t sx8_kv4_pages_workspace_bytes(int64_t n_slots, int64_t n_pages);
 int32_t sx8_kv4_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* add, int64_t n_slots,
                         int64_t max_pages, int64_t n_pages, int32_t page_tokens, int32_t* status, void* workspace,

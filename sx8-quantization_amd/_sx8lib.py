@@ -22,7 +22,7 @@ LIB_NAME = "libsx8_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["sx8_abi.hip", "sx8_dequant.hip", "sx8_layout.hip", "sx8_quant.hip", "sx8_gemv.hip",
            "sx8_gemm.hip", "sx8_gemm_small.hip", "sx8_decoder.hip", "sx8_attn_varlen.hip", "sx8_kv4.hip",
-           "sx8_pages.hip"]
+           "sx8_kv4_rope.hip", "sx8_kv4_tree.hip", "sx8_pages.hip", "sx8_draft.hip"]
 PY_SOURCE, PY_PATH = "sx8_py.cpp", os.path.join(PKG_DIR, "_sx8py.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -129,13 +129,26 @@ SIGNATURES = [
     ("sx8_kv4_attend", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32,
                               _I32, ctypes.c_float, _I32, _P, _I64, _P]),
     ("sx8_kv4_attend_workspace_bytes", _I64, [_I32]),
+    ("sx8_kv4_append_rope", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+                                   _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _I32, _I32, _P, _P, _P,
+                                   ctypes.c_double, _I32, _I32, _P]),
+    ("sx8_kv4_attend_tree", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I32, _I32,
+                                   _I32, _I32, _I32, ctypes.c_float, _I32, _P, _I64, _P]),
+    ("sx8_kv4_attend_tree_workspace_bytes", _I64, [_I32]),
     ("sx8_kv4_pages_workspace_bytes", _I64, [_I64, _I64]),
     ("sx8_kv4_reserve", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P, _P, _I64, _P]),
     ("sx8_kv4_fork", _I32, [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _I64, _P]),
     ("sx8_kv4_free", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P]),
     ("sx8_kv4_compact", _I32, [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    ("sx8_kv4_keep_workspace_bytes", _I64, [_I64, _I64]),
+    ("sx8_kv4_keep", _I32, [_P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _I64, _P]),
+    # include/sx8_draft.h
+    ("sx8_draft_tree", _I32, [_P, _P, _I64, _I64, _I32, _P, _P, _P]),
+    ("sx8_draft_verify_workspace_bytes", _I64, [_I64, _I64, _I64]),
+    ("sx8_draft_verify", _I32, [_P, _I64, _I32, _P, _P, _P, _I64, _I64, _I64, _P, _P, ctypes.c_float, _P, _I64, _I32, _P,
+                                _P, _P, _P, _I64, _P]),
 ]
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 _lib = None
 _py = None

@@ -89,15 +89,41 @@ struct Kv4Run {
 };
 // a / b; the wide division only where it is needed
 SX8_KV4_FN int64_t kv4_div(int64_t a, int b) { return (uint64_t)a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
-SX8_KV4_FN Kv4Run kv4_run(int64_t x, int64_t off, int64_t x1, int nb) {
-    const int all = nb + kKv4Begin;
+SX8_KV4_FN Kv4Run kv4_run(int64_t x, int64_t off, int64_t x1, int nb, int before = kKv4Begin) {
+    const int all = nb + before;
     const int64_t unit = kv4_div(off, all);
     const int v0 = (int)(off - unit * all), v1 = all - v0 < x1 - x ? all : v0 + (int)(x1 - x);
-    return Kv4Run{unit, v0 > kKv4Begin ? v0 - kKv4Begin : 0, v1 > kKv4Begin ? v1 - kKv4Begin : 0, v1 - v0};
+    return Kv4Run{unit, v0 > before ? v0 - before : 0, v1 > before ? v1 - before : 0, v1 - v0};
 }
 // How many waves have blocks of a unit whose first block lies at place `at`, in the share of `wave`.
 SX8_KV4_FN int kv4_parts(int64_t at, int nb, int64_t share, int wave) {
     return (int)((at + nb - 1) / share - wave + 1);
+}
+
+// ---- the pieces of the attention of drafted trees ----------------------------------------------
+// The same line, for units of `cols` query rows of a KV head (row r of a slot's n G: token r / G) that work-groups of
+// four waves share; a share has a block for each wave at least.
+constexpr int kTreeBegin = 8, kTreeWaves = 4;
+SX8_KV4_FN int kv4_tree_tiles(int n, int G, int cols) { return (int)(((int64_t)n * G + cols - 1) / cols); }
+SX8_KV4_FN int64_t kv4_tree_places(const Kv4Shape& sh, int cols, int n, int len) {
+    return (int64_t)sh.nk * kv4_tree_tiles(n, sh.G, cols) * (kv4_unit_blocks(len) + kTreeBegin);
+}
+SX8_KV4_FN int64_t kv4_tree_share(int64_t total, int groups) {
+    const int64_t p = (total + groups - 1) / groups;
+    return p < kTreeWaves ? kTreeWaves : p;
+}
+// Which of the 32 keys from `key0` on a row attends whose slot had `first` tokens before its new ones: those, and new ones
+// j with bit j of its mask (words of 64).
+SX8_KV4_FN uint32_t kv4_tree_bits(const uint64_t* mask, int words, int first, int key0) {
+    const int64_t at = (int64_t)key0 - first;
+    if (at + 32 <= 0) return 0xFFFFFFFFu;
+    if (at < 0) return (uint32_t)(mask[0] << -at) | ((1u << -at) - 1u);
+    const int64_t w = at >> 6;
+    const int sh = (int)(at & 63);
+    if (w >= words) return 0;
+    uint64_t v = mask[w] >> sh;
+    if (sh > 32 && w + 1 < words) v |= mask[w + 1] << (64 - sh);
+    return (uint32_t)v;
 }
 
 // Blocks of tokens that the new tokens of a slot touch (append, read): first block, and how many.  Positions

@@ -1,4 +1,4 @@
-// sx8_pages.hip -- page operations of the paged KV cache: reserve, fork, free and compact
+// sx8_pages.hip -- page operations of the paged KV cache: reserve, fork, free, compact and keep
 // (include/sx8_paged.h).
 //
 // The tables are small and the decisions on them ordered (lowest free page first, all or nothing), so one work-group
@@ -343,6 +343,173 @@ __global__ __launch_bounds__(256) void k_compact_copy(uint8_t* pages, int64_t pa
     }
 }
 
+// ---- keep --------------------------------------------------------------------------------------
+// Workspace of keep: header (0: nothing to do), then by slot the tokens before its new rows and where its pages begin
+// in a list of those pages, which the table loses before the rows move.
+struct KeepWs {
+    int32_t* head;                 // [4]
+    int32_t* base;                 // [n_slots]
+    int32_t* at;                   // [n_slots]
+    int32_t* pages;                // [rows / page_tokens + 2 n_slots]
+};
+int64_t keep_ws_bytes(int64_t n_slots, int64_t rows) { return 16 + 4 * (2 * n_slots + rows / 32 + 2 * n_slots); }
+KeepWs keep_ws(void* w, int64_t n_slots) {
+    int32_t* b = reinterpret_cast<int32_t*>(w);
+    return KeepWs{b, b + 4, b + 4 + n_slots, b + 4 + 2 * n_slots};
+}
+
+// A slot of n new rows keeps rows path[0] < path[1] < .. (counts of them) of these.
+__global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const int32_t* path, const int32_t* counts,
+                                                       const int32_t* cu, Kv4Shape sh, const KeepWs ws) {
+    const int tid = threadIdx.x, pt = t.page_tokens;
+    const int64_t cap = (int64_t)t.max_pages * pt;
+    int code = 0, item = 0, total = 0;
+    for (int s0 = 0; s0 < t.n_slots; s0 += kPageThreads) {
+        const int s = s0 + tid;
+        int held = 0;                                                // pages with new rows
+        if (s < t.n_slots) {
+            int first, n;
+            kv4_rows(sh, cu, s, &first, &n);
+            const int len = t.lens[s], c = counts[s], base = len - n;
+            bool bad = false;
+            if (n > 0) {
+                bad = c < 0 || c > n || base < 0 || len > cap;
+                for (int i = 0, last = -1; !bad && i < c; ++i) {
+                    const int at = path[first + i];
+                    bad = at <= last || at >= n;
+                    last = at;
+                }
+                if (!bad) held = (len + pt - 1) / pt - base / pt;
+            } else {
+                bad = c != 0;
+            }
+            if (bad && !code) {
+                code = 1;
+                item = s;
+            }
+            ws.base[s] = n > 0 ? base : -1;
+        }
+        int all;
+        const int before = total + scan_before(held, &all);
+        if (s < t.n_slots) ws.at[s] = before;
+        total = total + all < 0 ? 0x7FFFFFFF : total + all;
+    }
+    // (a cu that runs backwards can name more rows than there are)
+    if (!code && total > sh.rows / 32 + 2 * t.n_slots) {
+        code = 1;
+        item = 0;
+    }
+    code = worst(code, item, &item);
+    if (tid == 0) ws.head[0] = code == 0;
+    if (code) {
+        report(t.status, code, item);
+        return;
+    }
+    for (int s = tid; s < t.n_slots; s += kPageThreads) {
+        const int base = ws.base[s], len = t.lens[s], at = ws.at[s];
+        if (base < 0) continue;
+        const int end = base + counts[s], have = (end + pt - 1) / pt;
+        for (int i = base / pt; i < (len + pt - 1) / pt; ++i) {
+            const int64_t e = (int64_t)s * t.max_pages + i;
+            const int page = t.table[e];
+            ws.pages[at + i - base / pt] = page;
+            if (i >= have) {
+                if (page >= 0 && page < t.n_pages) atomicSub(&t.refs[page], 1);
+                t.table[e] = -1;
+            }
+        }
+        t.lens[s] = end;
+    }
+}
+
+// Work-group (slot, head, layer): the kept rows, a block of the places they go to at a time.  Rows only move to
+// the front, so a block's rows come from it or from later ones: read all of them, then write.  K's words belong to one
+// token each; a V word holds eight tokens of a dimension and keeps those that are not replaced.
+template <int HD>
+__global__ __launch_bounds__(256) void k_keep_move(uint8_t* pages, const int32_t* path, const int32_t* counts,
+                                                   const int32_t* cu, Kv4Shape sh, int page_tokens, int64_t n_pages,
+                                                   int64_t page_bytes, const KeepWs ws) {
+    constexpr int kBB = kv4_block_bytes(HD), NG = HD / kKv4Group, kK = 32 * (HD / 8) / 256, kV = 4 * HD / 256 > 0 ? 4 * HD / 256 : 1;
+    constexpr int kP = (32 * 4 * NG + 255) / 256;
+    __shared__ const uint8_t* from[32];                              // block of the row that goes to token t, null: none
+    __shared__ int row[32];                                          // and its token there
+    const int s = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+    int first, n;
+    kv4_rows(sh, cu, s, &first, &n);
+    if (n == 0 || ws.head[0] == 0) return;
+    const int c = counts[s];
+    if (c == 0 || path[first + c - 1] == c - 1) return;              // (they lie together already)
+    const int base = ws.base[s], bpp = page_tokens / 32;
+    const int32_t* const list = ws.pages + ws.at[s];
+    uint8_t* const layer = pages + (int64_t)blockIdx.z * n_pages * page_bytes + (int64_t)head * bpp * kBB;
+    auto block = [&](int pos) -> uint8_t* {
+        const int page = list[pos / page_tokens - base / page_tokens];
+        return page < 0 || page >= n_pages ? nullptr : layer + page * page_bytes + (int64_t)(pos % page_tokens / 32) * kBB;
+    };
+    for (int b = base / 32; b * 32 < base + c; ++b) {
+        uint8_t* const dst = block(b * 32 < base ? base : b * 32);
+        __syncthreads();                                             // (the list of the last block is read)
+        bool moves = false;
+        if (tid < 32) {
+            const int i = b * 32 + tid - base;
+            const uint8_t* src = nullptr;
+            if (i >= 0 && i < c) {
+                const int at = path[first + i];
+                if (at != i) {
+                    src = block(base + at);
+                    row[tid] = (base + at) % 32;
+                }
+            }
+            from[tid] = src;
+            moves = src != nullptr;
+        }
+        if (!__syncthreads_or(moves) || dst == nullptr) continue;
+        uint32_t k[kK], v[kV];
+        uint16_t prm[kP];
+#pragma unroll
+        for (int u = 0; u < kK; ++u) {
+            const int i = tid + 256 * u, t = i % 32, d = i / 32 * 8;
+            if (from[t]) k[u] = *reinterpret_cast<const uint32_t*>(from[t] + kv4_k_word(HD, row[t], d));
+        }
+#pragma unroll
+        for (int u = 0; u < kV; ++u) {
+            const int i = tid + 256 * u, d = i % HD, h = i / HD;
+            if (i >= 4 * HD) break;
+            const uint32_t old = *reinterpret_cast<const uint32_t*>(dst + kv4_v_word(HD, 4 * h, d));
+            v[u] = old;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int t = e / 4 * 16 + 4 * h + e % 4;
+                if (!from[t]) continue;
+                const uint32_t lv = *reinterpret_cast<const uint32_t*>(from[t] + kv4_v_word(HD, row[t], d)) >> kv4_v_shift(row[t]) & 15u;
+                v[u] = (v[u] & ~(15u << kv4_shift(e))) | lv << kv4_shift(e);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kP; ++u) {
+            const int i = tid + 256 * u, t = i % 32, which = i / 32 % 4, g = i / 128;
+            if (g < NG && from[t]) prm[u] = *reinterpret_cast<const uint16_t*>(from[t] + kv4_param(HD, which, row[t], g));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kK; ++u) {
+            const int i = tid + 256 * u, t = i % 32, d = i / 32 * 8;
+            if (from[t]) *reinterpret_cast<uint32_t*>(dst + kv4_k_word(HD, t, d)) = k[u];
+        }
+#pragma unroll
+        for (int u = 0; u < kV; ++u) {
+            const int i = tid + 256 * u, d = i % HD, h = i / HD;
+            if (i >= 4 * HD) break;
+            *reinterpret_cast<uint32_t*>(dst + kv4_v_word(HD, 4 * h, d)) = v[u];
+        }
+#pragma unroll
+        for (int u = 0; u < kP; ++u) {
+            const int i = tid + 256 * u, t = i % 32, which = i / 32 % 4, g = i / 128;
+            if (g < NG && from[t]) *reinterpret_cast<uint16_t*>(dst + kv4_param(HD, which, t, g)) = prm[u];
+        }
+    }
+}
+
 int32_t make_tab(const char* what, PageTab* t, int32_t* table, int32_t* lens, int32_t* refs, int64_t n_slots,
                  int64_t max_pages, int64_t n_pages, int32_t page_tokens, int32_t* status) {
     if (!table || !refs) return fail(SX8_ERR_INVALID, "%s: null pointer", what);
@@ -447,5 +614,45 @@ extern "C" int32_t sx8_kv4_compact(uint8_t* pages, int64_t n_layers, int64_t pag
     hipLaunchKernelGGL(k_compact, dim3(1), dim3(kPageThreads), 0, as_stream(stream), t, ws);
     hipLaunchKernelGGL(k_compact_copy, dim3((unsigned)(most < 2048 ? most : 2048)), dim3(256), 0, as_stream(stream), pages,
                        page_bytes, (int)chunks, n_layers, t, ws);
+    return check_launch(what);
+}
+
+extern "C" int64_t sx8_kv4_keep_workspace_bytes(int64_t n_slots, int64_t rows) {
+    using namespace sx8;
+    if (n_slots <= 0 || n_slots > kKv4MaxSlots || rows < 0 || rows > 0x7FFFFFFF) return -1;
+    return keep_ws_bytes(n_slots, rows);
+}
+
+extern "C" int32_t sx8_kv4_keep(uint8_t* pages, int64_t n_layers, int32_t* table, int32_t* lens, int32_t* refs,
+                                const int32_t* cu, const int32_t* path, const int32_t* counts, int64_t rows, int64_t n_slots,
+                                int64_t max_pages, int64_t n_pages, int32_t nk, int32_t hd, int32_t page_tokens,
+                                int32_t* status, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace sx8;
+    const char* what = "sx8_kv4_keep";
+    if (!lens || !status || !counts || (!path && rows > 0)) return fail(SX8_ERR_INVALID, "%s: null pointer", what);
+    PageTab t;
+    int32_t rc = make_tab(what, &t, table, lens, refs, n_slots, max_pages, n_pages, page_tokens, status);
+    if (rc != SX8_OK) return rc;
+    const int64_t pb = sx8_kv4_page_bytes(nk, hd, page_tokens);
+    if (pb < 0) return fail(SX8_ERR_INVALID, "%s: bad shape (hd 64, 128 or 256, 1 <= nk <= 256)", what);
+    rc = check_pages(what, pages, n_layers, pb);
+    if (rc != SX8_OK) return rc;
+    if (rows < 0 || rows > 0x7FFFFFFF || (!cu && rows != n_slots))
+        return fail(SX8_ERR_INVALID, "%s: bad rows (without cu one row a slot)", what);
+    if (!aligned(cu, 4) || !aligned(path, 4) || !aligned(counts, 4))
+        return fail(SX8_ERR_INVALID, "%s: cu, path and counts must be 4-byte aligned", what);
+    if (!workspace || workspace_bytes < keep_ws_bytes(n_slots, rows) || !aligned(workspace, 16))
+        return fail(SX8_ERR_INVALID, "%s: workspace needs %lld bytes, 16-byte aligned", what, (long long)keep_ws_bytes(n_slots, rows));
+    if (rows == 0) return ok();
+    const Kv4Shape sh{(int)n_slots, nk, 1, (int)(max_pages * page_tokens), (int)rows};
+    const KeepWs ws = keep_ws(workspace, n_slots);
+    hipLaunchKernelGGL(k_keep, dim3(1), dim3(kPageThreads), 0, as_stream(stream), t, path, counts, cu, sh, ws);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n_slots, (unsigned)nk, (unsigned)n_layers), dim3(256), 0, as_stream(stream),
+                           pages, path, counts, cu, sh, page_tokens, n_pages, pb, ws);
+    };
+    if (hd == 64) go(k_keep_move<64>);
+    else if (hd == 128) go(k_keep_move<128>);
+    else go(k_keep_move<256>);
     return check_launch(what);
 }

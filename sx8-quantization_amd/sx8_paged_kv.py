@@ -3,7 +3,8 @@
 ``attn_varlen`` is the prompt attention of a packed batch; ``PagedKV4`` holds the K and V rows of
 n_slots sequences in pages of 4-bit values (4.5 bits with their scales, a quarter of an fp16 cache), which
 ``append`` writes, ``attend`` reads for the new tokens of every slot and ``reserve``, ``fork``, ``free`` and
-``compact`` manage.  The kernels and the format are those of include/sx8_paged.h; lengths, tables and
+``compact`` manage; ``append_rope``, ``attend_tree`` and ``keep`` are for drafted tokens that are checked together
+(sx8_draft).  The kernels and the format are those of include/sx8_paged.h; lengths, tables and
 counts live on the device and no call waits for it, so a step of all of them can be captured in a
 graph.  The reference serves one sequence with the Hugging Face cache (scripts/infer_sx8.py:109-173).
 """
@@ -27,15 +28,16 @@ def _dtype(name, t):
     return _DTYPES[t.dtype]
 
 
-def _rows(name, t, heads, hd, device, dtype=None, min_ts=0):
-    """A (rows, heads, hd) tensor that the kernels can read in place, or a contiguous copy of it."""
+def _rows(name, t, heads, hd, device, dtype=None, min_ts=0, wide=False):
+    """A (rows, heads, hd) tensor that the kernels can read in place, or a contiguous copy of it (wide: float32 too)."""
     if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd:
         raise RuntimeError(f"{name} must be (rows, {heads}, {hd}), got {tuple(t.shape)}")
     if t.device != device:
         raise RuntimeError(f"{name} must be on {device}, got {t.device}")
     if dtype is not None and t.dtype != dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
-    _dtype(name, t)
+    if not (wide and t.dtype == torch.float32):
+        _dtype(name, t)
     t = t.resolve_neg()                                             # (a view that negates on reading)
     return t if _in_place(t, min_ts) else t.clone(memory_format=torch.contiguous_format)
 
@@ -66,6 +68,25 @@ def _ints(name, t, n, device):
             or (n is not None and t.numel() != n) or not t.is_contiguous() or t.is_neg():
         raise RuntimeError(f"{name} must be a contiguous int32 vector{'' if n is None else f' of {n}'} on {device}")
     return t
+
+
+def _table(name, t, device):
+    """A table of cosines or sines (positions, half of the rotated dimensions) float32, 16-byte aligned and contiguous."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.dim() != 2 or t.device != device:
+        raise RuntimeError(f"{name} must be a (positions, half of the rotated dimensions) float32 tensor on {device}")
+    if t.is_neg() or not t.is_contiguous() or t.data_ptr() % 16:
+        t = t.resolve_neg().clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _weights(name, t, hd, dtype, device):
+    """hd norm weights of dtype, or None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != (hd,) or t.device != device:
+        raise RuntimeError(f"{name} must be {hd} values of {dtype} on {device}")
+    t = t.resolve_neg()
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _scale(scale, hd):
@@ -169,6 +190,7 @@ class PagedKV4:
         if self._ws_pages < 0 or self.max_pages * self.page_tokens > 1 << 22:
             raise RuntimeError("a cache has 1..4096 slots of up to 2^22 tokens and up to 2^28 pages")
         self._ws_attend = int(_L.lib().sx8_kv4_attend_workspace_bytes(self.head_dim))
+        self._ws_tree = int(_L.lib().sx8_kv4_attend_tree_workspace_bytes(self.head_dim))
         self._t = (pages, table, lens, refs, status, nb, self.n_kv, self.head_dim, self.page_tokens, self._ws_attend,
                    self._ws_pages)
 
@@ -241,6 +263,66 @@ class PagedKV4:
                     _L.stream(self.device))
         return out
 
+    def append_rope(self, layer, q, k, v, cos, sin, cu=None, depth=None, q_norm=None, k_norm=None, eps=1e-6,
+                    interleaved=False, dtype=None, out=None):
+        """`append` of rows as the linears leave them: q (rows, heads, head_dim) and k are normed per head (where q_norm,
+        k_norm, head_dim values, are given: x / sqrt(mean x^2 + eps) w) and rotated; k and v go into the pages, the new
+        query rows are returned (into `out`).  cos and sin (positions, r / 2) float32 rotate the first r dimensions (a
+        multiple of 16) in pairs (i, i + r / 2), or (2 i, 2 i + 1) where interleaved; tables of scaled angles serve long contexts.
+        A row's position is that of the slot's first new row plus depth[row] (int32; without depth: its number in the
+        slot), where trees of drafted tokens have several rows of one depth (sx8_draft.draft_tree).  Rows are fp16, bf16, or
+        float32 (then dtype, fp16 unless given, is what they are rounded to, once).  A row whose position lies outside the tables
+        gives zeros and is not written.  out shares no memory with q, k and v."""
+        if dtype is None:
+            dtype = torch.float16 if q.dtype == torch.float32 else q.dtype
+        with torch.cuda.device(self.device):
+            nh = q.shape[1] if q.dim() == 3 else 0
+            q = _rows("q", q, nh, self.head_dim, self.device, wide=True)
+            k = _rows("k", k, self.n_kv, self.head_dim, self.device, q.dtype, wide=True)
+            v = _rows("v", v, self.n_kv, self.head_dim, self.device, q.dtype, wide=True)
+            if k.shape[0] != q.shape[0] or v.shape[0] != q.shape[0]:
+                raise RuntimeError(f"q, k and v have {q.shape[0]}, {k.shape[0]} and {v.shape[0]} rows")
+            if dtype not in _DTYPES or q.dtype not in (dtype, torch.float32):
+                raise RuntimeError(f"dtype must be float16 or bfloat16, and that of rows that are not float32, got {dtype}")
+            cos, sin = (_table(n, t, self.device) for n, t in (("cos", cos), ("sin", sin)))
+            if cos.shape != sin.shape:
+                raise RuntimeError(f"cos and sin must be of one shape, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+            q_norm, k_norm = (_weights(n, t, self.head_dim, dtype, self.device) for n, t in (("q_norm", q_norm), ("k_norm", k_norm)))
+            if depth is not None:
+                _ints("depth", depth, q.shape[0], self.device)
+            like = q if q.dtype == dtype else torch.empty(q.shape[0], 0, 0, dtype=dtype, device=self.device)
+            out = _out("out", out, like, nh, self.head_dim)
+            if out.shape[0] and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+                raise RuntimeError("out may not be q, k or v")
+            _L.call("sx8_kv4_append_rope", *self._slots(layer, cu), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                    q.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
+                    out.stride(1), nh, self.n_kv, self.head_dim, self.page_tokens, cos.data_ptr(), sin.data_ptr(),
+                    cos.shape[0], 2 * cos.shape[1], int(bool(interleaved)), None if depth is None else depth.data_ptr(),
+                    None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                    float(eps), 2 if q.dtype == torch.float32 else _DTYPES[dtype], _DTYPES[dtype], _L.stream(self.device))
+        return out
+
+    def attend_tree(self, layer, q, mask, cu=None, scale=None, out=None):
+        """`attend` for rows that form trees: row i of a slot's n new ones attends the lens - n tokens before them and those new
+        rows j of the slot whose bit is set in mask (rows, words) int64 (bit j % 64 of word j // 64; 1 to 4 words;
+        sx8_draft.draft_tree makes them from parents; a row's own bit is no exception).  New rows from 64 words on are attended
+        by none.  A row that attends nothing gives zeros.  Returns out (rows, heads, head_dim), which shares no memory with q."""
+        with torch.cuda.device(self.device):
+            nh = q.shape[1] if q.dim() == 3 else 0
+            q = _rows("q", q, nh, self.head_dim, self.device)
+            if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != q.shape[0] or not 1 <= mask.shape[1] <= 4 \
+                    or mask.device != self.device or not mask.is_contiguous() or mask.is_neg():
+                raise RuntimeError(f"mask must be a contiguous ({q.shape[0]}, 1 to 4) int64 tensor on {self.device}")
+            out = _out("out", out, q, nh, self.head_dim)
+            if out.shape[0] and out.data_ptr() == q.data_ptr():
+                raise RuntimeError("out may not be q")
+            ws = torch.empty(self._ws_tree, dtype=torch.uint8, device=self.device)
+            _L.call("sx8_kv4_attend_tree", *self._slots(layer, cu), q.data_ptr(), out.data_ptr(), q.shape[0], q.stride(0),
+                    q.stride(1), out.stride(0), out.stride(1), mask.data_ptr(), mask.shape[1], nh, self.n_kv, self.head_dim,
+                    self.page_tokens, _scale(scale, self.head_dim), _DTYPES[q.dtype], ws.data_ptr(), self._ws_tree,
+                    _L.stream(self.device))
+        return out
+
     # ---------------------------------------------------------------- pages
     def _ws(self):
         return torch.empty(self._ws_pages, dtype=torch.uint8, device=self.device)
@@ -290,8 +372,25 @@ class PagedKV4:
                     self.refs.data_ptr(), self.n_slots, self.max_pages, self.n_pages, ws.data_ptr(), self._ws_pages,
                     _L.stream(self.device))
 
+    def keep(self, path, counts, cu=None):
+        """Of its n new rows slot s keeps counts[s], the rows path[cu[s]] < path[cu[s] + 1] < .. (numbers in the slot; both
+        int32 on the device, as sx8_draft.verify_draft returns them): in all layers they move together behind the tokens
+        before the new ones, lens becomes lens - n + counts[s] and pages behind that are given back.  Slots without new rows have
+        counts 0.  The rows' pages must be the slot's own, as for `append`."""
+        with torch.cuda.device(self.device):
+            _ints("path", path, None, self.device)
+            _ints("counts", counts, self.n_slots, self.device)
+            if cu is not None:
+                _ints("cu", cu, self.n_slots + 1, self.device)
+            nb = int(_L.lib().sx8_kv4_keep_workspace_bytes(self.n_slots, path.numel()))
+            ws = torch.empty(max(nb, 0), dtype=torch.uint8, device=self.device)
+            _L.call("sx8_kv4_keep", self.pages.data_ptr(), self.n_layers, self.table.data_ptr(), self.lens.data_ptr(),
+                    self.refs.data_ptr(), None if cu is None else cu.data_ptr(), path.data_ptr(), counts.data_ptr(),
+                    path.numel(), self.n_slots, self.max_pages, self.n_pages, self.n_kv, self.head_dim, self.page_tokens,
+                    self.status.data_ptr(), ws.data_ptr(), nb, _L.stream(self.device))
+
     def check(self):
-        """Wait for the device and raise the first error that reserve, fork or free met since the last check."""
+        """Wait for the device and raise the first error that reserve, fork, free or keep met since the last check."""
         code, item = self.status.tolist()
         if code:
             self.status.zero_()
