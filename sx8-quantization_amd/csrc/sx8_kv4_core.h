@@ -187,51 +187,62 @@ struct Kv4Regs {                          // a lane's share of one block
     uint32_t km[2][(NG + 1) / 2];
     bool bad;
 };
+// A lane's share of the block at `base`: K's words and parameters, and V's.
+template <int HD>
+__device__ __forceinline__ void load_block_k(Kv4Regs<HD>& rg, const uint8_t* base, int lane) {
+    constexpr int W = Kv4Regs<HD>::W, NG = Kv4Regs<HD>::NG;
+    const int c = lane & 15, h = lane >> 4;
+    const uint8_t* prm = base + 32 * HD;
+    if constexpr (W == 2) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(base + a * 512 + lane * 8);
+            rg.kw[a][0] = v.x;
+            rg.kw[a][1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int q4 = 0; q4 < W / 4; ++q4) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(base + a * (256 * W) + q4 * 1024 + lane * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rg.kw[a][4 * q4 + e] = v[e];
+            }
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) rg.ks[g] = *reinterpret_cast<const u32x4*>(prm + (g * 32 + h * 8) * 2);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        const uint8_t* at = prm + NG * 64 + (16 * a + c) * NG * 2;
+        if constexpr (NG == 1) rg.km[a][0] = *reinterpret_cast<const uint16_t*>(at);
+        else if constexpr (NG == 2) rg.km[a][0] = *reinterpret_cast<const uint32_t*>(at);
+        else {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(at);
+            rg.km[a][0] = v.x;
+            rg.km[a][1] = v.y;
+        }
+    }
+}
+template <int HD>
+__device__ __forceinline__ void load_block_v(Kv4Regs<HD>& rg, const uint8_t* base, int lane) {
+    constexpr int NT = Kv4Regs<HD>::NT, NG = Kv4Regs<HD>::NG;
+    const int c = lane & 15, h = lane >> 4;
+    const uint8_t* prm = base + 32 * HD;
+#pragma unroll
+    for (int q4 = 0; q4 < NT / 4; ++q4) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(base + 16 * HD + q4 * 1024 + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rg.vw[4 * q4 + e] = v[e];
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) rg.vs[g] = *reinterpret_cast<const u32x4*>(prm + 2 * NG * 64 + (g * 32 + h * 8) * 2);
+    rg.vm = *reinterpret_cast<const u32x4*>(prm + 3 * NG * 64 + ((c < NG ? c : 0) * 32 + h * 8) * 2);
+}
 template <int HD>
 __device__ __forceinline__ void load_block(Kv4Regs<HD>& rg, const uint8_t* base, int lane) {
-    constexpr int W = Kv4Regs<HD>::W, NT = Kv4Regs<HD>::NT, NG = Kv4Regs<HD>::NG;
-    const int c = lane & 15, h = lane >> 4;
-                const uint8_t* prm = base + 32 * HD;
-                if constexpr (W == 2) {
-    #pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        const u32x2 v = *reinterpret_cast<const u32x2*>(base + a * 512 + lane * 8);
-                        rg.kw[a][0] = v.x;
-                        rg.kw[a][1] = v.y;
-                    }
-                } else {
-    #pragma unroll
-                    for (int a = 0; a < 2; ++a)
-    #pragma unroll
-                        for (int q4 = 0; q4 < W / 4; ++q4) {
-                            const u32x4 v = *reinterpret_cast<const u32x4*>(base + a * (256 * W) + q4 * 1024 + lane * 16);
-    #pragma unroll
-                            for (int e = 0; e < 4; ++e) rg.kw[a][4 * q4 + e] = v[e];
-                        }
-                }
-    #pragma unroll
-                for (int g = 0; g < NG; ++g) rg.ks[g] = *reinterpret_cast<const u32x4*>(prm + (g * 32 + h * 8) * 2);
-    #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const uint8_t* at = prm + NG * 64 + (16 * a + c) * NG * 2;
-                    if constexpr (NG == 1) rg.km[a][0] = *reinterpret_cast<const uint16_t*>(at);
-                    else if constexpr (NG == 2) rg.km[a][0] = *reinterpret_cast<const uint32_t*>(at);
-                    else {
-                        const u32x2 v = *reinterpret_cast<const u32x2*>(at);
-                        rg.km[a][0] = v.x;
-                        rg.km[a][1] = v.y;
-                    }
-                }
-    #pragma unroll
-                for (int q4 = 0; q4 < NT / 4; ++q4) {
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(base + 16 * HD + q4 * 1024 + lane * 16);
-    #pragma unroll
-                    for (int e = 0; e < 4; ++e) rg.vw[4 * q4 + e] = v[e];
-                }
-    #pragma unroll
-                for (int g = 0; g < NG; ++g)
-                    rg.vs[g] = *reinterpret_cast<const u32x4*>(prm + 2 * NG * 64 + (g * 32 + h * 8) * 2);
-                rg.vm = *reinterpret_cast<const u32x4*>(prm + 3 * NG * 64 + ((c < NG ? c : 0) * 32 + h * 8) * 2);
+    load_block_k<HD>(rg, base, lane);
+    load_block_v<HD>(rg, base, lane);
 }
 
 __device__ __forceinline__ f16x8 levels(uint32_t w) {

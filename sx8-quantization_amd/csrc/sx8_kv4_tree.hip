@@ -1,11 +1,18 @@
 // sx8_kv4_tree.hip -- attention of trees of drafted tokens over the paged 4-bit cache (include/sx8_paged.h).
 //
 // The products are those of sx8_kv4.hip: S^T = K Q^T with the levels as fp16 subnormals, O^T += V^T P^T with p * s as two
-// fp16 numbers, the minima's parts in matrix products of their own.  What differs is the shape of the work: a tree brings
-// tens of query rows a KV head, so a unit is 16 kCt of them, and a block's levels are unpacked once for all; a work-group's
-// four waves take a unit's blocks in turn and add their results up in LDS, so that a unit cut over many
-// work-groups leaves one partial result for each.  A block that ends at or behind the first new token is masked
-// by 32 bits of each column's mask.
+// fp16 numbers (cut, not rounded: 21 bits), the minima's parts in matrix products of their own, where a row of ones gives the
+// weights' sum as well.  What differs is the shape of the work: a tree brings tens of query rows a KV head, so a unit is
+// one or two tiles of 16 of them (a block's levels are unpacked once for both); a work-group's four waves take a unit's
+// blocks in turn and add their results up in LDS, so that a unit cut over many work-groups leaves one partial
+// result for each.  A block that ends at or behind the first new token is masked by 32 bits of each column's mask.
+// Bound by the VALU and its chains: for 16 rows and a block of 32 tokens of a head of 128 there are 29 matrix instructions
+// (16 cycles each) and 140 others besides 190 for the block.  A wave keeps one block in registers: K of the next one
+// is requested when the scores are done, V when the products are; no branch lies between, so that the compiler keeps the
+// scores' sums apart from neither (with one: 316 us instead of 108 for the case below).  Query fragments stay in LDS.  Four tiles a
+// unit spill (506 us) or, with one work-group a CU, wait (121).  p * s by mixed multiply-adds that write halves of a register: 102.
+// 8 trees of 64 rows after 2500 .. 4100 tokens, 32 heads over 8 of 128: 97 us; two of 31 after 61000 and 100000, 32 over 4: 222;
+// 24 of 1 .. 24 after up to 8000: 45 (the combine 4.2 more).
 #include "sx8_kv4_core.h"
 
 namespace sx8 {
@@ -32,14 +39,25 @@ struct TreeIo {
 constexpr int kMaxWords = 4;              // of a row's mask: 256 drafted tokens a slot
 // Work-groups a CU by tiles of 16 query rows, as registers allow.
 template <int HD, int kCt>
-constexpr int groups_per_cu() { return HD < 256 && HD * kCt <= 256 ? 2 : 1; }
-constexpr int kMaxGroups = 512;
+constexpr int groups_per_cu() { return HD < 256 && kCt == 1 ? 3 : 2; }
+constexpr int kMaxGroups = 768;
 // Query rows of all partial results: the most that 256 groups_per_cu work-groups have, two units each.
-constexpr int64_t part_rows(int64_t hd) { return hd == 64 ? 2 * 512 * 64 : 2 * 256 * 64; }
+constexpr int64_t part_rows(int64_t hd) { return hd == 256 ? 2 * 512 * 16 : 2 * 512 * 32; }
 constexpr int64_t tree_ws(int64_t hd) { return part_rows(hd) * (hd + 2) * 4 + kMaxGroups * (int64_t)sizeof(TreePiece); }
 
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
+
+// x of eight values as two fp16 numbers each, hi + lo
+__device__ __forceinline__ void halves8(const float* x, u32x4* hi, u32x4* lo) {
+    typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const h2 h = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
+        (*hi)[i] = __builtin_bit_cast(uint32_t, h);
+        (*lo)[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.f, x[2 * i]), __builtin_fmaf((float)h[1], -1.f, x[2 * i + 1])));
+    }
+}
 template <int HD, bool kBf16, int kCt>
 __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(const Kv4Pool p, const TreeIo io) {
     using Regs = Kv4Regs<HD>;
@@ -103,14 +121,13 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
             const int b = b0 + w + 4 * (i0 + lane);
             pages = b < end ? p.table[(int64_t)slot * p.max_pages + (b >> p.bpp_log2)] : -1;
         };
-        auto load = [&](Regs& rg, int i) __attribute__((always_inline)) {
+        // where block i of the wave lies (a page that is none: its place in page 0, and bad)
+        auto where = [&](int i, bool* bad) -> const uint8_t* {
             if (i != 0 && (i & 63) == 0) load_pages(i);
             const int b = b0 + w + 4 * i;
-            int page = __builtin_amdgcn_readlane(pages, i & 63);
-            rg.bad = page < 0 || page >= p.n_pages;
-            page = rg.bad ? 0 : page;
-            load_block<HD>(rg, p.pages + page * p.page_bytes +
-                                   (int64_t)((head << p.bpp_log2) + (b & ((1 << p.bpp_log2) - 1))) * kBB, lane);
+            const int page = __builtin_amdgcn_readlane(pages, i & 63);
+            *bad = page < 0 || page >= p.n_pages;
+            return p.pages + (*bad ? 0 : page) * p.page_bytes + (int64_t)((head << p.bpp_log2) + (b & ((1 << p.bpp_log2) - 1))) * kBB;
         };
         load_pages(0);
         __syncthreads();                                             // the last unit's LDS is free
@@ -170,25 +187,25 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
             }
             masks[col][word] = m;
         }
-        Regs r0, r1;
-        if (cnt > 0) load(r0, 0);
+        Regs rg;
+        bool bad = false;
+        if (cnt > 0) load_block<HD>(rg, where(0, &bad), lane);
         __syncthreads();
-        f16x8 qf[kCt][W];
         float kscale[kCt], m[kCt];
         f32x4 o[kCt][NT], om[kCt];
 #pragma unroll
         for (int ct = 0; ct < kCt; ++ct) {
-#pragma unroll
-            for (int j = 0; j < W; ++j) qf[ct][j] = __builtin_bit_cast(f16x8, frag[ct][j][lane]);
             kscale[ct] = unscale[16 * ct + c];
             m[ct] = -kInf;
             om[ct] = zero4();
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[ct][t] = zero4();
         }
-        auto step = [&](Regs& rg, int i) __attribute__((always_inline)) {
-            if (rg.bad) return;                                      // (no page: no tokens)
+        for (int i = 0; i < cnt; ++i) {
+            bool bad_next;
+            const uint8_t* const next = where(i + 1 < cnt ? i + 1 : i, &bad_next);    // (the last block is loaded again)
             const int b = b0 + w + 4 * i;
+            asm volatile("" ::: "memory");                           // (query fragments stay in LDS: registers)
             float pv[kCt][8];
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
@@ -210,23 +227,25 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     for (int e = 0; e < 4; ++e) ks[e] = sx8_h2f(half_of(rg.ks[g][2 * a + (e >> 1)], e)) * 1048576.f;
 #pragma unroll
                     for (int ct = 0; ct < kCt; ++ct) {
-                        f32x4 acc = mfma16(l0, qf[ct][2 * g], zero4());
-                        acc = mfma16(l1, qf[ct][2 * g + 1], acc);
+                        f32x4 acc = mfma16(l0, __builtin_bit_cast(f16x8, frag[ct][2 * g][lane]), zero4());
+                        acc = mfma16(l1, __builtin_bit_cast(f16x8, frag[ct][2 * g + 1][lane]), acc);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[ct][e] = __builtin_fmaf(ks[e], acc[e], s[ct][e]);
                     }
+                    
                 }
 #pragma unroll
                 for (int ct = 0; ct < kCt; ++ct)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) pv[ct][4 * a + e] = s[ct][e];
             }
+            load_block_k<HD>(rg, next, lane);
             u32x4 vm = rg.vm;
-            if (b * 32 + 31 >= first) {
+            if (b * 32 + 31 >= first || bad) {
                 asm volatile("");                // (a branch: as selects these would run for every block)
 #pragma unroll
                 for (int ct = 0; ct < kCt; ++ct) {
-                    const uint32_t see = kv4_tree_bits(masks[16 * ct + c], kMaxWords, first, b * 32) >> 4 * h;
+                    const uint32_t see = bad ? 0u : kv4_tree_bits(masks[16 * ct + c], kMaxWords, first, b * 32) >> 4 * h;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) pv[ct][e] = see >> (e / 4 * 16 + e % 4) & 1u ? pv[ct][e] : -kInf;
                 }
@@ -252,7 +271,7 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                         nan[g] |= __shfl_xor((int)nan[g], 32, 64);
 #pragma unroll
                         for (int ct = 0; ct < kCt; ++ct)
-                            if (kv4_tree_bits(masks[16 * ct + c], kMaxWords, first, b * 32) & nan[g])
+                            if (!bad && (kv4_tree_bits(masks[16 * ct + c], kMaxWords, first, b * 32) & nan[g]))
 #pragma unroll
                                 for (int t = 4 * g; t < 4 * g + 4; ++t) o[ct][t] += __builtin_nanf("");
                     }
@@ -263,23 +282,33 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     }
                 }
             }
+            float mx[kCt];
+            bool over = false;
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
-                float mx = pv[ct][0];
+                mx[ct] = pv[ct][0];
 #pragma unroll
-                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, pv[ct][e]);
-                mx *= kscale[ct];
-                if (__builtin_amdgcn_ballot_w64(mx > m[ct] + (kUp + kSlack)) != 0) {
-                    const float mn = fmaxf(m[ct], max4(mx - kUp));
+                for (int e = 1; e < 8; ++e) mx[ct] = fmaxf(mx[ct], pv[ct][e]);
+                mx[ct] *= kscale[ct];
+                over |= mx[ct] > m[ct] + (kUp + kSlack);
+            }
+            if (__builtin_amdgcn_ballot_w64(over) != 0) {
+#pragma unroll
+                for (int ct = 0; ct < kCt; ++ct) {
+                    const float mn = fmaxf(m[ct], max4(mx[ct] - kUp));
                     const float alpha = m[ct] == mn ? 1.f : __builtin_amdgcn_exp2f(m[ct] - mn);
                     m[ct] = mn;
                     om[ct] *= alpha;
 #pragma unroll
                     for (int t = 0; t < NT; ++t) o[ct][t] *= alpha;
                 }
+            }
+#pragma unroll
+            for (int ct = 0; ct < kCt; ++ct) {
                 const float nm = m[ct] == -kInf ? 0.f : -m[ct];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(pv[ct][e], kscale[ct], nm));
+                
             }
             // rows of the minima's product: a group's minima, and behind them ones, whose sum is the weights'
             constexpr uint32_t kOnes = 0x3C003C00u;
@@ -289,7 +318,7 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
                 u32x4 hi, lo;
-                split8(pv[ct], u32x4{kOnes, kOnes, kOnes, kOnes}, &hi, &lo);
+                halves8(pv[ct], &hi, &lo);
                 om[ct] = mfma16(vm8, __builtin_bit_cast(f16x8, hi), om[ct]);
                 om[ct] = mfma16(vm8, __builtin_bit_cast(f16x8, lo), om[ct]);
             }
@@ -307,8 +336,11 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                         s = __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, s) * f16x8(down));
 #pragma unroll
                         for (int ct = 0; ct < kCt; ++ct) {
+                            float ps[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) ps[e] = pv[ct][e] * sx8_h2f(half_of(s[e >> 1], e));
                             u32x4 hi, lo;
-                            split8(pv[ct], s, &hi, &lo);
+                            halves8(ps, &hi, &lo);
 #pragma unroll
                             for (int t = 4 * g; t < 4 * g + 4; ++t) {
                                 uint32_t word = rg.vw[t];
@@ -325,31 +357,26 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                f16x8 h8[kCt], l8[kCt];
+                f16x8 lv[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) lv[t] = levels(rg.vw[4 * g + t]);
 #pragma unroll
                 for (int ct = 0; ct < kCt; ++ct) {
                     u32x4 hi, lo;
-                    split8(pv[ct], rg.vs[g], &hi, &lo);
-                    h8[ct] = __builtin_bit_cast(f16x8, hi);
-                    l8[ct] = __builtin_bit_cast(f16x8, lo);
-                }
+                    float ps[8];
 #pragma unroll
-                for (int t = 4 * g; t < 4 * g + 4; ++t) {
-                    const f16x8 lv = levels(rg.vw[t]);
+                    for (int e = 0; e < 8; ++e) ps[e] = pv[ct][e] * sx8_h2f(half_of(rg.vs[g][e >> 1], e));
+                    halves8(ps, &hi, &lo);
 #pragma unroll
-                    for (int ct = 0; ct < kCt; ++ct) {
-                        o[ct][t] = mfma16(lv, h8[ct], o[ct][t]);
-                        o[ct][t] = mfma16(lv, l8[ct], o[ct][t]);
+                    for (int t = 0; t < 4; ++t) {
+                        o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, hi), o[ct][4 * g + t]);
+                        o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, lo), o[ct][4 * g + t]);
                     }
+                    
                 }
             }
-        };
-        for (int i = 0; i < cnt; i += 2) {
-            if (i + 1 < cnt) load(r1, i + 1);
-            step(r0, i);
-            if (i + 1 >= cnt) break;
-            if (i + 2 < cnt) load(r0, i + 2);
-            step(r1, i + 1);
+            load_block_v<HD>(rg, next, lane);
+            bad = bad_next;
         }
         // O = 2^20 (levels) + (the minima's sum of the group, row g of om); the weights' sum in row NG
         float l[kCt];
@@ -529,9 +556,12 @@ extern "C" int32_t sx8_kv4_attend_tree(const uint8_t* pages, const int32_t* tabl
             hipLaunchKernelGGL((k_kv4_tree_combine<HD, kBf, 16 * kCt>), dim3(groups, (unsigned)(most + 3) / 4), dim3(256), 0,
                                as_stream(stream), io, p.sh.G);
         };
-        if (tiles <= 1) go(std::integral_constant<int, 1>{});
-        else if (tiles <= 2 || HD == 256) go(std::integral_constant<int, 2>{});
-        else if constexpr (HD < 256) go(std::integral_constant<int, 4>{});
+        // Two tiles a unit from four tiles a slot on (8 slots of about 3300 tokens, 8 KV heads of 128, 64 rows of 4 heads: 97 us
+        // instead of 112; of 2 rows: 28 instead of 25), where registers allow it (heads of 256: 229 instead of 106).
+        if constexpr (HD < 256) {
+            if (tiles >= 4) return go(std::integral_constant<int, 2>{});
+        }
+        go(std::integral_constant<int, 1>{});
     });
     return check_launch(what);
 }
