@@ -52,10 +52,14 @@ __global__ __launch_bounds__(256) void k_draft_tree(const int32_t* parents, cons
 
 // ---- verification ------------------------------------------------------------------------------
 // Two launches: every row's largest logit and the sum of its weights exp((logit - largest) / temperature), by
-// parts of kPart logits; then a work-group for each slot walks its tree, where a test needs one logit, and draws the next token, where
-// the parts' sums say in which part it lies.  All in binary64: a token must not depend on the order in which 150000 weights
-// were added, and a border of the cumulated sum lies within a binary32 rounding of u once in some hundred draws.
-constexpr int kPart = 8192, kThreads = 256;
+// parts of kPart logits; then a work-group for each slot walks its tree, where a test needs one logit of a row, and draws the
+// next token, where the parts' sums say in which part it lies.  With draft probabilities a refused token costs a sum over the
+// vocabulary: the walk stops there, a launch sums the parts of all slots that wait, and a second walk goes on (further
+// refusals, which trees can have, it sums by itself).  All in binary64: the token must not depend on the order in which 150000
+// weights were added, and of so many borders of the cumulated sum one lies within a binary32 rounding of u once in some
+// hundred draws.  The first launch reads all rows, which is little more than a path's where trees are small, and needs no
+// wait between its work-groups.
+constexpr int kPart = 8192, kRowThreads = 256, kWalkThreads = 1024;
 
 struct RowPart {
     double sum;                           // of exp((x - top) / temperature), or 0 (greedy)
@@ -63,6 +67,12 @@ struct RowPart {
     int32_t arg;                          // its first index
 };
 static_assert(sizeof(RowPart) == 16, "part");
+
+// Where a walk waits for the sums of its slot's parts: weights max(a w / sum - b q, 0) of row `cur`, for the child `row`.
+struct Wait {
+    double a, b;
+    int32_t cur, count, row, open;        // open 0: the slot is done
+};
 
 struct VerifyIo {
     const void* logits;
@@ -79,23 +89,54 @@ struct VerifyIo {
     int32_t *path, *counts;
     int64_t* next;
     RowPart* part;                        // [rows][parts]
+    RowPart* row;                         // [rows]: the whole row
+    double* p;                            // [rows]: probability of a row's token at its parent, below zero: none
     int64_t* gone;                        // [rows]: tokens of a slot that are out of p at its current row
     double* slot_sum;                     // [n_slots][parts]: sums of what is left of p
+    Wait* wait;                           // [n_slots]
 };
 
-template <int kType>                      // 0 fp16, 1 bf16, 2 float32; NaN: -infinity
+template <int kType>                      // 0 fp16, 1 bf16, 2 float32
 __device__ __forceinline__ float value(const void* base, int64_t at) {
     if constexpr (kType == 2) return static_cast<const float*>(base)[at];
     else return ld16<kType == 1>(static_cast<const uint16_t*>(base)[at]);
 }
 __device__ __forceinline__ float logit(float x) { return x == x ? x : -__builtin_inff(); }
 
-// exp((x - top) / temperature): 1 for the largest (an infinity too)
-__device__ __forceinline__ double weight(float x, float top, double scale) {
-    return x == top ? 1.0 : x - top == -__builtin_inff() ? 0.0 : exp(((double)x - (double)top) * scale);
-}
+// exp((x - top) / temperature) for x <= top; scale = log2(e) / temperature.  2^y = 2^n 2^f with n the nearest integer, 2^f by its
+// interpolation in the Chebyshev nodes of [-1/2, 1/2] (degree 10: within 3e-16 of itself).  An infinite top has the weights
+// of a row of -infinity and 0.
+struct Weigh {
+    double top, scale;
+    bool all;                             // top is infinite
+    __device__ __forceinline__ Weigh(float t, double s) : top(t == __builtin_inff() ? 0.0 : t), scale(s), all(t == __builtin_inff()) {}
+    __device__ __forceinline__ double operator()(float x) const {
+        if (all) return x == __builtin_inff() ? 1.0 : 0.0;
+        double y = ((double)x - top) * scale;
+        const bool none = !(y >= -1000.0);                           // (-infinity, and 0 * infinity)
+        y = none ? 0.0 : y;
+        const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
+        double r = 0x1.e6063f7217bc6p-28;
+        r = __builtin_fma(r, f, 0x1.b675bca4eeebbp-24);
+        r = __builtin_fma(r, f, 0x1.62bfd47773353p-20);
+        r = __builtin_fma(r, f, 0x1.ffcb54062e698p-17);
+        r = __builtin_fma(r, f, 0x1.430913096fd9fp-13);
+        r = __builtin_fma(r, f, 0x1.5d87fe9d7a584p-10);
+        r = __builtin_fma(r, f, 0x1.3b2ab6fba1ddap-7);
+        r = __builtin_fma(r, f, 0x1.c6b08d703ce49p-5);
+        r = __builtin_fma(r, f, 0x1.ebfbdff82c598p-3);
+        r = __builtin_fma(r, f, 0x1.62e42fefa3a19p-1);
+        r = __builtin_fma(r, f, 1.0);
+        const uint64_t bits = __builtin_bit_cast(uint64_t, r) + (__builtin_bit_cast(uint64_t, shifted) << 52);
+        return none ? 0.0 : __builtin_bit_cast(double, bits);
+    }
+};
 __device__ __forceinline__ float temperature_of(const VerifyIo& io, int slot) { return io.temperature ? io.temperature[slot] : io.t; }
+__device__ __forceinline__ double scale_of(float temperature) { return 1.4426950408889634 / (double)temperature; }
 
+__device__ __forceinline__ double lane_of_double(double v, int lane) {
+    return __builtin_bit_cast(double, lane_of(__builtin_bit_cast(int64_t, v), lane));
+}
 __device__ __forceinline__ double wave_add(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -111,16 +152,17 @@ __device__ __forceinline__ double wave_prefix_sum(double v) {
     }
     return v;
 }
-// The sum over the work-group, the same in every thread.
+// The sum over the work-group's kT threads, the same in every thread.
+template <int kT>
 __device__ __forceinline__ double group_add(double v) {
-    __shared__ double s[kThreads / 64];
+    __shared__ double s[kT / 64];
     v = wave_add(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     double r = 0.0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) r += s[i];
+    for (int i = 0; i < kT / 64; ++i) r += s[i];
     return r;
 }
 // (top, first index) of two candidates
@@ -149,73 +191,122 @@ __device__ __forceinline__ int slot_of(const Kv4Shape& sh, const int32_t* cu, in
     return s;
 }
 
-template <int kType>
-__global__ __launch_bounds__(kThreads) void k_verify_rows(const VerifyIo io) {
-    constexpr int kE = kPart / kThreads;
+// kWide: rows begin on 16 bytes, and a thread takes 16 bytes at a time.
+template <int kType, bool kWide>
+__global__ __launch_bounds__(kRowThreads) void k_verify_rows(const VerifyIo io) {
+    constexpr int kE = kPart / kRowThreads, kN = !kWide ? 1 : kType == 2 ? 4 : 8;
     const int r = blockIdx.x, part = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-    const int slot = slot_of(io.sh, io.cu, r);
-    if (slot < 0) return;
-    const int64_t base = (int64_t)part * kPart;
+    const int64_t base = (int64_t)part * kPart, from = r * io.stride + base;
     const int n = (int)min((int64_t)kPart, io.V - base);
     float x[kE], top = -__builtin_inff();
-    int arg = 0x7FFFFFFF;
+    auto place = [&](int i) { return (i / kN * kRowThreads + tid) * kN + i % kN; };
+    if constexpr (kWide) {
+        u32x4 raw[kE / kN];
 #pragma unroll
-    for (int i = 0; i < kE; ++i) {
-        const int at = tid + kThreads * i;
-        x[i] = at < n ? logit(value<kType>(io.logits, r * io.stride + base + at)) : -__builtin_inff();
-    }
-#pragma unroll
-    for (int i = 0; i < kE; ++i)
-        if (x[i] > top) {
-            top = x[i];
-            arg = (int)base + tid + kThreads * i;
+        for (int i = 0; i < kE / kN; ++i) {
+            raw[i] = u32x4{0u, 0u, 0u, 0u};
+            const int at = place(i * kN);
+            if (at + kN <= n) raw[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(io.logits) + (from + at) * (kType == 2 ? 4 : 2));
+            else
+                for (int e = 0; e < kN && at + e < n; ++e) {
+                    if constexpr (kType == 2) raw[i][e] = __builtin_bit_cast(uint32_t, value<2>(io.logits, from + at + e));
+                    else raw[i][e >> 1] |= (uint32_t)static_cast<const uint16_t*>(io.logits)[from + at + e] << 16 * (e & 1);
+                }
         }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) better(top, arg, __shfl_xor(top, o, 64), __shfl_xor(arg, o, 64));
-    __shared__ float tops[kThreads / 64];
-    __shared__ int args[kThreads / 64];
-    if (lane == 0) {
-        tops[tid >> 6] = top;
-        args[tid >> 6] = arg;
+        for (int i = 0; i < kE; ++i) {
+            float v;
+            if constexpr (kType == 2) v = __builtin_bit_cast(float, (uint32_t)raw[i / kN][i % kN]);
+            else v = ld16<kType == 1>(half_of(raw[i / kN][i % kN >> 1], i));
+            x[i] = place(i) < n ? logit(v) : -__builtin_inff();
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kE; ++i) x[i] = place(i) < n ? value<kType>(io.logits, from + place(i)) : -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < kE; ++i) x[i] = logit(x[i]);
     }
+    const int slot = slot_of(io.sh, io.cu, r);
+    if (slot < 0) return;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) top = fmaxf(top, x[i]);
+    float all = top;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, 64));
+    __shared__ float tops[kRowThreads / 64];
+    __shared__ int first;
+    if (lane == 0) tops[tid >> 6] = all;
+    if (tid == 0) first = 0x7FFFFFFF;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) better(top, arg, tops[i], args[i]);
+    for (int i = 0; i < kRowThreads / 64; ++i) all = fmaxf(all, tops[i]);
+    if (all > -__builtin_inff() && top == all) {
+        int arg = 0x7FFFFFFF;
+#pragma unroll
+        for (int i = kE - 1; i >= 0; --i)
+            if (x[i] == all) arg = place(i);
+        atomicMin(&first, arg);
+    }
     const float temp = temperature_of(io, slot);
     double sum = 0.0;
-    if (temp > 0.f && top > -__builtin_inff()) {
-        const double scale = 1.0 / (double)temp;
+    if (temp > 0.f && all > -__builtin_inff()) {
+        const Weigh w(all, scale_of(temp));
 #pragma unroll
-        for (int i = 0; i < kE; ++i) sum += weight(x[i], top, scale);
-        sum = group_add(sum);
+        for (int i = 0; i < kE; ++i) sum += w(x[i]);
     }
-    if (tid == 0) io.part[(int64_t)r * io.parts + part] = RowPart{sum, top, arg};
+    sum = group_add<kRowThreads>(sum);                               // (behind its barriers `first` is whole)
+    if (tid == 0) io.part[(int64_t)r * io.parts + part] = RowPart{sum, all, all > -__builtin_inff() ? (int)base + first : 0x7FFFFFFF};
 }
 
-// The largest logit of a row, its first index and the sum of its weights (wave-wide; every lane gets them).
-struct RowSum {
-    double sum;
-    float top;
-    int arg;
-};
-__device__ __forceinline__ RowSum row_sum(const VerifyIo& io, int64_t row, bool greedy, double scale) {
+// A row's parts as one (wave-wide; every lane gets it).
+__device__ __forceinline__ RowPart whole_row(const VerifyIo& io, int64_t row, bool greedy, double scale) {
     const int lane = threadIdx.x & 63;
     const RowPart* const p = io.part + row * io.parts;
-    RowSum r = {0.0, -__builtin_inff(), 0x7FFFFFFF};
+    RowPart r = {0.0, -__builtin_inff(), 0x7FFFFFFF};
     for (int i = lane; i < io.parts; i += 64) better(r.top, r.arg, p[i].top, p[i].arg);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) better(r.top, r.arg, __shfl_xor(r.top, o, 64), __shfl_xor(r.arg, o, 64));
-    if (!greedy)
-        for (int i = lane; i < io.parts; i += 64)
-            if (p[i].top > -__builtin_inff()) r.sum += p[i].sum * weight(p[i].top, r.top, scale);
+    if (greedy) return r;
+    const Weigh w(r.top, scale);
+    for (int i = lane; i < io.parts; i += 64)
+        if (p[i].top > -__builtin_inff()) r.sum += p[i].sum * w(p[i].top);
     r.sum = wave_add(r.sum);
     return r;
 }
 
-// What is left of p at a row: weights max(a w(x) / sum - b q(x), 0), without the tokens in `gone`.
-template <int kType, int kProbs>          // kProbs -1: no draft probabilities
-__global__ __launch_bounds__(kThreads) void k_verify_walk(const VerifyIo io) {
-    __shared__ double sums[kThreads];
+// The sums of the parts of rows that wait: work-group (part, slot).
+template <int kType, int kProbs>
+__global__ __launch_bounds__(kRowThreads) void k_verify_left(const VerifyIo io) {
+    const int slot = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
+    const Wait wt = io.wait[slot];
+    if (!wt.open) return;
+    int first, n;
+    kv4_rows(io.sh, io.cu, slot, &first, &n);
+    const int64_t row = (int64_t)first + wt.cur, base = (int64_t)part * kPart;
+    const RowPart rs = io.row[row];
+    const Weigh w(rs.top, scale_of(temperature_of(io, slot)));
+    const double a = wt.a / rs.sum;
+    const int m = (int)min((int64_t)kPart, io.V - base);
+    double s = 0.0;
+    for (int e0 = 0; e0 < m; e0 += 8 * kRowThreads) {
+        float x[8], q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = e0 + i * kRowThreads + tid;
+            x[i] = e < m ? value<kType>(io.logits, row * io.stride + base + e) : -__builtin_inff();
+            q[i] = e < m ? value<kProbs>(io.probs, row * io.probs_stride + base + e) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += fmax(a * w(logit(x[i])) - wt.b * (double)q[i], 0.0);
+    }
+    s = group_add<kRowThreads>(s);
+    if (tid == 0) io.slot_sum[(int64_t)slot * io.parts + part] = s;
+}
+
+// kProbs -1: no draft probabilities.  kGoOn: the second walk, from where the first one waits.
+template <int kType, int kProbs, bool kGoOn>
+__global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io) {
+    constexpr bool kFirst = kProbs >= 0 && !kGoOn;                    // (stops at a refused token)
     const int slot = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     int first, n;
     kv4_rows(io.sh, io.cu, slot, &first, &n);
@@ -223,26 +314,63 @@ __global__ __launch_bounds__(kThreads) void k_verify_walk(const VerifyIo io) {
         if (tid == 0) {
             io.counts[slot] = 0;
             io.next[slot] = -1;
+            if constexpr (kProbs >= 0) io.wait[slot].open = 0;
         }
         return;
     }
-    for (int i = tid; i < n; i += kThreads) io.path[first + i] = i == 0 ? 0 : -1;
     const float temp = temperature_of(io, slot);
     const bool greedy = !(temp > 0.f);
-    const double scale = greedy ? 0.0 : 1.0 / (double)temp;
-    __syncthreads();
-    int64_t* const gone = io.gone + first;
-    // the walk: every wave does it alike
-    int cur = 0, count = 1, n_gone = 0;
-    double left = 1.0, a = 1.0, b = 0.0;
-    RowSum rs = row_sum(io, first, greedy, scale);
+    const double scale = greedy ? 0.0 : scale_of(temp);
     double* const slot_sum = io.slot_sum + (int64_t)slot * io.parts;
-    // the weight that is left of token x at the current row, of coefficients ca, cb
-    auto weigh = [&](int64_t x, double ca, double cb) -> double {
-        const float l = logit(value<kType>(io.logits, ((int64_t)first + cur) * io.stride + x));
-        double v = rs.top > -__builtin_inff() ? weight(l, rs.top, scale) / rs.sum : 0.0;
+    int64_t* const gone = io.gone + first;
+    int cur = 0, count = 1, n_gone = 0, i0 = 0;
+    double left = 1.0, a = 1.0, b = 0.0, total = 1.0;
+    uint64_t above = ~0ull;                                           // rows of the first 64 that are still to be tried
+    if constexpr (kGoOn) {
+        const Wait wt = io.wait[slot];
+        if (!wt.open) return;
+        cur = wt.cur;
+        count = wt.count;
+        i0 = wt.row & ~63;
+        above = wt.row % 64 == 63 ? 0ull : ~0ull << (wt.row % 64 + 1);
+        a = wt.a;
+        b = wt.b;
+        double s = 0.0;
+        for (int i = tid; i < io.parts; i += kWalkThreads) s += slot_sum[i];
+        total = group_add<kWalkThreads>(s);
+        if (!(total > 0.0)) {
+            a = total = 1.0;
+            b = 0.0;
+        }
+    } else {
+        // whole rows, then every token's probability at its parent: all of them at once
+        for (int i = tid >> 6; i < n; i += kWalkThreads / 64) {
+            const RowPart r = whole_row(io, (int64_t)first + i, greedy, scale);
+            if (lane == 0) io.row[first + i] = r;
+        }
+        for (int i = tid; i < n; i += kWalkThreads) io.path[first + i] = i == 0 ? 0 : -1;
+        __syncthreads();
+        for (int i = tid; i < n; i += kWalkThreads) {
+            const int up = io.parents[first + i];
+            const int64_t x = io.tokens[first + i];
+            double p = -1.0;
+            if (i > 0 && up >= 0 && up < i && x >= 0 && x < io.V) {
+                const RowPart r = io.row[first + up];
+                if (r.top > -__builtin_inff()) {
+                    if (greedy) p = x == r.arg;
+                    else p = Weigh(r.top, scale)(logit(value<kType>(io.logits, ((int64_t)first + up) * io.stride + x))) / r.sum;
+                }
+            }
+            io.p[first + i] = p;
+        }
+        __syncthreads();
+    }
+    RowPart rs = io.row[first + cur];
+    // the weight that is left of token x at the current row
+    auto weigh = [&](const Weigh& w, double per, int64_t x, double cb) -> double {
+        double v = w(logit(value<kType>(io.logits, ((int64_t)first + cur) * io.stride + x))) * per;
         if constexpr (kProbs >= 0) {
-            if (cb != 0.0) v = fmax(ca * v - cb * (double)value<kProbs < 0 ? 0 : kProbs>(io.probs, ((int64_t)first + cur) * io.probs_stride + x), 0.0);
+            if (cb != 0.0) v = fmax(v - cb * (double)value<kProbs < 0 ? 0 : kProbs>(io.probs, ((int64_t)first + cur) * io.probs_stride + x), 0.0);
         }
         return v;
     };
@@ -251,26 +379,45 @@ __global__ __launch_bounds__(kThreads) void k_verify_walk(const VerifyIo io) {
             if (gone[i] == x) return true;
         return false;
     };
-    double total = 1.0;                    // of the weights of coefficients a, b
-    for (int i0 = 0; i0 < n; i0 += 64) {
+    // the sums of the parts for coefficients a, b by this work-group; their sum
+    auto sum_parts = [&]() {
+        const Weigh w(rs.top, scale);
+        const double per = a / rs.sum;
+        double all = 0.0;
+        for (int part = 0; part < io.parts; ++part) {
+            double s = 0.0;
+            const int64_t base = (int64_t)part * kPart, m = min((int64_t)kPart, io.V - base);
+            for (int e = tid; e < m; e += kWalkThreads) s += weigh(w, per, base + e, b);
+            s = group_add<kWalkThreads>(s);
+            if (tid == 0) slot_sum[part] = s;
+            all += s;
+        }
+        return all;
+    };
+    // the walk: every wave does it alike, a row a lane
+    for (; i0 < n; i0 += 64, above = ~0ull) {
         const int row = i0 + lane;
-        const int par = row < n && row > 0 ? io.parents[first + row] : -1;
-        const int64_t tok = row < n ? io.tokens[first + row] : -1;
-        const float un = row < n && io.u ? io.u[first + row] : 0.f;
-        uint64_t todo = __builtin_amdgcn_ballot_w64(par == cur);
+        const bool in = row < n;
+        const int par = in && row > 0 ? io.parents[first + row] : -1;
+        const int64_t tok = in ? io.tokens[first + row] : -1;
+        const double pr = in ? io.p[first + row] : -1.0;
+        const double un = in && io.u ? (double)io.u[first + row] : 0.0;
+        double qr = 0.0;
+        if constexpr (kProbs >= 0)
+            if (pr >= 0.0 && !greedy) qr = (double)value<kProbs < 0 ? 0 : kProbs>(io.probs, ((int64_t)first + par) * io.probs_stride + tok);
+        uint64_t todo = __builtin_amdgcn_ballot_w64(par == cur && pr >= 0.0) & above;
         while (todo) {
             const int k = __builtin_ctzll(todo);
             todo &= todo - 1;
-            const int64_t x = lane_of(tok, k);
-            const double uk = (double)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, un), k));
-            const bool in = x >= 0 && x < io.V;
+            const double p = lane_of_double(pr, k), uk = lane_of_double(un, k);
             bool keep;
             if (greedy) {
-                keep = in && rs.top > -__builtin_inff() && x == rs.arg;
+                keep = p > 0.0;
             } else if constexpr (kProbs < 0) {
-                const double p = in && !is_gone(x) ? weigh(x, 1.0, 0.0) : 0.0;
-                keep = p > 0.0 && uk < 1.0 && uk * left < p;
-                if (!keep && p > 0.0) {
+                const int64_t x = lane_of(tok, k);
+                const bool some = p > 0.0 && !is_gone(x);
+                keep = some && uk < 1.0 && uk * left < p;
+                if (some && !keep) {
                     __syncthreads();
                     if (tid == 0) gone[n_gone] = x;
                     __syncthreads();
@@ -278,25 +425,18 @@ __global__ __launch_bounds__(kThreads) void k_verify_walk(const VerifyIo io) {
                     left -= p;
                 }
             } else {
-                const double p = in ? weigh(x, a, b) / total : 0.0;
-                const double q = in ? (double)value<kProbs>(io.probs, ((int64_t)first + cur) * io.probs_stride + x) : 0.0;
-                keep = p > 0.0 && uk * q < p;
-                if (!keep && in && rs.top > -__builtin_inff()) {
+                const double q = lane_of_double(qr, k), now = (b != 0.0 ? fmax(a * p - b * q, 0.0) : p) / total;
+                keep = now > 0.0 && uk * q < now;
+                if (!keep) {
                     // max(p - q, 0) with p = max(a w - b q, 0) / total: coefficients a / total and b / total + 1
-                    const double na = a / total, nb = b / total + 1.0;
-                    double all = 0.0;
-                    for (int part = 0; part < io.parts; ++part) {
-                        double s = 0.0;
-                        const int64_t base = (int64_t)part * kPart, m = min((int64_t)kPart, io.V - base);
-                        for (int e = tid; e < m; e += kThreads) s += weigh(base + e, na, nb);
-                        s = group_add(s);
-                        if (tid == 0) slot_sum[part] = s;
-                        all += s;
+                    a /= total;
+                    b = b / total + 1.0;
+                    if constexpr (kFirst) {
+                        if (tid == 0) io.wait[slot] = Wait{a, b, cur, count, i0 + k, 1};
+                        return;
                     }
-                    a = na;
-                    b = nb;
-                    total = all;
-                    if (!(all > 0.0)) {
+                    total = sum_parts();
+                    if (!(total > 0.0)) {
                         a = total = 1.0;
                         b = 0.0;
                     }
@@ -304,48 +444,58 @@ __global__ __launch_bounds__(kThreads) void k_verify_walk(const VerifyIo io) {
             }
             if (keep) {
                 cur = i0 + k;
+                rs = io.row[first + cur];
                 if (tid == 0) io.path[first + count] = cur;
                 ++count;
                 n_gone = 0;
                 left = a = total = 1.0;
                 b = 0.0;
-                rs = row_sum(io, (int64_t)first + cur, greedy, scale);
-                todo = __builtin_amdgcn_ballot_w64(par == cur && lane > k);
+                todo = __builtin_amdgcn_ballot_w64(par == cur && pr >= 0.0 && lane > k);
             }
         }
     }
-    if (tid == 0) io.counts[slot] = count;
+    if (tid == 0) {
+        io.counts[slot] = count;
+        if constexpr (kProbs >= 0) io.wait[slot].open = 0;
+    }
     if (greedy || !(rs.top > -__builtin_inff())) {
         if (tid == 0) io.next[slot] = rs.top > -__builtin_inff() ? rs.arg : -1;
         return;
     }
     // the sums of the parts of what is left
-    const RowPart* const rp = io.part + ((int64_t)first + cur) * io.parts;
-    auto left_of = [&](int64_t x) { return is_gone(x) ? 0.0 : weigh(x, a, b); };
+    const Weigh w(rs.top, scale);
+    const double per = a / rs.sum;
+    auto left_of = [&](int64_t x) { return is_gone(x) ? 0.0 : weigh(w, per, x, b); };
     if (b == 0.0) {
-        for (int i = tid; i < io.parts; i += kThreads)
-            slot_sum[i] = rp[i].top > -__builtin_inff() ? rp[i].sum * weight(rp[i].top, rs.top, scale) / rs.sum : 0.0;
-        __syncthreads();
-        for (int i = 0; i < n_gone; ++i) {
-            const int part = (int)(gone[i] / kPart);
+        const RowPart* const rp = io.part + ((int64_t)first + cur) * io.parts;
+        auto fill = [&]() {
+            __syncthreads();
             double s = 0.0;
-            const int64_t base = (int64_t)part * kPart, m = min((int64_t)kPart, io.V - base);
-            for (int e = tid; e < m; e += kThreads) s += left_of(base + e);
-            s = group_add(s);
-            if (tid == 0) slot_sum[part] = s;
-        }
-        __syncthreads();
-        double s = 0.0;
-        for (int i = tid; i < io.parts; i += kThreads) s += slot_sum[i];
-        total = group_add(s);
+            for (int i = tid; i < io.parts; i += kWalkThreads) {
+                double v = rp[i].top > -__builtin_inff() ? rp[i].sum * w(rp[i].top) / rs.sum : 0.0;
+                for (int j = 0; j < n_gone; ++j)
+                    if (gone[j] / kPart == i) v = -1.0;              // (to be summed without it)
+                slot_sum[i] = v;
+                s += v > 0.0 ? v : 0.0;
+            }
+            s = group_add<kWalkThreads>(s);
+            for (int j = 0; j < n_gone; ++j) {
+                const int part = (int)(gone[j] / kPart);
+                if (slot_sum[part] >= 0.0) continue;
+                const int64_t base = (int64_t)part * kPart, m = min((int64_t)kPart, io.V - base);
+                double v = 0.0;
+                for (int e = tid; e < m; e += kWalkThreads) v += left_of(base + e);
+                v = group_add<kWalkThreads>(v);
+                if (tid == 0) slot_sum[part] = v;
+                s += v;
+                __syncthreads();
+            }
+            return s;
+        };
+        total = fill();
         if (!(total > 0.0)) {                 // nothing left: the target's own
             n_gone = 0;
-            for (int i = tid; i < io.parts; i += kThreads)
-                slot_sum[i] = rp[i].top > -__builtin_inff() ? rp[i].sum * weight(rp[i].top, rs.top, scale) / rs.sum : 0.0;
-            __syncthreads();
-            s = 0.0;
-            for (int i = tid; i < io.parts; i += kThreads) s += slot_sum[i];
-            total = group_add(s);
+            total = fill();
         }
     }
     __syncthreads();
@@ -373,39 +523,48 @@ __global__ __launch_bounds__(kThreads) void k_verify_walk(const VerifyIo io) {
         part = last;
         before = last_before;
     }
-    // a thread's kMine tokens of the part, then the tokens of the thread in which the sum passes
-    constexpr int kMine = kPart / kThreads;
+    // a thread's kMine tokens of the part, the wave in which the sum passes, its thread, and the token
+    constexpr int kMine = kPart / kWalkThreads;
+    __shared__ double sums[kWalkThreads / 64];
     const int64_t base = (int64_t)part * kPart;
     const int m = (int)min((int64_t)kPart, io.V - base);
-    double mine = 0.0;
-    for (int e = tid * kMine; e < min(m, (tid + 1) * kMine); ++e) mine += left_of(base + e);
-    sums[tid] = mine;
+    double mine[kMine], s = 0.0;
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) {
+        const int at = tid * kMine + e;
+        mine[e] = at < m ? left_of(base + at) : 0.0;
+        s += mine[e];
+    }
+    const double end = wave_prefix_sum(s);
+    if (lane == 63) sums[tid >> 6] = end;
     __syncthreads();
-    int64_t who = -1, last_who = 0;
-    for (int t0 = 0; t0 < kThreads && who < 0; t0 += 64) {
-        const double s = sums[t0 + lane], end = wave_prefix_sum(s);
-        const uint64_t some = __builtin_amdgcn_ballot_w64(s > 0.0), past = __builtin_amdgcn_ballot_w64(s > 0.0 && before + end > goal);
-        if (past) {
-            const int k = __builtin_ctzll(past);
-            who = t0 + k;
-            before += __shfl(end - s, k, 64);
-        } else {
-            if (some) last_who = t0 + 63 - __builtin_clzll(some);
-            before += __shfl(end, 63, 64);
-        }
+    int who = -1, last_who = 0;
+#pragma unroll
+    for (int i = 0; i < kWalkThreads / 64; ++i) {
+        if (who >= 0) continue;
+        if (sums[i] > 0.0) last_who = i;
+        if (sums[i] > 0.0 && before + sums[i] > goal) who = i;
+        else before += sums[i];
     }
     const bool behind = who < 0;              // (roundings again: the last token of all)
-    if (behind) who = last_who;
-    static_assert(kMine <= 64, "a wave");
-    const int e = (int)who * kMine + lane;
-    const double s = lane < kMine && e < m ? left_of(base + e) : 0.0, end = wave_prefix_sum(s);
+    if ((tid >> 6) != (behind ? last_who : who)) return;
     const uint64_t some = __builtin_amdgcn_ballot_w64(s > 0.0), past = __builtin_amdgcn_ballot_w64(s > 0.0 && !behind && before + end > goal);
-    if (tid == 0) io.next[slot] = base + who * kMine + (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some | 1));
+    if (lane != (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some | 1))) return;
+    double sum = before + (end - s);
+    int64_t token = -1;
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) {
+        if (!(mine[e] > 0.0) || (past && token >= 0 && sum > goal)) continue;
+        token = base + tid * kMine + e;
+        sum += mine[e];
+    }
+    io.next[slot] = token;
 }
 
+// Bytes of the workspace's lists, in the order of VerifyIo.
 constexpr int64_t verify_ws(int64_t n_slots, int64_t rows, int64_t V) {
     const int64_t parts = (V + kPart - 1) / kPart;
-    return rows * (parts * (int64_t)sizeof(RowPart) + 8) + n_slots * parts * 8;
+    return rows * (parts + 1) * (int64_t)sizeof(RowPart) + rows * 16 + n_slots * (parts * 8 + (int64_t)sizeof(Wait));
 }
 
 }  // namespace
@@ -456,21 +615,31 @@ extern "C" int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, i
         return fail(SX8_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", what, (long long)verify_ws(n_slots, rows, V));
     const int parts = (int)((V + kPart - 1) / kPart);
     VerifyIo io{logits, logits_stride, tokens, parents, cu, Kv4Shape{(int)n_slots, 1, 1, 0, (int)rows}, V, parts, u, temperature, t,
-                probs, probs_stride, path, counts, next, nullptr, nullptr, nullptr};
+                probs, probs_stride, path, counts, next, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     io.part = reinterpret_cast<RowPart*>(workspace);
-    io.gone = reinterpret_cast<int64_t*>(io.part + rows * parts);
-    io.slot_sum = reinterpret_cast<double*>(io.gone + rows);
+    io.row = io.part + rows * parts;
+    io.p = reinterpret_cast<double*>(io.row + rows);
+    io.gone = reinterpret_cast<int64_t*>(io.p + rows);
+    io.wait = reinterpret_cast<Wait*>(io.gone + rows);
+    io.slot_sum = reinterpret_cast<double*>(io.wait + n_slots);
+    const bool wide = aligned(logits, 16) && logits_stride * la % 16 == 0;
     auto with = [&](auto ty) {
         constexpr int kType = decltype(ty)::value;
-        if (rows > 0)
-            hipLaunchKernelGGL((k_verify_rows<kType>), dim3((unsigned)rows, (unsigned)parts), dim3(kThreads), 0, as_stream(stream), io);
-        auto walk = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)n_slots), dim3(kThreads), 0, as_stream(stream), io);
+        const hipStream_t st = as_stream(stream);
+        auto row = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)rows, (unsigned)parts), dim3(kRowThreads), 0, st, io); };
+        auto walk = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)n_slots), dim3(kWalkThreads), 0, st, io); };
+        if (rows > 0 && wide) row(k_verify_rows<kType, true>);
+        else if (rows > 0) row(k_verify_rows<kType, false>);
+        if (!probs) return walk(k_verify_walk<kType, -1, false>);
+        auto drawn = [&](auto pt) {
+            constexpr int kProbs = decltype(pt)::value;
+            walk(k_verify_walk<kType, kProbs, false>);
+            hipLaunchKernelGGL((k_verify_left<kType, kProbs>), dim3((unsigned)parts, (unsigned)n_slots), dim3(kRowThreads), 0, st, io);
+            walk(k_verify_walk<kType, kProbs, true>);
         };
-        if (!probs) walk(k_verify_walk<kType, -1>);
-        else if (probs_dtype == 0) walk(k_verify_walk<kType, 0>);
-        else if (probs_dtype == 1) walk(k_verify_walk<kType, 1>);
-        else walk(k_verify_walk<kType, 2>);
+        if (probs_dtype == 0) drawn(std::integral_constant<int, 0>{});
+        else if (probs_dtype == 1) drawn(std::integral_constant<int, 1>{});
+        else drawn(std::integral_constant<int, 2>{});
     };
     if (dtype == 0) with(std::integral_constant<int, 0>{});
     else if (dtype == 1) with(std::integral_constant<int, 1>{});
