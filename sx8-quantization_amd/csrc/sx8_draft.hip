@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void k_draft_tree(const int32_t* parents, cons
 // weights were added, and of so many borders of the cumulated sum one lies within a binary32 rounding of u once in some
 // hundred draws.  The first launch reads all rows, which is little more than a path's where trees are small, and needs no
 // wait between its work-groups.
-constexpr int kPart = 8192, kRowThreads = 256, kWalkThreads = 1024;
+constexpr int kPart = 4096, kRowThreads = 256, kWalkThreads = 1024, kNear = 256;
 
 struct RowPart {
     double sum;                           // of exp((x - top) / temperature), or 0 (greedy)
@@ -91,7 +91,7 @@ struct VerifyIo {
     RowPart* part;                        // [rows][parts]
     RowPart* row;                         // [rows]: the whole row
     double* p;                            // [rows]: probability of a row's token at its parent, below zero: none
-    int64_t* gone;                        // [rows]: tokens of a slot that are out of p at its current row
+    int32_t* gone;                        // [rows]: rows of a slot whose tokens are out of p at its current row
     double* slot_sum;                     // [n_slots][parts]: sums of what is left of p
     Wait* wait;                           // [n_slots]
 };
@@ -234,7 +234,9 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(const VerifyIo io) 
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, 64));
     __shared__ float tops[kRowThreads / 64];
+    __shared__ double root[32];
     __shared__ int first;
+    if (tid < 32) root[tid] = Weigh(0.f, 1.0 / 32.0)(tid - 32) * 2.0;
     if (lane == 0) tops[tid >> 6] = all;
     if (tid == 0) first = 0x7FFFFFFF;
     __syncthreads();
@@ -250,9 +252,32 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(const VerifyIo io) 
     const float temp = temperature_of(io, slot);
     double sum = 0.0;
     if (temp > 0.f && all > -__builtin_inff()) {
-        const Weigh w(all, scale_of(temp));
+        // 2^y as 2^(j / 32) from LDS times 2^f by its interpolation in the Chebyshev nodes of [-1/64, 1/64] (degree 4, within
+        // 8e-14 of itself), where no weight is below e^-690 for it: 11 operations of 64 bits a logit, 18 by Weigh
+        const float lowest = all - 690.f * temp;
+        if (all < __builtin_inff() && lowest > -__builtin_inff()) {
+            const double top64 = all, scale = 32.0 * scale_of(temp);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) sum += w(x[i]);
+            for (int i = 0; i < kE; ++i) {
+                const double y = ((double)fmaxf(x[i], lowest) - top64) * scale, shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
+                const int n = (int)__builtin_bit_cast(uint64_t, shifted);
+                double r = __builtin_fma(0x1.3b2b1bee88b09p-27, f, 0x1.c6b167e571135p-20);
+                r = __builtin_fma(r, f, 0x1.ebfbdff8131c3p-13);
+                r = __builtin_fma(r, f, 0x1.62e42fef6d01ap-6);
+                r = __builtin_fma(r, f, 1.0);
+                const uint64_t bits = __builtin_bit_cast(uint64_t, root[n & 31]) + ((uint64_t)(uint32_t)(n >> 5) << 52);
+                sum = __builtin_fma(__builtin_bit_cast(double, bits), r, sum);
+            }
+        } else {
+            const Weigh w(all, scale_of(temp));
+#pragma unroll 1
+            for (int i = 0; i < kE; ++i) {
+                float v = x[0];
+#pragma unroll
+                for (int j = 1; j < kE; ++j) v = i == j ? x[j] : v;
+                sum += w(v);
+            }
+        }
     }
     sum = group_add<kRowThreads>(sum);                               // (behind its barriers `first` is whole)
     if (tid == 0) io.part[(int64_t)r * io.parts + part] = RowPart{sum, all, all > -__builtin_inff() ? (int)base + first : 0x7FFFFFFF};
@@ -321,8 +346,15 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
     const float temp = temperature_of(io, slot);
     const bool greedy = !(temp > 0.f);
     const double scale = greedy ? 0.0 : scale_of(temp);
-    double* const slot_sum = io.slot_sum + (int64_t)slot * io.parts;
-    int64_t* const gone = io.gone + first;
+    // the slot's lists: in LDS where they fit and nobody else reads them
+    __shared__ RowPart row_lds[kProbs < 0 ? kNear : 1];
+    __shared__ double p_lds[kProbs < 0 ? kNear : 1], sum_lds[kNear];
+    __shared__ int gone_lds[kNear];
+    const bool near = kProbs < 0 && n <= kNear;
+    RowPart* const whole = near ? row_lds : io.row + first;
+    double* const prob = near ? p_lds : io.p + first;
+    double* const slot_sum = !kGoOn && io.parts <= kNear ? sum_lds : io.slot_sum + (int64_t)slot * io.parts;
+    int* const gone = n <= kNear ? gone_lds : io.gone + first;       // rows of the tokens that are out of p
     int cur = 0, count = 1, n_gone = 0, i0 = 0;
     double left = 1.0, a = 1.0, b = 0.0, total = 1.0;
     uint64_t above = ~0ull;                                           // rows of the first 64 that are still to be tried
@@ -346,7 +378,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         // whole rows, then every token's probability at its parent: all of them at once
         for (int i = tid >> 6; i < n; i += kWalkThreads / 64) {
             const RowPart r = whole_row(io, (int64_t)first + i, greedy, scale);
-            if (lane == 0) io.row[first + i] = r;
+            if (lane == 0) whole[i] = r;
         }
         for (int i = tid; i < n; i += kWalkThreads) io.path[first + i] = i == 0 ? 0 : -1;
         __syncthreads();
@@ -355,17 +387,17 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
             const int64_t x = io.tokens[first + i];
             double p = -1.0;
             if (i > 0 && up >= 0 && up < i && x >= 0 && x < io.V) {
-                const RowPart r = io.row[first + up];
+                const RowPart r = whole[up];
                 if (r.top > -__builtin_inff()) {
                     if (greedy) p = x == r.arg;
                     else p = Weigh(r.top, scale)(logit(value<kType>(io.logits, ((int64_t)first + up) * io.stride + x))) / r.sum;
                 }
             }
-            io.p[first + i] = p;
+            prob[i] = p;
         }
         __syncthreads();
     }
-    RowPart rs = io.row[first + cur];
+    RowPart rs = whole[cur];
     // the weight that is left of token x at the current row
     auto weigh = [&](const Weigh& w, double per, int64_t x, double cb) -> double {
         double v = w(logit(value<kType>(io.logits, ((int64_t)first + cur) * io.stride + x))) * per;
@@ -374,9 +406,10 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         }
         return v;
     };
+    auto token_of = [&](int row) { return io.tokens[first + row]; };
     auto is_gone = [&](int64_t x) {
         for (int i = 0; i < n_gone; ++i)
-            if (gone[i] == x) return true;
+            if (token_of(gone[i]) == x) return true;
         return false;
     };
     // the sums of the parts for coefficients a, b by this work-group; their sum
@@ -400,7 +433,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         const bool in = row < n;
         const int par = in && row > 0 ? io.parents[first + row] : -1;
         const int64_t tok = in ? io.tokens[first + row] : -1;
-        const double pr = in ? io.p[first + row] : -1.0;
+        const double pr = in ? prob[row] : -1.0;
         const double un = in && io.u ? (double)io.u[first + row] : 0.0;
         double qr = 0.0;
         if constexpr (kProbs >= 0)
@@ -419,7 +452,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
                 keep = some && uk < 1.0 && uk * left < p;
                 if (some && !keep) {
                     __syncthreads();
-                    if (tid == 0) gone[n_gone] = x;
+                    if (tid == 0) gone[n_gone] = i0 + k;
                     __syncthreads();
                     ++n_gone;
                     left -= p;
@@ -444,7 +477,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
             }
             if (keep) {
                 cur = i0 + k;
-                rs = io.row[first + cur];
+                rs = whole[cur];
                 if (tid == 0) io.path[first + count] = cur;
                 ++count;
                 n_gone = 0;
@@ -465,32 +498,38 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
     // the sums of the parts of what is left
     const Weigh w(rs.top, scale);
     const double per = a / rs.sum;
-    auto left_of = [&](int64_t x) { return is_gone(x) ? 0.0 : weigh(w, per, x, b); };
     if (b == 0.0) {
+        // A part's sum without the tokens that are out: less their weights, which keeps the sums' precision where most of the
+        // part is left; summed anew where less than 2^-20 of it is.
         const RowPart* const rp = io.part + ((int64_t)first + cur) * io.parts;
         auto fill = [&]() {
             __syncthreads();
             double s = 0.0;
+            bool anew = false;
             for (int i = tid; i < io.parts; i += kWalkThreads) {
-                double v = rp[i].top > -__builtin_inff() ? rp[i].sum * w(rp[i].top) / rs.sum : 0.0;
+                const double of = rp[i].top > -__builtin_inff() ? rp[i].sum * w(rp[i].top) / rs.sum : 0.0;
+                double v = of;
                 for (int j = 0; j < n_gone; ++j)
-                    if (gone[j] / kPart == i) v = -1.0;              // (to be summed without it)
-                slot_sum[i] = v;
-                s += v > 0.0 ? v : 0.0;
+                    if (token_of(gone[j]) / kPart == i) v -= prob[gone[j]];
+                const bool again = v < of * 0x1p-20;
+                anew |= again;
+                slot_sum[i] = again ? -1.0 : v;
+                s += again ? 0.0 : v;
             }
-            s = group_add<kWalkThreads>(s);
-            for (int j = 0; j < n_gone; ++j) {
-                const int part = (int)(gone[j] / kPart);
-                if (slot_sum[part] >= 0.0) continue;
-                const int64_t base = (int64_t)part * kPart, m = min((int64_t)kPart, io.V - base);
-                double v = 0.0;
-                for (int e = tid; e < m; e += kWalkThreads) v += left_of(base + e);
-                v = group_add<kWalkThreads>(v);
-                if (tid == 0) slot_sum[part] = v;
-                s += v;
-                __syncthreads();
-            }
-            return s;
+            if (__syncthreads_or(anew))
+                for (int part = 0; part < io.parts; ++part) {
+                    if (slot_sum[part] >= 0.0) continue;             // (alike in all threads)
+                    const int64_t base = (int64_t)part * kPart, m = min((int64_t)kPart, io.V - base);
+                    double v = 0.0;
+                    for (int e = tid; e < m; e += kWalkThreads) v += is_gone(base + e) ? 0.0 : weigh(w, per, base + e, 0.0);
+                    v = group_add<kWalkThreads>(v);
+                    if (tid == 0) {
+                        slot_sum[part] = v;
+                        s += v;
+                    }
+                    __syncthreads();
+                }
+            return group_add<kWalkThreads>(s);
         };
         total = fill();
         if (!(total > 0.0)) {                 // nothing left: the target's own
@@ -532,9 +571,16 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
 #pragma unroll
     for (int e = 0; e < kMine; ++e) {
         const int at = tid * kMine + e;
-        mine[e] = at < m ? left_of(base + at) : 0.0;
-        s += mine[e];
+        mine[e] = at < m ? weigh(w, per, base + at, b) : 0.0;
     }
+    for (int j = 0; j < n_gone; ++j) {
+        const int64_t at = token_of(gone[j]) - base - tid * kMine;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e)
+            if (at == e) mine[e] = 0.0;
+    }
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) s += mine[e];
     const double end = wave_prefix_sum(s);
     if (lane == 63) sums[tid >> 6] = end;
     __syncthreads();
@@ -564,7 +610,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
 // Bytes of the workspace's lists, in the order of VerifyIo.
 constexpr int64_t verify_ws(int64_t n_slots, int64_t rows, int64_t V) {
     const int64_t parts = (V + kPart - 1) / kPart;
-    return rows * (parts + 1) * (int64_t)sizeof(RowPart) + rows * 16 + n_slots * (parts * 8 + (int64_t)sizeof(Wait));
+    return rows * (parts + 1) * (int64_t)sizeof(RowPart) + rows * 12 + n_slots * (parts * 8 + (int64_t)sizeof(Wait));
 }
 
 }  // namespace
@@ -619,9 +665,9 @@ extern "C" int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, i
     io.part = reinterpret_cast<RowPart*>(workspace);
     io.row = io.part + rows * parts;
     io.p = reinterpret_cast<double*>(io.row + rows);
-    io.gone = reinterpret_cast<int64_t*>(io.p + rows);
-    io.wait = reinterpret_cast<Wait*>(io.gone + rows);
+    io.wait = reinterpret_cast<Wait*>(io.p + rows);
     io.slot_sum = reinterpret_cast<double*>(io.wait + n_slots);
+    io.gone = reinterpret_cast<int32_t*>(io.slot_sum + n_slots * parts);
     const bool wide = aligned(logits, 16) && logits_stride * la % 16 == 0;
     auto with = [&](auto ty) {
         constexpr int kType = decltype(ty)::value;
