@@ -449,38 +449,34 @@ __global__ __launch_bounds__(256) void k_keep_move(uint8_t* pages, const int32_t
     for (int b = base / 32; b * 32 < base + c; ++b) {
         uint8_t* const dst = block(b * 32 < base ? base : b * 32);
         __syncthreads();                                             // (the list of the last block is read)
-        bool moves = false;
-        if (tid < 32) {
-            const int i = b * 32 + tid - base;
-            const uint8_t* src = nullptr;
-            if (i >= 0 && i < c) {
-                const int at = path[first + i];
-                if (at != i) {
-                    src = block(base + at);
-                    row[tid] = (base + at) % 32;
-                }
-            }
-            from[tid] = src;
-            moves = src != nullptr;
+        // (every wave finds them; the first one writes them down)
+        const int lane = tid & 63, i = b * 32 + lane - base;
+        const uint8_t* src = nullptr;
+        if (lane < 32 && i >= 0 && i < c) {
+            const int at = path[first + i];
+            if (at != i) src = block(base + at);
+            if (tid < 32) row[lane] = (base + at) % 32;
         }
-        if (!__syncthreads_or(moves) || dst == nullptr) continue;
+        if (tid < 32) from[lane] = src;
+        const uint32_t moves = (uint32_t)__builtin_amdgcn_ballot_w64(src != nullptr);
+        __syncthreads();
+        if (moves == 0 || dst == nullptr) continue;
         uint32_t k[kK], v[kV];
         uint16_t prm[kP];
 #pragma unroll
         for (int u = 0; u < kK; ++u) {
             const int i = tid + 256 * u, t = i % 32, d = i / 32 * 8;
-            if (from[t]) k[u] = *reinterpret_cast<const uint32_t*>(from[t] + kv4_k_word(HD, row[t], d));
+            if (moves >> t & 1u) k[u] = *reinterpret_cast<const uint32_t*>(from[t] + kv4_k_word(HD, row[t], d));
         }
 #pragma unroll
         for (int u = 0; u < kV; ++u) {
-            const int i = tid + 256 * u, d = i % HD, h = i / HD;
-            if (i >= 4 * HD) break;
-            const uint32_t old = *reinterpret_cast<const uint32_t*>(dst + kv4_v_word(HD, 4 * h, d));
-            v[u] = old;
+            const int i = tid + 256 * u, d = i % HD, h = __builtin_amdgcn_readfirstlane(i / HD);   // (HD >= 64: a wave's alike)
+            if (i >= 4 * HD || !(moves >> 4 * h & 0x000F000Fu)) continue;
+            v[u] = *reinterpret_cast<const uint32_t*>(dst + kv4_v_word(HD, 4 * h, d));
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int t = e / 4 * 16 + 4 * h + e % 4;
-                if (!from[t]) continue;
+                if (!(moves >> t & 1u)) continue;
                 const uint32_t lv = *reinterpret_cast<const uint32_t*>(from[t] + kv4_v_word(HD, row[t], d)) >> kv4_v_shift(row[t]) & 15u;
                 v[u] = (v[u] & ~(15u << kv4_shift(e))) | lv << kv4_shift(e);
             }
@@ -488,24 +484,23 @@ __global__ __launch_bounds__(256) void k_keep_move(uint8_t* pages, const int32_t
 #pragma unroll
         for (int u = 0; u < kP; ++u) {
             const int i = tid + 256 * u, t = i % 32, which = i / 32 % 4, g = i / 128;
-            if (g < NG && from[t]) prm[u] = *reinterpret_cast<const uint16_t*>(from[t] + kv4_param(HD, which, row[t], g));
+            if (g < NG && moves >> t & 1u) prm[u] = *reinterpret_cast<const uint16_t*>(from[t] + kv4_param(HD, which, row[t], g));
         }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < kK; ++u) {
             const int i = tid + 256 * u, t = i % 32, d = i / 32 * 8;
-            if (from[t]) *reinterpret_cast<uint32_t*>(dst + kv4_k_word(HD, t, d)) = k[u];
+            if (moves >> t & 1u) *reinterpret_cast<uint32_t*>(dst + kv4_k_word(HD, t, d)) = k[u];
         }
 #pragma unroll
         for (int u = 0; u < kV; ++u) {
-            const int i = tid + 256 * u, d = i % HD, h = i / HD;
-            if (i >= 4 * HD) break;
-            *reinterpret_cast<uint32_t*>(dst + kv4_v_word(HD, 4 * h, d)) = v[u];
+            const int i = tid + 256 * u, d = i % HD, h = __builtin_amdgcn_readfirstlane(i / HD);
+            if (i < 4 * HD && moves >> 4 * h & 0x000F000Fu) *reinterpret_cast<uint32_t*>(dst + kv4_v_word(HD, 4 * h, d)) = v[u];
         }
 #pragma unroll
         for (int u = 0; u < kP; ++u) {
             const int i = tid + 256 * u, t = i % 32, which = i / 32 % 4, g = i / 128;
-            if (g < NG && from[t]) *reinterpret_cast<uint16_t*>(dst + kv4_param(HD, which, t, g)) = prm[u];
+            if (g < NG && moves >> t & 1u) *reinterpret_cast<uint16_t*>(dst + kv4_param(HD, which, t, g)) = prm[u];
         }
     }
 }

@@ -27,6 +27,7 @@
 #include <cstring>
 #include <string>
 
+#include "sx8_draft.h"
 #include "sx8_hip.h"
 #include "sx8_paged.h"
 
@@ -54,6 +55,13 @@ struct Lib {
     decltype(&sx8_kv4_fork) kv4_fork;
     decltype(&sx8_kv4_free) kv4_free;
     decltype(&sx8_kv4_compact) kv4_compact;
+    decltype(&sx8_kv4_append_rope) kv4_append_rope;
+    decltype(&sx8_kv4_attend_tree) kv4_attend_tree;
+    decltype(&sx8_kv4_keep) kv4_keep;
+    decltype(&sx8_kv4_keep_workspace_bytes) kv4_keep_ws;
+    decltype(&sx8_draft_tree) draft_tree;
+    decltype(&sx8_draft_verify) draft_verify;
+    decltype(&sx8_draft_verify_workspace_bytes) draft_verify_ws;
 } lib;
 
 constexpr int32_t kUnsupported = SX8_ERR_UNSUPPORTED;
@@ -140,6 +148,13 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     SX8_BIND(kv4_fork, "sx8_kv4_fork")
     SX8_BIND(kv4_free, "sx8_kv4_free")
     SX8_BIND(kv4_compact, "sx8_kv4_compact")
+    SX8_BIND(kv4_append_rope, "sx8_kv4_append_rope")
+    SX8_BIND(kv4_attend_tree, "sx8_kv4_attend_tree")
+    SX8_BIND(kv4_keep, "sx8_kv4_keep")
+    SX8_BIND(kv4_keep_ws, "sx8_kv4_keep_workspace_bytes")
+    SX8_BIND(draft_tree, "sx8_draft_tree")
+    SX8_BIND(draft_verify, "sx8_draft_verify")
+    SX8_BIND(draft_verify_ws, "sx8_draft_verify_workspace_bytes")
 #undef SX8_BIND
     Py_RETURN_NONE;
 }
@@ -423,11 +438,12 @@ PyObject* py_to_host(PyObject*, PyObject* const* a, Py_ssize_t na) {
 }
 
 // ---- packed sequences and the paged cache (sx8_paged_kv.py) ------------------------------------
-// A (rows, heads, hd) tensor of fp16 or bf16 that the kernels read in place (sx8_paged_kv._in_place), else null.
-const at::Tensor* head_rows(PyObject* o, int64_t min_ts) {
+// A (rows, heads, hd) tensor of fp16 or bf16 (wide: or float32) that the kernels read in place (sx8_paged_kv._in_place), else
+// null.
+const at::Tensor* head_rows(PyObject* o, int64_t min_ts, bool wide = false) {
     const at::Tensor* x = plain(o);
     if (!x || !x->is_cuda() || x->layout() != at::kStrided || x->dim() != 3 || x->size(0) < 1 ||
-        (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16))
+        (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16 && !(wide && x->scalar_type() == at::kFloat)))
         return nullptr;
     const int64_t ts = x->stride(0), hs = x->stride(1);
     const bool ok = x->stride(2) == 1 && ts % 8 == 0 && hs % 8 == 0 && hs >= 0 && ts >= min_ts && ts <= 1 << 23 &&
@@ -480,28 +496,29 @@ PyObject* py_varlen(PyObject*, PyObject* const* a, Py_ssize_t na) {
 }
 
 // What PagedKV4 keeps for these calls: (pages, table, lens, refs, status, page_bytes, n_kv, head_dim, page_tokens,
-// bytes of attend's workspace, bytes of the page operations' workspace); the wrapper checked it.
+// bytes of attend's workspace, of the page operations', of attend_tree's); the wrapper checked it.
 struct Cache {
     const at::Tensor *pages, *table, *lens, *refs, *status;
-    int64_t layers, n_pages, slots, width, page_bytes, ws_attend, ws_pages;
+    int64_t layers, n_pages, slots, width, page_bytes, ws_attend, ws_pages, ws_tree;
     int32_t nk, hd, pt;
     void* stream;
     int32_t* ints(const at::Tensor* t) const { return t->data_ptr<int32_t>(); }
     uint8_t* layer(int64_t i) const { return pages->data_ptr<uint8_t>() + i * n_pages * page_bytes; }
 };
 bool cache(PyObject* o, Cache* c) {
-    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 11) return false;
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 12) return false;
     const at::Tensor** t[5] = {&c->pages, &c->table, &c->lens, &c->refs, &c->status};
     for (int i = 0; i < 5; ++i)
         if (!(*t[i] = plain(PyTuple_GET_ITEM(o, i)))) return false;
-    int64_t n[6];
-    for (int i = 0; i < 6; ++i) n[i] = num(PyTuple_GET_ITEM(o, 5 + i));
+    int64_t n[7];
+    for (int i = 0; i < 7; ++i) n[i] = num(PyTuple_GET_ITEM(o, 5 + i));
     c->page_bytes = n[0];
     c->nk = (int32_t)n[1];
     c->hd = (int32_t)n[2];
     c->pt = (int32_t)n[3];
     c->ws_attend = n[4];
     c->ws_pages = n[5];
+    c->ws_tree = n[6];
     c->layers = c->pages->size(0);
     c->n_pages = c->pages->size(1);
     c->slots = c->table->size(0);
@@ -649,6 +666,214 @@ PyObject* py_kv4_pages(PyObject*, PyObject* const* a, Py_ssize_t na) {
     END_HANDLE_TH_ERRORS
 }
 
+// None, or a dense vector of n values of type t on the device of `like`; ok false: something else.
+const at::Tensor* vector_or_none(PyObject* o, at::ScalarType t, int64_t n, const at::Tensor& like, bool* ok) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor* x = dense(o, t);
+    if (x && x->dim() == 1 && x->numel() == n && x->device() == like.device()) return x;
+    *ok = false;
+    return nullptr;
+}
+bool aligned16(const at::Tensor* x) { return !x || reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0; }
+PyObject* tuple_of(std::initializer_list<at::Tensor*> ts) {
+    PyObject* t = PyTuple_New((Py_ssize_t)ts.size());
+    Py_ssize_t i = 0;
+    for (at::Tensor* x : ts) {
+        PyObject* o = t ? THPVariable_Wrap(std::move(*x)) : nullptr;
+        if (!o) {
+            Py_XDECREF(t);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(t, i++, o);
+    }
+    return t;
+}
+
+// kv4_append_rope(cache, layer, q, k, v, cos, sin, cu, depth, q_norm, k_norm, eps, interleaved, bf16) -> the query rows; cu,
+// depth and the norms may be None
+PyObject* py_kv4_append_rope(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(14)
+    Cache c;
+    int64_t layer;
+    const int32_t* cu;
+    const at::Tensor* q = head_rows(a[2], 0, true);
+    const at::Tensor* k = head_rows(a[3], 0, true);
+    const at::Tensor* v = head_rows(a[4], 0, true);
+    const at::Tensor* cs = dense(a[5], at::kFloat);
+    const at::Tensor* sn = dense(a[6], at::kFloat);
+    if (!q || !k || !v || !cs || !sn || !cache_call(a[0], a[1], a[7], &c, &layer, &cu) || !PyFloat_Check(a[11]) ||
+        !PyBool_Check(a[12]) || !PyBool_Check(a[13]))
+        Py_RETURN_NONE;
+    const at::Device on = c.pages->device();
+    const bool bf = a[13] == Py_True, wide = q->scalar_type() == at::kFloat;
+    const at::ScalarType to = bf ? at::kBFloat16 : at::kHalf;
+    bool fits = true;
+    const at::Tensor* depth = vector_or_none(a[8], at::kInt, q->size(0), *c.pages, &fits);
+    const at::Tensor* qw = vector_or_none(a[9], to, c.hd, *c.pages, &fits);
+    const at::Tensor* kw = vector_or_none(a[10], to, c.hd, *c.pages, &fits);
+    if (!fits || !aligned16(qw) || !aligned16(kw) || !aligned16(cs) || !aligned16(sn) || q->size(2) != c.hd ||
+        k->sizes() != v->sizes() || k->size(0) != q->size(0) || k->size(1) != c.nk || k->size(2) != c.hd ||
+        k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || (!wide && q->scalar_type() != to) ||
+        cs->dim() != 2 || cs->sizes() != sn->sizes() || q->device() != on || k->device() != on || v->device() != on ||
+        cs->device() != on || sn->device() != on)
+        Py_RETURN_NONE;
+    const double eps = PyFloat_AS_DOUBLE(a[11]);
+    int32_t rc;
+    at::Tensor o;
+    {
+        Unlocked u;
+        c10::DeviceGuard guard(on);
+        o = empty_like_device(q->sizes(), to, *q);
+        rc = lib.kv4_append_rope(c.layer(layer), c.ints(c.table), c.ints(c.lens), cu, c.slots, c.width, c.n_pages, q->data_ptr(),
+                                 k->data_ptr(), v->data_ptr(), o.data_ptr(), q->size(0), q->stride(0), q->stride(1), k->stride(0),
+                                 k->stride(1), v->stride(0), v->stride(1), o.stride(0), o.stride(1), (int32_t)q->size(1), c.nk,
+                                 c.hd, c.pt, cs->data_ptr<float>(), sn->data_ptr<float>(), cs->size(0),
+                                 (int32_t)(2 * cs->size(1)), a[12] == Py_True, depth ? depth->data_ptr<int32_t>() : nullptr,
+                                 qw ? qw->data_ptr() : nullptr, kw ? kw->data_ptr() : nullptr, eps, wide ? 2 : bf, bf, c.stream);
+    }
+    if (rc) return failed("sx8_kv4_append_rope", rc);
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_attend_tree(cache, layer, q, mask, cu or None, scale) -> out
+PyObject* py_kv4_attend_tree(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(6)
+    Cache c;
+    int64_t layer;
+    const int32_t* cu;
+    const at::Tensor* q = head_rows(a[2], 0);
+    const at::Tensor* m = dense(a[3], at::kLong);
+    if (!q || !m || !PyFloat_Check(a[5]) || !cache_call(a[0], a[1], a[4], &c, &layer, &cu) || q->size(2) != c.hd ||
+        m->dim() != 2 || m->size(0) != q->size(0) || m->size(1) < 1 || m->size(1) > 4 || q->device() != c.pages->device() ||
+        m->device() != c.pages->device())
+        Py_RETURN_NONE;
+    const float scale = (float)PyFloat_AS_DOUBLE(a[5]);
+    int32_t rc;
+    at::Tensor o;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(c.pages->device());
+        o = empty_like_device(q->sizes(), q->scalar_type(), *q);
+        const at::Tensor ws = empty_like_device({c.ws_tree}, at::kByte, *q);
+        rc = lib.kv4_attend_tree(c.layer(layer), c.ints(c.table), c.ints(c.lens), cu, c.slots, c.width, c.n_pages, q->data_ptr(),
+                                 o.data_ptr(), q->size(0), q->stride(0), q->stride(1), o.stride(0), o.stride(1),
+                                 reinterpret_cast<const uint64_t*>(m->data_ptr()), (int32_t)m->size(1), (int32_t)q->size(1), c.nk,
+                                 c.hd, c.pt, scale, dtype_of(*q), ws.data_ptr(), c.ws_tree, c.stream);
+    }
+    if (rc) return failed("sx8_kv4_attend_tree", rc);
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// kv4_keep(cache, path, counts, cu or None) -> True
+PyObject* py_kv4_keep(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(4)
+    Cache c;
+    if (!cache(a[0], &c)) Py_RETURN_NONE;
+    const at::Tensor* path = int_vector(a[1], -1, *c.pages);
+    const at::Tensor* counts = int_vector(a[2], c.slots, *c.pages);
+    const at::Tensor* cu = a[3] == Py_None ? nullptr : int_vector(a[3], c.slots + 1, *c.pages);
+    if (!path || !counts || (a[3] != Py_None && !cu)) Py_RETURN_NONE;
+    int32_t rc;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(c.pages->device());
+        const int64_t nb = lib.kv4_keep_ws(c.slots, path->numel());
+        const at::Tensor ws = empty_like_device({nb > 0 ? nb : 0}, at::kByte, *c.pages);
+        rc = lib.kv4_keep(c.layer(0), c.layers, c.ints(c.table), c.ints(c.lens), c.ints(c.refs), cu ? c.ints(cu) : nullptr,
+                          c.ints(path), c.ints(counts), path->numel(), c.slots, c.width, c.n_pages, c.nk, c.hd, c.pt,
+                          c.ints(c.status), ws.data_ptr(), nb, c.stream);
+    }
+    if (rc) return failed("sx8_kv4_keep", rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- drafted tokens (sx8_draft.py) -------------------------------------------------------------
+// draft_tree(parents, cu, words) -> (mask, depth)
+PyObject* py_draft_tree(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(3)
+    const at::Tensor* p = dense(a[0], at::kInt);
+    const int64_t words = num(a[2]);
+    SX8_SIZES_OK()
+    if (!p || p->dim() != 1 || p->numel() < 1 || words < 1 || words > 4) Py_RETURN_NONE;
+    const at::Tensor* cu = int_vector(a[1], -1, *p);
+    if (!cu) Py_RETURN_NONE;
+    int32_t rc;
+    at::Tensor mask, depth;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(p->device());
+        mask = empty_like_device({p->numel(), words}, at::kLong, *p);
+        depth = empty_like_device({p->numel()}, at::kInt, *p);
+        rc = lib.draft_tree(p->data_ptr<int32_t>(), cu->data_ptr<int32_t>(), cu->numel() - 1, p->numel(), (int32_t)words,
+                            reinterpret_cast<uint64_t*>(mask.data_ptr()), depth.data_ptr<int32_t>(), stream_of(*p));
+    }
+    if (rc) return failed("sx8_draft_tree", rc);
+    return tuple_of({&mask, &depth});
+    END_HANDLE_TH_ERRORS
+}
+
+// (rows, vocabulary) values of a type that sx8_draft_verify takes, rows one after another or apart; null: something else
+const at::Tensor* matrix(PyObject* o, int32_t* type) {
+    const at::Tensor* x = plain(o);
+    if (!x || !x->is_cuda() || x->layout() != at::kStrided || x->dim() != 2 || x->size(0) < 1 || x->size(1) < 1 || x->stride(1) != 1 ||
+        x->stride(0) < x->size(1))
+        return nullptr;
+    *type = x->scalar_type() == at::kHalf ? 0 : x->scalar_type() == at::kBFloat16 ? 1 : x->scalar_type() == at::kFloat ? 2 : -1;
+    return *type < 0 ? nullptr : x;
+}
+
+// draft_verify(logits, tokens, parents, cu, uniforms or None, temperature (a float or a vector), probs or None)
+//   -> (path, counts, next)
+PyObject* py_draft_verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    HANDLE_TH_ERRORS
+    SX8_ARGS(7)
+    int32_t type = 0, ptype = 0;
+    const at::Tensor* x = matrix(a[0], &type);
+    if (!x) Py_RETURN_NONE;
+    const int64_t rows = x->size(0), V = x->size(1);
+    const at::Tensor* tok = dense(a[1], at::kLong);
+    const at::Tensor* par = int_vector(a[2], rows, *x);
+    const at::Tensor* cu = int_vector(a[3], -1, *x);
+    if (!tok || tok->dim() != 1 || tok->numel() != rows || tok->device() != x->device() || !par || !cu || cu->numel() < 2)
+        Py_RETURN_NONE;
+    const int64_t slots = cu->numel() - 1;
+    bool fits = true;
+    const at::Tensor* un = vector_or_none(a[4], at::kFloat, rows, *x, &fits);
+    const at::Tensor* temp = nullptr;
+    float t = 0.f;
+    if (PyFloat_Check(a[5])) t = (float)PyFloat_AS_DOUBLE(a[5]);
+    else temp = vector_or_none(a[5], at::kFloat, slots, *x, &fits);
+    const at::Tensor* pr = a[6] == Py_None ? nullptr : matrix(a[6], &ptype);
+    if (!fits || (!temp && !PyFloat_Check(a[5])) || (a[6] != Py_None && (!pr || pr->sizes() != x->sizes() || pr->device() != x->device())))
+        Py_RETURN_NONE;
+    int32_t rc;
+    at::Tensor path, counts, next;
+    {
+        Unlocked u;
+        c10::DeviceGuard on(x->device());
+        path = empty_like_device({rows}, at::kInt, *x);
+        counts = empty_like_device({slots}, at::kInt, *x);
+        next = empty_like_device({slots}, at::kLong, *x);
+        const int64_t nb = lib.draft_verify_ws(slots, rows, V);
+        const at::Tensor ws = empty_like_device({nb > 0 ? nb : 0}, at::kByte, *x);
+        rc = lib.draft_verify(x->data_ptr(), x->stride(0), type, tok->data_ptr<int64_t>(), par->data_ptr<int32_t>(),
+                              cu->data_ptr<int32_t>(), slots, rows, V, un ? un->data_ptr<float>() : nullptr,
+                              temp ? temp->data_ptr<float>() : nullptr, t, pr ? pr->data_ptr() : nullptr, pr ? pr->stride(0) : 0,
+                              ptype, path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), next.data_ptr<int64_t>(), ws.data_ptr(),
+                              nb, stream_of(*x));
+    }
+    if (rc) return failed("sx8_draft_verify", rc);
+    return tuple_of({&path, &counts, &next});
+    END_HANDLE_TH_ERRORS
+}
+
 #define SX8_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
 PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"linear", SX8_FAST(py_linear), nullptr},
@@ -663,6 +888,11 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"kv4_read", SX8_FAST(py_kv4_read), nullptr},
                          {"kv4_attend", SX8_FAST(py_kv4_attend), nullptr},
                          {"kv4_pages", SX8_FAST(py_kv4_pages), nullptr},
+                         {"kv4_append_rope", SX8_FAST(py_kv4_append_rope), nullptr},
+                         {"kv4_attend_tree", SX8_FAST(py_kv4_attend_tree), nullptr},
+                         {"kv4_keep", SX8_FAST(py_kv4_keep), nullptr},
+                         {"draft_tree", SX8_FAST(py_draft_tree), nullptr},
+                         {"draft_verify", SX8_FAST(py_draft_verify), nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_sx8py", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -23,6 +23,9 @@ def draft_tree(parents, cu, words=1):
     j % 64 of a mask's word j // 64 is set where row j is the row itself or above it; depth counts the rows above it.  words (1 to
     4) are for slots of up to 64 words rows: later rows get mask 0 and a depth far below zero, so that append_rope and
     attend_tree leave them out.  Rows of no slot: unset."""
+    got = _L.py().draft_tree(parents, cu, words)
+    if got is not None:
+        return got
     if not isinstance(parents, torch.Tensor) or parents.device.type != "cuda":
         raise RuntimeError("parents must be an int32 vector on the GPU")
     device = parents.device
@@ -63,6 +66,11 @@ def verify_draft(logits, tokens, parents, cu, uniforms=None, temperature=0.0, dr
 
     Returns path (rows,) int32: the rows that slot s keeps, in path[cu[s]] .. (row 0 first, then -1); counts (slots,) int32: how
     many; and the tokens that follow, (slots,) int64 (-1: none).  PagedKV4.keep takes path and counts.  Outputs have no gradient."""
+    if not isinstance(temperature, torch.Tensor):
+        temperature = float(temperature)
+    got = _L.py().draft_verify(logits, tokens, parents, cu, uniforms, temperature, draft_probs)
+    if got is not None:
+        return got
     if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda" or logits.dim() != 2:
         raise RuntimeError("logits must be a (rows, tokens) tensor on the GPU")
     device = logits.device

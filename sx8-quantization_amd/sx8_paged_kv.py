@@ -192,7 +192,7 @@ class PagedKV4:
         self._ws_attend = int(_L.lib().sx8_kv4_attend_workspace_bytes(self.head_dim))
         self._ws_tree = int(_L.lib().sx8_kv4_attend_tree_workspace_bytes(self.head_dim))
         self._t = (pages, table, lens, refs, status, nb, self.n_kv, self.head_dim, self.page_tokens, self._ws_attend,
-                   self._ws_pages)
+                   self._ws_pages, self._ws_tree)
 
     pages = property(lambda self: self._t[0])
     table = property(lambda self: self._t[1])
@@ -275,6 +275,11 @@ class PagedKV4:
         gives zeros and is not written.  out shares no memory with q, k and v."""
         if dtype is None:
             dtype = torch.float16 if q.dtype == torch.float32 else q.dtype
+        if out is None and dtype in _DTYPES:
+            got = _L.py().kv4_append_rope(self._t, layer, q, k, v, cos, sin, cu, depth, q_norm, k_norm, float(eps),
+                                          bool(interleaved), dtype is torch.bfloat16)
+            if got is not None:
+                return got
         with torch.cuda.device(self.device):
             nh = q.shape[1] if q.dim() == 3 else 0
             q = _rows("q", q, nh, self.head_dim, self.device, wide=True)
@@ -307,6 +312,10 @@ class PagedKV4:
         rows j of the slot whose bit is set in mask (rows, words) int64 (bit j % 64 of word j // 64; 1 to 4 words;
         sx8_draft.draft_tree makes them from parents; a row's own bit is no exception).  New rows from 64 words on are attended
         by none.  A row that attends nothing gives zeros.  Returns out (rows, heads, head_dim), which shares no memory with q."""
+        if out is None:
+            got = _L.py().kv4_attend_tree(self._t, layer, q, mask, cu, _scale(scale, self.head_dim))
+            if got is not None:
+                return got
         with torch.cuda.device(self.device):
             nh = q.shape[1] if q.dim() == 3 else 0
             q = _rows("q", q, nh, self.head_dim, self.device)
@@ -377,6 +386,8 @@ class PagedKV4:
         int32 on the device, as sx8_draft.verify_draft returns them): in all layers they move together behind the tokens
         before the new ones, lens becomes lens - n + counts[s] and pages behind that are given back.  Slots without new rows have
         counts 0.  The rows' pages must be the slot's own, as for `append`."""
+        if _L.py().kv4_keep(self._t, path, counts, cu):
+            return
         with torch.cuda.device(self.device):
             _ints("path", path, None, self.device)
             _ints("counts", counts, self.n_slots, self.device)
