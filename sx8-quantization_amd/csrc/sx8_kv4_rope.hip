@@ -110,7 +110,7 @@ __device__ __forceinline__ u32x4 turned(const typename Row<kIn>::T* row, int d0,
 
 // Work-groups (block, y): y < nk encodes the K and V rows of a head, the others turn the rows of `heads` of
 // the query heads that share one.
-template <int HD, int kIn, bool kBf16, bool kInter>
+template <int HD, int kIn, bool kBf16, bool kInter, bool kOne>       // kOne: one query head
 __global__ __launch_bounds__(256) void k_kv4_append_rope(const Kv4Pool p, const RopeIn in) {
     using T = typename Row<kIn>::T;
     constexpr int kBB = kv4_block_bytes(HD), CPR = HD / 8;
@@ -126,25 +126,18 @@ __global__ __launch_bounds__(256) void k_kv4_append_rope(const Kv4Pool p, const 
     }
     __syncthreads();
     if (head >= p.sh.nk) {
-        const int G = p.sh.G, cuts = (G + in.heads - 1) / in.heads, y = head - p.sh.nk, h0 = y % cuts * in.heads;
-        const int h = y / cuts * G + h0, per = min(in.heads, G - h0);
+        const int G = p.sh.G, hs = kOne ? 1 : in.heads, cuts = (G + hs - 1) / hs, y = head - p.sh.nk, h0 = kOne ? 0 : y % cuts * hs;
+        const int h = kOne ? y : y / cuts * G + h0, per = kOne ? 1 : min(hs, G - h0);
         const T* const q = static_cast<const T*>(in.q) + t.row0 * in.q_ts + h * in.q_hs;
         uint16_t* const out = in.out + t.row0 * in.o_ts + h * in.o_hs;
-        auto row = [&](int i, int g, int d0) {
-            const int at = place[t.t0 + i];
+        for (int ch = tid; ch < nt * per * CPR; ch += 256) {
+            const int hr = ch / CPR, i = kOne ? hr : hr / per, g = kOne ? 0 : hr - i * per, d0 = ch % CPR * 8, at = place[t.t0 + i];
             u32x4 r = {0u, 0u, 0u, 0u};
             if (at >= 0)
                 r = turned<HD, kIn, kBf16, kInter>(q + i * in.q_ts + g * in.q_hs, d0, in.qw, in.eps, in.cos + (int64_t)at * half,
                                                    in.sin + (int64_t)at * half, in.rot);
             *reinterpret_cast<u32x4*>(out + i * in.o_ts + g * in.o_hs + d0) = r;
-        };
-        if (per == 1)
-            for (int ch = tid; ch < nt * CPR; ch += 256) row(ch / CPR, 0, ch % CPR * 8);
-        else
-            for (int ch = tid; ch < nt * per * CPR; ch += 256) {
-                const int hr = ch / CPR, i = hr / per;
-                row(i, hr - i * per, ch % CPR * 8);
-            }
+        }
         return;
     }
     const int64_t off = block_offset(p, t.slot, head, t.block, kBB);
@@ -230,8 +223,8 @@ extern "C" int32_t sx8_kv4_append_rope(uint8_t* pages, const int32_t* table, con
     if (rc == SX8_OK) rc = check_rows(what, "v", v, v_ts, v_hs, rows);
     if (rc == SX8_OK) rc = check_rows(what, "out", out, o_ts, o_hs, rows);
     if (rc != SX8_OK) return rc;
-    if (nh <= 0 || nh % nk || nh / nk > 256)
-        return fail(SX8_ERR_INVALID, "%s: nh must be a multiple of nk, at most 256 nk", what);
+    if (nh <= 0 || nh % nk || nh / nk > 256 || nh + nk > 65535)
+        return fail(SX8_ERR_INVALID, "%s: nh must be a multiple of nk, at most 256 nk (and 65535 - nk)", what);
     rc = check_apart(what, "out", o_ts, o_hs, rows, nh, hd);
     if (rc != SX8_OK) return rc;
     if (in_dtype != 2 && in_dtype != dtype)
@@ -258,13 +251,18 @@ extern "C" int32_t sx8_kv4_append_rope(uint8_t* pages, const int32_t* table, con
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, grid, dim3(256), cu && n_slots > 64 ? prefix_bytes(p) : 0, as_stream(stream), p, in);
         };
-        if (in_dtype == 2) {
-            if (interleaved) go(k_kv4_append_rope<HD, 2, kBf, true>);
-            else go(k_kv4_append_rope<HD, 2, kBf, false>);
-        } else {
-            if (interleaved) go(k_kv4_append_rope<HD, kBf, kBf, true>);
-            else go(k_kv4_append_rope<HD, kBf, kBf, false>);
-        }
+        auto of = [&](auto in_kind, auto inter) {
+            constexpr int kIn = decltype(in_kind)::value;
+            constexpr bool kInter = decltype(inter)::value;
+            if (heads == 1) go(k_kv4_append_rope<HD, kIn, kBf, kInter, true>);
+            else go(k_kv4_append_rope<HD, kIn, kBf, kInter, false>);
+        };
+        auto kind = [&](auto in_kind) {
+            if (interleaved) of(in_kind, std::true_type{});
+            else of(in_kind, std::false_type{});
+        };
+        if (in_dtype == 2) kind(std::integral_constant<int, 2>{});
+        else kind(std::integral_constant<int, kBf>{});
     });
     return check_launch(what);
 }
