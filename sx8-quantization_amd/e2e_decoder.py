@@ -26,6 +26,7 @@ import torch
 import torch.nn as nn
 
 import _sx8lib as _L
+from sx8_draft import draft_tree, verify_draft
 from sx8_paged_kv import PagedKV4, attn_varlen
 from integrate_fused_v44 import SX8LinearV44
 from prepare_v44 import to_v44_device
@@ -587,8 +588,8 @@ class PagedDecoder:
     """Several sequences of one SX8Decoder, each in a slot of a paged 4-bit KV cache (sx8_paged_kv).
 
     ``prompt`` runs the prompts of any slots as one packed pass (a slot that has tokens already goes on from them),
-    ``step`` decodes one token of every slot in use, replayed from a HIP graph; ``fork``, ``free`` and ``compact`` are the
-    cache's.  Linears, norms and RoPE are the kernels of prefill_fused with one row per new token; K and V rows go
+    ``step`` decodes one token of every slot in use, replayed from a HIP graph; ``verify`` checks several drafted tokens a slot
+    in one pass and goes on behind those that the model keeps; ``fork``, ``free`` and ``compact`` are the cache's.  Linears, norms and RoPE are the kernels of prefill_fused with one row per new token; K and V rows go
     into the pages as they leave RoPE.  New prompts attend their own fp16 rows (attn_varlen), whatever else the call
     brings; rows with earlier tokens, and every decoded token, attend the pages (PagedKV4.attend; many rows at once
     read the pages' values back and attend those).  The reference serves one sequence
@@ -616,25 +617,29 @@ class PagedDecoder:
         self.active.copy_(self._ints(int(n > 0) for n in self.lens))
 
     def _rows(self, pb, ids, pos, attend):
-        """The layers over T packed rows at positions `pos`; attend(layer, q, k, v) -> (T, heads, hd).  The residual
-        stream of the rows is left in pb["resid"] + pb["d"]."""
+        """The layers over T packed rows at positions `pos`; attend(layer, q, k, v) -> (T, heads, hd).  pos None: q, k and v are
+        those of the linears, float32, without norm and RoPE.  The residual stream of the rows is left in pb["resid"] + pb["d"]."""
         d = self.dec
         cfg, P = d.cfg, _L.ptr
         H, nh, nk, hd, eps, T = cfg["hidden"], cfg["n_heads"], cfg["n_kv"], cfg["head_dim"], cfg["eps"], pb["T"]
         st = _L.stream(d.device)
         emb = d.embed.rows(ids, pb["emb"])                          # (the captured step's own: the module's may be replaced)
         # RoPE and its K/V rows as a prompt's at position 0 of a table and a cache of T rows
-        cos, sin = d.cos.index_select(0, pos), d.sin.index_select(0, pos)
+        if pos is not None:
+            cos, sin = d.cos.index_select(0, pos), d.sin.index_select(0, pos)
         pend, last = (None, 0, 0), len(d.layers) - 1
         for li, ly in enumerate(d.layers):
             g_qkv, g_mlp, g_o, g_down = pb["groups"][li]
             d._norm_packed(pb, g_qkv, pb["resid"], None if li == 0 else pb["d"], emb if li == 0 else None, ly.in_norm, pend,
                            eps, st)
-            qp = d._gemm_packed(g_qkv, pb["xn"], pb["zn"], T, H, pb["ws"], st)
-            _L.call("sx8_dec_qk_rope_cache_rows_parts", P(pb["q"]), P(pb["k"]), P(pb["v"]), P(ly.q_norm), P(ly.k_norm),
-                    P(cos), P(sin), P(pb["pos0"]), T, P(pb["qh"]), P(pb["kr"]), P(pb["vr"]), nh, nk, hd, T, eps, qp[0],
-                    qp[1], qp[2], st)
-            a = attend(li, pb["qh"], pb["kr"].permute(1, 0, 2), pb["vr"].permute(1, 0, 2))
+            qp = d._gemm_packed(g_qkv, pb["xn"], pb["zn"], T, H, pb["ws"], st, defer=pos is not None)
+            if pos is None:
+                a = attend(li, pb["q"].view(T, nh, hd), pb["k"].view(T, nk, hd), pb["v"].view(T, nk, hd))
+            else:
+                _L.call("sx8_dec_qk_rope_cache_rows_parts", P(pb["q"]), P(pb["k"]), P(pb["v"]), P(ly.q_norm), P(ly.k_norm),
+                        P(cos), P(sin), P(pb["pos0"]), T, P(pb["qh"]), P(pb["kr"]), P(pb["vr"]), nh, nk, hd, T, eps, qp[0],
+                        qp[1], qp[2], st)
+                a = attend(li, pb["qh"], pb["kr"].permute(1, 0, 2), pb["vr"].permute(1, 0, 2))
             op = d._gemm_group_deferred(g_o, a.view(T, nh * hd), pb["ws"], st)
             d._norm_packed(pb, g_mlp, pb["resid"], pb["o"], None, ly.post_norm, op, eps, st)
             _, hdrs, lvls, bas, sca, _, gcb, _ = g_mlp
@@ -787,6 +792,90 @@ class PagedDecoder:
             self.logits = self._step()
         self.tok.copy_(self.logits.argmax(-1))
         return self.tok.clone()
+
+    @_on_device
+    @torch.no_grad()
+    def verify(self, slots, drafts, parents=None, uniforms=None, temperature=0.0, draft_probs=None):
+        """Check drafted tokens of any slots in use in one pass, and go on behind those that are kept.  drafts: for each slot an int64
+        vector of up to 255 tokens (none: a step of that slot alone), which follow its last token one after another, or, with
+        parents (a list a slot), form a tree: token j follows row parents[j] of 0 .. j, 0 the last token and i + 1 token i.
+        temperature (a number, or one a slot), uniforms (a float32 vector of 1 + tokens a slot) and draft_probs ((1 +
+        tokens, vocabulary) a slot, row 0 what the last token's followers were drawn from) are those of sx8_draft.verify_draft.
+        Returns for each slot its new tokens, int64 on the device: the kept ones and the one that follows, which is the
+        input of the next pass.  ``logits`` are those of all rows, packed by slot number.  Rows that are not kept leave no
+        trace in the cache.  Waits for the device once, for the numbers of kept tokens."""
+        slots = _numbers(slots)
+        dev, n_all = self.dec.device, self.n_slots
+        each = dict(zip(slots, drafts))
+        if not slots or len(slots) != len(drafts) or len(each) != len(slots):
+            raise ValueError("as many different slots as drafts, and at least one")
+        rows = {s: 1 + t.numel() for s, t in each.items()}
+        for s, n in rows.items():
+            if not 0 <= s < n_all or not self.lens[s] or n > 256 or self.lens[s] + n > self.max_len:
+                raise ValueError(f"slot {s}: out of range, not in use, over 255 drafted tokens or past {self.max_len} tokens")
+        up = {s: list(range(-1, n - 1)) for s, n in rows.items()}
+        if parents is not None:
+            if len(parents) != len(slots):
+                raise ValueError("as many lists of parents as slots")
+            for s, p in zip(slots, parents):
+                up[s] = [-1, *_numbers(p)]
+                if len(up[s]) != rows[s] or any(not 0 <= b < i for i, b in enumerate(up[s]) if i):
+                    raise ValueError(f"slot {s}: a parent for each drafted token, a row before it")
+        order = sorted(rows)
+
+        def packed(name, xs, width=()):                             # a tensor a slot -> rows in the order of the slots
+            if xs is None:
+                return None
+            by = dict(zip(slots, xs))
+            if len(xs) != len(slots) or any(by[s].shape != (rows[s], *width) for s in order):
+                raise ValueError(f"{name}: one a slot, with 1 + its drafted tokens rows")
+            return torch.cat([by[s].to(dev) for s in order])
+
+        uniforms, draft_probs = packed("uniforms", uniforms), packed("draft_probs", draft_probs, (self.dec.cfg["vocab"],))
+        if uniforms is not None:
+            uniforms = uniforms.float()
+        elif isinstance(temperature, (list, tuple, torch.Tensor)) or temperature > 0:
+            raise ValueError("uniforms: needed where a temperature is above zero")
+        if draft_probs is not None and draft_probs.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+            raise ValueError("draft_probs: float16, bfloat16 or float32")
+        if isinstance(temperature, (list, tuple, torch.Tensor)):
+            t = torch.as_tensor(temperature, dtype=torch.float32, device=dev)
+            if t.shape != (len(slots),):
+                raise ValueError("temperature: a number, or one a slot")
+            temperature = torch.zeros(n_all, device=dev)
+            temperature[torch.tensor(slots, device=dev)] = t
+        last = self.tok[torch.tensor(order, device=dev)].split(1)
+        ids = torch.cat([x for s, t in zip(order, last) for x in (t, each[s].to(dev))])
+        counts = [rows.get(s, 0) for s in range(n_all)]
+        cu, par = self._ints([0, *itertools.accumulate(counts), *(p for s in order for p in up[s])]).split((n_all + 1, ids.numel()))
+        self.cache.reserve(self._ints(counts))
+        self.cache.check()
+        self.lens = [a + b for a, b in zip(self.lens, counts)]
+        mask, depth = draft_tree(par, cu, -(-max(rows.values()) // 64))
+        d, scale = self.dec, 1.0 / math.sqrt(self.dec.cfg["head_dim"])
+
+        def attend(li, q, k, v):
+            ly = d.layers[li]
+            q = self.cache.append_rope(li, q, k, v, d.cos, d.sin, cu, depth=depth, q_norm=ly.q_norm, k_norm=ly.k_norm,
+                                       eps=d.cfg["eps"], dtype=torch.float16)
+            return self.cache.attend_tree(li, q, mask, cu, scale)
+
+        pb = self._bufs(ids.numel())
+        self._rows(pb, ids, None, attend)
+        self.logits = self._head(pb["resid"], pb["d"], ids.numel())
+        path, kept, following = verify_draft(self.logits, ids, par, cu, uniforms, temperature, draft_probs)
+        self.cache.keep(path, kept, cu)
+        kept = kept.tolist()
+        self.cache.check()
+        self.lens = [a - b + k for a, b, k in zip(self.lens, counts, kept)]
+        at = torch.tensor(order, device=dev)
+        self.tok[at] = following[at]
+        starts = dict(zip(order, itertools.accumulate([0, *(rows[s] for s in order)])))
+        out = {}
+        for s in order:
+            a = starts[s]
+            out[s] = torch.cat([ids[a + path[a + 1:a + kept[s]].long()], following[s:s + 1]])
+        return [out[s] for s in slots]
 
     def fork(self, src, dst):
         """The empty slots dst[i] go on from where the slots src[i] are."""
