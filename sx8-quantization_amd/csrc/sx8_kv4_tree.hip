@@ -6,13 +6,16 @@
 // one or two tiles of 16 of them (a block's levels are unpacked once for both); a work-group's four waves take a unit's
 // blocks in turn and add their results up in LDS, so that a unit cut over many work-groups leaves one partial
 // result for each.  A block that ends at or behind the first new token is masked by 32 bits of each column's mask.
-// Bound by the VALU and its chains: for 16 rows and a block of 32 tokens of a head of 128 there are 29 matrix instructions
-// (16 cycles each) and 140 others besides 190 for the block.  A wave keeps one block in registers: K of the next one
-// is requested when the scores are done, V when the products are; no branch lies between, so that the compiler keeps the
-// scores' sums apart from neither (with one: 316 us instead of 108 for the case below).  Query fragments stay in LDS.  Four tiles a
-// unit spill (506 us) or, with one work-group a CU, wait (121).  p * s by mixed multiply-adds that write halves of a register: 102.
-// 8 trees of 64 rows after 2500 .. 4100 tokens, 32 heads over 8 of 128: 97 us; two of 31 after 61000 and 100000, 32 over 4: 222;
-// 24 of 1 .. 24 after up to 8000: 45 (the combine 4.2 more).
+// Bound by instructions: for 16 rows and a block of 32 tokens of a head of 128 there are 29 matrix instructions of 16 cycles
+// and about 140 others of 4 (exponentials 16, multiply-adds of fp16 with float32 8), beside 190 for the block; they take turns on
+// a SIMD (two long trees: the VALU is busy 71% of its cycles, the matrix cores 31%), and a second wave there makes neither faster.
+// A wave keeps one block in registers: K of the next one is requested when the scores are done, V when the products are;
+// no branch lies between, so that the compiler keeps the scores' sums apart from neither (with one: 316 us instead of 108 for
+// the case below).  Query fragments stay in LDS.  Three or four tiles a unit spill (120 us) or need half of their sums moved
+// through accumulator registers (109); p * s by mixed multiply-adds that write halves of a register: 102; a block's scores computed
+// beside the products of the one before: 155.
+// 8 trees of 64 rows after 2500 .. 4100 tokens, 32 heads over 8 of 128: 93 us; two of 31 after 61000 and 100000, 32 over 4: 214
+// (198 on other machines); 24 of 1 .. 24 after up to 8000: 45 (the combine 4.2 more).
 #include "sx8_kv4_core.h"
 
 namespace sx8 {
@@ -46,7 +49,6 @@ constexpr int64_t part_rows(int64_t hd) { return hd == 256 ? 2 * 512 * 16 : 2 * 
 constexpr int64_t tree_ws(int64_t hd) { return part_rows(hd) * (hd + 2) * 4 + kMaxGroups * (int64_t)sizeof(TreePiece); }
 
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
-
 
 // x of eight values as two fp16 numbers each, hi + lo
 __device__ __forceinline__ void halves8(const float* x, u32x4* hi, u32x4* lo) {
@@ -225,13 +227,15 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     float ks[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) ks[e] = sx8_h2f(half_of(rg.ks[g][2 * a + (e >> 1)], e)) * 1048576.f;
+                    f32x4 acc[kCt];
 #pragma unroll
-                    for (int ct = 0; ct < kCt; ++ct) {
-                        f32x4 acc = mfma16(l0, __builtin_bit_cast(f16x8, frag[ct][2 * g][lane]), zero4());
-                        acc = mfma16(l1, __builtin_bit_cast(f16x8, frag[ct][2 * g + 1][lane]), acc);
+                    for (int ct = 0; ct < kCt; ++ct) acc[ct] = mfma16(l0, __builtin_bit_cast(f16x8, frag[ct][2 * g][lane]), zero4());
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[ct][e] = __builtin_fmaf(ks[e], acc[e], s[ct][e]);
-                    }
+                    for (int ct = 0; ct < kCt; ++ct) acc[ct] = mfma16(l1, __builtin_bit_cast(f16x8, frag[ct][2 * g + 1][lane]), acc[ct]);
+#pragma unroll
+                    for (int ct = 0; ct < kCt; ++ct)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[ct][e] = __builtin_fmaf(ks[e], acc[ct][e], s[ct][e]);
                     
                 }
 #pragma unroll
@@ -368,10 +372,9 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     for (int e = 0; e < 8; ++e) ps[e] = pv[ct][e] * sx8_h2f(half_of(rg.vs[g][e >> 1], e));
                     halves8(ps, &hi, &lo);
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, hi), o[ct][4 * g + t]);
-                        o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, lo), o[ct][4 * g + t]);
-                    }
+                    for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, hi), o[ct][4 * g + t]);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, lo), o[ct][4 * g + t]);
                     
                 }
             }
@@ -557,7 +560,7 @@ extern "C" int32_t sx8_kv4_attend_tree(const uint8_t* pages, const int32_t* tabl
                                as_stream(stream), io, p.sh.G);
         };
         // Two tiles a unit from four tiles a slot on (8 slots of about 3300 tokens, 8 KV heads of 128, 64 rows of 4 heads: 97 us
-        // instead of 112; of 2 rows: 28 instead of 25), where registers allow it (heads of 256: 229 instead of 106).
+        // instead of 112; of 2 rows: 28 instead of 25), where registers allow it (16 heads over 2 of 256: 229 instead of 106).
         if constexpr (HD < 256) {
             if (tiles >= 4) return go(std::integral_constant<int, 2>{});
         }
