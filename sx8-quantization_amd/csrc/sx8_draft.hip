@@ -254,8 +254,10 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(const VerifyIo io) 
     if (temp > 0.f && all > -__builtin_inff()) {
         // 2^y as 2^(j / 32) from LDS times 2^f by its interpolation in the Chebyshev nodes of [-1/64, 1/64] (degree 4, within
         // 8e-14 of itself), where no weight is below e^-690 for it: 11 operations of 64 bits a logit, 18 by Weigh
-        const float lowest = all - 690.f * temp;
-        if (all < __builtin_inff() && lowest > -__builtin_inff()) {
+        // (a temperature that the logits' float32 steps do not resolve leaves no such clamp)
+        const float lowest = all - 680.f * temp;
+        const double gap = (double)all - (double)lowest;
+        if (all < __builtin_inff() && lowest > -__builtin_inff() && gap >= 600.0 * (double)temp && gap <= 690.0 * (double)temp) {
             const double top64 = all, scale = 32.0 * scale_of(temp);
 #pragma unroll
             for (int i = 0; i < kE; ++i) {
@@ -407,9 +409,11 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         return v;
     };
     auto token_of = [&](int row) { return io.tokens[first + row]; };
+    // (a cu that runs backwards gives slots the same rows, and their lists in memory the same places)
+    auto gone_row = [&](int i) { return (int)min((unsigned)gone[i], (unsigned)n - 1u); };
     auto is_gone = [&](int64_t x) {
         for (int i = 0; i < n_gone; ++i)
-            if (token_of(gone[i]) == x) return true;
+            if (token_of(gone_row(i)) == x) return true;
         return false;
     };
     // the sums of the parts for coefficients a, b by this work-group; their sum
@@ -510,7 +514,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
                 const double of = rp[i].top > -__builtin_inff() ? rp[i].sum * w(rp[i].top) / rs.sum : 0.0;
                 double v = of;
                 for (int j = 0; j < n_gone; ++j)
-                    if (token_of(gone[j]) / kPart == i) v -= prob[gone[j]];
+                    if (token_of(gone_row(j)) / kPart == i) v -= prob[gone_row(j)];
                 const bool again = v < of * 0x1p-20;
                 anew |= again;
                 slot_sum[i] = again ? -1.0 : v;
@@ -574,7 +578,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         mine[e] = at < m ? weigh(w, per, base + at, b) : 0.0;
     }
     for (int j = 0; j < n_gone; ++j) {
-        const int64_t at = token_of(gone[j]) - base - tid * kMine;
+        const int64_t at = token_of(gone_row(j)) - base - tid * kMine;
 #pragma unroll
         for (int e = 0; e < kMine; ++e)
             if (at == e) mine[e] = 0.0;
@@ -633,7 +637,7 @@ extern "C" int32_t sx8_draft_tree(const int32_t* parents, const int32_t* cu, int
 
 extern "C" int64_t sx8_draft_verify_workspace_bytes(int64_t n_slots, int64_t rows, int64_t V) {
     using namespace sx8;
-    if (n_slots <= 0 || n_slots > kKv4MaxSlots || rows < 0 || rows > 1 << 22 || V <= 0 || V > 1 << 28) return -1;
+    if (n_slots <= 0 || n_slots > kKv4MaxSlots || rows < 0 || rows > 1 << 22 || V <= 0 || V > 1 << 27) return -1;
     return verify_ws(n_slots, rows, V);
 }
 
@@ -647,7 +651,7 @@ extern "C" int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, i
     if (!cu || !counts || !next || (rows > 0 && (!logits || !tokens || !parents || !path)))
         return fail(SX8_ERR_INVALID, "%s: null pointer", what);
     if (sx8_draft_verify_workspace_bytes(n_slots, rows, V) < 0)
-        return fail(SX8_ERR_INVALID, "%s: bad sizes (n_slots 1..%d, rows up to 2^22, V 1..2^28)", what, kKv4MaxSlots);
+        return fail(SX8_ERR_INVALID, "%s: bad sizes (n_slots 1..%d, rows up to 2^22, V 1..2^27)", what, kKv4MaxSlots);
     if (dtype < 0 || dtype > 2 || (probs && (probs_dtype < 0 || probs_dtype > 2)))
         return fail(SX8_ERR_INVALID, "%s: dtypes must be 0 (fp16), 1 (bf16) or 2 (float32)", what);
     const int64_t la = dtype == 2 ? 4 : 2, pa = probs_dtype == 2 ? 4 : 2;
@@ -656,7 +660,7 @@ extern "C" int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, i
         return fail(SX8_ERR_INVALID, "%s: pointers must be aligned to their values", what);
     if (logits_stride < V || logits_stride > (int64_t)1 << 40 || (probs && (probs_stride < V || probs_stride > (int64_t)1 << 40)))
         return fail(SX8_ERR_INVALID, "%s: row strides must be V or more", what);
-    if (!u && (temperature || t > 0.f)) return fail(SX8_ERR_INVALID, "%s: random numbers needed where a temperature is above zero", what);
+    if (rows > 0 && !u && (temperature || t > 0.f)) return fail(SX8_ERR_INVALID, "%s: random numbers needed where a temperature is above zero", what);
     if (!workspace || workspace_bytes < verify_ws(n_slots, rows, V) || !aligned(workspace, 256))
         return fail(SX8_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", what, (long long)verify_ws(n_slots, rows, V));
     const int parts = (int)((V + kPart - 1) / kPart);

@@ -236,7 +236,6 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     for (int ct = 0; ct < kCt; ++ct)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[ct][e] = __builtin_fmaf(ks[e], acc[ct][e], s[ct][e]);
-                    
                 }
 #pragma unroll
                 for (int ct = 0; ct < kCt; ++ct)
@@ -254,8 +253,13 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     for (int e = 0; e < 8; ++e) pv[ct][e] = see >> (e / 4 * 16 + e % 4) & 1u ? pv[ct][e] : -kInf;
                 }
                 // A token whose V is no number must not reach a column that may not attend it through 0 * NaN: its scale and
-                // minimum become zeros, and the columns that attend it get the NaN by themselves, however small its weight.
-                uint32_t nan[NG], any = 0;
+                // minimum (each may be one, in bytes that no token was written to) become zeros, and the columns that attend it
+                // get the NaN by themselves, however small its weight.
+                uint32_t nan[NG], any = 0, low = 0;                   // low: of lane c the minima of group c
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((half_of(vm[e >> 1], e) & 0x7FFFu) >= 0x7C00u) low |= 1u << (e / 4 * 16 + e % 4);
+                any = low;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     nan[g] = 0;
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             if (nan[g] >> (e / 4 * 16 + e % 4) & 1u) rg.vs[g][e >> 1] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
-                        nan[g] <<= 4 * h;
+                        nan[g] = (nan[g] | __shfl((int)low, 16 * h + g, 64)) << 4 * h;
                         nan[g] |= __shfl_xor((int)nan[g], 16, 64);
                         nan[g] |= __shfl_xor((int)nan[g], 32, 64);
 #pragma unroll
@@ -312,7 +316,6 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                 const float nm = m[ct] == -kInf ? 0.f : -m[ct];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(pv[ct][e], kscale[ct], nm));
-                
             }
             // rows of the minima's product: a group's minima, and behind them ones, whose sum is the weights'
             constexpr uint32_t kOnes = 0x3C003C00u;
@@ -375,7 +378,6 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, hi), o[ct][4 * g + t]);
 #pragma unroll
                     for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, lo), o[ct][4 * g + t]);
-                    
                 }
             }
             load_block_v<HD>(rg, next, lane);

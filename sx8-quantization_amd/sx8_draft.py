@@ -62,7 +62,7 @@ def verify_draft(logits, tokens, parents, cu, uniforms=None, temperature=0.0, dr
     from, child i is kept if uniform * draft_probs(token) < probability, otherwise the distribution becomes
     max(p - draft_probs, 0), scaled.  Where it is not above zero, tokens are kept while they are the first of the largest
     logits (uniforms may be None if that goes for all slots: a number as temperature).  NaN logits count as
-    -infinity; a row of -infinities gives no token.  Sums are held in 64 bits.  Include/sx8_draft.h has every case.
+    -infinity; a row of -infinities gives no token.  Sums are held in 64 bits.  Every case is written down in include/sx8_draft.h.
 
     Returns path (rows,) int32: the rows that slot s keeps, in path[cu[s]] .. (row 0 first, then -1); counts (slots,) int32: how
     many; and the tokens that follow, (slots,) int64 (-1: none).  PagedKV4.keep takes path and counts.  Outputs have no gradient."""

@@ -636,3 +636,436 @@ def test_round_captured(hiplib, cuda):
             want_k = turn(k[at], None, cos[place], sin[place], False).float().half()
             assert torch.equal(q4v[0][a + first:a + ln], q4(want_k).half()) and torch.equal(q4v[1][a + first:a + ln], q4(v[at]).half())
         a += ln
+
+
+def test_round_of_long_trees(hiplib, cuda):
+    """Trees of more than 64 rows through the whole pass: four words a mask, rows past them out of every later step."""
+    from sx8_draft import draft_tree
+    new, before = [200, 300, 256], [10, 0, 33]
+    p, k0, v0 = make(cuda, before, 2, 64, 32, spare=40, width=12)
+    cos, sin = tables(400, 64, cuda)
+    ps, T, cu = trees(new, 6), sum(new), cum(new, cuda)
+    p.reserve(ints(new, cuda))
+    q, k, v = (rand((T, n, 64), 30 + i, F16, cuda) for i, n in enumerate((4, 2, 2)))
+    p.append(0, torch.zeros_like(k), torch.zeros_like(v), cu)
+    mask, depth = draft_tree(ints(flat(ps), cuda), cu, 4)
+    qr = p.append_rope(0, q, k, v, cos, sin, cu, depth=depth)
+    out = p.attend_tree(0, qr, mask, cu)
+    a, b, want = 0, 0, []
+    for n, f, tree in zip(new, before, ps):
+        sets = [s if i < 256 else frozenset() for i, s in enumerate(ancestors(tree))]
+        at = [f + len(s) - 1 for s in sets[:256]]
+        turned = torch.zeros(n, 2, 64, dtype=F16, device=cuda)
+        turned[:256] = turn(k[a:a + min(n, 256)], None, cos[at], sin[at], False).float().half()
+        vv = v[a:a + n].clone()
+        vv[256:] = 0
+        kk, vv = torch.cat([k0[b:b + f], turned]), torch.cat([v0[b:b + f], vv])
+        want.append(want_tree(qr[a:a + n].double(), q4(kk), q4(vv), f, sets))
+        assert not qr[a + 256:a + n].any() or n <= 256
+        a, b = a + n, b + f
+    close(out, torch.cat(want), F16, q4(v).abs().max().item())
+    kept = [list(range(0, n, 7))[:20] for n in new]
+    was = p.read(0, sum(before) + T, cum([f + n for f, n in zip(before, new)], cuda))
+    p.keep(ints(flat([x + [-1] * (n - len(x)) for x, n in zip(kept, new)]), cuda), ints([len(x) for x in kept], cuda), cu)
+    p.check()
+    lens = [f + len(x) for f, x in zip(before, kept)]
+    assert p.lens.tolist() == lens
+    starts = [0, 210, 510]
+    at = flat([list(range(s, s + f)) + [s + f + j for j in x] for s, f, x in zip(starts, before, kept)])
+    for g, w in zip(p.read(0, sum(lens), cum(lens, cuda)), was):
+        assert torch.equal(g, w[at])
+
+
+def test_two_rounds_at_once(hiplib, cuda):
+    """Two caches on two streams at once, then as two captured graphs replayed side by side."""
+    cos, sin = tables(1500, 64, cuda)
+    pools = [make(cuda, [700 + 100 * i, 3, 40], 2, 64, 32, spare=12, width=32, seed=i)[0] for i in range(2)]
+    states = [[t.clone() for t in (p.pages, p.table, p.lens, p.refs)] for p in pools]
+    work = [round_of(p, 20 + i, [9, 1, 30], trees([9, 1, 30], i), cuda, cos, sin) for i, p in enumerate(pools)]
+
+    def back(i):
+        for t, w in zip((pools[i].pages, pools[i].table, pools[i].lens, pools[i].refs), states[i]):
+            t.copy_(w)
+
+    def grown(i):
+        back(i)
+        pools[i].reserve(ints([9, 1, 30], cuda))
+
+    def all_of(i, outs):
+        return [t.clone() for t in (*outs, pools[i].pages, pools[i].table, pools[i].lens, pools[i].refs)]
+
+    want = []
+    for i in range(2):
+        grown(i)
+        want.append(all_of(i, work[i][0](*work[i][1])))
+    streams, graphs = [torch.cuda.Stream() for _ in range(2)], []
+    add = ints([9, 1, 30], cuda)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                back(i)
+                pools[i].reserve(add)
+                got.append(all_of(i, work[i][0](*work[i][1])))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+    for i in range(2):
+        grown(i)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = work[i][0](*work[i][1])
+        graphs.append((g, outs))
+    for _ in range(5):
+        torch.cuda.synchronize()
+        for i in range(2):
+            grown(i)
+        torch.cuda.synchronize()
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i, (_, outs) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(all_of(i, outs), want[i]))
+    for p in pools:
+        p.check()
+
+
+# ------------------------------------------------------------------------------ where calls could go wrong
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_attend_tree_query_sizes(hiplib, cuda, dt):
+    """Queries from tiny to large (bf16: far past fp16's range) keep their precision."""
+    p, k, v = make(cuda, [300] * 6, 1, 64, 64, F16)
+    q = rand((6, 2, 64), 4, F32, cuda)
+    mags = [1e-6, 1e-3, 1.0, 30.0, 300.0, 0.0] if dt is F16 else [1e-30, 1e-3, 1.0, 1e6, 1e20, 0.0]
+    q = (q * torch.tensor(mags, device=cuda)[:, None, None]).to(dt)
+    ones = torch.ones(6, 1, dtype=torch.int64, device=cuda)
+    kk, vv = q4(k), q4(v)
+    for scale, rows in ((0.125, [0, 1, 2, 5]), (2.0 ** -9, [3] if dt is F16 else []), (2.0 ** -23, [3] if dt is BF16 else [4]),
+                        (2.0 ** -69, [4] if dt is BF16 else [])):
+        if rows:
+            got = p.attend_tree(0, q, ones, scale=scale)
+            want = torch.cat([want_tree(q[i:i + 1].double(), kk[300 * i:300 * i + 300], vv[300 * i:300 * i + 300], 299, [{0}], scale)
+                              for i in rows])
+            close(got[rows], want, dt, vv.abs().max().item())
+
+
+@pytest.mark.parametrize("hd,rep", [(64, 16), (128, 32), (256, 16)])
+def test_attend_tree_value_sizes(hiplib, cuda, hd, rep):
+    """Blocks whose values grow from nothing to fp16's ends and back, for one tile of rows a unit and for two."""
+    sizes = [0.0, 1e-6, 1e-3, 1.0, 100.0, 65504.0, 1.0, 0.0, 30.0]
+    from sx8_paged_kv import PagedKV4
+    n = 32 * len(sizes)
+    p = PagedKV4(1, 1, hd, 9, 1, 9, 32, device=cuda)
+    p.reserve(ints([n], cuda))
+    k, v = rand((n, 1, hd), 1, F16, cuda), torch.zeros(n, 1, hd, dtype=F16, device=cuda)
+    for i, size in enumerate(sizes):
+        g = torch.Generator().manual_seed(i)
+        v[32 * i:32 * i + 32] = ((torch.rand(32, 1, hd, generator=g) * 2 - 1) * size).half().to(cuda)
+    p.append(0, k, v, cum([n], cuda))
+    T = 8
+    q = rand((T, rep, hd), 3, F16, cuda)
+    for i in range(9):                                               # (heads that pick out one block each)
+        q[:, i] = k[32 * i + 5, 0] * 4
+    sets = [{j for j in range(T) if (i + j) % 3} for i in range(T)]
+    got = p.attend_tree(0, q, words_of(sets, 1).to(cuda), cum([T], cuda)).double()
+    kk, vv = q4(k), q4(v)
+    want = want_tree(q.double(), kk, vv, n - T, sets)
+    # a row's bound goes by the values that it gives weight, as in the test of `attend`
+    top = want_tree(q.double(), kk, vv.abs().amax(-1, keepdim=True).expand(-1, -1, hd).contiguous(), n - T, sets)
+    err = (got - want).abs()
+    assert (err <= (2.0 ** -11 + LOOSE) * torch.maximum(top, want.abs()) + 2.0 ** -25).all(), (err / top.clamp(min=1e-9)).max()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attend_tree_bits_do_not_depend_on_old_bytes(hiplib, cuda, hd):
+    """What lies behind a slot's last token in its page does not change a bit of the result, whatever it is."""
+    from sx8_paged_kv import PagedKV4
+    lens, new, got = [45, 1, 130], [3, 1, 33], []
+    k, v = rand((sum(lens), 2, hd), 1, F16, cuda), rand((sum(lens), 2, hd), 2, F16, cuda)
+    q = rand((sum(new), 4, hd), 3, F16, cuda)
+    mask = words_of(flat([ancestors(t) for t in trees(new, 3)]), 1).to(cuda)
+    for seed in range(4):
+        p = PagedKV4(1, 2, hd, 8, 3, 3, 64, device=cuda)
+        if seed == 3:
+            p.pages.fill_(255)                                       # (scales and minima that are NaN)
+        elif seed:
+            p.pages.copy_(torch.randint(0, 256, p.pages.shape, generator=torch.Generator().manual_seed(seed), dtype=torch.uint8))
+        p.reserve(ints(lens, cuda))
+        p.append(0, k, v, cum(lens, cuda))
+        got.append(p.attend_tree(0, q, mask, cum(new, cuda)))
+    assert not torch.isnan(got[0]).any() and all(torch.equal(g, got[0]) for g in got)
+
+
+@pytest.mark.parametrize("n_slots", [64, 65, 4096])
+def test_many_slots(hiplib, cuda, n_slots):
+    """Slots without rows, with one, with trees, at 64 (the last number whose line a wave holds) and far more."""
+    from sx8_draft import draft_tree, verify_draft
+    from sx8_paged_kv import PagedKV4
+    hd, nk, rng = 64, 2, random.Random(n_slots)
+    new = [rng.choice([0, 0, 1, 2, 5]) for _ in range(n_slots)]
+    new[n_slots // 2] = 20
+    lens = [n + rng.choice([0, 1, 40]) for n in new]
+    p = PagedKV4(1, nk, hd, 3 * n_slots, n_slots, 4, 32, device=cuda)
+    p.reserve(ints(lens, cuda))
+    k, v = rand((sum(lens), nk, hd), 1, F16, cuda), rand((sum(lens), nk, hd), 2, F16, cuda)
+    p.append(0, k, v, cum(lens, cuda))
+    cos, sin = tables(80, hd, cuda)
+    T, cu, ps = sum(new), cum(new, cuda), trees(new, 1)
+    q, nkr, nvr = (rand((T, n, hd), 5 + i, F16, cuda) for i, n in enumerate((4, nk, nk)))
+    mask, depth = draft_tree(ints(flat(ps), cuda), cu)
+    sets = [ancestors(t) for t in ps]
+    assert torch.equal(mask.cpu(), words_of(flat(sets), 1)) and depth.tolist() == [len(s) - 1 for x in sets for s in x]
+    qr = p.append_rope(0, q, nkr, nvr, cos, sin, cu, depth=depth)
+    at = [ln - n + len(s) - 1 for ln, n, x in zip(lens, new, sets) for s in x]
+    assert torch.equal(qr, turn(q, None, cos[at], sin[at], False).float().half())
+    kt = turn(nkr, None, cos[at], sin[at], False).float().half()
+    out = p.attend_tree(0, qr, mask, cu)
+    a, b, checked = 0, 0, 0
+    for n, ln, x in zip(new, lens, sets):
+        if n and checked < 150:
+            checked += 1
+            kk, vv = (q4(torch.cat([old[b:b + ln - n], fresh[a:a + n]])) for old, fresh in ((k, kt), (v, nvr)))
+            close(out[a:a + n], want_tree(qr[a:a + n].double(), kk, vv, ln - n, x), F16, 6.0)
+        a, b = a + n, b + ln
+    logits, _, tokens, u, _ = drafts(cuda, new, 40, 3)
+    path, counts, nxt = run_verify(cuda, logits, ps, tokens, u, [0.8] * n_slots)
+    assert [t.tolist() for t in verify_draft(logits, torch.tensor(tokens, device=cuda), ints(flat(ps), cuda), cu,
+                                             torch.tensor(u, device=cuda), 0.8)] == [path.tolist(), counts.tolist(), nxt.tolist()]
+    p.keep(path, counts, cu)
+    p.check()
+    assert p.lens.tolist() == [ln - n + c for ln, n, c in zip(lens, new, counts.tolist())]
+
+
+@pytest.mark.parametrize("top,temp", [(20.0, 1e-9), (20.0, 1e-8), (20.0, 1e-6), (1.0, 1e-30), (1.0, 1e-44), (1e10, 1.0), (1e30, 1.0),
+                                      (65504.0, 1e-6), (1e10, 1e9), (3e38, 3e37), (-1e30, 0.7), (1e-30, 1.0), (1e-42, 1e-42)])
+@pytest.mark.parametrize("drawn", [False, True])
+def test_verify_steep(hiplib, cuda, top, temp, drawn):
+    """Temperatures far below a step of the logits, and logits whose steps are far above the temperature: the weights are
+    those of the formula."""
+    V, n = 5000, 6
+    g = torch.Generator().manual_seed(4)
+    logits = (torch.randn(n, V, generator=g) * abs(top) / 10).clamp(-abs(top), abs(top))
+    logits[:, 17], logits[:, 4321] = abs(top), abs(top)
+    logits = logits - (2 * abs(top) if top < 0 else 0)
+    tokens, u = [0, 5, 17, 4321, 17, 4321], [0.51, 0.0, 0.7, 0.3, 0.2, 0.9]
+    probs = torch.softmax(torch.randn(n, V, generator=g), -1).to(cuda) if drawn else None
+    run_verify(cuda, logits.to(cuda), [[-1, 0, 0, 0, 2, 3]], tokens, u, [temp], probs)
+    run_verify(cuda, logits.to(cuda), [[-1]] * n, tokens, [0.1, 0.4, 0.499, 0.501, 0.8, 0.99], [temp] * n)
+
+
+def test_cu_backwards(hiplib, cuda):
+    """A cu that names the same rows for many slots, and ends below its beginnings: no call leaves its memory."""
+    from sx8_draft import draft_tree, verify_draft
+    from sx8_paged_kv import PagedKV4
+    n_slots = 4096
+    p = PagedKV4(1, 1, 64, 2, n_slots, 1, 32, device=cuda)
+    p.reserve(ints([1, 1] + [0] * (n_slots - 2), cuda))
+    q, k = rand((64, 256, 64), 1, F16, cuda), rand((64, 1, 64), 1, F16, cuda)
+    cos, sin = tables(40, 64, cuda)
+    for cu in (ints([0, 64] * 2048 + [64], cuda), ints([-5, 70, 3] + [64, -2 ** 31] * 2047, cuda), ints([64] * 4097, cuda),
+               ints([2 ** 31 - 1, 0] * 2048 + [9], cuda)):
+        mask, depth = draft_tree(ints([-1] + [0] * 63, cuda), cu, 2)
+        assert p.append_rope(0, q, k, k, cos, sin, cu).shape == q.shape
+        ones = torch.full((64, 2), -1, dtype=torch.int64, device=cuda)
+        assert p.attend_tree(0, q, ones, cu).shape == q.shape
+        torch.cuda.synchronize()
+        assert p.refs.tolist() == [1, 1]
+    # long slots over the same rows, whose lists of refused tokens share their places
+    T, V = 600, 50
+    logits = torch.randn(T, V, generator=torch.Generator().manual_seed(1)).to(cuda)
+    tokens, parents = (torch.arange(T, device=cuda) % V), ints([-1] + [0] * (T - 1), cuda)
+    u = torch.full((T,), 0.999, device=cuda)
+    for cu in ([0, 600, 300, 600, 0, 500], [300, 600, 0, 600, 100, 600]):
+        path, counts, nxt = verify_draft(logits, tokens, parents, ints(cu, cuda), u, 1.0)
+        torch.cuda.synchronize()
+        assert path.shape == (T,) and (counts >= 0).all() and (counts <= T).all()
+
+
+def test_past_four_gib(hiplib, cuda):
+    """Pages whose bytes lie past 2^32: rows rotated into them, read as a tree, kept."""
+    from sx8_paged_kv import PagedKV4
+    nk, hd, pt = 8, 128, 128
+    n_pages = (1 << 32) // PagedKV4._page_bytes(nk, hd, pt) + 40
+    big = PagedKV4(1, nk, hd, n_pages, 2, 4, pt, device=cuda)
+    small = PagedKV4(1, nk, hd, 8, 2, 4, pt, device=cuda)
+    big.refs[:n_pages - 8] = 1                                      # all but the last pages are taken
+    cos, sin = tables(400, hd, cuda)
+    new, got = [20, 64], []
+    q, k, v = (rand((300, n, hd), i, F16, cuda) for i, n in enumerate((2 * nk, nk, nk)))
+    mask = words_of(flat([ancestors(t) for t in trees(new, 2)]), 1).to(cuda)
+    path = flat([[j for j in range(0, n, 3)] + [-1] * (n - len(range(0, n, 3))) for n in new])
+    for p in (big, small):
+        p.reserve(ints([200, 100], cuda))
+        p.append_rope(0, q, k, v, cos, sin, cum([200, 100], cuda))
+        p.reserve(ints(new, cuda))
+        qr = p.append_rope(0, q[:84], k[84:168], v[84:168], cos, sin, cum(new, cuda))
+        out = p.attend_tree(0, qr, mask, cum(new, cuda))
+        p.keep(ints(path, cuda), ints([7, 22], cuda), cum(new, cuda))
+        p.check()
+        got.append((qr, out, *p.read(0, 329, cum([207, 122], cuda)), p.lens))
+    assert big.table.max() == n_pages - 8 + small.table.max() and (n_pages - 8) * big.page_bytes > 1 << 32
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_rows_past_four_gib(hiplib, cuda):
+    """Query rows, logits and probabilities whose offsets pass 2^32 bytes."""
+    from sx8_draft import verify_draft
+    T, ts = 2100, 1 << 20
+    big = torch.zeros(T * ts, dtype=F16, device=cuda)
+    far = torch.as_strided(big, (T, 2, 64), (ts, 64, 1))
+    far.copy_(rand((T, 2, 64), 1, F16, cuda))
+    out = torch.as_strided(big, (T, 2, 64), (ts, 64, 1), 256)
+    p, _, _ = make(cuda, [T + 50], 1, 64, 64)
+    near, k = far.clone(), far[:, :1].clone()
+    cos, sin = tables(T + 50, 64, cuda)
+    cu = cum([T], cuda)
+    p.append_rope(0, far, far[:, :1], far[:, 1:], cos, sin, cu, out=out)
+    pages = p.pages.clone()
+    assert torch.equal(out, p.append_rope(0, near, k, near[:, 1:].clone(), cos, sin, cu)) and torch.equal(p.pages, pages)
+    mask = torch.full((T, 4), 0x5A5A5A5A, dtype=torch.int64, device=cuda)
+    assert torch.equal(p.attend_tree(0, far, mask, cu, out=out), p.attend_tree(0, near, mask, cu))
+    del big, far, out
+    rows, V, stride = 20, 9000, 1 << 28
+    pool = torch.empty(rows * stride, dtype=F16, device=cuda)
+    logits, probs = (torch.as_strided(pool, (rows, V), (stride, 1), i << 20) for i in range(2))
+    x, ps, tokens, u, pr = drafts(cuda, [12, 8], V, 5, F16, probs=True)
+    logits.copy_(x)
+    probs.copy_(pr.half())
+    run_verify(cuda, logits, ps, tokens, u, [0.8, 1.2], probs)
+
+
+def test_rows_with_gradients(hiplib, cuda):
+    """Rows that require a gradient are read as values; outputs have none."""
+    from sx8_draft import verify_draft
+    p, k, v = make(cuda, [40, 9], 2, 64, 32)
+    cos, sin = tables(60, 64, cuda)
+    q, kk = rand((2, 4, 64), 5, F16, cuda).requires_grad_(), rand((2, 2, 64), 6, F16, cuda).requires_grad_()
+    w = torch.nn.Parameter(torch.ones(64, dtype=F16, device=cuda))
+    got = p.append_rope(0, q, kk, kk, cos, sin, q_norm=w, k_norm=w)
+    ones = torch.ones(2, 1, dtype=torch.int64, device=cuda)
+    x = torch.randn(2, 30, device=cuda, requires_grad=True)
+    outs = [got, p.attend_tree(0, q, ones), *verify_draft(x, torch.zeros(2, dtype=torch.int64, device=cuda), ints([-1, -1], cuda), cum([1, 1], cuda))]
+    assert not any(o.requires_grad for o in outs)
+
+
+def test_general_path_gives_the_same(hiplib, cuda, monkeypatch):
+    """Without the host module every call takes the wrappers' general path: the same results."""
+    import _sx8lib
+    from sx8_draft import draft_tree, verify_draft
+
+    def run():
+        p, _, _ = make(cuda, [40, 0, 70], 2, 128, 32, spare=8, width=8, layers=2)
+        cos, sin = tables(200, 64, cuda)
+        new = [5, 0, 20]
+        ps, cu, T = trees(new, 4), cum(new, cuda), 25
+        p.reserve(ints(new, cuda))
+        w = rand((128,), 9, F16, cuda)
+        outs = []
+        for dt in (F16, F32):
+            q, k, v = (rand((T, n, 128), 20 + i, dt, cuda) for i, n in enumerate((4, 2, 2)))
+            mask, depth = draft_tree(ints(flat(ps), cuda), cu, 2)
+            qr = p.append_rope(1, q, k, v, cos, sin, cu, depth=depth, q_norm=w, k_norm=w, eps=1e-5, interleaved=dt is F32)
+            outs += [mask, depth, qr, p.attend_tree(1, qr, mask, cu), p.attend_tree(0, qr, mask, cu, scale=0.3), p.pages.clone()]
+        outs.append(p.append_rope(0, q[:3], k[:3], v[:3], cos, sin, dtype=BF16))
+        for dt, probs, temp in ((F32, False, 0.8), (BF16, True, torch.tensor([0.5, 1.0, 0.0], device=cuda)), (F16, False, 0.0)):
+            logits, _, tokens, u, pr = drafts(cuda, new, 900, 3, dt, probs=probs)
+            u = None if dt is F16 else torch.tensor(u, device=cuda)
+            got = verify_draft(logits, torch.tensor(tokens, device=cuda), ints(flat(ps), cuda), cu, u, temp, pr)
+            outs += got
+        p.keep(got[0], got[1], cu)
+        p.keep(ints([0, 0, 0], cuda), ints([1, 0, 1], cuda), ints([0, 1, 1, 2], cuda))
+        p.check()
+        return outs + [p.pages, p.table, p.lens, p.refs]
+
+    fast = run()
+    assert isinstance(_sx8lib.py().kv4_attend_tree, type(len))      # the module is there
+    monkeypatch.setattr(_sx8lib, "_py", _sx8lib._NoHostModule())
+    for i, (a, b) in enumerate(zip(fast, run())):
+        assert torch.equal(a, b), i
+
+
+def test_views_that_negate(hiplib, cuda):
+    """They are read as the values they stand for; as outputs, masks or whole numbers they are refused."""
+    from sx8_draft import draft_tree, verify_draft
+    p, _, _ = make(cuda, [40, 9], 2, 64, 32)
+    cos, sin = tables(60, 64, cuda)
+    n = torch._neg_view
+    q, k, v, w = (rand(s, i, F16, cuda) for i, s in enumerate(((2, 4, 64), (2, 2, 64), (2, 2, 64), (64,))))
+    want = p.append_rope(0, q, k, v, cos, sin, q_norm=w, k_norm=w)
+    pages = p.pages.clone()
+    got = p.append_rope(0, n(-q), n(-k), n(-v), n(-cos), n(-sin), q_norm=n(-w), k_norm=n(-w))
+    assert torch.equal(got, want) and torch.equal(p.pages, pages)
+    ones = torch.ones(2, 1, dtype=torch.int64, device=cuda)
+    assert torch.equal(p.attend_tree(0, n(-q), ones), p.attend_tree(0, q, ones))
+    x, pr, u = torch.randn(2, 30, device=cuda), torch.rand(2, 30, device=cuda), torch.rand(2, device=cuda)
+    tokens, parents, cu, temp = torch.tensor([3, 4], device=cuda), ints([-1, 0], cuda), cum([2], cuda), torch.tensor([0.7], device=cuda)
+    for a, b in zip(verify_draft(x, tokens, parents, cu, u, temp, pr), verify_draft(n(-x), tokens, parents, cu, n(-u), n(-temp), n(-pr))):
+        assert torch.equal(a, b)
+    for call in (lambda: p.append_rope(0, q, k, v, cos, sin, out=n(torch.empty_like(q))), lambda: p.append_rope(0, q, k, v, cos, sin, n(-cum([1, 1], cuda))),
+                 lambda: p.append_rope(0, q, k, v, cos, sin, depth=n(ints([0, 0], cuda))), lambda: p.attend_tree(0, q, n(-ones)),
+                 lambda: p.attend_tree(0, q, ones, out=n(torch.empty_like(q))), lambda: draft_tree(n(parents), cu), lambda: draft_tree(parents, n(-cu)),
+                 lambda: verify_draft(x, n(tokens), parents, cu, u, 0.8), lambda: verify_draft(x, tokens, n(parents), cu, u, 0.8),
+                 lambda: verify_draft(x, tokens, parents, n(-cu), u, 0.8), lambda: p.keep(n(ints([0, 0], cuda)), ints([1, 1], cuda)),
+                 lambda: p.keep(ints([0, 0], cuda), n(ints([1, 1], cuda)))):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@pytest.mark.parametrize("general", [False, True])
+def test_wrappers_refuse(hiplib, cuda, monkeypatch, general):
+    """What the documentation does not allow, by the host module and by the general path."""
+    import _sx8lib
+    from sx8_draft import draft_tree, verify_draft
+    p, _, _ = make(cuda, [40], 1, 64, 32)
+    if general:
+        monkeypatch.setattr(_sx8lib, "_py", _sx8lib._NoHostModule())
+    cos, sin = tables(60, 64, cuda)
+    q, k, w = rand((1, 2, 64), 1, F16, cuda), rand((1, 1, 64), 2, F16, cuda), rand((64,), 3, F16, cuda)
+    cu, ones = cum([1], cuda), torch.ones(1, 1, dtype=torch.int64, device=cuda)
+    x, tokens, parents, u = torch.randn(1, 30, device=cuda), torch.zeros(1, dtype=torch.int64, device=cuda), ints([-1], cuda), torch.rand(1, device=cuda)
+    before = p.pages.clone()
+
+    def rope(q=q, k=k, v=k, cos=cos, sin=sin, layer=0, **kw):
+        return lambda: p.append_rope(layer, q, k, v, cos, sin, **kw)
+
+    def tree(q=q, mask=ones, cu=None, **kw):
+        return lambda: p.attend_tree(0, q, mask, cu, **kw)
+
+    def verify(x=x, tokens=tokens, parents=parents, cu=cu, u=u, t=0.8, probs=None):
+        return lambda: verify_draft(x, tokens, parents, cu, u, t, probs)
+
+    for i, call in enumerate((
+            rope(layer=1), rope(layer=-1), rope(q=q.double()), rope(q=q[..., :32]), rope(q=q[0]), rope(k=k.bfloat16()), rope(v=k.float()),
+            rope(k=k[:0]), rope(k=q), rope(q=rand((1, 2, 64), 1, F16, cuda).cpu()), rope(cos=cos.half()), rope(cos=cos[:, :8]), rope(cos=cos[0], sin=sin[0]),
+            rope(cos=cos[:, :20], sin=sin[:, :20]), rope(cos=torch.ones(60, 40, device=cuda), sin=torch.ones(60, 40, device=cuda)), rope(cos=cos.cpu()),
+            rope(cos=cos[:0], sin=sin[:0]), rope(depth=ints([0, 0], cuda)), rope(depth=ints([0], cuda).long()), rope(q_norm=w.float()),
+            rope(k_norm=w[:32]), rope(q_norm=w.cpu()), rope(eps=-1.0), rope(eps=math.nan), rope(eps=math.inf), rope(dtype=BF16), rope(dtype=F32),
+            rope(out=q), rope(out=q.float()), rope(out=q[:, :1].expand(1, 2, 64)), rope(q=torch.cat([q, q]), k=torch.cat([k, k]), v=torch.cat([k, k])),
+            rope(cu=cu.long()), rope(cu=cum([1, 1], cuda)),
+            tree(mask=ones.int()), tree(mask=ones[0]), tree(mask=ones.expand(1, 5).contiguous()), tree(mask=torch.ones(2, 1, dtype=torch.int64, device=cuda)),
+            tree(mask=ones.cpu()), tree(mask=torch.ones(1, 0, dtype=torch.int64, device=cuda)), tree(q=q.float()), tree(scale=0.0), tree(scale=math.nan),
+            tree(out=q), tree(out=q.bfloat16()), tree(cu=cum([1, 1], cuda)), tree(q=torch.cat([q, q]), mask=torch.cat([ones, ones])),
+            lambda: draft_tree(parents, cu, 0), lambda: draft_tree(parents, cu, 5), lambda: draft_tree(parents, cu, -1), lambda: draft_tree(parents.long(), cu),
+            lambda: draft_tree(parents, cu.cpu()), lambda: draft_tree(parents.cpu(), cu), lambda: draft_tree([0], cu), lambda: draft_tree(parents, cu[:0]),
+            lambda: draft_tree(parents, ints([0], cuda)), lambda: draft_tree(ints([0, 1, 2, 3], cuda)[::2], cu),
+            verify(x=x.double()), verify(x=x[0]), verify(x=x.cpu()), verify(x=x[:, :0]), verify(tokens=tokens.int()), verify(tokens=torch.cat([tokens, tokens])),
+            verify(parents=parents.long()), verify(parents=ints([0, 0], cuda)), verify(cu=cu.long()), verify(cu=cu[:1]), verify(u=None), verify(u=u.half()),
+            verify(u=torch.rand(2, device=cuda)), verify(u=None, t=torch.zeros(1, device=cuda)), verify(t=torch.ones(2, device=cuda)),
+            verify(t=torch.ones(1, device=cuda).half()), verify(t=torch.ones(1)), verify(probs=x[:, :29]), verify(probs=x.double()), verify(probs=x.cpu()),
+            lambda: p.keep(ints([0], cuda).long(), ints([1], cuda)), lambda: p.keep(ints([0], cuda), ints([1, 1], cuda)),
+            lambda: p.keep(ints([0, 0], cuda), ints([1], cuda)), lambda: p.keep([0], ints([1], cuda)), lambda: p.keep(ints([0], cuda), ints([1], cuda), cu.long()),
+            lambda: p.keep(ints([0], cuda), ints([1], cuda).cpu()), lambda: p.keep(ints([0], cuda), ints([1], cuda), cum([1, 1], cuda)))):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} is not refused")
+    assert torch.equal(p.pages, before) and p.lens.tolist() == [40]
+    # calls without rows
+    none = ints([0, 0], cuda)
+    assert p.append_rope(0, q[:0], k[:0], k[:0], cos, sin, none).shape == (0, 2, 64) and p.attend_tree(0, q[:0], ones[:0], none).shape == (0, 2, 64)
+    mask, depth = draft_tree(parents[:0], none)
+    path, counts, nxt = verify_draft(x[:0], tokens[:0], parents[:0], none, u[:0], 0.8, x[:0])
+    p.keep(path, counts, none)
+    p.check()
+    assert mask.shape == (0, 1) and depth.shape == (0,) and counts.tolist() == [0] and nxt.tolist() == [-1] and p.lens.tolist() == [40]
