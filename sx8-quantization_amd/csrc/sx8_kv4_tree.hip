@@ -51,14 +51,29 @@ constexpr int64_t tree_ws(int64_t hd) { return part_rows(hd) * (hd + 2) * 4 + kM
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
 // x of eight values as two fp16 numbers each, hi + lo
-__device__ __forceinline__ void halves8(const float* x, u32x4* hi, u32x4* lo) {
+__device__ __forceinline__ void halves8(const float* x, f16x8* hi, f16x8* lo) {
     typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+    u32x4 a, b;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const h2 h = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-        (*hi)[i] = __builtin_bit_cast(uint32_t, h);
-        (*lo)[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.f, x[2 * i]), __builtin_fmaf((float)h[1], -1.f, x[2 * i + 1])));
+        a[i] = __builtin_bit_cast(uint32_t, h);
+        b[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.f, x[2 * i]), __builtin_fmaf((float)h[1], -1.f, x[2 * i + 1])));
     }
+    *hi = __builtin_bit_cast(f16x8, a);
+    *lo = __builtin_bit_cast(f16x8, b);
+}
+// (hi + lo) s of eight values as two fp16 numbers each: the product of the upper halves rounded, and what that left (one multiply-add:
+// the exact product of two fp16 numbers less its rounding is an fp16 number, down to the type's smallest) plus the lower halves' product
+__device__ __forceinline__ void scaled8(f16x8 hi, f16x8 lo, f16x8 s, f16x8* a, f16x8* b) {
+    *a = hi * s;
+    *b = __builtin_elementwise_fma(lo, s, __builtin_elementwise_fma(hi, s, -*a));
+}
+// Levels of K as `levels` gives them but for values 0, 1, 4 and 5, which are a 16th of it (two shifts less; their query values are 16 times as large).
+__device__ __forceinline__ f16x8 levels_k(uint32_t w) {
+    const uint32_t up = w >> 8;
+    const u32x4 v = {w & 0x000F000Fu, w & 0x00F000F0u, up & 0x000F000Fu, up & 0x00F000F0u};
+    return __builtin_bit_cast(f16x8, v);
 }
 template <int HD, bool kBf16, int kCt>
 __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(const Kv4Pool p, const TreeIo io) {
@@ -161,6 +176,7 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                 for (int e = 0; e < 8; ++e) {
                     f[e] = (_Float16)(row_ok ? ld16<kBf16>(half_of(raw[j][e >> 1], e)) * mul : 0.f);
                     qs[j / 2] += (float)f[e];
+                    if ((e & 2) == 0) f[e] *= (_Float16)16.f;        // (levels_k)
                 }
                 frag[ct][j][lane] = __builtin_bit_cast(u32x4, f);
             }
@@ -223,7 +239,7 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     s[ct] = mfma16(__builtin_bit_cast(f16x8, mw), __builtin_bit_cast(f16x8, frag[ct][W][lane]), zero4());
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const f16x8 l0 = levels(rg.kw[a][2 * g]), l1 = levels(rg.kw[a][2 * g + 1]);
+                    const f16x8 l0 = levels_k(rg.kw[a][2 * g]), l1 = levels_k(rg.kw[a][2 * g + 1]);
                     float ks[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) ks[e] = sx8_h2f(half_of(rg.ks[g][2 * a + (e >> 1)], e)) * 1048576.f;
@@ -322,12 +338,12 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
             if (c == NG) vm = u32x4{kOnes, kOnes, kOnes, kOnes};
             if (c > NG) vm = u32x4{0u, 0u, 0u, 0u};
             const f16x8 vm8 = __builtin_bit_cast(f16x8, vm);
+            f16x8 ph[kCt], pl[kCt];
 #pragma unroll
             for (int ct = 0; ct < kCt; ++ct) {
-                u32x4 hi, lo;
-                halves8(pv[ct], &hi, &lo);
-                om[ct] = mfma16(vm8, __builtin_bit_cast(f16x8, hi), om[ct]);
-                om[ct] = mfma16(vm8, __builtin_bit_cast(f16x8, lo), om[ct]);
+                halves8(pv[ct], &ph[ct], &pl[ct]);
+                om[ct] = mfma16(vm8, ph[ct], om[ct]);
+                om[ct] = mfma16(vm8, pl[ct], om[ct]);
             }
             uint32_t large = 0;                  // bits 14 and 30: a scale of 2 or more (or NaN)
 #pragma unroll
@@ -343,18 +359,15 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                         s = __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, s) * f16x8(down));
 #pragma unroll
                         for (int ct = 0; ct < kCt; ++ct) {
-                            float ps[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) ps[e] = pv[ct][e] * sx8_h2f(half_of(s[e >> 1], e));
-                            u32x4 hi, lo;
-                            halves8(ps, &hi, &lo);
+                            f16x8 hi, lo;
+                            scaled8(ph[ct], pl[ct], __builtin_bit_cast(f16x8, s), &hi, &lo);
 #pragma unroll
                             for (int t = 4 * g; t < 4 * g + 4; ++t) {
                                 uint32_t word = rg.vw[t];
                                 asm volatile("" : "+v"(word));          // (here, not ahead of the loop: registers)
                                 const f16x8 lv = levels(word) * f16x8(up);
-                                o[ct][t] = mfma16(lv, __builtin_bit_cast(f16x8, hi), o[ct][t]);
-                                o[ct][t] = mfma16(lv, __builtin_bit_cast(f16x8, lo), o[ct][t]);
+                                o[ct][t] = mfma16(lv, hi, o[ct][t]);
+                                o[ct][t] = mfma16(lv, lo, o[ct][t]);
                             }
                         }
                     }
@@ -369,15 +382,12 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                 for (int t = 0; t < 4; ++t) lv[t] = levels(rg.vw[4 * g + t]);
 #pragma unroll
                 for (int ct = 0; ct < kCt; ++ct) {
-                    u32x4 hi, lo;
-                    float ps[8];
+                    f16x8 hi, lo;
+                    scaled8(ph[ct], pl[ct], __builtin_bit_cast(f16x8, rg.vs[g]), &hi, &lo);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) ps[e] = pv[ct][e] * sx8_h2f(half_of(rg.vs[g][e >> 1], e));
-                    halves8(ps, &hi, &lo);
+                    for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], hi, o[ct][4 * g + t]);
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, hi), o[ct][4 * g + t]);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], __builtin_bit_cast(f16x8, lo), o[ct][4 * g + t]);
+                    for (int t = 0; t < 4; ++t) o[ct][4 * g + t] = mfma16(lv[t], lo, o[ct][4 * g + t]);
                 }
             }
             load_block_v<HD>(rg, next, lane);
