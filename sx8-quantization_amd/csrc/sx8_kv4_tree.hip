@@ -50,7 +50,7 @@ constexpr int64_t tree_ws(int64_t hd) { return part_rows(hd) * (hd + 2) * 4 + kM
 
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
-// x of eight values as two fp16 numbers each, hi + lo
+// x of eight values as two fp16 numbers each, hi + lo, both cut (rounded ones spill registers: 191 us and 174 for the long case below)
 __device__ __forceinline__ void halves8(const float* x, f16x8* hi, f16x8* lo) {
     typedef __fp16 h2 __attribute__((ext_vector_type(2)));
     u32x4 a, b;
@@ -63,17 +63,12 @@ __device__ __forceinline__ void halves8(const float* x, f16x8* hi, f16x8* lo) {
     *hi = __builtin_bit_cast(f16x8, a);
     *lo = __builtin_bit_cast(f16x8, b);
 }
-// (hi + lo) s of eight values as two fp16 numbers each: the product of the upper halves rounded, and what that left (one multiply-add:
-// the exact product of two fp16 numbers less its rounding is an fp16 number, down to the type's smallest) plus the lower halves' product
+// (hi + lo) s of eight values as two fp16 numbers each: the product of the upper halves rounded, and what that left (the exact
+// product of two fp16 numbers less its rounding is an fp16 number, down to the type's smallest) plus the lower halves'
+// product: 12 instructions, 24 by products in float32 that are taken apart again (174 us and 191 for the long case below).
 __device__ __forceinline__ void scaled8(f16x8 hi, f16x8 lo, f16x8 s, f16x8* a, f16x8* b) {
     *a = hi * s;
     *b = __builtin_elementwise_fma(lo, s, __builtin_elementwise_fma(hi, s, -*a));
-}
-// Levels of K as `levels` gives them but for values 0, 1, 4 and 5, which are a 16th of it (two shifts less; their query values are 16 times as large).
-__device__ __forceinline__ f16x8 levels_k(uint32_t w) {
-    const uint32_t up = w >> 8;
-    const u32x4 v = {w & 0x000F000Fu, w & 0x00F000F0u, up & 0x000F000Fu, up & 0x00F000F0u};
-    return __builtin_bit_cast(f16x8, v);
 }
 template <int HD, bool kBf16, int kCt>
 __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(const Kv4Pool p, const TreeIo io) {
@@ -176,7 +171,6 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                 for (int e = 0; e < 8; ++e) {
                     f[e] = (_Float16)(row_ok ? ld16<kBf16>(half_of(raw[j][e >> 1], e)) * mul : 0.f);
                     qs[j / 2] += (float)f[e];
-                    if ((e & 2) == 0) f[e] *= (_Float16)16.f;        // (levels_k)
                 }
                 frag[ct][j][lane] = __builtin_bit_cast(u32x4, f);
             }
@@ -239,7 +233,7 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
                     s[ct] = mfma16(__builtin_bit_cast(f16x8, mw), __builtin_bit_cast(f16x8, frag[ct][W][lane]), zero4());
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const f16x8 l0 = levels_k(rg.kw[a][2 * g]), l1 = levels_k(rg.kw[a][2 * g + 1]);
+                    const f16x8 l0 = levels(rg.kw[a][2 * g]), l1 = levels(rg.kw[a][2 * g + 1]);
                     float ks[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) ks[e] = sx8_h2f(half_of(rg.ks[g][2 * a + (e >> 1)], e)) * 1048576.f;
