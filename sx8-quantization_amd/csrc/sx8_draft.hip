@@ -335,6 +335,7 @@ template <int kType, int kProbs, bool kGoOn>
 __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io) {
     constexpr bool kFirst = kProbs >= 0 && !kGoOn;                    // (stops at a refused token)
     const int slot = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const float temp = temperature_of(io, slot);                     // (asked for with cu)
     int first, n;
     kv4_rows(io.sh, io.cu, slot, &first, &n);
     if (n == 0) {
@@ -345,7 +346,18 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         }
         return;
     }
-    const float temp = temperature_of(io, slot);
+    // parent, token and uniform of row i0 + lane, the first ones on their way before the sums of rows
+    int par = -1;
+    int64_t tok = -1;
+    float un = 0.f;
+    auto load_rows = [&](int i0) {
+        const int row = i0 + lane;
+        par = row > 0 && row < n ? io.parents[first + row] : -1;
+        tok = row < n ? io.tokens[first + row] : -1;
+        un = row < n && io.u ? io.u[first + row] : 0.f;
+    };
+    if constexpr (!kGoOn) load_rows(0);
+    const float u0 = io.u ? io.u[first] : 0.f;
     const bool greedy = !(temp > 0.f);
     const double scale = greedy ? 0.0 : scale_of(temp);
     // the slot's lists: in LDS where they fit and nobody else reads them
@@ -366,6 +378,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         cur = wt.cur;
         count = wt.count;
         i0 = wt.row & ~63;
+        load_rows(i0);
         above = wt.row % 64 == 63 ? 0ull : ~0ull << (wt.row % 64 + 1);
         a = wt.a;
         b = wt.b;
@@ -385,8 +398,8 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         for (int i = tid; i < n; i += kWalkThreads) io.path[first + i] = i == 0 ? 0 : -1;
         __syncthreads();
         for (int i = tid; i < n; i += kWalkThreads) {
-            const int up = io.parents[first + i];
-            const int64_t x = io.tokens[first + i];
+            const int up = i < 64 ? par : io.parents[first + i];
+            const int64_t x = i < 64 ? tok : io.tokens[first + i];
             double p = -1.0;
             if (i > 0 && up >= 0 && up < i && x >= 0 && x < io.V) {
                 const RowPart r = whole[up];
@@ -432,13 +445,9 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         return all;
     };
     // the walk: every wave does it alike, a row a lane
-    for (; i0 < n; i0 += 64, above = ~0ull) {
-        const int row = i0 + lane;
-        const bool in = row < n;
-        const int par = in && row > 0 ? io.parents[first + row] : -1;
-        const int64_t tok = in ? io.tokens[first + row] : -1;
-        const double pr = in ? prob[row] : -1.0;
-        const double un = in && io.u ? (double)io.u[first + row] : 0.0;
+    for (bool loaded = true; i0 < n; i0 += 64, above = ~0ull, loaded = false) {
+        if (!loaded) load_rows(i0);
+        const double pr = i0 + lane < n ? prob[i0 + lane] : -1.0;
         double qr = 0.0;
         if constexpr (kProbs >= 0)
             if (pr >= 0.0 && !greedy) qr = (double)value<kProbs < 0 ? 0 : kProbs>(io.probs, ((int64_t)first + par) * io.probs_stride + tok);
@@ -446,7 +455,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         while (todo) {
             const int k = __builtin_ctzll(todo);
             todo &= todo - 1;
-            const double p = lane_of_double(pr, k), uk = lane_of_double(un, k);
+            const double p = lane_of_double(pr, k), uk = lane_of_double((double)un, k);
             bool keep;
             if (greedy) {
                 keep = p > 0.0;
@@ -543,7 +552,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
     }
     __syncthreads();
     // the part in which the sum passes u * total (or, by roundings, the last one that has any)
-    const double goal = (io.u ? (double)io.u[first] : 0.0) * total;
+    const double goal = (double)u0 * total;
     double before = 0.0, last_before = 0.0;
     int part = -1, last = 0;
     for (int p0 = 0; p0 < io.parts && part < 0; p0 += 64) {
