@@ -470,7 +470,7 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
 // 2 (group + j)).
 template <int HD, bool kBf16, int kCols>
 __global__ __launch_bounds__(256) void k_kv4_tree_combine(const TreeIo io, int G) {
-    constexpr int N = HD / 64, kU = 8;                            // kU: parts requested together
+    constexpr int N = HD / 64;
     typedef float vecN __attribute__((ext_vector_type(N)));
     const TreePiece pc = io.piece[blockIdx.x];
     const int row = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -478,31 +478,40 @@ __global__ __launch_bounds__(256) void k_kv4_tree_combine(const TreeIo io, int G
     auto at = [&](int i) { return (int64_t)(i == 0 ? pc.first : 2 * (pc.first / 2 + i)) * kCols + row; };
     float m = -__builtin_inff(), den = 0.f;
     vecN acc = 0.f;
-    for (int i = 0; i < pc.parts; i += kU) {
-        float pm[kU], pl[kU];
-        vecN v[kU];
+    for (int i0 = 0; i0 < pc.parts; i0 += 64) {                   // lane j: what part i0 + j weighs
+        const int n = min(64, pc.parts - i0);
+        const int64_t mine = at(i0 + min(lane, n - 1)) * 2;
+        const float pm = io.part_ml[mine], pl = io.part_ml[mine + 1];
+        float f = 0.f;
+        // kU parts requested together
+        auto add = [&](auto together, int i) {
+            constexpr int kU = decltype(together)::value;
+            vecN v[kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int64_t a = at(min(i + u, pc.parts - 1));
-            pm[u] = io.part_ml[a * 2];
-            pl[u] = io.part_ml[a * 2 + 1];
-            v[u] = reinterpret_cast<const vecN*>(io.part_o + a * HD)[lane];
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        float mn = m;
+            for (int u = 0; u < kU; ++u) v[u] = reinterpret_cast<const vecN*>(io.part_o + at(i0 + min(i + u, n - 1)) * HD)[lane];
+            __builtin_amdgcn_sched_barrier(0);
+            if (i == 0) {
+                float mn = fmaxf(m, pm);
 #pragma unroll
-        for (int u = 0; u < kU; ++u) mn = fmaxf(mn, pm[u]);
-        const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        den *= alpha;
-        acc *= alpha;
+                for (int o = 32; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
+                const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                f = lane >= n ? 0.f : pm == mn ? 1.f : __builtin_amdgcn_exp2f(pm - mn);
+                float sum = lane < n ? f * pl : 0.f;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            if (i + u >= pc.parts) continue;
-            const float f = pm[u] == m ? 1.f : __builtin_amdgcn_exp2f(pm[u] - m);
-            den = __builtin_fmaf(f, pl[u], den);
-            acc = __builtin_elementwise_fma(vecN(f), v[u], acc);
-        }
+                for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+                m = mn;
+                den = __builtin_fmaf(den, alpha, sum);
+                acc *= alpha;
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                if (i + u >= n) continue;
+                acc = __builtin_elementwise_fma(vecN(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i + u))), v[u], acc);
+            }
+        };
+        if (n <= 8) add(std::integral_constant<int, 8>{}, 0);
+        else
+            for (int i = 0; i < n; i += 16) add(std::integral_constant<int, 16>{}, i);
     }
     acc *= den == 0.f ? 0.f : 1.f / den;
     const int r = kCols * pc.tile + row, tok = r / G;
