@@ -1,21 +1,19 @@
 // sx8_kv4_tree.hip -- attention of trees of drafted tokens over the paged 4-bit cache (include/sx8_paged.h).
 //
 // The products are those of sx8_kv4.hip: S^T = K Q^T with the levels as fp16 subnormals, O^T += V^T P^T with p * s as two
-// fp16 numbers (cut, not rounded: 21 bits), the minima's parts in matrix products of their own, where a row of ones gives the
-// weights' sum as well.  What differs is the shape of the work: a tree brings tens of query rows a KV head, so a unit is
-// one or two tiles of 16 of them (a block's levels are unpacked once for both); a work-group's four waves take a unit's
-// blocks in turn and add their results up in LDS, so that a unit cut over many work-groups leaves one partial
-// result for each.  A block that ends at or behind the first new token is masked by 32 bits of each column's mask.
-// Bound by instructions: for 16 rows and a block of 32 tokens of a head of 128 there are 29 matrix instructions of 16 cycles
-// and about 140 others of 4 (exponentials 16, multiply-adds of fp16 with float32 8), beside 190 for the block; they take turns on
-// a SIMD (two long trees: the VALU is busy 71% of its cycles, the matrix cores 31%), and a second wave there makes neither faster.
+// fp16 numbers, the minima's parts in matrix products of their own, where a row of ones gives the weights' sum as well.  What
+// differs is the shape of the work: a tree brings tens of query rows a KV head, so a unit is one or two tiles of 16 of them (a
+// block's levels are unpacked once for both); a work-group's four waves take a unit's blocks in turn and add their results up in
+// LDS, so that a unit cut over many work-groups leaves one partial result for each.  A block that ends at or behind the
+// first new token is masked by 32 bits of each column's mask.
+// Bound by instructions: for 16 rows and a block of 32 tokens of a head of 128 there are 28 matrix instructions of 16 cycles
+// and 95 others of 4 (exponentials 16), beside 180 for the block; they take turns on a SIMD (two long trees: the VALU is busy 66%
+// of its cycles, the matrix cores 33%, together 99%), and a second wave there makes neither faster.
 // A wave keeps one block in registers: K of the next one is requested when the scores are done, V when the products are;
-// no branch lies between, so that the compiler keeps the scores' sums apart from neither (with one: 316 us instead of 108 for
-// the case below).  Query fragments stay in LDS.  Three or four tiles a unit spill (120 us) or need half of their sums moved
-// through accumulator registers (109); p * s by mixed multiply-adds that write halves of a register: 102; a block's scores computed
-// beside the products of the one before: 155.
-// 8 trees of 64 rows after 2500 .. 4100 tokens, 32 heads over 8 of 128: 93 us; two of 31 after 61000 and 100000, 32 over 4: 214
-// (198 on other machines); 24 of 1 .. 24 after up to 8000: 45 (the combine 4.2 more).
+// no branch lies between (with one the sums are copied: 316 us for the two long trees below, at that stage 237).  Query fragments
+// stay in LDS.  Three tiles a unit spill registers (245 us beside 198 on one machine), four leave one wave a SIMD (220).
+// Measured, with combine: 24 trees of 1 .. 24 rows after up to 8000 tokens, 32 heads over 8 of 128: 46 us; 8 of 64 rows after
+// 2500 .. 4100: 84; two of 31 after 61000 and 100000, 32 over 4: 175 (under a profiler's clock 205).
 #include "sx8_kv4_core.h"
 
 namespace sx8 {
@@ -50,7 +48,7 @@ constexpr int64_t tree_ws(int64_t hd) { return part_rows(hd) * (hd + 2) * 4 + kM
 
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
-// x of eight values as two fp16 numbers each, hi + lo, both cut (rounded ones spill registers: 191 us and 174 for the long case below)
+// x of eight values as two fp16 numbers each, hi + lo, both cut (rounded ones spill registers: 191 us beside 175 for two long trees)
 __device__ __forceinline__ void halves8(const float* x, f16x8* hi, f16x8* lo) {
     typedef __fp16 h2 __attribute__((ext_vector_type(2)));
     u32x4 a, b;
@@ -65,7 +63,7 @@ __device__ __forceinline__ void halves8(const float* x, f16x8* hi, f16x8* lo) {
 }
 // (hi + lo) s of eight values as two fp16 numbers each: the product of the upper halves rounded, and what that left (the exact
 // product of two fp16 numbers less its rounding is an fp16 number, down to the type's smallest) plus the lower halves'
-// product: 12 instructions, 24 by products in float32 that are taken apart again (174 us and 191 for the long case below).
+// product: 12 instructions, 24 by products in float32 that are taken apart again (two long trees: 175 us, 191).
 __device__ __forceinline__ void scaled8(f16x8 hi, f16x8 lo, f16x8 s, f16x8* a, f16x8* b) {
     *a = hi * s;
     *b = __builtin_elementwise_fma(lo, s, __builtin_elementwise_fma(hi, s, -*a));
@@ -466,8 +464,9 @@ __global__ __launch_bounds__(256, (groups_per_cu<HD, kCt>())) void k_kv4_tree(co
     }
 }
 
-// Units that were cut: wave (record, row) adds a row's parts up in their order (part 0 at its place, part j at place
-// 2 (group + j)).
+// Units that were cut: wave (record, row) adds a row's parts up (part 0 at its place, part j at place 2 (group + j)), 64 of them at
+// a time: each lane weighs one, and the sums are added in the parts' order, 16 requested together (96 parts: 6.2 us, 13.9 where
+// every lane computes every weight).
 template <int HD, bool kBf16, int kCols>
 __global__ __launch_bounds__(256) void k_kv4_tree_combine(const TreeIo io, int G) {
     constexpr int N = HD / 64;
@@ -574,8 +573,8 @@ extern "C" int32_t sx8_kv4_attend_tree(const uint8_t* pages, const int32_t* tabl
             hipLaunchKernelGGL((k_kv4_tree_combine<HD, kBf, 16 * kCt>), dim3(groups, (unsigned)(most + 3) / 4), dim3(256), 0,
                                as_stream(stream), io, p.sh.G);
         };
-        // Two tiles a unit from four tiles a slot on (8 slots of about 3300 tokens, 8 KV heads of 128, 64 rows of 4 heads: 97 us
-        // instead of 112; of 2 rows: 28 instead of 25), where registers allow it (16 heads over 2 of 256: 229 instead of 106).
+        // Two tiles a unit from four tiles a slot on, where registers allow it (8 slots of about 3300 tokens, 8 KV heads of 128,
+        // groups of 4: 64 new rows 92 us instead of 108, 16 rows 37 instead of 40, 12 rows 36 instead of 34, 2 rows 27 instead of 23).
         if constexpr (HD < 256) {
             if (tiles >= 4) return go(std::integral_constant<int, 2>{});
         }
