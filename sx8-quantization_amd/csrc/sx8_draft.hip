@@ -176,22 +176,21 @@ __device__ __forceinline__ void better(float& top, int& arg, float t, int a) {
     }
 }
 
-// The slot that has row r, or -1.
-__device__ __forceinline__ int slot_of(const Kv4Shape& sh, const int32_t* cu, int r) {
+// The slot that has row r, or -1.  mine: where slot `lane` ends, 2^31 - 1 for none; begin: where slot 0 begins.
+__device__ __forceinline__ int slot_of(const Kv4Shape& sh, const int32_t* cu, int r, int mine, int begin) {
     const int lane = threadIdx.x & 63;
     // (ends grow: the slots that end at or before r come first; 64 at a time)
-    int s = 0;
-    for (; s < sh.n_slots; s += 64) {
-        const int at = s + lane;
-        const uint64_t before = __builtin_amdgcn_ballot_w64(at < sh.n_slots && cu[at + 1] <= r);
-        const int k = __builtin_popcountll(before);
-        if (k < 64) {
-            s += k;
-            break;
+    int s = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine <= r));
+    if (s < 64) {
+        if (s > 0) begin = __builtin_amdgcn_readlane(mine, s - 1);
+    } else {
+        for (int k = 64; k == 64 && s < sh.n_slots; s += k) {
+            const int at = s + lane;
+            k = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at < sh.n_slots && cu[at + 1] <= r));
         }
+        if (s < sh.n_slots) begin = cu[s];
     }
-    if (s >= sh.n_slots || cu[s] > r) return -1;
-    return s;
+    return s >= sh.n_slots || begin > r ? -1 : s;
 }
 
 // kWide: rows begin on 16 bytes, and a thread takes 16 bytes at a time.
@@ -201,36 +200,42 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(const VerifyIo io) 
     const int r = blockIdx.x, part = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int64_t base = (int64_t)part * kPart, from = r * io.stride + base;
     const int n = (int)min((int64_t)kPart, io.V - base);
+    const int mine = lane < io.sh.n_slots ? io.cu[lane + 1] : 0x7FFFFFFF, begin = io.cu[0];   // (asked for before the logits)
     float x[kE], top = -__builtin_inff();
     auto place = [&](int i) { return (i / kN * kRowThreads + tid) * kN + i % kN; };
     if constexpr (kWide) {
         u32x4 raw[kE / kN];
+        auto load = [&](int at) { return *reinterpret_cast<const u32x4*>(static_cast<const char*>(io.logits) + (from + at) * (kType == 2 ? 4 : 2)); };
+        if (n == kPart) {
 #pragma unroll
-        for (int i = 0; i < kE / kN; ++i) {
-            raw[i] = u32x4{0u, 0u, 0u, 0u};
-            const int at = place(i * kN);
-            if (at + kN <= n) raw[i] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(io.logits) + (from + at) * (kType == 2 ? 4 : 2));
-            else
-                for (int e = 0; e < kN && at + e < n; ++e) {
-                    if constexpr (kType == 2) raw[i][e] = __builtin_bit_cast(uint32_t, value<2>(io.logits, from + at + e));
-                    else raw[i][e >> 1] |= (uint32_t)static_cast<const uint16_t*>(io.logits)[from + at + e] << 16 * (e & 1);
-                }
+            for (int i = 0; i < kE / kN; ++i) raw[i] = load(place(i * kN));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kE / kN; ++i) {
+                constexpr uint32_t kNone = kType == 2 ? 0xFF800000u : kType == 1 ? 0xFF80FF80u : 0xFC00FC00u;   // -infinity
+                raw[i] = u32x4{kNone, kNone, kNone, kNone};
+                const int at = place(i * kN);
+                if (at + kN <= n) raw[i] = load(at);
+                else
+                    for (int e = 0; e < kN && at + e < n; ++e) {
+                        if constexpr (kType == 2) raw[i][e] = __builtin_bit_cast(uint32_t, value<2>(io.logits, from + at + e));
+                        else raw[i][e >> 1] = (raw[i][e >> 1] & (e & 1 ? 0xFFFFu : 0xFFFF0000u)) | (uint32_t)static_cast<const uint16_t*>(io.logits)[from + at + e] << 16 * (e & 1);
+                    }
+            }
         }
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
-            float v;
-            if constexpr (kType == 2) v = __builtin_bit_cast(float, (uint32_t)raw[i / kN][i % kN]);
-            else v = ld16<kType == 1>(half_of(raw[i / kN][i % kN >> 1], i));
-            x[i] = place(i) < n ? logit(v) : -__builtin_inff();
+            if constexpr (kType == 2) x[i] = __builtin_bit_cast(float, (uint32_t)raw[i / kN][i % kN]);
+            else x[i] = ld16<kType == 1>(half_of(raw[i / kN][i % kN >> 1], i));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < kE; ++i) x[i] = place(i) < n ? value<kType>(io.logits, from + place(i)) : -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < kE; ++i) x[i] = logit(x[i]);
     }
-    const int slot = slot_of(io.sh, io.cu, r);
+    // (a NaN is no maximum here, equals none, and weighs what -infinity does: fmaxf takes the other number)
+    const int slot = slot_of(io.sh, io.cu, r, mine, begin);
     if (slot < 0) return;
+    const float temp = temperature_of(io, slot);
 #pragma unroll
     for (int i = 0; i < kE; ++i) top = fmaxf(top, x[i]);
     float all = top;
@@ -252,27 +257,31 @@ __global__ __launch_bounds__(kRowThreads) void k_verify_rows(const VerifyIo io) 
             if (x[i] == all) arg = place(i);
         atomicMin(&first, arg);
     }
-    const float temp = temperature_of(io, slot);
     double sum = 0.0;
     if (temp > 0.f && all > -__builtin_inff()) {
         // 2^y as 2^(j / 32) from LDS times 2^f by its interpolation in the Chebyshev nodes of [-1/64, 1/64] (degree 4, within
-        // 8e-14 of itself), where no weight is below e^-690 for it: 11 operations of 64 bits a logit, 18 by Weigh
+        // 8e-14 of itself), where no weight is below e^-690 for it: 9 operations of 64 bits a logit, 18 by Weigh.  32 y is
+        // x scale - top32 for an integer top32, and the sum takes the rest of the top once.
         // (a temperature that the logits' float32 steps do not resolve leaves no such clamp)
         const float lowest = all - 680.f * temp;
-        const double gap = (double)all - (double)lowest;
-        if (all < __builtin_inff() && lowest > -__builtin_inff() && gap >= 600.0 * (double)temp && gap <= 690.0 * (double)temp) {
-            const double top64 = all, scale = 32.0 * scale_of(temp);
-#pragma unroll
-            for (int i = 0; i < kE; ++i) {
-                const double y = ((double)fmaxf(x[i], lowest) - top64) * scale, shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
-                const int n = (int)__builtin_bit_cast(uint64_t, shifted);
+        const double gap = (double)all - (double)lowest, scale = 32.0 * scale_of(temp), top32 = rint((double)all * scale);
+        if (all < __builtin_inff() && lowest > -__builtin_inff() && gap >= 600.0 * (double)temp && gap <= 690.0 * (double)temp &&
+            __builtin_fabs(top32) < 0x1p40) {
+            auto root_of = [](double f) {                            // 2^(f / 32)
                 double r = __builtin_fma(0x1.3b2b1bee88b09p-27, f, 0x1.c6b167e571135p-20);
                 r = __builtin_fma(r, f, 0x1.ebfbdff8131c3p-13);
                 r = __builtin_fma(r, f, 0x1.62e42fef6d01ap-6);
-                r = __builtin_fma(r, f, 1.0);
+                return __builtin_fma(r, f, 1.0);
+            };
+            const double c = 0x1.8p52 - top32;
+#pragma unroll
+            for (int i = 0; i < kE; ++i) {
+                const double v = fmaxf(x[i], lowest), shifted = __builtin_fma(v, scale, c), f = __builtin_fma(v, scale, c - shifted);
+                const int n = (int)__builtin_bit_cast(uint64_t, shifted);
                 const uint64_t bits = __builtin_bit_cast(uint64_t, root[n & 31]) + ((uint64_t)(uint32_t)(n >> 5) << 52);
-                sum = __builtin_fma(__builtin_bit_cast(double, bits), r, sum);
+                sum = __builtin_fma(__builtin_bit_cast(double, bits), root_of(f), sum);
             }
+            sum *= root_of(__builtin_fma(-(double)all, scale, top32));
         } else {
             const Weigh w(all, scale_of(temp));
 #pragma unroll 1
