@@ -59,9 +59,9 @@ __global__ __launch_bounds__(256) void k_draft_tree(const int32_t* parents, cons
 // weights were added, and of so many borders of the cumulated sum one lies within a binary32 rounding of u once in some
 // hundred draws.  The first launch reads all rows, which is little more than a path's where trees are small, and needs no
 // wait between its work-groups.
-// The rows of 16 trees (515 of 151936 float32 logits, 313 MB) take 66-70 us, where reading them takes 49 (11 operations of 64 bits
-// a logit), the walk 16; 32 chains of 187 rows with draft probabilities 33, 8.4, 14.6 (the left sums) and 10; a chain of five 5 and
-// 10.8, which are about seven dependent round trips.
+// The rows of 16 trees (515 of 151936 float32 logits, 313 MB) take 62 us, where reading them takes 49 (18 instructions a logit, nine of
+// them of 64 bits), the walk 16; 32 chains of 187 rows with draft probabilities 29, 8.2, 14.6 (the left sums) and 10; a chain of
+// five 5 and 10.8, which are about seven dependent round trips.
 constexpr int kPart = 4096, kRowThreads = 256, kWalkThreads = 1024, kNear = 256;
 
 struct RowPart {
