@@ -376,10 +376,16 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
             bool bad = false;
             if (n > 0) {
                 bad = c < 0 || c > n || base < 0 || len > cap;
-                for (int i = 0, last = -1; !bad && i < c; ++i) {
-                    const int at = path[first + i];
-                    bad = at <= last || at >= n;
-                    last = at;
+                for (int i = 0, last = -1; !bad && i < c; i += 8) {  // (eight asked for together)
+                    int at[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) at[u] = path[first + min(i + u, c - 1)];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        if (i + u >= c) continue;
+                        bad |= at[u] <= last || at[u] >= n;
+                        last = at[u];
+                    }
                 }
                 if (!bad) held = (len + pt - 1) / pt - base / pt;
             } else {

@@ -5,7 +5,7 @@ Tolerances.  append_rope computes in 64 bits and rounds once, as the reference d
 exact value within 2^-50 of a rounding's border is not to be expected among the 10^6 here), so its rows and what is read back are
 equal.  attend_tree is the arithmetic of PagedKV4.attend, with the bound that test_paged_kv.py derives: half a step of the output
 and LOOSE = 2^-15 of the largest value averaged (the weights' sum is taken from the matrix cores here: two fp16 numbers a
-weight, 22 bits, 2^-22 of the sum, and sums cut by 2^-24 a product: within 2^-15 with the rest).  verify_draft and keep
+weight, cut, 2^-21 of it, their products with a scale within 2^-22 of that or 2^-24: within 2^-15 with the rest).  verify_draft and keep
 return whole numbers and moved bits: equal."""
 import math
 import random
@@ -561,6 +561,30 @@ def test_keep_refuses(hiplib, cuda):
     # a cu that runs backwards names more rows than there are
     p.keep(ints([0] * 6, cuda), ints([0, 0], cuda), ints([0, 6, 0], cuda))
     p.check()
+
+
+def test_keep_many_rows(hiplib, cuda):
+    """Hundreds of kept rows of a slot; one of them out of order, anywhere, refuses the call."""
+    n, before = 700, 50
+    p, _, _ = make(cuda, [before + n, 3], 1, 64, 32, spare=2, width=30)
+    kept = sorted(random.Random(3).sample(range(n), 403))
+    was = p.read(0, before + n + 3, cum([before + n, 3], cuda))
+    cu, counts = cum([n, 1], cuda), ints([len(kept), 1], cuda)
+    state = [t.clone() for t in (p.pages, p.table, p.lens, p.refs)]
+    for i in (1, 7, 8, 200, 402):
+        for value in (kept[i - 1], n, -1):
+            path = kept[:i] + [value] + kept[i + 1:] + [-1] * (n - len(kept)) + [0]
+            p.keep(ints(path, cuda), counts, cu)
+            with pytest.raises(RuntimeError, match=r"bad slot or count \(slot or entry 0\)"):
+                p.check()
+    assert all(torch.equal(a, b) for a, b in zip(state, (p.pages, p.table, p.lens, p.refs)))
+    p.keep(ints(kept + [-1] * (n - len(kept)) + [0], cuda), counts, cu)
+    p.check()
+    lens = [before + len(kept), 3]
+    at = list(range(before)) + [before + j for j in kept] + [before + n + j for j in range(3)]
+    assert p.lens.tolist() == lens
+    for g, w in zip(p.read(0, sum(lens), cum(lens, cuda)), was):
+        assert torch.equal(g, w[at])
 
 
 # ------------------------------------------------------------------------------ together
