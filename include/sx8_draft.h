@@ -42,7 +42,7 @@ int32_t sx8_draft_tree(const int32_t* parents, const int32_t* cu, int64_t n_slot
  * not depend on the order of a sum.
  * path (rows) int32: slot s has the row numbers in the slot of what it keeps, row 0 first, in path[cu[s]] .. , then -1;
  * counts (n_slots) int32: how many (0: no rows); next (n_slots) int64: the token that follows (-1: none).
- * workspace (256-byte aligned, sx8_draft_verify_workspace_bytes, no clearing needed). */
+ * rows up to 2^22, V up to 2^27; workspace (256-byte aligned, sx8_draft_verify_workspace_bytes, no clearing needed). */
 int64_t sx8_draft_verify_workspace_bytes(int64_t n_slots, int64_t rows, int64_t V);
 int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, int32_t dtype, const int64_t* tokens,
                          const int32_t* parents, const int32_t* cu, int64_t n_slots, int64_t rows, int64_t V,

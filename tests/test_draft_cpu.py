@@ -145,7 +145,7 @@ def test_draft_tree_refuses(hiplib, change, word):
 
 
 @pytest.mark.parametrize("change,word", [
-    ({"logits": None}, "null"), ({"next": None}, "null"), ({"path": None}, "null"), ({"V": 0}, "sizes"), ({"V": 1 << 29}, "sizes"),
+    ({"logits": None}, "null"), ({"next": None}, "null"), ({"path": None}, "null"), ({"V": 0}, "sizes"), ({"V": 1 << 29}, "sizes"), ({"V": (1 << 27) + 1}, "sizes"), ({"rows": (1 << 22) + 1}, "sizes"),
     ({"rows": -1}, "sizes"), ({"dtype": 3}, "dtypes"), ({"probs_dtype": -1}, "dtypes"), ({"logits": ODD}, "aligned"), ({"tokens": P(4100)}, "aligned"),
     ({"logits_stride": 99}, "strides"), ({"probs_stride": 99}, "strides"), ({"u": None}, "random"), ({"u": None, "temperature": None, "t": 0.5}, "random"),
     ({"workspace_bytes": 8}, "workspace"), ({"workspace": None}, "workspace")])
