@@ -40,6 +40,9 @@ int32_t sx8_draft_tree(const int32_t* parents, const int32_t* cu, int64_t n_slot
  * A NaN logit counts as -infinity; +infinities share a row between them; a row of -infinities keeps no child and gives no
  * token (-1).  A token outside 0 .. V - 1 is never kept.  Exponentials and sums are held in 64 bits, so that tokens do
  * not depend on the order of a sum.
+ * sx8_draft_verify_within: with depth (rows) int32 as sx8_draft_tree gives it (NULL: as sx8_draft_verify).  A row whose depth is below
+ * zero is no part of its tree: neither sx8_kv4_append_rope nor sx8_kv4_attend_tree knew it, so it is never kept; a slot whose
+ * row 0 is such a row keeps nothing (counts 0, next -1).
  * path (rows) int32: slot s has the row numbers in the slot of what it keeps, row 0 first, in path[cu[s]] .. , then -1;
  * counts (n_slots) int32: how many (0: no rows); next (n_slots) int64: the token that follows (-1: none).
  * rows up to 2^22, V up to 2^27; workspace (256-byte aligned, sx8_draft_verify_workspace_bytes, no clearing needed). */
@@ -49,6 +52,11 @@ int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, int32_t dtyp
                          const float* u, const float* temperature, float t, const void* probs, int64_t probs_stride,
                          int32_t probs_dtype, int32_t* path, int32_t* counts, int64_t* next, void* workspace,
                          int64_t workspace_bytes, void* stream);
+int32_t sx8_draft_verify_within(const void* logits, int64_t logits_stride, int32_t dtype, const int64_t* tokens,
+                                const int32_t* parents, const int32_t* depth, const int32_t* cu, int64_t n_slots, int64_t rows,
+                                int64_t V, const float* u, const float* temperature, float t, const void* probs,
+                                int64_t probs_stride, int32_t probs_dtype, int32_t* path, int32_t* counts, int64_t* next,
+                                void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -43,8 +43,10 @@ extern "C" {
  *    sx8_dec_attn_prefill_packed, sx8_dec_gemm_gateup_silu(_workspace_bytes)
  * 6: sx8_linear_f16, sx8_quant_pca(_workspace_bytes); sx8_dec_attn_workspace_bytes returns the
  *    bytes of 64 chunks (the entry points still run with those of 16)
- * 7: sx8_paged.h: sx8_attn_varlen, sx8_kv4_* */
-#define SX8_ABI_VERSION 8
+ * 7: sx8_paged.h: sx8_attn_varlen, sx8_kv4_*
+ * 8: sx8_draft.h; sx8_kv4_append_rope, sx8_kv4_attend_tree, sx8_kv4_keep
+ * 9: sx8_draft_verify_within */
+#define SX8_ABI_VERSION 9
 
 #define SX8_OK 0
 #define SX8_ERR_INVALID 1      /* bad argument (null pointer, size, hdr_bytes, alignment) */

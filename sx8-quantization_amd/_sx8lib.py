@@ -147,8 +147,10 @@ SIGNATURES = [
     ("sx8_draft_verify_workspace_bytes", _I64, [_I64, _I64, _I64]),
     ("sx8_draft_verify", _I32, [_P, _I64, _I32, _P, _P, _P, _I64, _I64, _I64, _P, _P, ctypes.c_float, _P, _I64, _I32, _P,
                                 _P, _P, _P, _I64, _P]),
+    ("sx8_draft_verify_within", _I32, [_P, _I64, _I32, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, ctypes.c_float, _P, _I64,
+                                       _I32, _P, _P, _P, _P, _I64, _P]),
 ]
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _lib = None
 _py = None

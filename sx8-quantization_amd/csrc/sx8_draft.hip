@@ -87,6 +87,7 @@ struct VerifyIo {
     int parts;                            // of a row
     const float *u, *temperature;
     float t;
+    const int32_t* depth;                 // below zero: the row is no part of its tree (null: all are)
     const void* probs;
     int64_t probs_stride;
     int32_t *path, *counts;
@@ -350,14 +351,17 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
     const float temp = temperature_of(io, slot);                     // (asked for with cu)
     int first, n;
     kv4_rows(io.sh, io.cu, slot, &first, &n);
-    if (n == 0) {
+    // a slot without rows, or whose first one is no part of a tree
+    auto none = [&]() {
+        for (int i = tid; i < n; i += kWalkThreads) io.path[first + i] = -1;
         if (tid == 0) {
             io.counts[slot] = 0;
             io.next[slot] = -1;
             if constexpr (kProbs >= 0) io.wait[slot].open = 0;
         }
-        return;
-    }
+    };
+    if (n == 0) return none();
+    const int root = io.depth ? io.depth[first] : 0;
     // parent, token and uniform of row i0 + lane, the first ones on their way before the sums of rows
     int par = -1;
     int64_t tok = -1;
@@ -370,6 +374,7 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
     };
     if constexpr (!kGoOn) load_rows(0);
     const float u0 = io.u ? io.u[first] : 0.f;
+    if (root < 0) return none();
     const bool greedy = !(temp > 0.f);
     const double scale = greedy ? 0.0 : scale_of(temp);
     // the slot's lists: in LDS where they fit and nobody else reads them
@@ -412,8 +417,9 @@ __global__ __launch_bounds__(kWalkThreads) void k_verify_walk(const VerifyIo io)
         for (int i = tid; i < n; i += kWalkThreads) {
             const int up = i < 64 ? par : io.parents[first + i];
             const int64_t x = i < 64 ? tok : io.tokens[first + i];
+            const int deep = io.depth ? io.depth[first + i] : 0;
             double p = -1.0;
-            if (i > 0 && up >= 0 && up < i && x >= 0 && x < io.V) {
+            if (i > 0 && deep >= 0 && up >= 0 && up < i && x >= 0 && x < io.V) {
                 const RowPart r = whole[up];
                 if (r.top > -__builtin_inff()) {
                     if (greedy) p = x == r.arg;
@@ -667,6 +673,16 @@ extern "C" int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, i
                                     const float* u, const float* temperature, float t, const void* probs,
                                     int64_t probs_stride, int32_t probs_dtype, int32_t* path, int32_t* counts, int64_t* next,
                                     void* workspace, int64_t workspace_bytes, void* stream) {
+    return sx8_draft_verify_within(logits, logits_stride, dtype, tokens, parents, nullptr, cu, n_slots, rows, V, u, temperature, t,
+                                   probs, probs_stride, probs_dtype, path, counts, next, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t sx8_draft_verify_within(const void* logits, int64_t logits_stride, int32_t dtype, const int64_t* tokens,
+                                           const int32_t* parents, const int32_t* depth, const int32_t* cu, int64_t n_slots,
+                                           int64_t rows, int64_t V, const float* u, const float* temperature, float t,
+                                           const void* probs, int64_t probs_stride, int32_t probs_dtype, int32_t* path,
+                                           int32_t* counts, int64_t* next, void* workspace, int64_t workspace_bytes,
+                                           void* stream) {
     using namespace sx8;
     const char* what = "sx8_draft_verify";
     if (!cu || !counts || !next || (rows > 0 && (!logits || !tokens || !parents || !path)))
@@ -676,7 +692,7 @@ extern "C" int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, i
     if (dtype < 0 || dtype > 2 || (probs && (probs_dtype < 0 || probs_dtype > 2)))
         return fail(SX8_ERR_INVALID, "%s: dtypes must be 0 (fp16), 1 (bf16) or 2 (float32)", what);
     const int64_t la = dtype == 2 ? 4 : 2, pa = probs_dtype == 2 ? 4 : 2;
-    if (!aligned(logits, la) || !aligned(tokens, 8) || !aligned(parents, 4) || !aligned(cu, 4) || !aligned(u, 4) ||
+    if (!aligned(logits, la) || !aligned(tokens, 8) || !aligned(parents, 4) || !aligned(depth, 4) || !aligned(cu, 4) || !aligned(u, 4) ||
         !aligned(temperature, 4) || !aligned(probs, pa) || !aligned(path, 4) || !aligned(counts, 4) || !aligned(next, 8))
         return fail(SX8_ERR_INVALID, "%s: pointers must be aligned to their values", what);
     if (logits_stride < V || logits_stride > (int64_t)1 << 40 || (probs && (probs_stride < V || probs_stride > (int64_t)1 << 40)))
@@ -685,7 +701,7 @@ extern "C" int32_t sx8_draft_verify(const void* logits, int64_t logits_stride, i
     if (!workspace || workspace_bytes < verify_ws(n_slots, rows, V) || !aligned(workspace, 256))
         return fail(SX8_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", what, (long long)verify_ws(n_slots, rows, V));
     const int parts = (int)((V + kPart - 1) / kPart);
-    VerifyIo io{logits, logits_stride, tokens, parents, cu, Kv4Shape{(int)n_slots, 1, 1, 0, (int)rows}, V, parts, u, temperature, t,
+    VerifyIo io{logits, logits_stride, tokens, parents, cu, Kv4Shape{(int)n_slots, 1, 1, 0, (int)rows}, V, parts, u, temperature, t, depth,
                 probs, probs_stride, path, counts, next, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     io.part = reinterpret_cast<RowPart*>(workspace);
     io.row = io.part + rows * parts;

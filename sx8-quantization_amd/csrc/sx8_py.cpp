@@ -60,7 +60,7 @@ struct Lib {
     decltype(&sx8_kv4_keep) kv4_keep;
     decltype(&sx8_kv4_keep_workspace_bytes) kv4_keep_ws;
     decltype(&sx8_draft_tree) draft_tree;
-    decltype(&sx8_draft_verify) draft_verify;
+    decltype(&sx8_draft_verify_within) draft_verify;
     decltype(&sx8_draft_verify_workspace_bytes) draft_verify_ws;
 } lib;
 
@@ -153,7 +153,7 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     SX8_BIND(kv4_keep, "sx8_kv4_keep")
     SX8_BIND(kv4_keep_ws, "sx8_kv4_keep_workspace_bytes")
     SX8_BIND(draft_tree, "sx8_draft_tree")
-    SX8_BIND(draft_verify, "sx8_draft_verify")
+    SX8_BIND(draft_verify, "sx8_draft_verify_within")
     SX8_BIND(draft_verify_ws, "sx8_draft_verify_workspace_bytes")
 #undef SX8_BIND
     Py_RETURN_NONE;
@@ -829,11 +829,11 @@ const at::Tensor* matrix(PyObject* o, int32_t* type) {
     return *type < 0 ? nullptr : x;
 }
 
-// draft_verify(logits, tokens, parents, cu, uniforms or None, temperature (a float or a vector), probs or None)
+// draft_verify(logits, tokens, parents, cu, uniforms or None, temperature (a float or a vector), probs or None, depth or None)
 //   -> (path, counts, next)
 PyObject* py_draft_verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
     HANDLE_TH_ERRORS
-    SX8_ARGS(7)
+    SX8_ARGS(8)
     int32_t type = 0, ptype = 0;
     const at::Tensor* x = matrix(a[0], &type);
     if (!x) Py_RETURN_NONE;
@@ -846,6 +846,7 @@ PyObject* py_draft_verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const int64_t slots = cu->numel() - 1;
     bool fits = true;
     const at::Tensor* un = vector_or_none(a[4], at::kFloat, rows, *x, &fits);
+    const at::Tensor* depth = vector_or_none(a[7], at::kInt, rows, *x, &fits);
     const at::Tensor* temp = nullptr;
     float t = 0.f;
     if (PyFloat_Check(a[5])) t = (float)PyFloat_AS_DOUBLE(a[5]);
@@ -864,7 +865,7 @@ PyObject* py_draft_verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
         const int64_t nb = lib.draft_verify_ws(slots, rows, V);
         const at::Tensor ws = empty_like_device({nb > 0 ? nb : 0}, at::kByte, *x);
         rc = lib.draft_verify(x->data_ptr(), x->stride(0), type, tok->data_ptr<int64_t>(), par->data_ptr<int32_t>(),
-                              cu->data_ptr<int32_t>(), slots, rows, V, un ? un->data_ptr<float>() : nullptr,
+                              depth ? depth->data_ptr<int32_t>() : nullptr, cu->data_ptr<int32_t>(), slots, rows, V, un ? un->data_ptr<float>() : nullptr,
                               temp ? temp->data_ptr<float>() : nullptr, t, pr ? pr->data_ptr() : nullptr, pr ? pr->stride(0) : 0,
                               ptype, path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), next.data_ptr<int64_t>(), ws.data_ptr(),
                               nb, stream_of(*x));

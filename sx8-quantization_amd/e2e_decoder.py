@@ -863,7 +863,7 @@ class PagedDecoder:
         pb = self._bufs(ids.numel())
         self._rows(pb, ids, None, attend)
         self.logits = self._head(pb["resid"], pb["d"], ids.numel())
-        path, kept, following = verify_draft(self.logits, ids, par, cu, uniforms, temperature, draft_probs)
+        path, kept, following = verify_draft(self.logits, ids, par, cu, uniforms, temperature, draft_probs, depth)
         self.cache.keep(path, kept, cu)
         kept = kept.tolist()
         self.cache.check()

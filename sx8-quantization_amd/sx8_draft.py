@@ -50,7 +50,7 @@ def _matrix(name, t, rows, vocab, device):
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.clone(memory_format=torch.contiguous_format)
 
 
-def verify_draft(logits, tokens, parents, cu, uniforms=None, temperature=0.0, draft_probs=None):
+def verify_draft(logits, tokens, parents, cu, uniforms=None, temperature=0.0, draft_probs=None, depth=None):
     """Which drafted tokens the target keeps.  logits (rows, vocabulary), fp16, bf16 or float32, are the target's behind each
     row; tokens (rows,) int64; parents and cu as draft_tree takes them; uniforms (rows,) float32 random numbers in [0, 1): a drafted row's
     decides on it, row 0's draws the token that follows; temperature a number or a (slots,) float32 vector.
@@ -63,12 +63,14 @@ def verify_draft(logits, tokens, parents, cu, uniforms=None, temperature=0.0, dr
     max(p - draft_probs, 0), scaled.  Where it is not above zero, tokens are kept while they are the first of the largest
     logits (uniforms may be None if that goes for all slots: a number as temperature).  NaN logits count as
     -infinity; a row of -infinities gives no token.  Sums are held in 64 bits.  Every case is written down in include/sx8_draft.h.
+    depth (rows,) int32, as draft_tree gives it: a row whose depth is below zero (those past its words) is in no cache and was
+    attended by none, so it is never kept, and a slot whose row 0 is one keeps none (counts 0, no token).  A pass over a cache gives it.
 
     Returns path (rows,) int32: the rows that slot s keeps, in path[cu[s]] .. (row 0 first, then -1); counts (slots,) int32: how
     many; and the tokens that follow, (slots,) int64 (-1: none).  PagedKV4.keep takes path and counts.  Outputs have no gradient."""
     if not isinstance(temperature, torch.Tensor):
         temperature = float(temperature)
-    got = _L.py().draft_verify(logits, tokens, parents, cu, uniforms, temperature, draft_probs)
+    got = _L.py().draft_verify(logits, tokens, parents, cu, uniforms, temperature, draft_probs, depth)
     if got is not None:
         return got
     if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda" or logits.dim() != 2:
@@ -82,6 +84,8 @@ def verify_draft(logits, tokens, parents, cu, uniforms=None, temperature=0.0, dr
         if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int64 or tokens.shape != (rows,) \
                 or tokens.device != device or not tokens.is_contiguous() or tokens.is_neg():
             raise RuntimeError(f"tokens must be a contiguous int64 vector of {rows} on {device}")
+        if depth is not None:
+            _ints("depth", depth, rows, device)
         slots = cu.numel() - 1
         temp, number = None, 0.0
         if isinstance(temperature, torch.Tensor):
@@ -97,8 +101,8 @@ def verify_draft(logits, tokens, parents, cu, uniforms=None, temperature=0.0, dr
         following = torch.empty(slots, dtype=torch.int64, device=device)
         nb = int(_L.lib().sx8_draft_verify_workspace_bytes(slots, rows, vocab))
         ws = torch.empty(max(nb, 0), dtype=torch.uint8, device=device)
-        _L.call("sx8_draft_verify", logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], tokens.data_ptr(), parents.data_ptr(),
-                cu.data_ptr(), slots, rows, vocab, _ptr(uniforms), _ptr(temp), number, _ptr(draft_probs),
+        _L.call("sx8_draft_verify_within", logits.data_ptr(), logits.stride(0), _TYPES[logits.dtype], tokens.data_ptr(),
+                parents.data_ptr(), _ptr(depth), cu.data_ptr(), slots, rows, vocab, _ptr(uniforms), _ptr(temp), number, _ptr(draft_probs),
                 0 if draft_probs is None else draft_probs.stride(0), 0 if draft_probs is None else _TYPES[draft_probs.dtype],
                 path.data_ptr(), counts.data_ptr(), following.data_ptr(), ws.data_ptr(), nb, _L.stream(device))
     return path, counts, following

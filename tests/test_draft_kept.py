@@ -1,0 +1,109 @@
+"""What a pass over drafted tokens may leave in the cache: only rows whose K and V were written there.  Whole numbers and moved
+bits: equal."""
+import random
+
+import pytest
+import torch
+
+from test_draft import F32, drafts, flat, run_verify, tables, trees, turn
+from test_paged_kv import F16, cum, ints, make, q4, rand
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------ rows that are no part of a tree
+def without(ps, dead):
+    """The trees with the rows of `dead` as no one's children."""
+    return [[-1 if (s, i) in dead else p for i, p in enumerate(tree)] for s, tree in enumerate(ps)]
+
+
+@pytest.mark.parametrize("words", [1, 2, 4])
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("dt", [F32, F16])
+def test_rows_past_the_words_are_not_kept(hiplib, cuda, words, probs, dt):
+    """Trees and chains with rows past the masks' words, greedy and drawn: the verification that knows the depths keeps what
+    it would if these rows followed none, and never one of them."""
+    from sx8_draft import draft_tree, verify_draft
+    ns, V = [70, 64, 3, 140, 0, 300, 65], 50
+    logits, ps, tokens, u, pr = drafts(cuda, ns, V, words, dt, probs=probs)
+    ps[0], ps[6] = trees([70], 0, chain=True)[0], trees([65], 0, chain=True)[0]
+    u = [0.0 if random.Random(i).random() < 0.9 else x for i, x in enumerate(u)]      # (most tokens are kept)
+    temp = [1.0, 0.0, 0.7, 1.3, 1.0, 0.9, 1.0]
+    cu, parents = cum(ns, cuda), ints(flat(ps), cuda)
+    _, depth = draft_tree(parents, cu, words)
+    dead = {(s, i) for s, n in enumerate(ns) for i in range(64 * words, n)}
+    assert (depth < 0).sum() == len(dead)
+    want = run_verify(cuda, logits, without(ps, dead), tokens, u, temp, pr)
+    args = (logits, torch.tensor(tokens, device=cuda), parents, cu, torch.tensor(u, dtype=F32, device=cuda), torch.tensor(temp, device=cuda), pr)
+    got = verify_draft(*args, depth=depth)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert got[0].max().item() < 64 * words
+    # every first child kept: the chains up to their masks' last row
+    u = [0.0] * len(u)
+    want = run_verify(cuda, logits, without(ps, dead), tokens, u, [1.0] * 7, pr)
+    got = verify_draft(*args[:4], torch.zeros(len(u), device=cuda), 1.0, pr, depth=depth)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert [got[1][s].item() for s in (0, 6)] == [min(70, 64 * words), min(65, 64 * words)]
+    # all rows are part of their trees: as without depths
+    _, depth = draft_tree(ints(flat(trees(ns, 3)), cuda), cu, 4)
+    if words == 4:
+        args = (*args[:2], ints([p if i < 256 else -1 for t in ps for i, p in enumerate(t)], cuda), *args[3:])
+        assert all(torch.equal(a, b) for a, b in zip(verify_draft(*args, depth=depth), verify_draft(*args)))
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("temp", [0.0, 0.9])
+@pytest.mark.parametrize("general", [False, True])
+def test_slots_whose_first_row_is_no_part(hiplib, cuda, monkeypatch, probs, temp, general):
+    """Such a slot keeps nothing and has no token; its neighbours are as they were; scattered rows without a place."""
+    import _sx8lib
+    from sx8_draft import verify_draft
+    if general:
+        monkeypatch.setattr(_sx8lib, "_py", _sx8lib._NoHostModule())
+    ns = [5, 1, 300, 7, 0, 20]
+    logits, ps, tokens, u, pr = drafts(cuda, ns, 33, 4, probs=probs)
+    u = [x / 3 for x in u]
+    dead = {(1, 0), (3, 0), (2, 7), (2, 280), (5, 1), (0, 3)}
+    starts = cum(ns, cuda).tolist()
+    depth = torch.zeros(sum(ns), dtype=torch.int32)
+    for s, i in dead:
+        depth[starts[s] + i] = -1 - s
+    want = run_verify(cuda, logits, without(ps, dead), tokens, u, [temp] * 6, pr)
+    got = verify_draft(logits, torch.tensor(tokens, device=cuda), ints(flat(ps), cuda), cum(ns, cuda), torch.tensor(u, dtype=F32, device=cuda),
+                       temp, pr, depth=depth.to(cuda))
+    for s in range(6):
+        rows = slice(starts[s], starts[s + 1])
+        if s in (1, 3):
+            assert got[1][s] == 0 and got[2][s] == -1 and (got[0][rows] == -1).all()
+        else:
+            assert all(torch.equal(a, b) for a, b in ((got[0][rows], want[0][rows]), (got[1][s], want[1][s]), (got[2][s], want[2][s])))
+    for bad in (depth, depth.to(cuda).long(), depth[1:].to(cuda), torch._neg_view(depth.to(cuda)), [0] * sum(ns)):
+        with pytest.raises(RuntimeError, match="depth"):
+            verify_draft(logits, torch.tensor(tokens, device=cuda), ints(flat(ps), cuda), cum(ns, cuda), torch.tensor(u, dtype=F32, device=cuda),
+                         temp, pr, depth=bad)
+
+
+@pytest.mark.parametrize("words,kept", [(1, 64), (2, 70)])
+def test_round_of_a_long_chain(hiplib, cuda, words, kept):
+    """A chain of 70 tokens, all of them to be kept, through a whole pass: with masks of one word 64 are, and every token of
+    the cache is one that was written."""
+    from sx8_draft import draft_tree, verify_draft
+    new, before = [70, 2], [40, 7]
+    p, k0, v0 = make(cuda, before, 2, 64, 32, spare=8, width=8)
+    cos, sin = tables(200, 64, cuda)
+    cu, parents = cum(new, cuda), ints([*range(-1, 69), -1, 0], cuda)
+    p.reserve(ints(new, cuda))
+    q, k, v = (rand((72, n, 64), 30 + i, F16, cuda) for i, n in enumerate((4, 2, 2)))
+    mask, depth = draft_tree(parents, cu, words)
+    qr = p.append_rope(0, q, k, v, cos, sin, cu, depth=depth)
+    p.attend_tree(0, qr, mask, cu)
+    logits = torch.randn(72, 30, generator=torch.Generator().manual_seed(1)).to(cuda)
+    tokens = torch.arange(72, device=cuda) % 30
+    path, counts, following = verify_draft(logits, tokens, parents, cu, torch.zeros(72, device=cuda), 1.0, depth=depth)
+    p.keep(path, counts, cu)
+    p.check()
+    assert counts.tolist() == [kept, 2] and p.lens.tolist() == [40 + kept, 9] and (following >= 0).all()
+    place = list(range(40, 40 + kept))
+    kk = torch.cat([k0[:40], turn(k[:kept], None, cos[place], sin[place], False).float().half()])
+    got = p.read(0, 40 + kept + 9, cum(p.lens.tolist(), cuda))
+    assert torch.equal(got[0][:40 + kept], q4(kk).half()) and torch.equal(got[1][:40 + kept], q4(torch.cat([v0[:40], v[:kept]])).half())
