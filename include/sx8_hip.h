@@ -45,7 +45,7 @@ extern "C" {
  *    bytes of 64 chunks (the entry points still run with those of 16)
  * 7: sx8_paged.h: sx8_attn_varlen, sx8_kv4_*
  * 8: sx8_draft.h; sx8_kv4_append_rope, sx8_kv4_attend_tree, sx8_kv4_keep
- * 9: sx8_draft_verify_within */
+ * 9: sx8_draft_verify_within; sx8_kv4_reserve_marked, sx8_kv4_append_rope_marked, sx8_kv4_keep_marked */
 #define SX8_ABI_VERSION 9
 
 #define SX8_OK 0

@@ -100,6 +100,15 @@ int32_t sx8_kv4_append_rope(uint8_t* pages, const int32_t* table, const int32_t*
                             int32_t interleaved, const int32_t* depth, const void* q_norm, const void* k_norm, double eps,
                             int32_t in_dtype, int32_t dtype, void* stream);
 
+int32_t sx8_kv4_append_rope_marked(uint8_t* pages, const int32_t* table, const int32_t* lens, const int32_t* cu,
+                                   int64_t n_slots, int64_t max_pages, int64_t n_pages, const void* q, const void* k,
+                                   const void* v, void* out, int64_t rows, int64_t q_ts, int64_t q_hs, int64_t k_ts,
+                                   int64_t k_hs, int64_t v_ts, int64_t v_hs, int64_t o_ts, int64_t o_hs, int32_t nh, int32_t nk,
+                                   int32_t hd, int32_t page_tokens, const float* cos_t, const float* sin_t,
+                                   int64_t table_rows, int32_t rot, int32_t interleaved, const int32_t* depth, int32_t* marks,
+                                   const void* q_norm, const void* k_norm, double eps, int32_t in_dtype, int32_t dtype,
+                                   void* stream);
+
 /* sx8_kv4_attend where the new rows form a tree: row i of a slot's n attends the lens - n tokens before them and those new rows
  * j whose bit (j % 64 of word j / 64) is set in mask (rows, words) uint64, words 1..4; new rows from 64 words on are attended by
  * none.  A row that attends nothing gives zeros.  out shares no memory with q.  Two launches; workspace:
@@ -117,6 +126,9 @@ int64_t sx8_kv4_attend_tree_workspace_bytes(int32_t hd);
  * is in use, named twice or a source.  workspace: sx8_kv4_pages_workspace_bytes bytes, 16-byte aligned.
  *
  * reserve: slot s grows by add[s] >= 0 tokens (lens[s] += add[s]), its new pages with one reference.
+ * *_marked: with marks (n_slots) int32, 2^31 - 1 at first (NULL: as without).  A refused reserve sets the marks of the slots with
+ *   add[s] != 0 to -1, one that is done sets them to 2^31 - 1.  For a slot whose mark is -1, append_rope gives zeros and writes no
+ *   page, and keep leaves all of it as it is: a pass that nobody checks in between cannot harm older tokens.
  * fork: for n entries, the empty slot dst[i] becomes a copy of slot src[i]: full pages are shared, a last page that is
  *   partly filled is copied (every layer: pages of layer l at pages + l * n_pages * page_bytes).
  * free: the slots' pages lose a reference, their rows become -1 and their lengths 0.  A slot named twice is freed
@@ -133,10 +145,17 @@ int32_t sx8_kv4_keep(uint8_t* pages, int64_t n_layers, int32_t* table, int32_t* 
                      const int32_t* path, const int32_t* counts, int64_t rows, int64_t n_slots, int64_t max_pages,
                      int64_t n_pages, int32_t nk, int32_t hd, int32_t page_tokens, int32_t* status, void* workspace,
                      int64_t workspace_bytes, void* stream);
+int32_t sx8_kv4_keep_marked(uint8_t* pages, int64_t n_layers, int32_t* table, int32_t* lens, int32_t* refs,
+                            const int32_t* cu, const int32_t* path, const int32_t* counts, int64_t rows, int64_t n_slots,
+                            int64_t max_pages, int64_t n_pages, int32_t nk, int32_t hd, int32_t page_tokens,
+                            int32_t* status, int32_t* marks, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t sx8_kv4_pages_workspace_bytes(int64_t n_slots, int64_t n_pages);
 int32_t sx8_kv4_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* add, int64_t n_slots,
                         int64_t max_pages, int64_t n_pages, int32_t page_tokens, int32_t* status, void* workspace,
                         int64_t workspace_bytes, void* stream);
+int32_t sx8_kv4_reserve_marked(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* add, int64_t n_slots,
+                               int64_t max_pages, int64_t n_pages, int32_t page_tokens, int32_t* status, int32_t* marks,
+                               void* workspace, int64_t workspace_bytes, void* stream);
 int32_t sx8_kv4_fork(uint8_t* pages, int64_t n_layers, int64_t page_bytes, int32_t* table, int32_t* lens, int32_t* refs,
                      const int32_t* src, const int32_t* dst, int64_t n, int64_t n_slots, int64_t max_pages,
                      int64_t n_pages, int32_t page_tokens, int32_t* status, void* workspace, int64_t workspace_bytes,

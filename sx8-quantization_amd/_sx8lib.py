@@ -132,16 +132,22 @@ SIGNATURES = [
     ("sx8_kv4_append_rope", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
                                    _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _I32, _I32, _P, _P, _P,
                                    ctypes.c_double, _I32, _I32, _P]),
+    ("sx8_kv4_append_rope_marked", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+                                          _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P,
+                                          ctypes.c_double, _I32, _I32, _P]),
     ("sx8_kv4_attend_tree", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I32, _I32,
                                    _I32, _I32, _I32, ctypes.c_float, _I32, _P, _I64, _P]),
     ("sx8_kv4_attend_tree_workspace_bytes", _I64, [_I32]),
     ("sx8_kv4_pages_workspace_bytes", _I64, [_I64, _I64]),
     ("sx8_kv4_reserve", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P, _P, _I64, _P]),
+    ("sx8_kv4_reserve_marked", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _P]),
     ("sx8_kv4_fork", _I32, [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _I64, _P]),
     ("sx8_kv4_free", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P]),
     ("sx8_kv4_compact", _I32, [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),
     ("sx8_kv4_keep_workspace_bytes", _I64, [_I64, _I64]),
     ("sx8_kv4_keep", _I32, [_P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _I64, _P]),
+    ("sx8_kv4_keep_marked", _I32, [_P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P,
+                                   _I64, _P]),
     # include/sx8_draft.h
     ("sx8_draft_tree", _I32, [_P, _P, _I64, _I64, _I32, _P, _P, _P]),
     ("sx8_draft_verify_workspace_bytes", _I64, [_I64, _I64, _I64]),

@@ -21,6 +21,7 @@ struct RopeIn {
     const float *cos, *sin;
     int64_t table_rows;
     const int32_t* depth;
+    const int32_t* marks;                   // of a slot: below zero, its reservation was refused (null: none was)
     const uint16_t *qw, *kw;
     double eps;
     int rot, heads;                         // heads: query heads of a work-group
@@ -122,9 +123,11 @@ __global__ __launch_bounds__(256) void k_kv4_append_rope(const Kv4Pool p, const 
     Touched t;
     if (!find_touched(p, blockIdx.x, pre, &t)) return;
     const int head = blockIdx.y, tid = threadIdx.x, nt = t.t1 - t.t0, half = in.rot / 2;
+    // (the last tokens of a slot that was refused its new ones are older: nothing of it may be overwritten)
+    const bool refused = in.marks && in.marks[t.slot] < 0;
     if (tid < nt) {
         const int64_t at = in.depth ? (int64_t)t.first + in.depth[t.row0 + tid] : (int64_t)t.block * 32 + t.t0 + tid;
-        place[t.t0 + tid] = at >= 0 && at < in.table_rows ? (int)at : -1;
+        place[t.t0 + tid] = !refused && at >= 0 && at < in.table_rows ? (int)at : -1;
     }
     __syncthreads();
     if (head >= p.sh.nk) {
@@ -216,6 +219,19 @@ extern "C" int32_t sx8_kv4_append_rope(uint8_t* pages, const int32_t* table, con
                                        int64_t table_rows, int32_t rot, int32_t interleaved, const int32_t* depth,
                                        const void* q_norm, const void* k_norm, double eps, int32_t in_dtype, int32_t dtype,
                                        void* stream) {
+    return sx8_kv4_append_rope_marked(pages, table, lens, cu, n_slots, max_pages, n_pages, q, k, v, out, rows, q_ts, q_hs, k_ts,
+                                      k_hs, v_ts, v_hs, o_ts, o_hs, nh, nk, hd, page_tokens, cos_t, sin_t, table_rows, rot,
+                                      interleaved, depth, nullptr, q_norm, k_norm, eps, in_dtype, dtype, stream);
+}
+
+extern "C" int32_t sx8_kv4_append_rope_marked(uint8_t* pages, const int32_t* table, const int32_t* lens, const int32_t* cu,
+                                              int64_t n_slots, int64_t max_pages, int64_t n_pages, const void* q, const void* k,
+                                              const void* v, void* out, int64_t rows, int64_t q_ts, int64_t q_hs, int64_t k_ts,
+                                              int64_t k_hs, int64_t v_ts, int64_t v_hs, int64_t o_ts, int64_t o_hs, int32_t nh,
+                                              int32_t nk, int32_t hd, int32_t page_tokens, const float* cos_t,
+                                              const float* sin_t, int64_t table_rows, int32_t rot, int32_t interleaved,
+                                              const int32_t* depth, int32_t* marks, const void* q_norm, const void* k_norm,
+                                              double eps, int32_t in_dtype, int32_t dtype, void* stream) {
     using namespace sx8;
     const char* what = "sx8_kv4_append_rope";
     Kv4Pool p;
@@ -234,8 +250,8 @@ extern "C" int32_t sx8_kv4_append_rope(uint8_t* pages, const int32_t* table, con
     if (!cos_t || !sin_t || !aligned(cos_t, 16) || !aligned(sin_t, 16) || table_rows <= 0 || table_rows > 0x7FFFFFFF)
         return fail(SX8_ERR_INVALID, "%s: cos and sin must be tables of 1..2^31 - 1 rows, 16-byte aligned", what);
     if (rot < 16 || rot > hd || rot % 16) return fail(SX8_ERR_INVALID, "%s: rot must be a multiple of 16 up to hd", what);
-    if (!aligned(depth, 4) || !aligned(q_norm, 16) || !aligned(k_norm, 16))
-        return fail(SX8_ERR_INVALID, "%s: depth must be 4-byte aligned, q_norm and k_norm 16-byte", what);
+    if (!aligned(depth, 4) || !aligned(marks, 4) || !aligned(q_norm, 16) || !aligned(k_norm, 16))
+        return fail(SX8_ERR_INVALID, "%s: depth and marks must be 4-byte aligned, q_norm and k_norm 16-byte", what);
     if (!(eps >= 0.0) || !(eps < __builtin_inff())) return fail(SX8_ERR_INVALID, "%s: eps must not be negative", what);
     if (out == q && rows > 0) return fail(SX8_ERR_INVALID, "%s: out may not be q", what);
     if (rows == 0) return ok();
@@ -244,7 +260,7 @@ extern "C" int32_t sx8_kv4_append_rope(uint8_t* pages, const int32_t* table, con
     // 32 heads of 128, one a slot: 6.7 us with four heads, 9.7 with one; 9761 rows of nine prompts: 48 and 44).
     const int64_t in_block = cu ? (rows + n_slots - 1) / n_slots : 1;
     const int fit = (int)(256 / ((in_block < 32 ? in_block : 32) * (hd / 8))), heads = fit < 1 ? 1 : fit > p.sh.G ? p.sh.G : fit;
-    const RopeIn in{q, k, v, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, (uint16_t*)out, o_ts, o_hs, cos_t, sin_t, table_rows, depth,
+    const RopeIn in{q, k, v, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, (uint16_t*)out, o_ts, o_hs, cos_t, sin_t, table_rows, depth, marks,
                     (const uint16_t*)q_norm, (const uint16_t*)k_norm, eps, rot, heads};
     const dim3 grid((unsigned)kv4_touched_most(n_slots, rows, cu != nullptr), (unsigned)(nk + nk * ((p.sh.G + heads - 1) / heads)));
     by_kind(hd, dtype, [&](auto d, auto b) {

@@ -108,7 +108,9 @@ __device__ __forceinline__ void report(int32_t* status, int code, int item) {
 }
 
 // ---- reserve -----------------------------------------------------------------------------------
-__global__ __launch_bounds__(kPageThreads) void k_reserve(const PageTab t, const int32_t* add, const PageWs ws) {
+constexpr int32_t kAllRows = 0x7FFFFFFF, kRefused = -1;              // a slot's mark (include/sx8_paged.h)
+
+__global__ __launch_bounds__(kPageThreads) void k_reserve(const PageTab t, const int32_t* add, const PageWs ws, int32_t* marks) {
     const int tid = threadIdx.x, pt = t.page_tokens;
     const int64_t cap = (int64_t)t.max_pages * pt;
     int total = 0, code = 0, item = 0;
@@ -136,6 +138,9 @@ __global__ __launch_bounds__(kPageThreads) void k_reserve(const PageTab t, const
     }
     if (code) {
         report(t.status, code, item);
+        if (marks)
+            for (int s = tid; s < t.n_slots; s += kPageThreads)
+                if (add[s] != 0) marks[s] = kRefused;
         return;
     }
     for (int s = tid; s < t.n_slots; s += kPageThreads) {
@@ -147,7 +152,10 @@ __global__ __launch_bounds__(kPageThreads) void k_reserve(const PageTab t, const
             t.table[(int64_t)s * t.max_pages + i] = page;
             t.refs[page] = 1;
         }
-        if (a) t.lens[s] = len + a;
+        if (a) {
+            t.lens[s] = len + a;
+            if (marks) marks[s] = kAllRows;
+        }
     }
 }
 
@@ -360,9 +368,10 @@ KeepWs keep_ws(void* w, int64_t n_slots) {
     return KeepWs{b, b + 4, b + 4 + n_slots, b + 4 + 2 * n_slots};
 }
 
-// A slot of n new rows keeps rows path[0] < path[1] < .. (counts of them) of these.
+// A slot of n new rows keeps rows path[0] < path[1] < .. (counts of them) of these.  A slot that its reservation was refused
+// has none (its last n tokens are older ones): it is passed over.
 __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const int32_t* path, const int32_t* counts,
-                                                       const int32_t* cu, Kv4Shape sh, const KeepWs ws) {
+                                                       const int32_t* cu, Kv4Shape sh, const KeepWs ws, const int32_t* marks) {
     const int tid = threadIdx.x, pt = t.page_tokens;
     const int64_t cap = (int64_t)t.max_pages * pt;
     int code = 0, item = 0, total = 0;
@@ -373,8 +382,11 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
             int first, n;
             kv4_rows(sh, cu, s, &first, &n);
             const int len = t.lens[s], c = counts[s], base = len - n;
+            const bool refused = n > 0 && marks && marks[s] < 0;
             bool bad = false;
-            if (n > 0) {
+            if (refused) {
+                n = 0;
+            } else if (n > 0) {
                 bad = c < 0 || c > n || base < 0 || len > cap;
                 for (int i = 0, last = -1; !bad && i < c; i += 8) {  // (eight asked for together)
                     int at[8];
@@ -444,7 +456,7 @@ __global__ __launch_bounds__(256) void k_keep_move(uint8_t* pages, const int32_t
     const int s = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
     int first, n;
     kv4_rows(sh, cu, s, &first, &n);
-    if (n == 0 || ws.head[0] == 0) return;
+    if (n == 0 || ws.head[0] == 0 || ws.base[s] < 0) return;
     const int c = counts[s];
     if (c == 0 || path[first + c - 1] == c - 1) return;              // (they lie together already)
     const int base = ws.base[s], bpp = page_tokens / 32;
@@ -552,6 +564,13 @@ extern "C" int64_t sx8_kv4_pages_workspace_bytes(int64_t n_slots, int64_t n_page
 extern "C" int32_t sx8_kv4_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* add, int64_t n_slots,
                                    int64_t max_pages, int64_t n_pages, int32_t page_tokens, int32_t* status,
                                    void* workspace, int64_t workspace_bytes, void* stream) {
+    return sx8_kv4_reserve_marked(table, lens, refs, add, n_slots, max_pages, n_pages, page_tokens, status, nullptr, workspace,
+                                  workspace_bytes, stream);
+}
+
+extern "C" int32_t sx8_kv4_reserve_marked(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* add, int64_t n_slots,
+                                          int64_t max_pages, int64_t n_pages, int32_t page_tokens, int32_t* status,
+                                          int32_t* marks, void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace sx8;
     const char* what = "sx8_kv4_reserve";
     if (!lens || !add || !status) return fail(SX8_ERR_INVALID, "%s: null pointer", what);
@@ -559,7 +578,8 @@ extern "C" int32_t sx8_kv4_reserve(int32_t* table, int32_t* lens, int32_t* refs,
     int32_t rc = make_tab(what, &t, table, lens, refs, n_slots, max_pages, n_pages, page_tokens, status);
     if (rc == SX8_OK) rc = check_ws(what, workspace, workspace_bytes, n_slots, n_pages);
     if (rc != SX8_OK) return rc;
-    hipLaunchKernelGGL(k_reserve, dim3(1), dim3(kPageThreads), 0, as_stream(stream), t, add, page_ws(workspace, n_pages));
+    if (!aligned(marks, 4)) return fail(SX8_ERR_INVALID, "%s: marks must be 4-byte aligned", what);
+    hipLaunchKernelGGL(k_reserve, dim3(1), dim3(kPageThreads), 0, as_stream(stream), t, add, page_ws(workspace, n_pages), marks);
     return check_launch(what);
 }
 
@@ -630,6 +650,15 @@ extern "C" int32_t sx8_kv4_keep(uint8_t* pages, int64_t n_layers, int32_t* table
                                 const int32_t* cu, const int32_t* path, const int32_t* counts, int64_t rows, int64_t n_slots,
                                 int64_t max_pages, int64_t n_pages, int32_t nk, int32_t hd, int32_t page_tokens,
                                 int32_t* status, void* workspace, int64_t workspace_bytes, void* stream) {
+    return sx8_kv4_keep_marked(pages, n_layers, table, lens, refs, cu, path, counts, rows, n_slots, max_pages, n_pages, nk, hd,
+                               page_tokens, status, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t sx8_kv4_keep_marked(uint8_t* pages, int64_t n_layers, int32_t* table, int32_t* lens, int32_t* refs,
+                                       const int32_t* cu, const int32_t* path, const int32_t* counts, int64_t rows,
+                                       int64_t n_slots, int64_t max_pages, int64_t n_pages, int32_t nk, int32_t hd,
+                                       int32_t page_tokens, int32_t* status, int32_t* marks, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
     using namespace sx8;
     const char* what = "sx8_kv4_keep";
     if (!lens || !status || !counts || (!path && rows > 0)) return fail(SX8_ERR_INVALID, "%s: null pointer", what);
@@ -642,14 +671,14 @@ extern "C" int32_t sx8_kv4_keep(uint8_t* pages, int64_t n_layers, int32_t* table
     if (rc != SX8_OK) return rc;
     if (rows < 0 || rows > 0x7FFFFFFF || (!cu && rows != n_slots))
         return fail(SX8_ERR_INVALID, "%s: bad rows (without cu one row a slot)", what);
-    if (!aligned(cu, 4) || !aligned(path, 4) || !aligned(counts, 4))
-        return fail(SX8_ERR_INVALID, "%s: cu, path and counts must be 4-byte aligned", what);
+    if (!aligned(cu, 4) || !aligned(path, 4) || !aligned(counts, 4) || !aligned(marks, 4))
+        return fail(SX8_ERR_INVALID, "%s: cu, path, counts and marks must be 4-byte aligned", what);
     if (!workspace || workspace_bytes < keep_ws_bytes(n_slots, rows) || !aligned(workspace, 16))
         return fail(SX8_ERR_INVALID, "%s: workspace needs %lld bytes, 16-byte aligned", what, (long long)keep_ws_bytes(n_slots, rows));
     if (rows == 0) return ok();
     const Kv4Shape sh{(int)n_slots, nk, 1, (int)(max_pages * page_tokens), (int)rows};
     const KeepWs ws = keep_ws(workspace, n_slots);
-    hipLaunchKernelGGL(k_keep, dim3(1), dim3(kPageThreads), 0, as_stream(stream), t, path, counts, cu, sh, ws);
+    hipLaunchKernelGGL(k_keep, dim3(1), dim3(kPageThreads), 0, as_stream(stream), t, path, counts, cu, sh, ws, marks);
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)n_slots, (unsigned)nk, (unsigned)n_layers), dim3(256), 0, as_stream(stream),
                            pages, path, counts, cu, sh, page_tokens, n_pages, pb, ws);

@@ -51,13 +51,13 @@ struct Lib {
     decltype(&sx8_kv4_append) kv4_append;
     decltype(&sx8_kv4_read) kv4_read;
     decltype(&sx8_kv4_attend) kv4_attend;
-    decltype(&sx8_kv4_reserve) kv4_reserve;
+    decltype(&sx8_kv4_reserve_marked) kv4_reserve;
     decltype(&sx8_kv4_fork) kv4_fork;
     decltype(&sx8_kv4_free) kv4_free;
     decltype(&sx8_kv4_compact) kv4_compact;
-    decltype(&sx8_kv4_append_rope) kv4_append_rope;
+    decltype(&sx8_kv4_append_rope_marked) kv4_append_rope;
     decltype(&sx8_kv4_attend_tree) kv4_attend_tree;
-    decltype(&sx8_kv4_keep) kv4_keep;
+    decltype(&sx8_kv4_keep_marked) kv4_keep;
     decltype(&sx8_kv4_keep_workspace_bytes) kv4_keep_ws;
     decltype(&sx8_draft_tree) draft_tree;
     decltype(&sx8_draft_verify_within) draft_verify;
@@ -144,13 +144,13 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     SX8_BIND(kv4_append, "sx8_kv4_append")
     SX8_BIND(kv4_read, "sx8_kv4_read")
     SX8_BIND(kv4_attend, "sx8_kv4_attend")
-    SX8_BIND(kv4_reserve, "sx8_kv4_reserve")
+    SX8_BIND(kv4_reserve, "sx8_kv4_reserve_marked")
     SX8_BIND(kv4_fork, "sx8_kv4_fork")
     SX8_BIND(kv4_free, "sx8_kv4_free")
     SX8_BIND(kv4_compact, "sx8_kv4_compact")
-    SX8_BIND(kv4_append_rope, "sx8_kv4_append_rope")
+    SX8_BIND(kv4_append_rope, "sx8_kv4_append_rope_marked")
     SX8_BIND(kv4_attend_tree, "sx8_kv4_attend_tree")
-    SX8_BIND(kv4_keep, "sx8_kv4_keep")
+    SX8_BIND(kv4_keep, "sx8_kv4_keep_marked")
     SX8_BIND(kv4_keep_ws, "sx8_kv4_keep_workspace_bytes")
     SX8_BIND(draft_tree, "sx8_draft_tree")
     SX8_BIND(draft_verify, "sx8_draft_verify_within")
@@ -496,9 +496,9 @@ PyObject* py_varlen(PyObject*, PyObject* const* a, Py_ssize_t na) {
 }
 
 // What PagedKV4 keeps for these calls: (pages, table, lens, refs, status, page_bytes, n_kv, head_dim, page_tokens,
-// bytes of attend's workspace, of the page operations', of attend_tree's); the wrapper checked it.
+// bytes of attend's workspace, of the page operations', of attend_tree's, marks); the wrapper checked it.
 struct Cache {
-    const at::Tensor *pages, *table, *lens, *refs, *status;
+    const at::Tensor *pages, *table, *lens, *refs, *status, *marks;
     int64_t layers, n_pages, slots, width, page_bytes, ws_attend, ws_pages, ws_tree;
     int32_t nk, hd, pt;
     void* stream;
@@ -506,10 +506,10 @@ struct Cache {
     uint8_t* layer(int64_t i) const { return pages->data_ptr<uint8_t>() + i * n_pages * page_bytes; }
 };
 bool cache(PyObject* o, Cache* c) {
-    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 12) return false;
-    const at::Tensor** t[5] = {&c->pages, &c->table, &c->lens, &c->refs, &c->status};
-    for (int i = 0; i < 5; ++i)
-        if (!(*t[i] = plain(PyTuple_GET_ITEM(o, i)))) return false;
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 13) return false;
+    const at::Tensor** t[6] = {&c->pages, &c->table, &c->lens, &c->refs, &c->status, &c->marks};
+    for (int i = 0; i < 6; ++i)
+        if (!(*t[i] = plain(PyTuple_GET_ITEM(o, i < 5 ? i : 12)))) return false;
     int64_t n[7];
     for (int i = 0; i < 7; ++i) n[i] = num(PyTuple_GET_ITEM(o, 5 + i));
     c->page_bytes = n[0];
@@ -648,7 +648,8 @@ PyObject* py_kv4_pages(PyObject*, PyObject* const* a, Py_ssize_t na) {
         int32_t *const table = c.ints(c.table), *const lens = c.ints(c.lens), *const refs = c.ints(c.refs),
                        *const status = c.ints(c.status);
         if (!std::strcmp(what, "reserve") && na == 3)
-            rc = lib.kv4_reserve(table, lens, refs, c.ints(x), c.slots, c.width, c.n_pages, c.pt, status, w, c.ws_pages, c.stream);
+            rc = lib.kv4_reserve(table, lens, refs, c.ints(x), c.slots, c.width, c.n_pages, c.pt, status, c.ints(c.marks), w,
+                                 c.ws_pages, c.stream);
         else if (!std::strcmp(what, "fork") && na == 4)
             rc = lib.kv4_fork(c.layer(0), c.layers, c.page_bytes, table, lens, refs, c.ints(x), c.ints(y), x->numel(), c.slots,
                               c.width, c.n_pages, c.pt, status, w, c.ws_pages, c.stream);
@@ -729,7 +730,7 @@ PyObject* py_kv4_append_rope(PyObject*, PyObject* const* a, Py_ssize_t na) {
                                  k->data_ptr(), v->data_ptr(), o.data_ptr(), q->size(0), q->stride(0), q->stride(1), k->stride(0),
                                  k->stride(1), v->stride(0), v->stride(1), o.stride(0), o.stride(1), (int32_t)q->size(1), c.nk,
                                  c.hd, c.pt, cs->data_ptr<float>(), sn->data_ptr<float>(), cs->size(0),
-                                 (int32_t)(2 * cs->size(1)), a[12] == Py_True, depth ? depth->data_ptr<int32_t>() : nullptr,
+                                 (int32_t)(2 * cs->size(1)), a[12] == Py_True, depth ? depth->data_ptr<int32_t>() : nullptr, c.ints(c.marks),
                                  qw ? qw->data_ptr() : nullptr, kw ? kw->data_ptr() : nullptr, eps, wide ? 2 : bf, bf, c.stream);
     }
     if (rc) return failed("sx8_kv4_append_rope", rc);
@@ -786,7 +787,7 @@ PyObject* py_kv4_keep(PyObject*, PyObject* const* a, Py_ssize_t na) {
         const at::Tensor ws = empty_like_device({nb > 0 ? nb : 0}, at::kByte, *c.pages);
         rc = lib.kv4_keep(c.layer(0), c.layers, c.ints(c.table), c.ints(c.lens), c.ints(c.refs), cu ? c.ints(cu) : nullptr,
                           c.ints(path), c.ints(counts), path->numel(), c.slots, c.width, c.n_pages, c.nk, c.hd, c.pt,
-                          c.ints(c.status), ws.data_ptr(), nb, c.stream);
+                          c.ints(c.status), c.ints(c.marks), ws.data_ptr(), nb, c.stream);
     }
     if (rc) return failed("sx8_kv4_keep", rc);
     Py_RETURN_TRUE;

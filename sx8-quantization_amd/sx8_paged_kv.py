@@ -192,13 +192,14 @@ class PagedKV4:
         self._ws_attend = int(_L.lib().sx8_kv4_attend_workspace_bytes(self.head_dim))
         self._ws_tree = int(_L.lib().sx8_kv4_attend_tree_workspace_bytes(self.head_dim))
         self._t = (pages, table, lens, refs, status, nb, self.n_kv, self.head_dim, self.page_tokens, self._ws_attend,
-                   self._ws_pages, self._ws_tree)
+                   self._ws_pages, self._ws_tree, torch.full((self.n_slots,), 2 ** 31 - 1, dtype=torch.int32, device=self.device))
 
     pages = property(lambda self: self._t[0])
     table = property(lambda self: self._t[1])
     lens = property(lambda self: self._t[2])
     refs = property(lambda self: self._t[3])
     status = property(lambda self: self._t[4])
+    marks = property(lambda self: self._t[12])                      # of a slot: -1 where its last reserve was refused
 
     # ---------------------------------------------------------------- rows
     def _slots(self, layer, cu):
@@ -272,7 +273,7 @@ class PagedKV4:
         A row's position is that of the slot's first new row plus depth[row] (int32; without depth: its number in the
         slot), where trees of drafted tokens have several rows of one depth (sx8_draft.draft_tree).  Rows are fp16, bf16, or
         float32 (then dtype, fp16 unless given, is what they are rounded to, once).  A row whose position lies outside the tables
-        gives zeros and is not written.  out shares no memory with q, k and v."""
+        gives zeros and is not written, nor are those of a slot whose reserve was refused.  out shares no memory with q, k and v."""
         if dtype is None:
             dtype = torch.float16 if q.dtype == torch.float32 else q.dtype
         if out is None and dtype in _DTYPES:
@@ -299,11 +300,11 @@ class PagedKV4:
             out = _out("out", out, like, nh, self.head_dim)
             if out.shape[0] and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
                 raise RuntimeError("out may not be q, k or v")
-            _L.call("sx8_kv4_append_rope", *self._slots(layer, cu), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            _L.call("sx8_kv4_append_rope_marked", *self._slots(layer, cu), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                     q.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
                     out.stride(1), nh, self.n_kv, self.head_dim, self.page_tokens, cos.data_ptr(), sin.data_ptr(),
                     cos.shape[0], 2 * cos.shape[1], int(bool(interleaved)), None if depth is None else depth.data_ptr(),
-                    None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                    self.marks.data_ptr(), None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
                     float(eps), 2 if q.dtype == torch.float32 else _DTYPES[dtype], _DTYPES[dtype], _L.stream(self.device))
         return out
 
@@ -337,15 +338,16 @@ class PagedKV4:
         return torch.empty(self._ws_pages, dtype=torch.uint8, device=self.device)
 
     def reserve(self, add):
-        """Slot s grows by add[s] tokens (int32 on the device): lens, and pages for them, lowest free page first."""
+        """Slot s grows by add[s] tokens (int32 on the device): lens, and pages for them, lowest free page first.  Where that
+        is refused, append_rope and keep leave the slots that were to grow alone until a reserve for them is done."""
         if _L.py().kv4_pages(self._t, "reserve", add):
             return
         with torch.cuda.device(self.device):
             _ints("add", add, self.n_slots, self.device)
             ws = self._ws()
-            _L.call("sx8_kv4_reserve", self.table.data_ptr(), self.lens.data_ptr(), self.refs.data_ptr(), add.data_ptr(),
-                    self.n_slots, self.max_pages, self.n_pages, self.page_tokens, self.status.data_ptr(), ws.data_ptr(),
-                    self._ws_pages, _L.stream(self.device))
+            _L.call("sx8_kv4_reserve_marked", self.table.data_ptr(), self.lens.data_ptr(), self.refs.data_ptr(), add.data_ptr(),
+                    self.n_slots, self.max_pages, self.n_pages, self.page_tokens, self.status.data_ptr(), self.marks.data_ptr(),
+                    ws.data_ptr(), self._ws_pages, _L.stream(self.device))
 
     def fork(self, src, dst):
         """The empty slots dst[i] become copies of the slots src[i] (int32 on the device): full pages are shared, a last
@@ -385,7 +387,7 @@ class PagedKV4:
         """Of its n new rows slot s keeps counts[s], the rows path[cu[s]] < path[cu[s] + 1] < .. (numbers in the slot; both
         int32 on the device, as sx8_draft.verify_draft returns them): in all layers they move together behind the tokens
         before the new ones, lens becomes lens - n + counts[s] and pages behind that are given back.  Slots without new rows have
-        counts 0.  The rows' pages must be the slot's own, as for `append`."""
+        counts 0, and those whose reserve was refused stay as they are.  The rows' pages must be the slot's own, as for `append`."""
         if _L.py().kv4_keep(self._t, path, counts, cu):
             return
         with torch.cuda.device(self.device):
@@ -395,10 +397,10 @@ class PagedKV4:
                 _ints("cu", cu, self.n_slots + 1, self.device)
             nb = int(_L.lib().sx8_kv4_keep_workspace_bytes(self.n_slots, path.numel()))
             ws = torch.empty(max(nb, 0), dtype=torch.uint8, device=self.device)
-            _L.call("sx8_kv4_keep", self.pages.data_ptr(), self.n_layers, self.table.data_ptr(), self.lens.data_ptr(),
+            _L.call("sx8_kv4_keep_marked", self.pages.data_ptr(), self.n_layers, self.table.data_ptr(), self.lens.data_ptr(),
                     self.refs.data_ptr(), None if cu is None else cu.data_ptr(), path.data_ptr(), counts.data_ptr(),
                     path.numel(), self.n_slots, self.max_pages, self.n_pages, self.n_kv, self.head_dim, self.page_tokens,
-                    self.status.data_ptr(), ws.data_ptr(), nb, _L.stream(self.device))
+                    self.status.data_ptr(), self.marks.data_ptr(), ws.data_ptr(), nb, _L.stream(self.device))
 
     def check(self):
         """Wait for the device and raise the first error that reserve, fork, free or keep met since the last check."""

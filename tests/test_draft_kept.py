@@ -107,3 +107,120 @@ def test_round_of_a_long_chain(hiplib, cuda, words, kept):
     kk = torch.cat([k0[:40], turn(k[:kept], None, cos[place], sin[place], False).float().half()])
     got = p.read(0, 40 + kept + 9, cum(p.lens.tolist(), cuda))
     assert torch.equal(got[0][:40 + kept], q4(kk).half()) and torch.equal(got[1][:40 + kept], q4(torch.cat([v0[:40], v[:kept]])).half())
+
+
+# ------------------------------------------------------------------------------ a reservation that is refused
+def a_pass(p, new, seed, cuda, cos, sin, reserve=True):
+    """One pass over drafted tokens of a single layer, nobody asking for the status in between; as a function of tensors."""
+    from sx8_draft import draft_tree, verify_draft
+    T = sum(new)
+    q, k, v = (rand((T, n, 64), seed + i, F16, cuda) for i, n in enumerate((4, 2, 2)))
+    logits, ps, tokens, u, _ = drafts(cuda, new, 40, seed)
+    add, cu, parents = ints(new, cuda), cum(new, cuda), ints(flat(ps), cuda)
+    tokens, u = torch.tensor(tokens, device=cuda), torch.tensor(u, dtype=F32, device=cuda) / 2
+
+    def run():
+        if reserve:
+            p.reserve(add)
+        mask, depth = draft_tree(parents, cu)
+        qr = p.append_rope(0, q, k, v, cos, sin, cu, depth=depth)
+        o = p.attend_tree(0, qr, mask, cu)
+        path, counts, nxt = verify_draft(logits, tokens, parents, cu, u, 0.8, depth=depth)
+        p.keep(path, counts, cu)
+        return qr, o, counts
+    return run
+
+
+def state(p):
+    return [t.clone() for t in (p.pages, p.table, p.lens, p.refs)]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("general", [False, True])
+@pytest.mark.parametrize("new,error", [([3, 40, 0], "no free pages"), ([3, 200, 2], "table row is full"), ([3, 5, 9], "no free pages"), ([0, 0, 70], "no free pages")])
+def test_refused_reservation_harms_no_token(hiplib, cuda, monkeypatch, general, new, error):
+    """No page left, or no place in the table: the whole pass changes nothing, in slots with room as well, one with fewer tokens
+    than rows among them; the error is there whenever it is asked for, and the next pass is that of a cache that never saw it."""
+    import _sx8lib
+    if general:
+        monkeypatch.setattr(_sx8lib, "_py", _sx8lib._NoHostModule())
+    p, _, _ = make(cuda, [60, 64, 1], 2, 64, 32, spare=0, width=6)
+    other, _, _ = make(cuda, [60, 64, 1], 2, 64, 32, spare=0, width=6)
+    cos, sin = tables(200, 64, cuda)
+    before = state(p)
+    qr, _, counts = a_pass(p, new, 30, cuda, cos, sin)()
+    assert same(state(p), before) and not qr.any() and counts.sum() > 0
+    qr = p.append_rope(0, *(rand((3, n, 64), 5, F16, cuda) for n in (4, 2, 2)), cos, sin)           # one row a slot
+    grown = torch.tensor([n == 0 for n in new], device=cuda)
+    assert torch.equal(qr.flatten(1).any(1), grown)
+    p.pages.copy_(before[0])
+    a_pass(p, new, 30, cuda, cos, sin)()                             # refused again
+    with pytest.raises(RuntimeError, match=error):
+        p.check()
+    assert same(state(p), before)
+    p.check()
+    outs = [a_pass(c, [4, 0, 20], 50, cuda, cos, sin)() for c in (p, other)]
+    for c in (p, other):
+        c.check()
+    assert same(*outs) and same(state(p), state(other)) and outs[0][2][0] > 0
+
+
+def test_refused_reservation_captured(hiplib, cuda):
+    """A captured pass, replayed while there is no page and again when there is one: nothing, then what the eager pass does."""
+    p, _, _ = make(cuda, [60, 64, 40], 2, 64, 32, spare=0, width=6)
+    other, _, _ = make(cuda, [60, 64, 40], 2, 64, 32, spare=0, width=6)
+    cos, sin = tables(200, 64, cuda)
+    run, want = a_pass(p, [3, 40, 0], 30, cuda, cos, sin), a_pass(other, [3, 40, 0], 30, cuda, cos, sin)
+    run()
+    with pytest.raises(RuntimeError, match="no free pages"):
+        p.check()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = run()
+    before = state(p)
+    for _ in range(3):
+        g.replay()
+        assert same(state(p), before)
+        run()
+        assert same(state(p), before)
+    with pytest.raises(RuntimeError, match="no free pages"):
+        p.check()
+    for c in (p, other):
+        c.free(ints([2], cuda))
+    g.replay()
+    got = [t.clone() for t in outs] + state(p)
+    assert same(got, [*want(), *state(other)])
+    for c in (p, other):
+        c.check()
+
+
+def test_marks_are_of_the_slot(hiplib, cuda):
+    """An error of another call stops no pass; a refusal for other slots neither; a slot's mark goes with its next reservation."""
+    cos, sin = tables(200, 64, cuda)
+    pools = [make(cuda, [60, 64, 1], 2, 64, 32, spare=1, width=6)[0] for _ in range(3)]
+    p, late, want = pools
+    p.fork(ints([0], cuda), ints([1], cuda))                         # the target is in use
+    a_pass(p, [3, 0, 5], 30, cuda, cos, sin)()
+    with pytest.raises(RuntimeError, match="in use"):
+        p.check()
+    # reserved, then other slots refused: the pass goes on
+    late.reserve(ints([3, 0, 5], cuda))
+    late.reserve(ints([0, 100, 0], cuda))
+    assert late.marks.tolist() == [2 ** 31 - 1, -1, 2 ** 31 - 1]
+    a_pass(late, [3, 0, 5], 30, cuda, cos, sin, reserve=False)()
+    with pytest.raises(RuntimeError, match="no free pages"):
+        late.check()
+    late.reserve(ints([0, 1, 0], cuda))
+    assert late.marks.tolist() == [2 ** 31 - 1] * 3 and late.lens[1] == 65
+    a_pass(want, [3, 0, 5], 30, cuda, cos, sin)()
+    want.check()
+    assert same(state(p), state(want))
+    want.reserve(ints([0, 1, 0], cuda))
+    assert same(state(late), state(want))
+    late.reserve(ints([-1, 0, 0], cuda))
+    assert late.marks.tolist() == [-1, 2 ** 31 - 1, 2 ** 31 - 1]
+    with pytest.raises(RuntimeError, match="bad slot or count"):
+        late.check()
