@@ -123,12 +123,14 @@ int64_t sx8_kv4_attend_tree_workspace_bytes(int32_t hd);
 /* Page operations.  Each takes free pages lowest number first, in the order of its slots or entries, and does all
  * of it or nothing: where it cannot, status (2 int32: code, slot or entry) is set if it was zero, and nothing
  * else changes.  Codes: 1 bad slot or count, 2 no free pages, 3 the slot's table row is full, 4 the target slot
- * is in use, named twice or a source.  workspace: sx8_kv4_pages_workspace_bytes bytes, 16-byte aligned.
+ * is in use, named twice or a source, 5 a row to be kept was never written.  workspace: sx8_kv4_pages_workspace_bytes bytes, 16-byte aligned.
  *
  * reserve: slot s grows by add[s] >= 0 tokens (lens[s] += add[s]), its new pages with one reference.
  * *_marked: with marks (n_slots) int32, 2^31 - 1 at first (NULL: as without).  A refused reserve sets the marks of the slots with
  *   add[s] != 0 to -1, one that is done sets them to 2^31 - 1.  For a slot whose mark is -1, append_rope gives zeros and writes no
- *   page, and keep leaves all of it as it is: a pass that nobody checks in between cannot harm older tokens.
+ *   page, and keep leaves all of it as it is: a pass that nobody checks in between cannot harm older tokens.  append_rope
+ *   lowers a slot's mark to the number of its first row that lies outside the tables, keep refuses (code 5) a row from there on
+ *   that is to be kept, and sets the marks of the slots that it has dealt with back.
  * fork: for n entries, the empty slot dst[i] becomes a copy of slot src[i]: full pages are shared, a last page that is
  *   partly filled is copied (every layer: pages of layer l at pages + l * n_pages * page_bytes).
  * free: the slots' pages lose a reference, their rows become -1 and their lengths 0.  A slot named twice is freed

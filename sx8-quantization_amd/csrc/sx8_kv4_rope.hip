@@ -21,7 +21,7 @@ struct RopeIn {
     const float *cos, *sin;
     int64_t table_rows;
     const int32_t* depth;
-    const int32_t* marks;                   // of a slot: below zero, its reservation was refused (null: none was)
+    int32_t* marks;                         // of a slot: new rows in the pages, below zero: its reservation was refused (or null)
     const uint16_t *qw, *kw;
     double eps;
     int rot, heads;                         // heads: query heads of a work-group
@@ -127,7 +127,9 @@ __global__ __launch_bounds__(256) void k_kv4_append_rope(const Kv4Pool p, const 
     const bool refused = in.marks && in.marks[t.slot] < 0;
     if (tid < nt) {
         const int64_t at = in.depth ? (int64_t)t.first + in.depth[t.row0 + tid] : (int64_t)t.block * 32 + t.t0 + tid;
-        place[t.t0 + tid] = !refused && at >= 0 && at < in.table_rows ? (int)at : -1;
+        const bool inside = at >= 0 && at < in.table_rows;
+        place[t.t0 + tid] = !refused && inside ? (int)at : -1;
+        if (in.marks && !inside && head == 0) atomicMin(&in.marks[t.slot], t.block * 32 + t.t0 + tid - t.first);
     }
     __syncthreads();
     if (head >= p.sh.nk) {

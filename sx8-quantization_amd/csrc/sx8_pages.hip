@@ -369,9 +369,9 @@ KeepWs keep_ws(void* w, int64_t n_slots) {
 }
 
 // A slot of n new rows keeps rows path[0] < path[1] < .. (counts of them) of these.  A slot that its reservation was refused
-// has none (its last n tokens are older ones): it is passed over.
+// has none (its last n tokens are older ones): it is passed over.  Rows from the slot's mark on were not all written.
 __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const int32_t* path, const int32_t* counts,
-                                                       const int32_t* cu, Kv4Shape sh, const KeepWs ws, const int32_t* marks) {
+                                                       const int32_t* cu, Kv4Shape sh, const KeepWs ws, int32_t* marks) {
     const int tid = threadIdx.x, pt = t.page_tokens;
     const int64_t cap = (int64_t)t.max_pages * pt;
     int code = 0, item = 0, total = 0;
@@ -382,13 +382,14 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
             int first, n;
             kv4_rows(sh, cu, s, &first, &n);
             const int len = t.lens[s], c = counts[s], base = len - n;
-            const bool refused = n > 0 && marks && marks[s] < 0;
-            bool bad = false;
-            if (refused) {
+            const int mark = n > 0 && marks ? marks[s] : kAllRows;
+            bool bad = false, missing = false;
+            if (mark < 0) {
                 n = 0;
             } else if (n > 0) {
                 bad = c < 0 || c > n || base < 0 || len > cap;
-                for (int i = 0, last = -1; !bad && i < c; i += 8) {  // (eight asked for together)
+                int last = -1;
+                for (int i = 0; !bad && i < c; i += 8) {             // (eight asked for together)
                     int at[8];
 #pragma unroll
                     for (int u = 0; u < 8; ++u) at[u] = path[first + min(i + u, c - 1)];
@@ -399,12 +400,13 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
                         last = at[u];
                     }
                 }
+                missing = !bad && last >= mark;
                 if (!bad) held = (len + pt - 1) / pt - base / pt;
             } else {
                 bad = c != 0;
             }
-            if (bad && !code) {
-                code = 1;
+            if ((bad || missing) && !code) {
+                code = bad ? 1 : 5;
                 item = s;
             }
             ws.base[s] = n > 0 ? base : -1;
@@ -439,6 +441,7 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
             }
         }
         t.lens[s] = end;
+        if (marks) marks[s] = kAllRows;
     }
 }
 

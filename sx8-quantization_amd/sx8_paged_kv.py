@@ -19,7 +19,7 @@ import _sx8lib as _L
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _STATUS = {1: "bad slot or count", 2: "no free pages", 3: "the slot's table row is full",
-           4: "the target slot is in use, named twice or a source"}
+           4: "the target slot is in use, named twice or a source", 5: "a row to be kept was never written"}
 
 
 def _dtype(name, t):
@@ -199,7 +199,7 @@ class PagedKV4:
     lens = property(lambda self: self._t[2])
     refs = property(lambda self: self._t[3])
     status = property(lambda self: self._t[4])
-    marks = property(lambda self: self._t[12])                      # of a slot: -1 where its last reserve was refused
+    marks = property(lambda self: self._t[12])                      # of a slot: new rows that are in the pages, -1: its reserve was refused
 
     # ---------------------------------------------------------------- rows
     def _slots(self, layer, cu):
@@ -387,7 +387,8 @@ class PagedKV4:
         """Of its n new rows slot s keeps counts[s], the rows path[cu[s]] < path[cu[s] + 1] < .. (numbers in the slot; both
         int32 on the device, as sx8_draft.verify_draft returns them): in all layers they move together behind the tokens
         before the new ones, lens becomes lens - n + counts[s] and pages behind that are given back.  Slots without new rows have
-        counts 0, and those whose reserve was refused stay as they are.  The rows' pages must be the slot's own, as for `append`."""
+        counts 0, and those whose reserve was refused stay as they are; a row
+        that append_rope left out (outside its tables, past draft_tree's words) is refused.  The rows' pages must be the slot's own, as for `append`."""
         if _L.py().kv4_keep(self._t, path, counts, cu):
             return
         with torch.cuda.device(self.device):

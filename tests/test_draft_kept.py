@@ -224,3 +224,78 @@ def test_marks_are_of_the_slot(hiplib, cuda):
     assert late.marks.tolist() == [-1, 2 ** 31 - 1, 2 ** 31 - 1]
     with pytest.raises(RuntimeError, match="bad slot or count"):
         late.check()
+
+
+# ------------------------------------------------------------------------------ rows that were never written
+@pytest.mark.parametrize("general", [False, True])
+@pytest.mark.parametrize("S", [3, 70])
+def test_keep_refuses_rows_that_were_not_written(hiplib, cuda, monkeypatch, general, S):
+    """Rows past the masks' words and behind the tables' end: a verification that does not know the depths keeps them, `keep` says
+    so and changes nothing; fewer rows are kept as ever, and the next pass is one without a trace."""
+    import _sx8lib
+    from sx8_draft import draft_tree, verify_draft
+    if general:
+        monkeypatch.setattr(_sx8lib, "_py", _sx8lib._NoHostModule())
+    for new, table, slot, good in (([70, 4], 400, 0, [64, 4]), ([5, 12], 40, 1, [5, 7]), ([2, 1], 33, 1, [2, 0])):
+        new, good = new + [0] * (S - 2), good + [0] * (S - 2)
+        p, _, _ = make(cuda, [10, 33] + [1] * (S - 2), 2, 64, 32, spare=8, width=8, layers=2)
+        cos, sin = tables(table, 64, cuda)
+        T, cu, parents = sum(new), cum(new, cuda), ints([j - 1 for n in new for j in range(n)], cuda)
+        p.reserve(ints(new, cuda))
+        q, k, v = (rand((T, n, 64), 30 + i, F16, cuda) for i, n in enumerate((4, 2, 2)))
+        mask, depth = draft_tree(parents, cu)
+        for layer in range(2):
+            p.attend_tree(layer, p.append_rope(layer, q, k, v, cos, sin, cu, depth=depth), mask, cu)
+        x, tokens, u = torch.randn(T, 30, generator=torch.Generator().manual_seed(1)).to(cuda), torch.arange(T, device=cuda) % 30, torch.zeros(T, device=cuda)
+        path, counts, _ = verify_draft(x, tokens, parents, cu, u, 1.0)
+        assert counts.tolist() == new
+        before = state(p)
+        for _ in range(2):                                           # (refused as often as it is asked)
+            p.keep(path, counts, cu)
+            with pytest.raises(RuntimeError, match=rf"never written \(slot or entry {slot}\)"):
+                p.check()
+            assert same(state(p), before)
+        p.keep(path, ints(good, cuda), cu)
+        p.check()
+        lens = [10 + good[0], 33 + good[1]]
+        assert p.lens.tolist()[:2] == lens and p.marks.tolist() == [2 ** 31 - 1] * S
+        at = list(range(10, lens[0]))
+        got = p.read(1, sum(lens), ints([0, lens[0], *[sum(lens)] * (S - 1)], cuda))
+        assert torch.equal(got[0][10:lens[0]], q4(turn(k[:good[0]], None, cos[at], sin[at], False).float().half()).half())
+        # a pass whose rows all have a place: nothing is left of the refusal
+        p.reserve(ints([1] + [0] * (S - 1), cuda))
+        one = cum([1] + [0] * (S - 1), cuda)
+        p.append_rope(0, q[:1], k[:1], v[:1], cos, sin, one)
+        p.keep(ints([0], cuda), ints([1] + [0] * (S - 1), cuda), one)
+        p.check()
+        assert p.lens[0] == lens[0] + 1
+
+
+def test_rows_that_were_not_written_and_not_kept(hiplib, cuda):
+    """Branches that end outside: what lies before them is kept, without depths too; a row that is out by its depth alone."""
+    from sx8_draft import draft_tree, verify_draft
+    p, _, _ = make(cuda, [10], 1, 64, 32, spare=4, width=8)
+    cos, sin = tables(100, 64, cuda)
+    new, parents = 80, ints([-1] + [0] * 79, cuda)
+    cu = cum([new], cuda)
+    p.reserve(ints([new], cuda))
+    q, k = rand((new, 2, 64), 1, F16, cuda), rand((new, 1, 64), 2, F16, cuda)
+    _, depth = draft_tree(parents, cu)
+    p.append_rope(0, q, k, k, cos, sin, cu, depth=depth)
+    assert p.marks.tolist() == [64]
+    x = torch.zeros(new, 100, device=cuda)
+    u = torch.full((new,), 0.999, device=cuda)
+    u[63] = 0.0
+    path, counts, _ = verify_draft(x, torch.arange(new, device=cuda), parents, cu, u, 1.0)
+    p.keep(path, counts, cu)
+    p.check()
+    assert path.tolist()[:3] == [0, 63, -1] and p.lens.tolist() == [12] and p.marks.tolist() == [2 ** 31 - 1]
+    p.reserve(ints([3], cuda))
+    p.append_rope(0, q[:3], k[:3], k[:3], cos, sin, cum([3], cuda), depth=ints([0, -13, 1], cuda))
+    assert p.marks.tolist() == [1]
+    p.keep(ints([0, 2, -1], cuda), ints([2], cuda), cum([3], cuda))
+    with pytest.raises(RuntimeError, match="never written"):
+        p.check()
+    p.keep(ints([0, 2, -1], cuda), ints([1], cuda), cum([3], cuda))
+    p.check()
+    assert p.lens.tolist() == [13]
