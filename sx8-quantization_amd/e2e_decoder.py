@@ -809,6 +809,9 @@ class PagedDecoder:
         each = dict(zip(slots, drafts))
         if not slots or len(slots) != len(drafts) or len(each) != len(slots):
             raise ValueError("as many different slots as drafts, and at least one")
+        for s, t in each.items():
+            if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.is_floating_point() or t.is_complex():
+                raise ValueError(f"slot {s}: drafts are a vector of whole numbers (none: an empty int64 one)")
         rows = {s: 1 + t.numel() for s, t in each.items()}
         for s, n in rows.items():
             if not 0 <= s < n_all or not self.lens[s] or n > 256 or self.lens[s] + n > self.max_len:
@@ -845,7 +848,7 @@ class PagedDecoder:
             temperature = torch.zeros(n_all, device=dev)
             temperature[torch.tensor(slots, device=dev)] = t
         last = self.tok[torch.tensor(order, device=dev)].split(1)
-        ids = torch.cat([x for s, t in zip(order, last) for x in (t, each[s].to(dev))])
+        ids = torch.cat([x for s, t in zip(order, last) for x in (t, each[s].to(dev, torch.int64))])
         counts = [rows.get(s, 0) for s in range(n_all)]
         cu, par = self._ints([0, *itertools.accumulate(counts), *(p for s in order for p in up[s])]).split((n_all + 1, ids.numel()))
         self.cache.reserve(self._ints(counts))

@@ -1,0 +1,50 @@
+"""What PagedDecoder.verify leaves behind where it refuses, raises or finds no token, and how often it waits."""
+import pytest
+import torch
+
+from test_e2e import TINY
+from test_paged_e2e import ids
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dec(hiplib, cuda):
+    from e2e_decoder import SX8Decoder
+    return SX8Decoder(TINY, device=cuda, seed=3, n_distinct=2, max_len=160)
+
+
+def start(dec, **kw):
+    """A decoder whose slots 0 and 2 of four hold tokens."""
+    from e2e_decoder import PagedDecoder
+    pd = PagedDecoder(dec, 4, max_len=120, page_tokens=32, **kw)
+    pd.prompt([0, 2], [ids(30, 1, dec.device), ids(20, 2, dec.device)])
+    return pd
+
+
+def state(pd):
+    """Everything that a later call reads: the slots' tokens, lengths, tables and counts, and the pages' used bytes as values."""
+    c, lens = pd.cache, pd.cache.lens.tolist()
+    cu = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32, device=c.device)
+    rows = [t for layer in range(c.n_layers) for t in c.read(layer, sum(lens), cu)]
+    return [list(pd.lens), pd.tok.clone(), c.table.clone(), c.lens.clone(), c.refs.clone(), *rows]
+
+
+def same(a, b):
+    return a[0] == b[0] and all(torch.equal(x, y) for x, y in zip(a[1:], b[1:]))
+
+
+def test_drafts_are_whole_numbers(dec, cuda):
+    """Vectors of another kind are refused before anything changes, an empty floating-point one too; other whole numbers are
+    taken as what they are."""
+    pd, other = start(dec), start(dec)
+    three, before = ids(3, 5, cuda), state(pd)
+    for bad in (torch.tensor([]), torch.tensor([], device=cuda), three.float(), three.half(), three[None], three[0], three.to(torch.complex64), three.tolist()):
+        for slots, drafts in (([0, 2], [three, bad]), ([2], [bad])):
+            with pytest.raises(ValueError, match="slot 2: drafts"):
+                pd.verify(slots, drafts)
+    assert same(state(pd), before)
+    none = torch.tensor([], dtype=torch.int64)
+    got, want = pd.verify([0, 2], [three.int(), none]), other.verify([0, 2], [three, none.to(cuda)])
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and same(state(pd), state(other))
+    assert torch.equal(pd.step()[[0, 2]], other.step()[[0, 2]])
