@@ -803,7 +803,7 @@ class PagedDecoder:
         tokens, vocabulary) a slot, row 0 what the last token's followers were drawn from) are those of sx8_draft.verify_draft.
         Returns for each slot its new tokens, int64 on the device: the kept ones and the one that follows, which is the
         input of the next pass.  ``logits`` are those of all rows, packed by slot number.  Rows that are not kept leave no
-        trace in the cache.  Waits for the device once, for the numbers of kept tokens."""
+        trace in the cache, nor does a pass that raises.  Waits for the device once, for the numbers of kept tokens."""
         slots = _numbers(slots)
         dev, n_all = self.dec.device, self.n_slots
         each = dict(zip(slots, drafts))
@@ -851,10 +851,29 @@ class PagedDecoder:
         ids = torch.cat([x for s, t in zip(order, last) for x in (t, each[s].to(dev, torch.int64))])
         counts = [rows.get(s, 0) for s in range(n_all)]
         cu, par = self._ints([0, *itertools.accumulate(counts), *(p for s in order for p in up[s])]).split((n_all + 1, ids.numel()))
+        none = torch.zeros(n_all, dtype=torch.int32, device=dev)
         self.cache.reserve(self._ints(counts))
-        self.cache.check()
-        self.lens = [a + b for a, b in zip(self.lens, counts)]
-        mask, depth = draft_tree(par, cu, -(-max(rows.values()) // 64))
+        try:
+            self.cache.check()
+            path, kept, following = self._verify(ids, par, cu, max(rows.values()), uniforms, temperature, draft_probs)
+            n_kept = kept.tolist()
+        except BaseException:
+            self.cache.keep(par, none, cu)                          # (slots that reserve refused are passed over)
+            raise
+        self.cache.keep(path, kept, cu)
+        self.lens = [a + k for a, k in zip(self.lens, n_kept)]
+        at = torch.tensor(order, device=dev)
+        self.tok[at] = following[at]
+        starts = dict(zip(order, itertools.accumulate([0, *(rows[s] for s in order)])))
+        out = {}
+        for s in order:
+            a = starts[s]
+            out[s] = torch.cat([ids[a + path[a + 1:a + n_kept[s]].long()], following[s:s + 1]])
+        return [out[s] for s in slots]
+
+    def _verify(self, ids, par, cu, most, uniforms, temperature, draft_probs):
+        """The layers over drafted rows that the cache has places for (up to `most` a slot), the lm_head and what is kept."""
+        mask, depth = draft_tree(par, cu, -(-most // 64))
         d, scale = self.dec, 1.0 / math.sqrt(self.dec.cfg["head_dim"])
 
         def attend(li, q, k, v):
@@ -866,19 +885,7 @@ class PagedDecoder:
         pb = self._bufs(ids.numel())
         self._rows(pb, ids, None, attend)
         self.logits = self._head(pb["resid"], pb["d"], ids.numel())
-        path, kept, following = verify_draft(self.logits, ids, par, cu, uniforms, temperature, draft_probs, depth)
-        self.cache.keep(path, kept, cu)
-        kept = kept.tolist()
-        self.cache.check()
-        self.lens = [a - b + k for a, b, k in zip(self.lens, counts, kept)]
-        at = torch.tensor(order, device=dev)
-        self.tok[at] = following[at]
-        starts = dict(zip(order, itertools.accumulate([0, *(rows[s] for s in order)])))
-        out = {}
-        for s in order:
-            a = starts[s]
-            out[s] = torch.cat([ids[a + path[a + 1:a + kept[s]].long()], following[s:s + 1]])
-        return [out[s] for s in slots]
+        return verify_draft(self.logits, ids, par, cu, uniforms, temperature, draft_probs, depth)
 
     def fork(self, src, dst):
         """The empty slots dst[i] go on from where the slots src[i] are."""

@@ -48,3 +48,53 @@ def test_drafts_are_whole_numbers(dec, cuda):
     got, want = pd.verify([0, 2], [three.int(), none]), other.verify([0, 2], [three, none.to(cuda)])
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and same(state(pd), state(other))
     assert torch.equal(pd.step()[[0, 2]], other.step()[[0, 2]])
+
+
+@pytest.mark.parametrize("where", ["head", "layer", "verify", "check"])
+@pytest.mark.parametrize("error", [torch.cuda.OutOfMemoryError, RuntimeError, KeyboardInterrupt])
+def test_a_pass_that_raises_leaves_no_trace(dec, cuda, monkeypatch, where, error):
+    """Whatever raises behind the reservation, with new pages among it: tokens, lengths, tables and counts are as before, and the
+    next pass and step those of a decoder that never saw it."""
+    import e2e_decoder
+    pd, other = start(dec), start(dec)
+    drafts, before = [ids(5, 5, cuda), ids(40, 6, cuda)], state(pd)
+
+    def fails(*a, **kw):
+        raise error("as if")
+
+    with monkeypatch.context() as m:
+        if where == "head":
+            m.setattr(pd, "_head", fails)
+        elif where == "layer":
+            real = pd.cache.attend_tree
+            m.setattr(pd.cache, "attend_tree", lambda li, *a: fails() if li == len(dec.layers) - 1 else real(li, *a))
+        elif where == "verify":
+            m.setattr(e2e_decoder, "verify_draft", fails)
+        else:
+            m.setattr(pd.cache, "check", fails)
+        for _ in range(2):
+            with pytest.raises(error, match="as if"):
+                pd.verify([0, 2], drafts)
+            assert same(state(pd), before)
+    got, want = pd.verify([0, 2], drafts), other.verify([0, 2], drafts)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and same(state(pd), state(other))
+    assert torch.equal(pd.step()[[0, 2]], other.step()[[0, 2]])
+    pd.cache.check()
+
+
+def test_an_earlier_error_is_raised_and_the_rows_are_dropped(dec, cuda):
+    """An error that the program's own call on the cache left behind: verify raises it, and its places are given back; where its own
+    reservation is refused, nothing is dropped."""
+    pd = start(dec)
+    before = state(pd)
+    pd.cache.fork(*(torch.tensor([i], dtype=torch.int32, device=cuda) for i in (0, 2)))
+    with pytest.raises(RuntimeError, match="in use"):
+        pd.verify([0, 2], [ids(5, 5, cuda), ids(40, 6, cuda)])
+    assert same(state(pd), before)
+    small = start(dec, n_pages=2)
+    before = state(small)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="no free pages"):
+            small.verify([2, 0], [ids(1, 5, cuda), ids(5, 6, cuda)])
+        assert same(state(small), before)
+    assert small.verify([2], [ids(1, 5, cuda)])[0].numel() >= 1 and small.lens == small.cache.lens.tolist()
