@@ -802,7 +802,7 @@ class PagedDecoder:
         temperature (a number, or one a slot), uniforms (a float32 vector of 1 + tokens a slot) and draft_probs ((1 +
         tokens, vocabulary) a slot, row 0 what the last token's followers were drawn from) are those of sx8_draft.verify_draft.
         Returns for each slot its new tokens, int64 on the device: the kept ones and the one that follows, which is the
-        input of the next pass.  ``logits`` are those of all rows, packed by slot number.  Rows that are not kept leave no
+        input of the next pass; a slot that none follows (the last kept row's logits are all NaN or -infinity) is a RuntimeError.  ``logits`` are those of all rows, packed by slot number.  Rows that are not kept leave no
         trace in the cache, nor does a pass that raises.  Waits for the device once, for the numbers of kept tokens."""
         slots = _numbers(slots)
         dev, n_all = self.dec.device, self.n_slots
@@ -856,7 +856,10 @@ class PagedDecoder:
         try:
             self.cache.check()
             path, kept, following = self._verify(ids, par, cu, max(rows.values()), uniforms, temperature, draft_probs)
-            n_kept = kept.tolist()
+            n_kept, token = torch.stack([kept.long(), following]).tolist()
+            lost = [s for s in order if token[s] < 0]
+            if lost:
+                raise RuntimeError(f"slots {lost}: no token follows, their logits are all NaN or -infinity; the pass is undone")
         except BaseException:
             self.cache.keep(par, none, cu)                          # (slots that reserve refused are passed over)
             raise

@@ -98,3 +98,27 @@ def test_an_earlier_error_is_raised_and_the_rows_are_dropped(dec, cuda):
             small.verify([2, 0], [ids(1, 5, cuda), ids(5, 6, cuda)])
         assert same(state(small), before)
     assert small.verify([2], [ids(1, 5, cuda)])[0].numel() >= 1 and small.lens == small.cache.lens.tolist()
+
+
+@pytest.mark.parametrize("value", [float("nan"), -float("inf")])
+@pytest.mark.parametrize("sampled", [False, True])
+def test_a_slot_that_no_token_follows(dec, cuda, monkeypatch, value, sampled):
+    """Logits that are no numbers give no token: the pass says which slots and is undone, and no slot's next input is -1."""
+    pd, other = start(dec), start(dec)
+    drafts, before = [ids(3, 5, cuda), ids(2, 6, cuda)], state(pd)
+    how = dict(uniforms=[torch.zeros(4, device=cuda), torch.zeros(3, device=cuda)], temperature=1.0) if sampled else {}
+    head = pd._head
+
+    def broken(resid, d, n):
+        x = head(resid, d, n)
+        x[4:] = value                                                # the rows of slot 2
+        return x
+
+    with monkeypatch.context() as m:
+        m.setattr(pd, "_head", broken)
+        with pytest.raises(RuntimeError, match=r"slots \[2\]: no token follows"):
+            pd.verify([0, 2], drafts, **how)
+    assert same(state(pd), before)
+    got, want = pd.verify([0, 2], drafts, **how), other.verify([0, 2], drafts, **how)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and same(state(pd), state(other)) and (pd.tok >= 0).all()
+    assert torch.equal(pd.step()[[0, 2]], other.step()[[0, 2]])
