@@ -589,8 +589,8 @@ class PagedDecoder:
 
     ``prompt`` runs the prompts of any slots as one packed pass (a slot that has tokens already goes on from them),
     ``step`` decodes one token of every slot in use, replayed from a HIP graph; ``verify`` checks several drafted tokens a slot
-    in one pass and goes on behind those that the model keeps; ``fork``, ``free`` and ``compact`` are the cache's.  Linears, norms and RoPE are the kernels of prefill_fused with one row per new token; K and V rows go
-    into the pages as they leave RoPE.  New prompts attend their own fp16 rows (attn_varlen), whatever else the call
+    in one pass and goes on behind those that the model keeps; ``fork``, ``free`` and ``compact`` are the cache's.  Linears,
+    norms and RoPE are the kernels of prefill_fused with one row per new token; K and V rows go into the pages as they leave RoPE.  New prompts attend their own fp16 rows (attn_varlen), whatever else the call
     brings; rows with earlier tokens, and every decoded token, attend the pages (PagedKV4.attend; many rows at once
     read the pages' values back and attend those).  The reference serves one sequence
     (scripts/infer_sx8.py:109-173)."""
@@ -609,9 +609,14 @@ class PagedDecoder:
         self.active = torch.zeros(n_slots, dtype=torch.int32, device=dec.device)
         self.logits = None                                          # of the last prompt or step
         self._pb, self._graph = {}, None
+        self._running = False                                       # whether a pass may still run on buffers that the next one replaces
 
     def _ints(self, xs):
         return torch.tensor(list(xs), dtype=torch.int32, device=self.dec.device)
+
+    def _sent(self, xs, dtype):
+        """A list on the device, behind earlier work, without a wait (torch.tensor's own copy waits for the stream)."""
+        return torch.tensor(xs, dtype=dtype, pin_memory=True).to(self.dec.device, non_blocking=True)
 
     def _set_active(self):
         self.active.copy_(self._ints(int(n > 0) for n in self.lens))
@@ -699,6 +704,7 @@ class PagedDecoder:
         self._set_active()
         # the last prompt's buffers may go now: check waited for this stream, whichever stream they were made on
         pb = self._bufs(ids.numel())
+        self._running = True
         scale = 1.0 / math.sqrt(self.dec.cfg["head_dim"])
 
         # From about 256 query rows of a KV head and slot on, reading the slots back and attending the values is the
@@ -802,8 +808,10 @@ class PagedDecoder:
         temperature (a number, or one a slot), uniforms (a float32 vector of 1 + tokens a slot) and draft_probs ((1 +
         tokens, vocabulary) a slot, row 0 what the last token's followers were drawn from) are those of sx8_draft.verify_draft.
         Returns for each slot its new tokens, int64 on the device: the kept ones and the one that follows, which is the
-        input of the next pass; a slot that none follows (the last kept row's logits are all NaN or -infinity) is a RuntimeError.  ``logits`` are those of all rows, packed by slot number.  Rows that are not kept leave no
-        trace in the cache, nor does a pass that raises.  Waits for the device once, for the numbers of kept tokens."""
+        input of the next pass; a slot that none follows (the last kept row's logits are all NaN or -infinity) is a RuntimeError.
+        ``logits`` are those of all rows, packed by slot number.  Rows that are not kept leave no trace in the cache, nor does a
+        pass that raises.  Waits for the device once, for the numbers of kept tokens, and before the layers only where a slot
+        needs a page or a prompt may still run on buffers that this pass replaces."""
         slots = _numbers(slots)
         dev, n_all = self.dec.device, self.n_slots
         each = dict(zip(slots, drafts))
@@ -842,21 +850,33 @@ class PagedDecoder:
         if draft_probs is not None and draft_probs.dtype not in (torch.float16, torch.bfloat16, torch.float32):
             raise ValueError("draft_probs: float16, bfloat16 or float32")
         if isinstance(temperature, (list, tuple, torch.Tensor)):
-            t = torch.as_tensor(temperature, dtype=torch.float32, device=dev)
+            t = torch.as_tensor(temperature, dtype=torch.float32)
             if t.shape != (len(slots),):
                 raise ValueError("temperature: a number, or one a slot")
-            temperature = torch.zeros(n_all, device=dev)
-            temperature[torch.tensor(slots, device=dev)] = t
-        last = self.tok[torch.tensor(order, device=dev)].split(1)
-        ids = torch.cat([x for s, t in zip(order, last) for x in (t, each[s].to(dev, torch.int64))])
+            t = t.to(dev) if t.is_cuda else self._sent(t.tolist(), torch.float32)
+        # everything that the host knows goes over in one transfer that nobody waits for
         counts = [rows.get(s, 0) for s in range(n_all)]
-        cu, par = self._ints([0, *itertools.accumulate(counts), *(p for s in order for p in up[s])]).split((n_all + 1, ids.numel()))
-        none = torch.zeros(n_all, dtype=torch.int32, device=dev)
-        self.cache.reserve(self._ints(counts))
+        cu, par = [0, *itertools.accumulate(counts)], [p for s in order for p in up[s]]
+        at, places, add, cu, par = self._sent([*order, *slots, *counts, *cu, *par], torch.int32).split(
+            (len(order), len(order), n_all, n_all + 1, len(par)))
+        at = at.long()
+        if isinstance(temperature, (list, tuple, torch.Tensor)):
+            temperature = torch.zeros(n_all, device=dev).index_copy_(0, places.long(), t)
+        ids = torch.cat([x for s, t in zip(order, self.tok[at].split(1)) for x in (t, each[s].to(dev, torch.int64))])
+        none, pt = torch.zeros(n_all, dtype=torch.int32, device=dev), self.cache.page_tokens
+        self.cache.reserve(add)
         try:
-            self.cache.check()
+            # (is there a page for a slot that needs one, and does nothing run on buffers that this pass replaces?)
+            if any((self.lens[s] + n - 1) // pt > (self.lens[s] - 1) // pt for s, n in rows.items()) \
+                    or (self._running and ids.numel() not in self._pb):
+                self.cache.check()
+            self._running = True
             path, kept, following = self._verify(ids, par, cu, max(rows.values()), uniforms, temperature, draft_probs)
-            n_kept, token = torch.stack([kept.long(), following]).tolist()
+            read = torch.cat([kept.long(), following, self.cache.status.long()]).tolist()
+            self._running = False
+            if read[-2]:
+                self.cache.check()                                  # (an error that an earlier call of the program's own left)
+            n_kept, token = read[:n_all], read[n_all:-2]
             lost = [s for s in order if token[s] < 0]
             if lost:
                 raise RuntimeError(f"slots {lost}: no token follows, their logits are all NaN or -infinity; the pass is undone")
@@ -865,7 +885,6 @@ class PagedDecoder:
             raise
         self.cache.keep(path, kept, cu)
         self.lens = [a + k for a, k in zip(self.lens, n_kept)]
-        at = torch.tensor(order, device=dev)
         self.tok[at] = following[at]
         starts = dict(zip(order, itertools.accumulate([0, *(rows[s] for s in order)])))
         out = {}

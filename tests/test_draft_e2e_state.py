@@ -1,4 +1,6 @@
 """What PagedDecoder.verify leaves behind where it refuses, raises or finds no token, and how often it waits."""
+import warnings
+
 import pytest
 import torch
 
@@ -122,3 +124,51 @@ def test_a_slot_that_no_token_follows(dec, cuda, monkeypatch, value, sampled):
     got, want = pd.verify([0, 2], drafts, **how), other.verify([0, 2], drafts, **how)
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and same(state(pd), state(other)) and (pd.tok >= 0).all()
     assert torch.equal(pd.step()[[0, 2]], other.step()[[0, 2]])
+
+
+def test_waits(dec, cuda, monkeypatch):
+    """One wait a pass; one more, before the buffers are replaced, where a slot needs a page or a prompt may still run on them."""
+    pd = start(dec)
+    order = []
+    check, bufs = pd.cache.check, pd._bufs
+    monkeypatch.setattr(pd.cache, "check", lambda: order.append("check") or check())
+    monkeypatch.setattr(pd, "_bufs", lambda n: order.append("bufs") or bufs(n))
+    torch.manual_seed(0)
+    drafts = {n: ids(n, n, cuda) for n in (1, 2, 20)}
+    u = {n: torch.rand(1 + n, device=cuda) for n in drafts}
+
+    def one(slots, ns, **kw):
+        order.clear()
+        torch.cuda.synchronize()
+        with warnings.catch_warnings(record=True) as said:
+            warnings.simplefilter("always")
+            torch.cuda.set_sync_debug_mode("warn")
+            try:
+                pd.verify(slots, [drafts[n] for n in ns], **kw)
+            finally:
+                torch.cuda.set_sync_debug_mode("default")
+        return order, sum("called a synchronizing" in str(w.message) for w in said)
+
+    assert one([2], [1]) == (["check", "bufs"], 2)                   # the prompt's buffers
+    assert one([2], [2]) == (["bufs"], 1)
+    assert one([2], [2], uniforms=[u[2]], temperature=[0.8]) == (["bufs"], 1)
+    assert one([2], [20], uniforms=[u[20]], temperature=0.8) == (["check", "bufs"], 2)       # a page
+    assert pd.lens == pd.cache.lens.tolist()
+    pd.prompt([1], [ids(3, 1, cuda)])
+    assert one([1], [2]) == (["bufs"], 1)                            # (three rows as well: the prompt's buffers stay)
+    pd.prompt([3], [ids(4, 1, cuda)])
+    assert one([3], [2]) == (["check", "bufs"], 2)
+    pd.cache.check()
+
+
+def test_an_earlier_error_where_no_page_is_needed(dec, cuda):
+    """It is read with the counts, and the pass is undone."""
+    pd, other = start(dec), start(dec)
+    pd.verify([2], [ids(1, 5, cuda)])
+    other.verify([2], [ids(1, 5, cuda)])
+    before = state(pd)
+    pd.cache.fork(*(torch.tensor([i], dtype=torch.int32, device=cuda) for i in (0, 2)))
+    with pytest.raises(RuntimeError, match="in use"):
+        pd.verify([2], [ids(2, 5, cuda)])
+    assert same(state(pd), before)
+    assert torch.equal(pd.verify([2], [ids(2, 5, cuda)])[0], other.verify([2], [ids(2, 5, cuda)])[0]) and same(state(pd), state(other))
