@@ -127,8 +127,8 @@ int64_t sx8_kv4_attend_tree_workspace_bytes(int32_t hd);
  *
  * reserve: slot s grows by add[s] >= 0 tokens (lens[s] += add[s]), its new pages with one reference.
  * *_marked: with marks (n_slots) int32, 2^31 - 1 at first (NULL: as without).  A refused reserve sets the marks of the slots with
- *   add[s] != 0 to -1, one that is done sets them to 2^31 - 1.  For a slot whose mark is -1, append_rope gives zeros and writes no
- *   page, and keep leaves all of it as it is: a pass that nobody checks in between cannot harm older tokens.  append_rope
+ *   add[s] != 0 to -1, one that is done sets them to 2^31 - 1.  For a slot whose mark is -1, append_rope writes no page (its
+ *   rows of out mean nothing), and keep leaves all of it as it is: a pass that nobody checks in between cannot harm older tokens.  append_rope
  *   lowers a slot's mark to the number of its first row that lies outside the tables, keep refuses (code 5) a row from there on
  *   that is to be kept, and sets the marks of the slots that it has dealt with back.
  * fork: for n entries, the empty slot dst[i] becomes a copy of slot src[i]: full pages are shared, a last page that is

@@ -273,7 +273,7 @@ class PagedKV4:
         A row's position is that of the slot's first new row plus depth[row] (int32; without depth: its number in the
         slot), where trees of drafted tokens have several rows of one depth (sx8_draft.draft_tree).  Rows are fp16, bf16, or
         float32 (then dtype, fp16 unless given, is what they are rounded to, once).  A row whose position lies outside the tables
-        gives zeros and is not written, nor are those of a slot whose reserve was refused.  out shares no memory with q, k and v."""
+        gives zeros and is not written; of a slot whose reserve was refused none is.  out shares no memory with q, k and v."""
         if dtype is None:
             dtype = torch.float16 if q.dtype == torch.float32 else q.dtype
         if out is None and dtype in _DTYPES:

@@ -151,11 +151,15 @@ def test_refused_reservation_harms_no_token(hiplib, cuda, monkeypatch, general, 
     other, _, _ = make(cuda, [60, 64, 1], 2, 64, 32, spare=0, width=6)
     cos, sin = tables(200, 64, cuda)
     before = state(p)
-    qr, _, counts = a_pass(p, new, 30, cuda, cos, sin)()
-    assert same(state(p), before) and not qr.any() and counts.sum() > 0
-    qr = p.append_rope(0, *(rand((3, n, 64), 5, F16, cuda) for n in (4, 2, 2)), cos, sin)           # one row a slot
-    grown = torch.tensor([n == 0 for n in new], device=cuda)
-    assert torch.equal(qr.flatten(1).any(1), grown)
+    _, _, counts = a_pass(p, new, 30, cuda, cos, sin)()
+    assert same(state(p), before) and counts.sum() > 0
+    k, v = (rand((3, 2, 64), i, F16, cuda) for i in (5, 6))
+    p.append_rope(0, rand((3, 4, 64), 4, F16, cuda), k, v, cos, sin)                                 # one row a slot
+    want, _, _ = make(cuda, [60, 64, 1], 2, 64, 32, spare=0, width=6)
+    want.append_rope(0, rand((3, 4, 64), 4, F16, cuda), k, v, cos, sin)
+    for got, new_row, old in zip(p.read(0, 3), want.read(0, 3), other.read(0, 3)):
+        grows = torch.tensor([n > 0 for n in new], device=cuda)[:, None, None]
+        assert torch.equal(got, torch.where(grows, old, new_row)) and not torch.equal(old, new_row)
     p.pages.copy_(before[0])
     a_pass(p, new, 30, cuda, cos, sin)()                             # refused again
     with pytest.raises(RuntimeError, match=error):
