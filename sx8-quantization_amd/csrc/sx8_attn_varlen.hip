@@ -18,9 +18,10 @@ namespace {
 // K and V go from memory to LDS directly, the next tile while this one is computed; rows past the sequence's
 // last key lie past the buffer and come as zeros.  A 16-byte chunk of a row lies at its position XOR a few bits of
 // the row, so that neither kind of read meets bank conflicts (the swap is made in the load's address).
-// Bound by the matrix cores and the softmax's VALU, which two waves a SIMD of different work-groups overlap: one prompt of
+// Bound by the matrix cores and the softmax's VALU, which take turns on a SIMD, whichever of its two waves (of different
+// work-groups, which hide each other's waits) they come from: one prompt of
 // 8192 tokens (32 heads over 8 of 128, bf16) takes 515-550 us by machine, 1000-1067 TFLOP/s, where a library product of
-// 8192^3 reaches 1100-1150: the MFMA is busy 51% of a SIMD's cycles and the VALU 46%.  Short prompts are bound by a
+// 8192^3 reaches 1100-1150: the MFMA is busy 51% of a SIMD's cycles and the VALU 46%, together 97%.  Short prompts are bound by a
 // work-group's start (about 5 us: lengths, query, first tile): 24 of
 // 40 .. 2000 tokens 230 us, three of up to 96 tokens 7.  s_setprio around the products (541 us against 533), tiles of 32
 // keys with three waves a SIMD (544 against 528) and work-groups that stay and request the next rows ahead (561 against

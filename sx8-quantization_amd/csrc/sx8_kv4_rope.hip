@@ -6,7 +6,8 @@
 // nothing here (the launch waits for memory) and makes the 16-bit values, and with them the levels, those of the exact
 // formula: a K value that falls to the other side of a rounding moves the ends of its group or its level.  Rounded once,
 // to float32 and from there to 16 bits; K and V are then encoded as sx8_kv4_append does it.
-// Bound by memory where rows are many (9761 rows of nine prompts, 32 heads over 8 of 128: 211 MB in 44 us, 4.8 TB/s) and by a launch of
+// Bound by memory where rows are many (9761 rows of nine prompts, 32 heads over 8 of 128: 211 MB in 56 us, 3.8 TB/s, and in 44 where the
+// rows lie in the last-level cache yet) and by a launch of
 // five dependent round trips where they are few (64 rows, one a slot: 6.7 us).
 #include "sx8_kv4_core.h"
 

@@ -11,7 +11,9 @@
 // of its cycles, the matrix cores 33%, together 99%), and a second wave there makes neither faster.
 // A wave keeps one block in registers: K of the next one is requested when the scores are done, V when the products are;
 // no branch lies between (with one the sums are copied: 316 us for the two long trees below, at that stage 237).  Query fragments
-// stay in LDS.  Three tiles a unit spill registers (245 us beside 198 on one machine), four leave one wave a SIMD (220).
+// stay in LDS.  Three tiles a unit spill registers (245 us beside 198 on one machine), four leave one wave a SIMD (220).  With two
+// (244 vector registers for heads of 128, two waves a SIMD; heads of 256 take 248 for one) no vector register is spilled, but 80 to 85 scalar
+// ones lie in vector lanes (64 to 67 with one tile).
 // Measured, with combine: 24 trees of 1 .. 24 rows after up to 8000 tokens, 32 heads over 8 of 128: 46 us; 8 of 64 rows after
 // 2500 .. 4100: 84; two of 31 after 61000 and 100000, 32 over 4: 175 (under a profiler's clock 205).
 #include "sx8_kv4_core.h"
