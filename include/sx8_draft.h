@@ -2,7 +2,8 @@
  *
  * A pass over drafted tokens brings each slot n rows: row 0 is the slot's last token, whose K/V is not in the cache yet, the
  * others are drafted ones; row i follows row parents[i] < i of its slot.  The pass is sx8_draft_tree, for every layer
- * sx8_kv4_append_rope and sx8_kv4_attend_tree, then sx8_draft_verify on the logits and sx8_kv4_keep (sx8_paged.h).
+ * sx8_kv4_append_rope and sx8_kv4_attend_tree, then sx8_draft_verify on the logits and sx8_kv4_keep (sx8_paged.h); with their forms
+ * sx8_draft_verify_within and *_marked nothing that was not written can become part of a sequence.
  * The reference has no counterpart (its runtime decodes one token a step, scripts/infer_sx8.py:109-173).
  * Conventions as in sx8_paged.h: rows are packed by slot (slot s has the rows cu[s] .. cu[s + 1] - 1; cu (n_slots + 1)
  * int32, kept within the call's rows), nothing is allocated and nothing synchronised, every call can be captured in

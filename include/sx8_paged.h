@@ -126,11 +126,12 @@ int64_t sx8_kv4_attend_tree_workspace_bytes(int32_t hd);
  * is in use, named twice or a source, 5 a row to be kept was never written.  workspace: sx8_kv4_pages_workspace_bytes bytes, 16-byte aligned.
  *
  * reserve: slot s grows by add[s] >= 0 tokens (lens[s] += add[s]), its new pages with one reference.
- * *_marked: with marks (n_slots) int32, 2^31 - 1 at first (NULL: as without).  A refused reserve sets the marks of the slots with
- *   add[s] != 0 to -1, one that is done sets them to 2^31 - 1.  For a slot whose mark is -1, append_rope writes no page (its
- *   rows of out mean nothing), and keep leaves all of it as it is: a pass that nobody checks in between cannot harm older tokens.  append_rope
- *   lowers a slot's mark to the number of its first row that lies outside the tables, keep refuses (code 5) a row from there on
- *   that is to be kept, and sets the marks of the slots that it has dealt with back.
+ * *_marked: with marks (n_slots, 9) int32 (NULL: as without), at first 2^31 - 1 and eight zeros for each slot; what the numbers
+ *   mean is up to these calls.  A refused reserve marks the slots with add[s] != 0, one that is done takes their marks
+ *   back.  For a slot marked so, append_rope writes no page (its rows of out mean nothing), and keep leaves all of it as it
+ *   is: a pass that nobody checks in between cannot harm older tokens.  append_rope marks the rows that lie outside its
+ *   tables (from row 256 on, that and all behind it); keep refuses such a row (code 5), and takes the marks of the slots that
+ *   it has dealt with back.
  * fork: for n entries, the empty slot dst[i] becomes a copy of slot src[i]: full pages are shared, a last page that is
  *   partly filled is copied (every layer: pages of layer l at pages + l * n_pages * page_bytes).
  * free: the slots' pages lose a reference, their rows become -1 and their lengths 0.  A slot named twice is freed

@@ -126,6 +126,10 @@ SX8_KV4_FN uint32_t kv4_tree_bits(const uint64_t* mask, int words, int first, in
     return (uint32_t)v;
 }
 
+// A slot's mark (include/sx8_paged.h): its first word, behind it a bit for each of its first 256 new rows.
+constexpr int kMarkRows = 256, kMarkWords = 1 + kMarkRows / 32;
+constexpr int32_t kMarkAll = 0x7FFFFFFF, kMarkSome = 0x7FFFFFFE, kMarkRefused = -1;
+
 // Blocks of tokens that the new tokens of a slot touch (append, read): first block, and how many.  Positions
 // len - n .. len - 1; those below zero (more rows than tokens) lie in blocks below zero, which have no page.
 SX8_KV4_FN int kv4_floor_block(int pos) { return pos >= 0 ? pos / kKv4Block : -((-pos + kKv4Block - 1) / kKv4Block); }

@@ -22,7 +22,7 @@ struct RopeIn {
     const float *cos, *sin;
     int64_t table_rows;
     const int32_t* depth;
-    int32_t* marks;                         // of a slot: new rows in the pages, below zero: its reservation was refused (or null)
+    int32_t* marks;                         // [n_slots][kMarkWords], or null
     const uint16_t *qw, *kw;
     double eps;
     int rot, heads;                         // heads: query heads of a work-group
@@ -125,10 +125,10 @@ __global__ __launch_bounds__(256) void k_kv4_append_rope(const Kv4Pool p, const 
     // prompts and their read 52.3 us, without marks 51.9, looked at by all work-groups 53.0).
     const bool looks = in.marks && (int)blockIdx.y < p.sh.nk, late = p.cu && p.sh.n_slots > 64;
     int mark = 0;
-    if (looks && !late) mark = in.marks[p.cu ? min((int)threadIdx.x & 63, p.sh.n_slots - 1) : (int)blockIdx.x];
+    if (looks && !late) mark = in.marks[kMarkWords * (p.cu ? min((int)threadIdx.x & 63, p.sh.n_slots - 1) : (int)blockIdx.x)];
     Touched t;
     if (!find_touched(p, blockIdx.x, pre, &t)) return;
-    if (looks && p.cu) mark = late ? in.marks[t.slot] : __builtin_amdgcn_readlane(mark, t.slot);
+    if (looks && p.cu) mark = late ? in.marks[kMarkWords * t.slot] : __builtin_amdgcn_readlane(mark, t.slot);
     const int head = blockIdx.y, tid = threadIdx.x, nt = t.t1 - t.t0, half = in.rot / 2;
     // (the last tokens of a slot that was refused its new ones are older: nothing of it may be overwritten)
     const bool refused = mark < 0;
@@ -136,7 +136,12 @@ __global__ __launch_bounds__(256) void k_kv4_append_rope(const Kv4Pool p, const 
         const int64_t at = in.depth ? (int64_t)t.first + in.depth[t.row0 + tid] : (int64_t)t.block * 32 + t.t0 + tid;
         const bool inside = at >= 0 && at < in.table_rows;
         place[t.t0 + tid] = !refused && inside ? (int)at : -1;
-        if (in.marks && !inside && head == 0) atomicMin(&in.marks[t.slot], t.block * 32 + t.t0 + tid - t.first);
+        if (in.marks && !inside && head == 0) {                      // (a row that stays out of the pages)
+            int32_t* const of = in.marks + kMarkWords * t.slot;
+            const int row = t.block * 32 + t.t0 + tid - t.first;
+            if (row < kMarkRows) atomicOr(&of[1 + row / 32], 1 << row % 32);
+            atomicMin(of, row < kMarkRows ? kMarkSome : row);
+        }
     }
     __syncthreads();
     if (head >= p.sh.nk) {

@@ -108,7 +108,11 @@ __device__ __forceinline__ void report(int32_t* status, int code, int item) {
 }
 
 // ---- reserve -----------------------------------------------------------------------------------
-constexpr int32_t kAllRows = 0x7FFFFFFF, kRefused = -1;              // a slot's mark (include/sx8_paged.h)
+__device__ __forceinline__ void clear_mark(int32_t* of) {
+    if (*of == kMarkAll) return;                                     // (no bit is set)
+#pragma unroll
+    for (int i = 0; i < kMarkWords; ++i) of[i] = i ? 0 : kMarkAll;
+}
 
 __global__ __launch_bounds__(kPageThreads) void k_reserve(const PageTab t, const int32_t* add, const PageWs ws, int32_t* marks) {
     const int tid = threadIdx.x, pt = t.page_tokens;
@@ -140,7 +144,7 @@ __global__ __launch_bounds__(kPageThreads) void k_reserve(const PageTab t, const
         report(t.status, code, item);
         if (marks)
             for (int s = tid; s < t.n_slots; s += kPageThreads)
-                if (add[s] != 0) marks[s] = kRefused;
+                if (add[s] != 0) marks[kMarkWords * s] = kMarkRefused;
         return;
     }
     for (int s = tid; s < t.n_slots; s += kPageThreads) {
@@ -154,7 +158,7 @@ __global__ __launch_bounds__(kPageThreads) void k_reserve(const PageTab t, const
         }
         if (a) {
             t.lens[s] = len + a;
-            if (marks) marks[s] = kAllRows;
+            if (marks) clear_mark(marks + kMarkWords * s);
         }
     }
 }
@@ -369,7 +373,7 @@ KeepWs keep_ws(void* w, int64_t n_slots) {
 }
 
 // A slot of n new rows keeps rows path[0] < path[1] < .. (counts of them) of these.  A slot that its reservation was refused
-// has none (its last n tokens are older ones): it is passed over.  Rows from the slot's mark on were not all written.
+// has none (its last n tokens are older ones): it is passed over.
 __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const int32_t* path, const int32_t* counts,
                                                        const int32_t* cu, Kv4Shape sh, const KeepWs ws, int32_t* marks) {
     const int tid = threadIdx.x, pt = t.page_tokens;
@@ -382,14 +386,14 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
             int first, n;
             kv4_rows(sh, cu, s, &first, &n);
             const int len = t.lens[s], c = counts[s], base = len - n;
-            const int mark = n > 0 && marks ? marks[s] : kAllRows;
+            const int32_t* const of = marks + kMarkWords * s;
+            const int mark = n > 0 && marks ? *of : kMarkAll;
             bool bad = false, missing = false;
             if (mark < 0) {
                 n = 0;
             } else if (n > 0) {
                 bad = c < 0 || c > n || base < 0 || len > cap;
-                int last = -1;
-                for (int i = 0; !bad && i < c; i += 8) {             // (eight asked for together)
+                for (int i = 0, last = -1; !bad && i < c; i += 8) {  // (eight asked for together)
                     int at[8];
 #pragma unroll
                     for (int u = 0; u < 8; ++u) at[u] = path[first + min(i + u, c - 1)];
@@ -400,7 +404,10 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
                         last = at[u];
                     }
                 }
-                missing = !bad && last >= mark;
+                for (int i = 0; !bad && mark != kMarkAll && i < c; ++i) {
+                    const int r = path[first + i];
+                    missing |= r < kMarkRows ? of[1 + r / 32] >> r % 32 & 1 : r >= mark;
+                }
                 if (!bad) held = (len + pt - 1) / pt - base / pt;
             } else {
                 bad = c != 0;
@@ -441,7 +448,7 @@ __global__ __launch_bounds__(kPageThreads) void k_keep(const PageTab t, const in
             }
         }
         t.lens[s] = end;
-        if (marks) marks[s] = kAllRows;
+        if (marks) clear_mark(marks + kMarkWords * s);
     }
 }
 

@@ -186,20 +186,22 @@ class PagedKV4:
         _ints("refs", refs, self.n_pages, self.device)
         self.n_kv, self.head_dim, self.page_tokens, self.page_bytes = int(n_kv), int(head_dim), int(page_tokens), nb
         status = torch.zeros(2, dtype=torch.int32, device=self.device)
+        marks = torch.zeros(self.n_slots, 9, dtype=torch.int32, device=self.device)
+        marks[:, 0] = 2 ** 31 - 1
         self._ws_pages = int(_L.lib().sx8_kv4_pages_workspace_bytes(self.n_slots, self.n_pages))
         if self._ws_pages < 0 or self.max_pages * self.page_tokens > 1 << 22:
             raise RuntimeError("a cache has 1..4096 slots of up to 2^22 tokens and up to 2^28 pages")
         self._ws_attend = int(_L.lib().sx8_kv4_attend_workspace_bytes(self.head_dim))
         self._ws_tree = int(_L.lib().sx8_kv4_attend_tree_workspace_bytes(self.head_dim))
         self._t = (pages, table, lens, refs, status, nb, self.n_kv, self.head_dim, self.page_tokens, self._ws_attend,
-                   self._ws_pages, self._ws_tree, torch.full((self.n_slots,), 2 ** 31 - 1, dtype=torch.int32, device=self.device))
+                   self._ws_pages, self._ws_tree, marks)
 
     pages = property(lambda self: self._t[0])
     table = property(lambda self: self._t[1])
     lens = property(lambda self: self._t[2])
     refs = property(lambda self: self._t[3])
     status = property(lambda self: self._t[4])
-    marks = property(lambda self: self._t[12])                      # of a slot: new rows that are in the pages, -1: its reserve was refused
+    marks = property(lambda self: self._t[12])                      # of a slot: was its reserve refused, which of its rows are not in the pages
 
     # ---------------------------------------------------------------- rows
     def _slots(self, layer, cu):

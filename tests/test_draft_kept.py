@@ -135,6 +135,10 @@ def state(p):
     return [t.clone() for t in (p.pages, p.table, p.lens, p.refs)]
 
 
+def unmarked(p):
+    return p.marks.tolist() == [[2 ** 31 - 1] + [0] * 8] * p.n_slots
+
+
 def same(a, b):
     return all(torch.equal(x, y) for x, y in zip(a, b))
 
@@ -213,19 +217,19 @@ def test_marks_are_of_the_slot(hiplib, cuda):
     # reserved, then other slots refused: the pass goes on
     late.reserve(ints([3, 0, 5], cuda))
     late.reserve(ints([0, 100, 0], cuda))
-    assert late.marks.tolist() == [2 ** 31 - 1, -1, 2 ** 31 - 1]
+    assert late.marks[:, 0].tolist() == [2 ** 31 - 1, -1, 2 ** 31 - 1]
     a_pass(late, [3, 0, 5], 30, cuda, cos, sin, reserve=False)()
     with pytest.raises(RuntimeError, match="no free pages"):
         late.check()
     late.reserve(ints([0, 1, 0], cuda))
-    assert late.marks.tolist() == [2 ** 31 - 1] * 3 and late.lens[1] == 65
+    assert unmarked(late) and late.lens[1] == 65
     a_pass(want, [3, 0, 5], 30, cuda, cos, sin)()
     want.check()
     assert same(state(p), state(want))
     want.reserve(ints([0, 1, 0], cuda))
     assert same(state(late), state(want))
     late.reserve(ints([-1, 0, 0], cuda))
-    assert late.marks.tolist() == [-1, 2 ** 31 - 1, 2 ** 31 - 1]
+    assert late.marks[:, 0].tolist() == [-1, 2 ** 31 - 1, 2 ** 31 - 1]
     with pytest.raises(RuntimeError, match="bad slot or count"):
         late.check()
 
@@ -262,7 +266,7 @@ def test_keep_refuses_rows_that_were_not_written(hiplib, cuda, monkeypatch, gene
         p.keep(path, ints(good, cuda), cu)
         p.check()
         lens = [10 + good[0], 33 + good[1]]
-        assert p.lens.tolist()[:2] == lens and p.marks.tolist() == [2 ** 31 - 1] * S
+        assert p.lens.tolist()[:2] == lens and unmarked(p)
         at = list(range(10, lens[0]))
         got = p.read(1, sum(lens), ints([0, lens[0], *[sum(lens)] * (S - 1)], cuda))
         assert torch.equal(got[0][10:lens[0]], q4(turn(k[:good[0]], None, cos[at], sin[at], False).float().half()).half())
@@ -286,20 +290,45 @@ def test_rows_that_were_not_written_and_not_kept(hiplib, cuda):
     q, k = rand((new, 2, 64), 1, F16, cuda), rand((new, 1, 64), 2, F16, cuda)
     _, depth = draft_tree(parents, cu)
     p.append_rope(0, q, k, k, cos, sin, cu, depth=depth)
-    assert p.marks.tolist() == [64]
+    assert not unmarked(p)
     x = torch.zeros(new, 100, device=cuda)
     u = torch.full((new,), 0.999, device=cuda)
     u[63] = 0.0
     path, counts, _ = verify_draft(x, torch.arange(new, device=cuda), parents, cu, u, 1.0)
     p.keep(path, counts, cu)
     p.check()
-    assert path.tolist()[:3] == [0, 63, -1] and p.lens.tolist() == [12] and p.marks.tolist() == [2 ** 31 - 1]
+    assert path.tolist()[:3] == [0, 63, -1] and p.lens.tolist() == [12] and unmarked(p)
     p.reserve(ints([3], cuda))
     p.append_rope(0, q[:3], k[:3], k[:3], cos, sin, cum([3], cuda), depth=ints([0, -13, 1], cuda))
-    assert p.marks.tolist() == [1]
-    p.keep(ints([0, 2, -1], cuda), ints([2], cuda), cum([3], cuda))
+    p.keep(ints([0, 1, -1], cuda), ints([2], cuda), cum([3], cuda))
     with pytest.raises(RuntimeError, match="never written"):
         p.check()
-    p.keep(ints([0, 2, -1], cuda), ints([1], cuda), cum([3], cuda))
+    p.keep(ints([0, 2, -1], cuda), ints([2], cuda), cum([3], cuda))
     p.check()
-    assert p.lens.tolist() == [13]
+    assert p.lens.tolist() == [14]
+
+
+def test_branches_beside_a_row_that_was_not_written(hiplib, cuda):
+    """A deep branch ends behind the tables; a row with a higher number that is written is kept, the deep ones are not: every
+    single row of a tree of 256 and rows behind them, where one that is out takes all behind it with it."""
+    p, _, _ = make(cuda, [10], 1, 64, 32, spare=14, width=20)
+    cos, sin = tables(20, 64, cuda)
+    q, k = rand((300, 2, 64), 1, F16, cuda), rand((300, 1, 64), 2, F16, cuda)
+    rng = random.Random(1)
+    depth = [0] + [rng.choice([1, 3, 9, 10, 11, 2 ** 31 - 1, -11, 2]) for _ in range(255)] + [1] * 20 + [10] + [1] * 23
+    cu, d = cum([300], cuda), ints(depth, cuda)
+    for row in [*range(1, 256, 5), 31, 32, 63, 64, 255, 256, 275, 276, 277, 299]:
+        p.reserve(ints([300], cuda))
+        p.append_rope(0, q, k, k, cos, sin, cu, depth=d)
+        p.keep(ints([0, row] + [-1] * 298, cuda), ints([2], cuda), cu)
+        if not 0 <= 10 + depth[row] < 20 or row > 276:
+            with pytest.raises(RuntimeError, match="never written"):
+                p.check()
+            p.keep(ints([0] + [-1] * 299, cuda), ints([0], cuda), cu)
+            assert p.lens.tolist() == [10]
+        else:
+            p.check()
+            assert p.lens.tolist() == [12] and unmarked(p)
+            p.lens.fill_(10)
+        p.check()
+        assert unmarked(p)
